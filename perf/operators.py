@@ -82,7 +82,7 @@ def draw(rng):
     new = _log(rng, 1 if kind == "prompt" else 16, min(8192, top))
     past = rng.choice([0, 0, _log(rng, 1, 1024)]) if new < min(8192, top) - 1024 else 0
     return dict(case, new=new, past=past, dim=rng.choice([16, 32, 40, 64, 64, 80, 96, 128, 128]),
-                window=_log(rng, 1, 4096), sinks=rng.choice([0, 1, 4, 4, rng.randint(2, 64)]),
+                window=_log(rng, 2, 4096), sinks=rng.choice([0, 1, 4, 4, rng.randint(2, 64)]),
                 ragged=case["batch"] > 1 and rng.random() < 0.5)
 
 
