@@ -420,6 +420,51 @@ int lnn_optimizer_step(int dev, int kind, uint64_t V, uint64_t G, uint64_t S1, u
 int lnn_optimizer_step_many(int dev, int kind, int count, const uint64_t* V, const uint64_t* G, const uint64_t* S1,
                             const uint64_t* S2, const int64_t* n, const uint32_t* seeds, const lnn_opt_params* p);
 
+/* ---- operators on tokens ---------------------------------------------------------------
+ * Token numbers and lengths are whole numbers in fp32 (exact to 2^24).  A token below zero marks a padded place: zeros,
+ * no gradient.  A number that is no row of the table, or a length that is none, counts as padding and leaves
+ * LNN_E_INVALID in the device status, which the next lnn_sync or lnn_d2h returns.
+ * Nothing in the reference corresponds to them. */
+
+/* Y[n] = scale * TABLE[IDS[n]];  dTABLE[v] (+)= scale * sum of dY[n] over the n with IDS[n] = v, in the order of n */
+int lnn_embedding_fwd(int dev, uint64_t Y, uint64_t TABLE, uint64_t IDS, int64_t tokens, int64_t vocab, int64_t dim,
+                      float scale);
+int lnn_embedding_bwd_acc(int dev, uint64_t dTABLE, uint64_t dY, uint64_t IDS, int64_t tokens, int64_t vocab, int64_t dim,
+                          float scale, int accumulate);
+
+/* LOGP[n] = X[n, id] - log(sum(exp(X[n]))).  LOSS[n] = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ * + kl (exp(REF - logp) - (REF - logp) - 1) with r = exp(logp - OLD), A = ADV; REF = 0: no KL term.
+ * STATS (optional, 3 floats per row) is what the gradient of either needs:
+ * dX[n, j] (+)= dOUT[n] * d OUT / d logp * ((j == id) - p_j). */
+int lnn_token_log_prob_fwd(int dev, uint64_t LOGP, uint64_t STATS, uint64_t X, uint64_t IDS, int64_t rows, int64_t vocab);
+int lnn_policy_loss_fwd(int dev, uint64_t LOSS, uint64_t STATS, uint64_t X, uint64_t IDS, uint64_t OLD, uint64_t ADV,
+                        uint64_t REF, int64_t rows, int64_t vocab, float clip_low, float clip_high, float kl);
+int lnn_token_logit_bwd_acc(int dev, uint64_t dX, uint64_t X, uint64_t STATS, uint64_t IDS, uint64_t dOUT, int64_t rows,
+                            int64_t vocab, int accumulate);
+
+/* Causal attention with a sliding window and `sinks` first tokens that stay visible.  Q, O [batch][q_heads][q_len][dim],
+ * K, V [batch][kv_heads][kv_len][dim]; query i is at position p = i + kv_len - q_len and sees key j when p < LEN[batch],
+ * j <= p and (p - j < window or j < sinks).  Rows that see nothing give zeros.  LEN may be 0 (kv_len everywhere).
+ * LSE [batch][q_heads][q_len] is kept for the gradients; a gradient whose pointer is 0 is not computed. */
+typedef struct lnn_attn_geom {
+  int batch, q_heads, kv_heads, q_len, kv_len, dim, window, sinks;
+  float scale;
+} lnn_attn_geom;
+int lnn_sink_attn_fwd(int dev, uint64_t O, uint64_t LSE, uint64_t Q, uint64_t K, uint64_t V, uint64_t LEN,
+                      const lnn_attn_geom* g);
+int lnn_sink_attn_bwd(int dev, uint64_t dQ, uint64_t dK, uint64_t dV, uint64_t Q, uint64_t K, uint64_t V, uint64_t O,
+                      uint64_t LSE, uint64_t LEN, uint64_t dO, const lnn_attn_geom* g, int acc_q, int acc_k, int acc_v);
+
+/* The cache that the same attention needs for one token after another: [batch][heads][sinks + window][dim], position p
+ * in slot p (p < sinks) or sinks + (p - sinks) % window.  lnn_sink_cache_store fills it from a prompt and writes the
+ * lengths to LEN_OUT (a batch entry whose LEN is below zero stays as it is); lnn_sink_attn_step appends K and V
+ * ([batch][kv_heads][dim]) and attends with Q ([batch][q_heads][dim]); LEN_OUT = LEN + 1 is other memory than LEN.  A
+ * batch entry of a length below zero is not in use: O is zero, its cache and length stay. */
+int lnn_sink_cache_store(int dev, uint64_t CK, uint64_t CV, uint64_t LEN_OUT, uint64_t K, uint64_t V, uint64_t LEN, int batch,
+                         int heads, int kv_len, int dim, int window, int sinks);
+int lnn_sink_attn_step(int dev, uint64_t O, uint64_t Q, uint64_t K, uint64_t V, uint64_t CK, uint64_t CV, uint64_t LEN,
+                       uint64_t LEN_OUT, int batch, int q_heads, int kv_heads, int dim, int window, int sinks, float scale);
+
 /* NCCL (loaded with dlopen on first use).  One communicator per device slot.
  * ref: optimizer/Optimizer.py:149-153 (host-staged replica averaging, replaced by a
  * gradient all-reduce) */

@@ -49,6 +49,16 @@ class ConvGeom(ctypes.Structure):
         self.address = ctypes.addressof(self)
 
 
+class AttnGeom(ctypes.Structure):
+    """Mirror of struct lnn_attn_geom."""
+    _fields_ = [(n, c_int) for n in ("batch", "q_heads", "kv_heads", "q_len", "kv_len", "dim", "window", "sinks")] + [
+        ("scale", c_float)]
+
+    def __init__(self, *values):
+        super().__init__(*values)
+        self.address = ctypes.addressof(self)
+
+
 _I64P = POINTER(c_int64)
 _SIGNATURES = {
     "lnn_version": (c_int, []),
@@ -140,6 +150,15 @@ _SIGNATURES = {
     "lnn_sgd_step": (c_int, [c_int, c_uint64, c_uint64, c_int64, c_float, c_float]),
     "lnn_optimizer_step": (c_int, [c_int, c_int, c_uint64, c_uint64, c_uint64, c_uint64, c_int64, c_void_p]),
     "lnn_optimizer_step_many": (c_int, [c_int, c_int, c_int] + [POINTER(c_uint64)] * 4 + [_I64P, POINTER(ctypes.c_uint32), c_void_p]),
+    "lnn_embedding_fwd": (c_int, [c_int, c_uint64, c_uint64, c_uint64, c_int64, c_int64, c_int64, c_float]),
+    "lnn_embedding_bwd_acc": (c_int, [c_int, c_uint64, c_uint64, c_uint64, c_int64, c_int64, c_int64, c_float, c_int]),
+    "lnn_token_log_prob_fwd": (c_int, [c_int] + [c_uint64] * 4 + [c_int64] * 2),
+    "lnn_policy_loss_fwd": (c_int, [c_int] + [c_uint64] * 7 + [c_int64] * 2 + [c_float] * 3),
+    "lnn_token_logit_bwd_acc": (c_int, [c_int] + [c_uint64] * 5 + [c_int64] * 2 + [c_int]),
+    "lnn_sink_attn_fwd": (c_int, [c_int] + [c_uint64] * 6 + [POINTER(AttnGeom)]),
+    "lnn_sink_attn_bwd": (c_int, [c_int] + [c_uint64] * 10 + [POINTER(AttnGeom)] + [c_int] * 3),
+    "lnn_sink_cache_store": (c_int, [c_int] + [c_uint64] * 6 + [c_int] * 6),
+    "lnn_sink_attn_step": (c_int, [c_int] + [c_uint64] * 8 + [c_int] * 6 + [c_float]),
     "lnn_nccl_unique_id": (c_int, [c_void_p]),
     "lnn_nccl_init_rank": (c_int, [c_int, c_int, c_int, c_void_p]),
     "lnn_nccl_init_all": (c_int, [POINTER(c_int), c_int]),
@@ -190,6 +209,15 @@ _CALLS = {
     "lnn_depthwise_conv2d_dx": "nnmpp",
     "lnn_depthwise_conv2d_dk": "nnmpp",
     "lnn_optimizer_step_many": "nnnLlLLnnn",
+    "lnn_embedding_fwd": "nwppnnnf",
+    "lnn_embedding_bwd_acc": "noppnnnfa",
+    "lnn_token_log_prob_fwd": "nwwppnn",
+    "lnn_policy_loss_fwd": "nwwpppppnnfff",
+    "lnn_token_logit_bwd_acc": "noppppnna",
+    "lnn_sink_attn_fwd": "nwwppppn",
+    "lnn_sink_attn_bwd": "nwwwpppppppnnnn",
+    "lnn_sink_cache_store": "nmmmpppnnnnnn",
+    "lnn_sink_attn_step": "nwpppmmpwnnnnnnf",
 }
 
 

@@ -1,0 +1,658 @@
+// Attention with a sliding window and sinks on the FP32 pipe, forward and backward, and the single-token step over a
+// cache.  One pass over the visible tiles of keys, the running maximum and sum of the softmax in registers; the
+// backward pass recomputes the probabilities from the stored denominators, once for the rows of dq and once for those
+// of dk and dv, so that every sum has one owner and a fixed order (no atomics).
+#include <cooperative_groups.h>
+#include <math_constants.h>
+#include <float.h>
+#include <algorithm>
+#include "lnn_attn.cuh"
+
+namespace {
+
+namespace cg = cooperative_groups;
+using lnn::AttnArgs;
+using lnn::exp2_fast;
+
+constexpr int kThreads = 256;           // 16 x 16
+
+// rows [r0, r0 + B) of a [len][dim] matrix into shared memory with pitch DP + 4, zeros outside
+template <int B, int DP>
+__device__ __forceinline__ void load_rows(float* dst, const float* src, int r0, int len, int dim) {
+  for (int i = threadIdx.x; i < B * DP; i += kThreads) {
+    const int r = i / DP, c = i % DP;
+    dst[r * (DP + 4) + c] = r0 + r < len && c < dim ? __ldg(src + (int64_t)(r0 + r) * dim + c) : 0.0f;
+  }
+}
+// s[r][c] = row (ty + 16 r) of A times row (tx + 16 c) of Bm
+template <int B, int DP>
+__device__ __forceinline__ void tile_product(float (&s)[B / 16][B / 16], const float* A, const float* Bm, int ty, int tx) {
+  constexpr int R = B / 16, PITCH = DP + 4;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < R; ++c) s[r][c] = 0.0f;
+  for (int d = 0; d < DP; d += 4) {
+    float4 a[R], b[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) a[r] = *reinterpret_cast<const float4*>(A + (ty + 16 * r) * PITCH + d);
+#pragma unroll
+    for (int c = 0; c < R; ++c) b[c] = *reinterpret_cast<const float4*>(Bm + (tx + 16 * c) * PITCH + d);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < R; ++c)
+        s[r][c] = fmaf(a[r].w, b[c].w, fmaf(a[r].z, b[c].z, fmaf(a[r].y, b[c].y, fmaf(a[r].x, b[c].x, s[r][c]))));
+  }
+}
+// o[r][..] += sum_j W[ty + 16 r][j] X[j][..]; a weight of zero leaves out what X holds there (it may not be finite)
+template <int B, int DP>
+__device__ __forceinline__ void tile_weighted(float (&o)[B / 16][DP / 16], const float* W, const float* X, int ty, int tx) {
+  constexpr int R = B / 16, PITCH = DP + 4;
+  for (int j = 0; j < B; ++j) {
+    float x[DP / 16];
+#pragma unroll
+    for (int u = 0; u < DP / 16; ++u) x[u] = X[j * PITCH + tx + 16 * u];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float w = W[(ty + 16 * r) * (B + 1) + j];
+      if (w != 0.0f)
+#pragma unroll
+        for (int u = 0; u < DP / 16; ++u) o[r][u] = fmaf(w, x[u], o[r][u]);
+    }
+  }
+}
+__device__ __forceinline__ float row_max(float v) {        // over the 16 threads of a row
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+template <int B, int DP>
+__global__ void __launch_bounds__(kThreads)
+simt_fwd_kernel(const AttnArgs a) {
+  constexpr int R = B / 16, PITCH = DP + 4;
+  extern __shared__ __align__(16) float smem[];
+  float *Q = smem, *K = Q + B * PITCH, *V = K + B * PITCH, *P = V + B * PITCH;
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int i0 = blockIdx.x * B, past = a.kv_len - a.q_len;
+  const int len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
+  const int64_t head = (int64_t)b * a.q_heads + h;
+  const int64_t kv = ((int64_t)b * a.kv_heads + h / (a.q_heads / a.kv_heads)) * a.kv_len * a.dim;
+  const float factor = a.scale * lnn::kLog2e;
+  float o[R][DP / 16], m[R], l[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -CUDART_INF_F;
+    l[r] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < DP / 16; ++u) o[r][u] = 0.0f;
+  }
+  const int p_hi = min(min(i0 + B, a.q_len) - 1 + past, len - 1);
+  if (p_hi >= i0 + past) {
+    load_rows<B, DP>(Q, a.q + head * a.q_len * a.dim, i0, a.q_len, a.dim);
+    const lnn::KeyTiles tiles(i0 + past, p_hi, a.window, a.sinks, B);
+    for (int t = 0; t < tiles.count; ++t) {
+      const int j0 = tiles.at(t) * B;
+      __syncthreads();
+      load_rows<B, DP>(K, a.k + kv, j0, a.kv_len, a.dim);
+      load_rows<B, DP>(V, a.v + kv, j0, a.kv_len, a.dim);
+      __syncthreads();
+      float s[R][R];
+      tile_product<B, DP>(s, Q, K, ty, tx);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int p = i0 + ty + 16 * r + past;
+        float top = -CUDART_INF_F;
+#pragma unroll
+        for (int c = 0; c < R; ++c) {
+          s[r][c] = p <= p_hi && lnn::attn_visible(p, j0 + tx + 16 * c, a.window, a.sinks) ? __fmul_rn(s[r][c], factor)
+                                                                                            : -CUDART_INF_F;
+          top = fmaxf(top, s[r][c]);
+        }
+        top = fmaxf(m[r], row_max(top));
+        const float base = top == -CUDART_INF_F ? 0.0f : top;
+        const float keep = exp2_fast(__fsub_rn(m[r], base));
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < R; ++c) {
+          const float e = exp2_fast(__fsub_rn(s[r][c], base));
+          sum = __fadd_rn(sum, e);
+          P[(ty + 16 * r) * (B + 1) + tx + 16 * c] = e;
+        }
+        l[r] = __fadd_rn(__fmul_rn(l[r], keep), row_sum(sum));
+        m[r] = top;
+#pragma unroll
+        for (int u = 0; u < DP / 16; ++u) o[r][u] = __fmul_rn(o[r][u], keep);
+      }
+      __syncthreads();
+      tile_weighted<B, DP>(o, P, V, ty, tx);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = i0 + ty + 16 * r;
+    if (i >= a.q_len) continue;
+    const bool empty = i + past > p_hi;
+    const float inv = empty ? 0.0f : __fdiv_rn(1.0f, l[r]);
+    float* to = a.o + (head * a.q_len + i) * a.dim;
+#pragma unroll
+    for (int u = 0; u < DP / 16; ++u)
+      if (tx + 16 * u < a.dim) to[tx + 16 * u] = empty ? 0.0f : __fmul_rn(o[r][u], inv);
+    if (tx == 0) a.lse[head * a.q_len + i] = empty ? CUDART_INF_F : __fadd_rn(m[r], log2f(l[r]));
+  }
+}
+
+// P = 2^(factor S - lse) and dS = scale P (dP - delta) of a tile: rows are queries (KEYS false) or keys (true)
+template <int B, int DP>
+__global__ void __launch_bounds__(kThreads)
+simt_dq_kernel(const AttnArgs a) {
+  constexpr int R = B / 16, PITCH = DP + 4;
+  extern __shared__ __align__(16) float smem[];
+  float *Q = smem, *D = Q + B * PITCH, *K = D + B * PITCH, *V = K + B * PITCH, *S = V + B * PITCH;
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int i0 = blockIdx.x * B, past = a.kv_len - a.q_len;
+  const int len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
+  const int64_t head = (int64_t)b * a.q_heads + h;
+  const int64_t kv = ((int64_t)b * a.kv_heads + h / (a.q_heads / a.kv_heads)) * a.kv_len * a.dim;
+  const float factor = a.scale * lnn::kLog2e;
+  float g[R][DP / 16], lse[R], delta[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = i0 + ty + 16 * r;
+    lse[r] = i < a.q_len ? a.lse[head * a.q_len + i] : CUDART_INF_F;
+    delta[r] = i < a.q_len ? a.delta[head * a.q_len + i] : 0.0f;
+#pragma unroll
+    for (int u = 0; u < DP / 16; ++u) g[r][u] = 0.0f;
+  }
+  const int p_hi = min(min(i0 + B, a.q_len) - 1 + past, len - 1);
+  if (p_hi >= i0 + past) {
+    load_rows<B, DP>(Q, a.q + head * a.q_len * a.dim, i0, a.q_len, a.dim);
+    load_rows<B, DP>(D, a.dout + head * a.q_len * a.dim, i0, a.q_len, a.dim);
+    const lnn::KeyTiles tiles(i0 + past, p_hi, a.window, a.sinks, B);
+    for (int t = 0; t < tiles.count; ++t) {
+      const int j0 = tiles.at(t) * B;
+      __syncthreads();
+      load_rows<B, DP>(K, a.k + kv, j0, a.kv_len, a.dim);
+      load_rows<B, DP>(V, a.v + kv, j0, a.kv_len, a.dim);
+      __syncthreads();
+      float s[R][R], dp[R][R];
+      tile_product<B, DP>(s, Q, K, ty, tx);
+      tile_product<B, DP>(dp, D, V, ty, tx);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int c = 0; c < R; ++c) {
+          const int p = i0 + ty + 16 * r + past;
+          const bool seen = p <= p_hi && lnn::attn_visible(p, j0 + tx + 16 * c, a.window, a.sinks);
+          const float e = exp2_fast(__fsub_rn(__fmul_rn(s[r][c], factor), lse[r]));
+          S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fsub_rn(dp[r][c], delta[r])), a.scale) : 0.0f;
+        }
+      __syncthreads();
+      tile_weighted<B, DP>(g, S, K, ty, tx);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = i0 + ty + 16 * r;
+    if (i >= a.q_len) continue;
+    float* to = a.dq + (head * a.q_len + i) * a.dim;
+#pragma unroll
+    for (int u = 0; u < DP / 16; ++u)
+      if (tx + 16 * u < a.dim) to[tx + 16 * u] = a.acc_q ? __fadd_rn(to[tx + 16 * u], g[r][u]) : g[r][u];
+  }
+}
+
+template <int B, int DP>
+__global__ void __launch_bounds__(kThreads)
+simt_dkv_kernel(const AttnArgs a) {
+  constexpr int R = B / 16, PITCH = DP + 4;
+  extern __shared__ __align__(16) float smem[];
+  float *Q = smem, *D = Q + B * PITCH, *K = D + B * PITCH, *V = K + B * PITCH, *P = V + B * PITCH, *S = P + B * (B + 1);
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  const int hk = blockIdx.y, b = blockIdx.z, group = a.q_heads / a.kv_heads;
+  const int j0 = blockIdx.x * B, past = a.kv_len - a.q_len;
+  const int len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
+  const int64_t kv = ((int64_t)b * a.kv_heads + hk) * a.kv_len * a.dim;
+  const float factor = a.scale * lnn::kLog2e;
+  float gk[R][DP / 16], gv[R][DP / 16];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int u = 0; u < DP / 16; ++u) gk[r][u] = gv[r][u] = 0.0f;
+  const lnn::QuerySpan span(j0, min(j0 + B, a.kv_len) - 1, a.window, a.sinks, past, len);
+  if (span.hi >= span.lo) {
+    load_rows<B, DP>(K, a.k + kv, j0, a.kv_len, a.dim);
+    load_rows<B, DP>(V, a.v + kv, j0, a.kv_len, a.dim);
+    for (int h = hk * group; h < (hk + 1) * group; ++h) {
+      const int64_t head = (int64_t)b * a.q_heads + h;
+      for (int i0 = (span.lo - past) / B * B; i0 + past <= span.hi; i0 += B) {
+        __syncthreads();
+        load_rows<B, DP>(Q, a.q + head * a.q_len * a.dim, i0, a.q_len, a.dim);
+        load_rows<B, DP>(D, a.dout + head * a.q_len * a.dim, i0, a.q_len, a.dim);
+        __syncthreads();
+        float s[R][R], dp[R][R];
+        tile_product<B, DP>(s, K, Q, ty, tx);
+        tile_product<B, DP>(dp, V, D, ty, tx);
+#pragma unroll
+        for (int c = 0; c < R; ++c) {
+          const int i = i0 + tx + 16 * c, p = i + past;
+          const float lse = i < a.q_len ? __ldg(a.lse + head * a.q_len + i) : CUDART_INF_F;
+          const float delta = i < a.q_len ? __ldg(a.delta + head * a.q_len + i) : 0.0f;
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const bool seen = i < a.q_len && p < len && lnn::attn_visible(p, j0 + ty + 16 * r, a.window, a.sinks);
+            const float e = seen ? exp2_fast(__fsub_rn(__fmul_rn(s[r][c], factor), lse)) : 0.0f;
+            P[(ty + 16 * r) * (B + 1) + tx + 16 * c] = e;
+            S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fsub_rn(dp[r][c], delta)), a.scale) : 0.0f;
+          }
+        }
+        __syncthreads();
+        tile_weighted<B, DP>(gv, P, D, ty, tx);
+        tile_weighted<B, DP>(gk, S, Q, ty, tx);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int j = j0 + ty + 16 * r;
+    if (j >= a.kv_len) continue;
+#pragma unroll
+    for (int u = 0; u < DP / 16; ++u) {
+      const int c = tx + 16 * u;
+      if (c >= a.dim) continue;
+      const int64_t at = kv + (int64_t)j * a.dim + c;
+      if (a.dk) a.dk[at] = a.acc_k ? __fadd_rn(a.dk[at], gk[r][u]) : gk[r][u];
+      if (a.dv) a.dv[at] = a.acc_v ? __fadd_rn(a.dv[at], gv[r][u]) : gv[r][u];
+    }
+  }
+}
+
+// one warp per row
+__global__ void __launch_bounds__(kThreads)
+attn_delta_kernel(float* __restrict__ delta, const float* __restrict__ dout, const float* __restrict__ o, int64_t rows, int dim) {
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  float s = 0.0f;
+  for (int c = threadIdx.x & 31; c < dim; c += 32) s = fmaf(__ldg(dout + row * dim + c), __ldg(o + row * dim + c), s);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, x));
+  if ((threadIdx.x & 31) == 0) delta[row] = s;
+}
+
+template <int B, int DP, class Kernel>
+int launch_simt(lnn::Device* d, Kernel kernel, int matrices, int tiles, dim3 grid, const AttnArgs& a) {
+  const size_t bytes = (size_t)(matrices * B * (DP + 4) + tiles * B * (B + 1)) * 4;
+  LNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  kernel<<<grid, kThreads, bytes, d->stream>>>(a);
+  LNN_CHECK_LAUNCH(d);
+  return LNN_OK;
+}
+
+template <int B, int DP>
+int simt_fwd(lnn::Device* d, const AttnArgs& a) {
+  return launch_simt<B, DP>(d, simt_fwd_kernel<B, DP>, 3, 1,
+                            dim3((unsigned)lnn_ceil_div(a.q_len, B), (unsigned)a.q_heads, (unsigned)a.batch), a);
+}
+template <int B, int DP>
+int simt_bwd(lnn::Device* d, const AttnArgs& a) {
+  int rc = LNN_OK;
+  if (a.dq)
+    rc = launch_simt<B, DP>(d, simt_dq_kernel<B, DP>, 4, 1,
+                            dim3((unsigned)lnn_ceil_div(a.q_len, B), (unsigned)a.q_heads, (unsigned)a.batch), a);
+  if (!rc && (a.dk || a.dv))
+    rc = launch_simt<B, DP>(d, simt_dkv_kernel<B, DP>, 4, 2,
+                            dim3((unsigned)lnn_ceil_div(a.kv_len, B), (unsigned)a.kv_heads, (unsigned)a.batch), a);
+  return rc;
+}
+
+// ---- the cache -----------------------------------------------------------------------------------
+// Slots of a sequence: the first `sinks` positions keep theirs, the later ones go round the other `window`.  A
+// position p that a query at the newest one sees is in slot p (p < sinks) or sinks + (p - sinks) % window, and
+// all slots below min(length, sinks + window) hold such positions: attention over the cache needs no mask.
+constexpr float kMaxLength = 16777216.0f;      // lengths are exact in fp32 up to 2^24
+
+// a sequence's length; below zero: the slot of the batch is not in use
+__device__ __forceinline__ int cache_length(float x, int b, int* status) {
+  if (x < 0.0f) return -1;
+  if (!(x < kMaxLength) || x != floorf(x)) {
+    if (atomicCAS(status, 0, LNN_E_INVALID) == 0) { status[1] = 5; status[2] = b; status[3] = (int)x; }
+    return -1;
+  }
+  return (int)x;
+}
+
+__global__ void __launch_bounds__(kThreads)
+cache_store_kernel(float* __restrict__ ck, float* __restrict__ cv, float* __restrict__ lengths_out, const float* __restrict__ k,
+                   const float* __restrict__ v, const float* __restrict__ lengths, int heads, int kv_len, int dim, int window,
+                   int sinks, int* status) {
+  const int b = blockIdx.z, h = blockIdx.y, slots = window + sinks;
+  if (lengths && __ldg(lengths + b) < 0.0f) return;               // this slot of the batch stays as it is
+  const int len = lnn::attn_length(lengths, b, kv_len, status);
+  if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) lengths_out[b] = (float)len;
+  const int64_t src = ((int64_t)b * heads + h) * kv_len * dim, dst = ((int64_t)b * heads + h) * slots * dim;
+  const int used = min(len, slots);
+  const int64_t n = (int64_t)used * dim;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+    const int slot = (int)(i / dim), c = (int)(i - (int64_t)slot * dim);
+    // the latest position that lives in this slot
+    const int p = slot < sinks ? slot : slot + (len - 1 - slot) / window * window;
+    ck[dst + i] = k[src + (int64_t)p * dim + c];
+    cv[dst + i] = v[src + (int64_t)p * dim + c];
+  }
+}
+
+struct StepArgs {
+  float* o;
+  const float *q, *k, *v;                // [batch][q_heads][dim], [batch][kv_heads][dim]
+  float *ck, *cv;                        // [batch][kv_heads][sinks + window][dim]
+  const float* lengths;
+  float* lengths_out;
+  int batch, q_heads, kv_heads, dim, window, sinks, splits, group_chunks;
+  float scale;
+  int* status;
+};
+
+// Eight lanes share a key: each holds 4 NV of its values, and of the queries and outputs of GC heads.  A warp takes
+// four keys at a time, and every group of eight lanes has a softmax of its own, which meet at the end: within the warp
+// by shuffles, in the block through shared memory and over the blocks of a cluster (the slots of one sequence and head,
+// cut into contiguous shares) through distributed shared memory.  The new key and value are read from the arguments
+// while one block writes them into the cache.
+template <int GC, int NV, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+step_kernel(const StepArgs a) {
+  extern __shared__ __align__(16) float smem[];
+  constexpr int kWarps = kThreads / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane & 7, sub = lane >> 3;
+  const int rank = blockIdx.x;                                    // the cluster runs along x
+  const int hk = blockIdx.y / a.group_chunks, chunk = blockIdx.y % a.group_chunks, b = blockIdx.z;
+  const int group = a.q_heads / a.kv_heads, dim = a.dim, slots = a.window + a.sinks;
+  const int h0 = hk * group + chunk * GC, heads = min(GC, group - chunk * GC);
+  const int len = cache_length(__ldg(a.lengths + b), b, a.status);
+  if (rank == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.lengths_out[b] = len < 0 ? a.lengths[b] : (float)(len + 1);
+  const int64_t oq = ((int64_t)b * a.q_heads + h0) * dim, okv = ((int64_t)b * a.kv_heads + hk) * dim, oc = okv * slots;
+  if (len < 0) {                                                  // the same for the whole cluster
+    if (rank == 0)
+      for (int i = threadIdx.x; i < heads * dim; i += kThreads) a.o[oq + i] = 0.0f;
+    return;
+  }
+  const int fresh = len < a.sinks ? len : a.sinks + (len - a.sinks) % a.window;
+  const int n = min(len + 1, slots);
+  const int per = ((n + a.splits - 1) / a.splits + 31) / 32 * 32;
+  const int begin = min(rank * per, n), end = min(begin + per, n);
+
+  const auto load = [&](const float* row, int u) {
+    const int c = u * 32 + part * 4;
+    if (VEC) return c < dim ? __ldg(reinterpret_cast<const float4*>(row + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    return make_float4(c < dim ? __ldg(row + c) : 0.0f, c + 1 < dim ? __ldg(row + c + 1) : 0.0f,
+                       c + 2 < dim ? __ldg(row + c + 2) : 0.0f, c + 3 < dim ? __ldg(row + c + 3) : 0.0f);
+  };
+  float4 q[GC][NV], o[GC][NV];
+  float m[GC], l[GC];
+  const float factor = a.scale * lnn::kLog2e;
+#pragma unroll
+  for (int g = 0; g < GC; ++g) {
+    m[g] = -FLT_MAX;
+    l[g] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      o[g][u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      q[g][u] = g < heads ? load(a.q + oq + g * dim, u) : o[g][u];
+      q[g][u].x *= factor; q[g][u].y *= factor; q[g][u].z *= factor; q[g][u].w *= factor;
+    }
+  }
+  for (int s0 = begin; s0 < end; s0 += 4 * kWarps) {
+    const int slot = s0 + warp * 4 + sub;
+    const bool in = slot < end;
+    const float* krow = slot == fresh ? a.k + okv : a.ck + oc + (int64_t)slot * dim;
+    const float* vrow = slot == fresh ? a.v + okv : a.cv + oc + (int64_t)slot * dim;
+    float4 k[NV], v[NV];
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      k[u] = in ? load(krow, u) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      v[u] = in ? load(vrow, u) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+#pragma unroll
+    for (int g = 0; g < GC; ++g) {
+      float s = 0.0f;
+#pragma unroll
+      for (int u = 0; u < NV; ++u)
+        s = fmaf(q[g][u].w, k[u].w, fmaf(q[g][u].z, k[u].z, fmaf(q[g][u].y, k[u].y, fmaf(q[g][u].x, k[u].x, s))));
+#pragma unroll
+      for (int x = 4; x > 0; x >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, x));
+      if (in) {
+        if (s > m[g]) {
+          const float keep = exp2_fast(__fsub_rn(m[g], s));
+          l[g] = __fmul_rn(l[g], keep);
+#pragma unroll
+          for (int u = 0; u < NV; ++u) {
+            o[g][u].x *= keep; o[g][u].y *= keep; o[g][u].z *= keep; o[g][u].w *= keep;
+          }
+          m[g] = s;
+        }
+        const float e = exp2_fast(__fsub_rn(s, m[g]));
+        l[g] = __fadd_rn(l[g], e);
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+          o[g][u].x = fmaf(e, v[u].x, o[g][u].x); o[g][u].y = fmaf(e, v[u].y, o[g][u].y);
+          o[g][u].z = fmaf(e, v[u].z, o[g][u].z); o[g][u].w = fmaf(e, v[u].w, o[g][u].w);
+        }
+      }
+    }
+  }
+  // one share per cluster and head writes the new row: nobody reads it from the cache in this launch
+  if (rank == 0 && chunk == 0)
+    for (int i = threadIdx.x; i < dim; i += kThreads) {
+      a.ck[oc + (int64_t)fresh * dim + i] = a.k[okv + i];
+      a.cv[oc + (int64_t)fresh * dim + i] = a.v[okv + i];
+    }
+  // shared memory: per warp GC heads of {values, m, l}; then the block's own
+  constexpr int kRow = NV * 32 + 2;
+  float* mine = smem + warp * GC * kRow;
+  float* block = smem + kWarps * GC * kRow;
+#pragma unroll
+  for (int g = 0; g < GC; ++g) {
+    float top = fmaxf(m[g], __shfl_xor_sync(0xffffffffu, m[g], 8));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    const float w = exp2_fast(__fsub_rn(m[g], top));
+    float sum = __fmul_rn(l[g], w);
+    sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, 8));
+    sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, 16));
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      float x[4] = {o[g][u].x, o[g][u].y, o[g][u].z, o[g][u].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = __fmul_rn(x[i], w);
+        x[i] = __fadd_rn(x[i], __shfl_xor_sync(0xffffffffu, x[i], 8));
+        x[i] = __fadd_rn(x[i], __shfl_xor_sync(0xffffffffu, x[i], 16));
+        if (sub == 0) mine[g * kRow + u * 32 + part * 4 + i] = x[i];
+      }
+    }
+    if (lane == 0) {
+      mine[g * kRow + NV * 32] = top;
+      mine[g * kRow + NV * 32 + 1] = sum;
+    }
+  }
+  __syncthreads();
+  // {values, m, l} of `count` partial results `stride` floats apart; column NV * 32 + 1 gives the sum of the l
+  const auto join = [&](auto&& from, int count, int g, int c) {
+    float top = from(0)[g * kRow + NV * 32];
+    for (int w = 1; w < count; ++w) top = fmaxf(top, from(w)[g * kRow + NV * 32]);
+    float sum = 0.0f;
+    for (int w = 0; w < count; ++w) sum = fmaf(exp2_fast(__fsub_rn(from(w)[g * kRow + NV * 32], top)), from(w)[g * kRow + c], sum);
+    return make_float2(sum, top);
+  };
+  const auto of_warp = [&](int w) { return smem + w * GC * kRow; };
+  for (int i = threadIdx.x; i < GC * (NV * 32 + 1); i += kThreads) {
+    const int g = i / (NV * 32 + 1), c = i % (NV * 32 + 1);
+    const float2 r = join(of_warp, kWarps, g, c < NV * 32 ? c : NV * 32 + 1);
+    if (c < NV * 32) block[g * kRow + c] = r.x;
+    else { block[g * kRow + NV * 32] = r.y; block[g * kRow + NV * 32 + 1] = r.x; }
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  if (a.splits > 1) cluster.sync();
+  else __syncthreads();
+  const auto of_rank = [&](int r) { return a.splits > 1 ? cluster.map_shared_rank(block, r) : block; };
+  for (int i = rank * kThreads + threadIdx.x; i < heads * dim; i += a.splits * kThreads) {
+    const int g = i / dim, c = i % dim;
+    const float sum = join(of_rank, a.splits, g, NV * 32 + 1).x;
+    a.o[oq + i] = __fdiv_rn(join(of_rank, a.splits, g, c).x, sum);
+  }
+  if (a.splits > 1) cluster.sync();                      // nobody leaves while its shared memory is being read
+}
+
+template <int GC, int NV>
+int launch_step(lnn::Device* d, StepArgs& a, bool vec) {
+  const int group = a.q_heads / a.kv_heads;
+  a.group_chunks = (group + GC - 1) / GC;
+  const int64_t clusters = (int64_t)a.batch * a.kv_heads * a.group_chunks;
+  a.splits = 1;
+  while (a.splits < 8 && clusters * a.splits < 2 * d->sm_count && a.window + a.sinks >= a.splits * 2 * 64) a.splits *= 2;
+  LNN_REQUIRE((int64_t)a.kv_heads * a.group_chunks < 65536, "too many heads");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.splits, (unsigned)(a.kv_heads * a.group_chunks), (unsigned)a.batch);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = (size_t)(kThreads / 32 + 1) * GC * (NV * 32 + 2) * 4;
+  cfg.stream = d->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)a.splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.splits > 1 ? 1 : 0;
+  LNN_CUDA(vec ? cudaLaunchKernelEx(&cfg, step_kernel<GC, NV, true>, a) : cudaLaunchKernelEx(&cfg, step_kernel<GC, NV, false>, a));
+  LNN_CHECK_LAUNCH(d);
+  return LNN_OK;
+}
+template <int NV>
+int launch_step(lnn::Device* d, StepArgs& a, bool vec) {
+  const int group = a.q_heads / a.kv_heads;
+  if (group == 1) return launch_step<1, NV>(d, a, vec);
+  if (group == 2 || NV > 4) return launch_step<2, NV>(d, a, vec);
+  return launch_step<4, NV>(d, a, vec);
+}
+
+const float* in(uint64_t p) { return (const float*)(uintptr_t)p; }
+float* out(uint64_t p) { return (float*)(uintptr_t)p; }
+
+int check_geom(const lnn_attn_geom* g) {
+  LNN_REQUIRE(g && g->batch > 0 && g->q_heads > 0 && g->kv_heads > 0 && g->q_len > 0 && g->kv_len > 0 && g->dim > 0, "bad geometry");
+  LNN_REQUIRE(g->q_heads % g->kv_heads == 0, "%d query heads over %d key heads", g->q_heads, g->kv_heads);
+  LNN_REQUIRE(g->q_len <= g->kv_len, "%d queries over %d keys", g->q_len, g->kv_len);
+  LNN_REQUIRE(g->dim <= 256, "heads of %d values: at most 256", g->dim);
+  LNN_REQUIRE(g->window > 0 && g->sinks >= 0, "window %d, sinks %d", g->window, g->sinks);
+  LNN_REQUIRE(g->batch < 65536 && g->q_heads < 65536 && g->kv_len <= (1 << 24), "geometry too large");
+  return LNN_OK;
+}
+
+AttnArgs attn_args(lnn::Device* d, const lnn_attn_geom* g, uint64_t Q, uint64_t K, uint64_t V, uint64_t LEN) {
+  AttnArgs a = {};
+  a.q = in(Q); a.k = in(K); a.v = in(V); a.lengths = in(LEN);
+  a.batch = g->batch; a.q_heads = g->q_heads; a.kv_heads = g->kv_heads; a.q_len = g->q_len; a.kv_len = g->kv_len;
+  a.dim = g->dim; a.scale = g->scale;
+  a.window = g->window < g->kv_len ? g->window : g->kv_len;       // (positions end there: no sum below passes 2^31)
+  a.sinks = g->sinks < g->kv_len ? g->sinks : g->kv_len;
+  a.status = d->status_dev;
+  return a;
+}
+
+}  // namespace
+
+namespace lnn {
+
+int attn_simt_fwd(Device* d, const AttnArgs& a) {
+  if (a.dim <= 32) return simt_fwd<64, 32>(d, a);
+  if (a.dim <= 64) return simt_fwd<64, 64>(d, a);
+  if (a.dim <= 128) return simt_fwd<64, 128>(d, a);
+  return simt_fwd<32, 256>(d, a);
+}
+
+int attn_simt_bwd(Device* d, const AttnArgs& a) {
+  if (a.dim <= 32) return simt_bwd<64, 32>(d, a);
+  if (a.dim <= 64) return simt_bwd<64, 64>(d, a);
+  if (a.dim <= 128) return simt_bwd<64, 128>(d, a);
+  return simt_bwd<32, 256>(d, a);
+}
+
+int attn_delta(Device* d, float* delta, const float* dout, const float* o, int64_t rows, int dim) {
+  attn_delta_kernel<<<(unsigned)lnn_ceil_div(rows, kThreads / 32), kThreads, 0, d->stream>>>(delta, dout, o, rows, dim);
+  LNN_CHECK_LAUNCH(d);
+  return LNN_OK;
+}
+
+}  // namespace lnn
+
+extern "C" {
+
+int lnn_sink_attn_fwd(int dev, uint64_t O, uint64_t LSE, uint64_t Q, uint64_t K, uint64_t V, uint64_t LEN, const lnn_attn_geom* g) {
+  LNN_DEV(d, dev);
+  int rc = check_geom(g);
+  if (rc) return rc;
+  LNN_REQUIRE(O && LSE && Q && K && V, "bad arguments");
+  AttnArgs a = attn_args(d, g, Q, K, V, LEN);
+  a.o = out(O); a.lse = out(LSE);
+  return lnn::attn_simt_fwd(d, a);
+}
+
+int lnn_sink_attn_bwd(int dev, uint64_t dQ, uint64_t dK, uint64_t dV, uint64_t Q, uint64_t K, uint64_t V, uint64_t O, uint64_t LSE,
+                      uint64_t LEN, uint64_t dO, const lnn_attn_geom* g, int acc_q, int acc_k, int acc_v) {
+  LNN_DEV(d, dev);
+  int rc = check_geom(g);
+  if (rc) return rc;
+  LNN_REQUIRE(Q && K && V && O && LSE && dO, "bad arguments");
+  AttnArgs a = attn_args(d, g, Q, K, V, LEN);
+  const int64_t rows = (int64_t)g->batch * g->q_heads * g->q_len;
+  lnn::Scratch delta(d);
+  rc = delta.get((uint64_t)rows * 4);
+  if (!rc) rc = lnn::attn_delta(d, delta.as<float>(), in(dO), in(O), rows, g->dim);
+  if (rc) return rc;
+  a.lse = out(LSE); a.dout = in(dO); a.delta = delta.as<float>();
+  a.dq = out(dQ); a.dk = out(dK); a.dv = out(dV);
+  a.acc_q = acc_q; a.acc_k = acc_k; a.acc_v = acc_v;
+  return lnn::attn_simt_bwd(d, a);
+}
+
+int lnn_sink_cache_store(int dev, uint64_t CK, uint64_t CV, uint64_t LEN_OUT, uint64_t K, uint64_t V, uint64_t LEN, int batch,
+                         int heads, int kv_len, int dim, int window, int sinks) {
+  LNN_DEV(d, dev);
+  LNN_REQUIRE(CK && CV && LEN_OUT && LEN_OUT != LEN && K && V && batch > 0 && heads > 0 && kv_len > 0 && dim > 0 && window > 0 && sinks >= 0,
+              "bad arguments");
+  LNN_REQUIRE(batch < 65536 && heads < 65536 && kv_len <= (1 << 24) && (int64_t)window + sinks <= (1 << 24), "geometry too large");
+  const int64_t elements = (int64_t)std::min(kv_len, window + sinks) * dim;
+  const int64_t blocks = std::min<int64_t>(lnn_ceil_div(elements, kThreads),
+                                           std::max<int64_t>(1, (int64_t)d->sm_count * 16 / ((int64_t)batch * heads)));
+  cache_store_kernel<<<dim3((unsigned)blocks, (unsigned)heads, (unsigned)batch), kThreads, 0, d->stream>>>(
+      out(CK), out(CV), out(LEN_OUT), in(K), in(V), in(LEN), heads, kv_len, dim, window, sinks, d->status_dev);
+  LNN_CHECK_LAUNCH(d);
+  return LNN_OK;
+}
+
+int lnn_sink_attn_step(int dev, uint64_t O, uint64_t Q, uint64_t K, uint64_t V, uint64_t CK, uint64_t CV, uint64_t LEN,
+                       uint64_t LEN_OUT, int batch, int q_heads, int kv_heads, int dim, int window, int sinks, float scale) {
+  LNN_DEV(d, dev);
+  LNN_REQUIRE(O && Q && K && V && CK && CV && LEN && LEN_OUT && LEN != LEN_OUT, "bad arguments");
+  LNN_REQUIRE(batch > 0 && q_heads > 0 && kv_heads > 0 && dim > 0 && window > 0 && sinks >= 0 && q_heads % kv_heads == 0,
+              "bad arguments");
+  LNN_REQUIRE(dim <= 256, "heads of %d values: at most 256", dim);
+  LNN_REQUIRE(batch < 65536 && (int64_t)window + sinks <= (1 << 24), "geometry too large");
+  StepArgs a = {};
+  a.o = out(O); a.q = in(Q); a.k = in(K); a.v = in(V); a.ck = out(CK); a.cv = out(CV);
+  a.lengths = in(LEN); a.lengths_out = out(LEN_OUT);
+  a.batch = batch; a.q_heads = q_heads; a.kv_heads = kv_heads; a.dim = dim; a.window = window; a.sinks = sinks;
+  a.scale = scale; a.status = d->status_dev;
+  const bool vec = dim % 4 == 0 && ((Q | K | V | CK | CV) & 15) == 0;
+  if (dim <= 32) return launch_step<1>(d, a, vec);
+  if (dim <= 64) return launch_step<2>(d, a, vec);
+  if (dim <= 96) return launch_step<3>(d, a, vec);
+  if (dim <= 128) return launch_step<4>(d, a, vec);
+  return launch_step<8>(d, a, vec);
+}
+
+}  // extern "C"

@@ -240,6 +240,15 @@ int lnn_h2d(int dev, uint64_t dst, const void* src, uint64_t bytes) {
 // stream in front of the sync the caller pays anyway): a bounded wait that expired in a tile
 // kernel makes the kernels after it return at once, so whatever the host is about to read is
 // not a result.  Reporting clears the word, so that work can go on afterwards.
+// A kernel met a token number or a length that it cannot use (and put nothing in its place).
+static int invalid_value(const int* st) {
+  static const char* const what[] = {"value", "token number of an embedding", "token number of an embedding's gradient",
+                                     "token number of a row of logits", "length of a sequence", "length of a cached sequence"};
+  return lnn::set_error(LNN_E_INVALID,
+                        "a %s (number %d, value %d) is not a whole number in its range; results computed since then are "
+                        "invalid (the status has been cleared)",
+                        what[st[1] >= 0 && st[1] < 6 ? st[1] : 0], st[2], st[3]);
+}
 static int sync_and_report(lnn::Device* d) {
   LNN_CUDA(cudaMemcpyAsync(d->status_host, d->status_dev, sizeof(int) * 4, cudaMemcpyDeviceToHost, d->stream));
   LNN_CUDA(cudaStreamSynchronize(d->stream));
@@ -248,6 +257,7 @@ static int sync_and_report(lnn::Device* d) {
     LNN_CUDA(cudaMemsetAsync(d->status_dev, 0, sizeof(int) * 4, d->stream));
     LNN_CUDA(cudaMemsetAsync(d->grid_barrier, 0, sizeof(unsigned int) * 2, d->stream));
     LNN_CUDA(cudaStreamSynchronize(d->stream));
+    if (st[0] == LNN_E_INVALID) return invalid_value(st);
     return lnn::set_error(LNN_E_TIMEOUT,
                           "device status %d (role %d, tile %d, step %d): a bounded wait expired in a tile kernel; "
                           "results computed since then are invalid (the status has been cleared)",
@@ -357,7 +367,9 @@ int lnn_device_status(int dev, int* status) {
   LNN_CUDA(cudaMemsetAsync(d->grid_barrier, 0, sizeof(unsigned int) * 2, d->stream));   // a wait that gave up leaves it set
   LNN_CUDA(cudaStreamSynchronize(d->stream));
   *status = d->status_host[0];
-  if (*status != 0)
+  if (*status == LNN_E_INVALID)
+    invalid_value(d->status_host);
+  else if (*status != 0)
     set_error(LNN_E_TIMEOUT, "device status %d (role %d, tile %d, step %d): a bounded wait expired",
               d->status_host[0], d->status_host[1], d->status_host[2], d->status_host[3]);
   return LNN_OK;

@@ -9,7 +9,7 @@ import weakref
 from pathlib import Path
 
 from . import initializer as _init
-from . import ops
+from . import ops, sequence
 from .devices import devices
 from .tensor import Tensor
 
@@ -378,5 +378,23 @@ class Dense(Module):
 
     def __str__(self):
         return f"{self.__class__.__name__} : in_ch:{self.in_ch} out_ch:{self.out_ch} "
+
+    __repr__ = __str__
+
+
+class Embedding(Module):
+    """Embedding(num_tokens, dim, scale=1.0, weight_initializer=None); forward = nn.embedding(ids, weight, scale): the
+    rows of the (num_tokens, dim) table that the ids name.  The default initializer is RandomNormal(0, 1)."""
+
+    def __init__(self, num_tokens, dim, scale=1.0, weight_initializer=None):
+        self.num_tokens, self.dim, self.scale = num_tokens, dim, scale
+        self.weight = Tensor((num_tokens, dim), init=weight_initializer or _init.RandomNormal(0.0, 1.0))
+        super().__init__(saveables=["weight"])
+
+    def forward(self, ids, **kwargs):
+        return sequence.embedding(ids, self.weight, self.scale)
+
+    def __str__(self):
+        return f"{self.__class__.__name__} : num_tokens:{self.num_tokens} dim:{self.dim} "
 
     __repr__ = __str__
