@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 SOURCES = ["lnn_runtime.cu", "lnn_eltwise.cu", "lnn_pool.cu", "lnn_reduce.cu", "lnn_move.cu",
            "lnn_tc.cu", "lnn_small.cu", "lnn_fewch.cu", "lnn_direct.cu", "lnn_depthwise.cu", "lnn_nccl.cu",
-           "lnn_token.cu", "lnn_attn.cu"]
+           "lnn_token.cu", "lnn_attn.cu", "lnn_attn_tc.cu"]
 HEADERS = ["lnn_common.cuh", "lnn_tc.cuh", "lnn_tc_dev.cuh", "lnn_attn.cuh", os.path.join("..", "..", "include", "litenn_b200.h")]
 LIB = os.path.join(PKG, "liblitenn_b200.so")
 NATIVE = os.path.join(PKG, "_native.so")

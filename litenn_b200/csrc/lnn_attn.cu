@@ -80,8 +80,13 @@ simt_fwd_kernel(const AttnArgs a) {
   extern __shared__ __align__(16) float smem[];
   float *Q = smem, *K = Q + B * PITCH, *V = K + B * PITCH, *P = V + B * PITCH;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  const int h = blockIdx.y, b = blockIdx.z;
-  const int i0 = blockIdx.x * B, past = a.kv_len - a.q_len;
+  if (a.info && !lnn::any_group_left(a)) return;
+  const int tiles_q = (a.q_len + B - 1) / B, past = a.kv_len - a.q_len;
+  for (int64_t work = blockIdx.x; work < (int64_t)tiles_q * a.q_heads * a.batch; work += gridDim.x) {
+  const int h = (int)(work / tiles_q % a.q_heads), b = (int)(work / tiles_q / a.q_heads);
+  const int i0 = (int)(work % tiles_q) * B;
+  if (a.info && lnn::group_ok(a, b, h / (a.q_heads / a.kv_heads))) continue;
+  __syncthreads();
   const int len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
   const int64_t head = (int64_t)b * a.q_heads + h;
   const int64_t kv = ((int64_t)b * a.kv_heads + h / (a.q_heads / a.kv_heads)) * a.kv_len * a.dim;
@@ -147,6 +152,7 @@ simt_fwd_kernel(const AttnArgs a) {
       if (tx + 16 * u < a.dim) to[tx + 16 * u] = empty ? 0.0f : __fmul_rn(o[r][u], inv);
     if (tx == 0) a.lse[head * a.q_len + i] = empty ? CUDART_INF_F : __fadd_rn(m[r], log2f(l[r]));
   }
+  }
 }
 
 // P = 2^(factor S - lse) and dS = scale P (dP - delta) of a tile: rows are queries (KEYS false) or keys (true)
@@ -157,8 +163,13 @@ simt_dq_kernel(const AttnArgs a) {
   extern __shared__ __align__(16) float smem[];
   float *Q = smem, *D = Q + B * PITCH, *K = D + B * PITCH, *V = K + B * PITCH, *S = V + B * PITCH;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  const int h = blockIdx.y, b = blockIdx.z;
-  const int i0 = blockIdx.x * B, past = a.kv_len - a.q_len;
+  if (a.info && !lnn::any_group_left(a)) return;
+  const int tiles_q = (a.q_len + B - 1) / B, past = a.kv_len - a.q_len;
+  for (int64_t work = blockIdx.x; work < (int64_t)tiles_q * a.q_heads * a.batch; work += gridDim.x) {
+  const int h = (int)(work / tiles_q % a.q_heads), b = (int)(work / tiles_q / a.q_heads);
+  const int i0 = (int)(work % tiles_q) * B;
+  if (a.info && lnn::group_ok(a, b, h / (a.q_heads / a.kv_heads))) continue;
+  __syncthreads();
   const int len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
   const int64_t head = (int64_t)b * a.q_heads + h;
   const int64_t kv = ((int64_t)b * a.kv_heads + h / (a.q_heads / a.kv_heads)) * a.kv_len * a.dim;
@@ -168,7 +179,7 @@ simt_dq_kernel(const AttnArgs a) {
   for (int r = 0; r < R; ++r) {
     const int i = i0 + ty + 16 * r;
     lse[r] = i < a.q_len ? a.lse[head * a.q_len + i] : CUDART_INF_F;
-    delta[r] = i < a.q_len ? a.delta[head * a.q_len + i] : 0.0f;
+    delta[r] = i < a.q_len ? a.delta[head * a.delta_pitch + i] : 0.0f;
 #pragma unroll
     for (int u = 0; u < DP / 16; ++u) g[r][u] = 0.0f;
   }
@@ -208,6 +219,7 @@ simt_dq_kernel(const AttnArgs a) {
     for (int u = 0; u < DP / 16; ++u)
       if (tx + 16 * u < a.dim) to[tx + 16 * u] = a.acc_q ? __fadd_rn(to[tx + 16 * u], g[r][u]) : g[r][u];
   }
+  }
 }
 
 template <int B, int DP>
@@ -217,8 +229,13 @@ simt_dkv_kernel(const AttnArgs a) {
   extern __shared__ __align__(16) float smem[];
   float *Q = smem, *D = Q + B * PITCH, *K = D + B * PITCH, *V = K + B * PITCH, *P = V + B * PITCH, *S = P + B * (B + 1);
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  const int hk = blockIdx.y, b = blockIdx.z, group = a.q_heads / a.kv_heads;
-  const int j0 = blockIdx.x * B, past = a.kv_len - a.q_len;
+  if (a.info && !lnn::any_group_left(a)) return;
+  const int tiles_k = (a.kv_len + B - 1) / B, past = a.kv_len - a.q_len, group = a.q_heads / a.kv_heads;
+  for (int64_t work = blockIdx.x; work < (int64_t)tiles_k * a.kv_heads * a.batch; work += gridDim.x) {
+  const int hk = (int)(work / tiles_k % a.kv_heads), b = (int)(work / tiles_k / a.kv_heads);
+  const int j0 = (int)(work % tiles_k) * B;
+  if (a.info && lnn::group_ok(a, b, hk)) continue;
+  __syncthreads();
   const int len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
   const int64_t kv = ((int64_t)b * a.kv_heads + hk) * a.kv_len * a.dim;
   const float factor = a.scale * lnn::kLog2e;
@@ -245,7 +262,7 @@ simt_dkv_kernel(const AttnArgs a) {
         for (int c = 0; c < R; ++c) {
           const int i = i0 + tx + 16 * c, p = i + past;
           const float lse = i < a.q_len ? __ldg(a.lse + head * a.q_len + i) : CUDART_INF_F;
-          const float delta = i < a.q_len ? __ldg(a.delta + head * a.q_len + i) : 0.0f;
+          const float delta = i < a.q_len ? __ldg(a.delta + head * a.delta_pitch + i) : 0.0f;
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             const bool seen = i < a.q_len && p < len && lnn::attn_visible(p, j0 + ty + 16 * r, a.window, a.sinks);
@@ -273,6 +290,7 @@ simt_dkv_kernel(const AttnArgs a) {
       if (a.dv) a.dv[at] = a.acc_v ? __fadd_rn(a.dv[at], gv[r][u]) : gv[r][u];
     }
   }
+  }
 }
 
 // one warp per row
@@ -288,7 +306,8 @@ attn_delta_kernel(float* __restrict__ delta, const float* __restrict__ dout, con
 }
 
 template <int B, int DP, class Kernel>
-int launch_simt(lnn::Device* d, Kernel kernel, int matrices, int tiles, dim3 grid, const AttnArgs& a) {
+int launch_simt(lnn::Device* d, Kernel kernel, int matrices, int tiles, int64_t works, const AttnArgs& a) {
+  const unsigned grid = (unsigned)std::min<int64_t>(works, a.info ? d->sm_count : 1 << 30);
   const size_t bytes = (size_t)(matrices * B * (DP + 4) + tiles * B * (B + 1)) * 4;
   LNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
   kernel<<<grid, kThreads, bytes, d->stream>>>(a);
@@ -299,17 +318,17 @@ int launch_simt(lnn::Device* d, Kernel kernel, int matrices, int tiles, dim3 gri
 template <int B, int DP>
 int simt_fwd(lnn::Device* d, const AttnArgs& a) {
   return launch_simt<B, DP>(d, simt_fwd_kernel<B, DP>, 3, 1,
-                            dim3((unsigned)lnn_ceil_div(a.q_len, B), (unsigned)a.q_heads, (unsigned)a.batch), a);
+                            lnn_ceil_div(a.q_len, B) * a.q_heads * a.batch, a);
 }
 template <int B, int DP>
 int simt_bwd(lnn::Device* d, const AttnArgs& a) {
   int rc = LNN_OK;
   if (a.dq)
     rc = launch_simt<B, DP>(d, simt_dq_kernel<B, DP>, 4, 1,
-                            dim3((unsigned)lnn_ceil_div(a.q_len, B), (unsigned)a.q_heads, (unsigned)a.batch), a);
+                            lnn_ceil_div(a.q_len, B) * a.q_heads * a.batch, a);
   if (!rc && (a.dk || a.dv))
     rc = launch_simt<B, DP>(d, simt_dkv_kernel<B, DP>, 4, 2,
-                            dim3((unsigned)lnn_ceil_div(a.kv_len, B), (unsigned)a.kv_heads, (unsigned)a.batch), a);
+                            lnn_ceil_div(a.kv_len, B) * a.kv_heads * a.batch, a);
   return rc;
 }
 
@@ -598,7 +617,7 @@ int lnn_sink_attn_fwd(int dev, uint64_t O, uint64_t LSE, uint64_t Q, uint64_t K,
   LNN_REQUIRE(O && LSE && Q && K && V, "bad arguments");
   AttnArgs a = attn_args(d, g, Q, K, V, LEN);
   a.o = out(O); a.lse = out(LSE);
-  return lnn::attn_simt_fwd(d, a);
+  return lnn::attn_tc_applicable(a) ? lnn::attn_tc_fwd(d, a) : lnn::attn_simt_fwd(d, a);
 }
 
 int lnn_sink_attn_bwd(int dev, uint64_t dQ, uint64_t dK, uint64_t dV, uint64_t Q, uint64_t K, uint64_t V, uint64_t O, uint64_t LSE,
@@ -608,14 +627,16 @@ int lnn_sink_attn_bwd(int dev, uint64_t dQ, uint64_t dK, uint64_t dV, uint64_t Q
   if (rc) return rc;
   LNN_REQUIRE(Q && K && V && O && LSE && dO, "bad arguments");
   AttnArgs a = attn_args(d, g, Q, K, V, LEN);
+  a.o = out(O); a.lse = out(LSE); a.dout = in(dO);
+  a.dq = out(dQ); a.dk = out(dK); a.dv = out(dV);
+  a.acc_q = acc_q; a.acc_k = acc_k; a.acc_v = acc_v;
+  if (lnn::attn_tc_applicable(a)) return lnn::attn_tc_bwd(d, a);
   const int64_t rows = (int64_t)g->batch * g->q_heads * g->q_len;
   lnn::Scratch delta(d);
   rc = delta.get((uint64_t)rows * 4);
   if (!rc) rc = lnn::attn_delta(d, delta.as<float>(), in(dO), in(O), rows, g->dim);
   if (rc) return rc;
-  a.lse = out(LSE); a.dout = in(dO); a.delta = delta.as<float>();
-  a.dq = out(dQ); a.dk = out(dK); a.dv = out(dV);
-  a.acc_q = acc_q; a.acc_k = acc_k; a.acc_v = acc_v;
+  a.delta = delta.as<float>(); a.delta_pitch = g->q_len;
   return lnn::attn_simt_bwd(d, a);
 }
 

@@ -9,19 +9,29 @@
 
 namespace lnn {
 
+// What is known about a head after its split into fp16 hi and lo.
+struct HeadInfo {
+  int e;                         // x 2^-e was split
+  int ok;                        // finite, and inside fp16's range with that scale
+  float norm;                    // the largest norm of a row, scaled
+};
+
 struct AttnArgs {
   const float *q, *k, *v;        // [batch][q_heads][q_len][dim], [batch][kv_heads][kv_len][dim]
   const float* lengths;          // [batch] whole numbers, or null: kv_len everywhere
   float* o;
   float* lse;                    // [batch][q_heads][q_len]: log2 of the softmax' denominator, +inf where nothing is seen
   const float* dout;             // gradient of o
-  const float* delta;            // [batch][q_heads][q_len]: rows of dout * o summed
+  const float* delta;            // [batch][q_heads][delta_pitch]: rows of dout * o summed
+  int64_t delta_pitch;
   float *dq, *dk, *dv;
   int acc_q, acc_k, acc_v;
   int batch, q_heads, kv_heads, q_len, kv_len, dim;
   int window, sinks;
   float scale;
   int* status;
+  const HeadInfo* info;          // of q's, k's, v's and (backward) dout's heads, or null: see group_ok
+  int backward;
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -67,6 +77,35 @@ __device__ __forceinline__ int attn_length(const float* lengths, int b, int kv_l
   return (int)x;
 }
 
+__device__ __forceinline__ HeadInfo info_of(const AttnArgs& a, int tensor, int head) {
+  const int nq = a.batch * a.q_heads, nk = a.batch * a.kv_heads;
+  const int* p = reinterpret_cast<const int*>(a.info + (tensor == 0 ? 0 : nq + (tensor - 1) * nk) + head);
+  return {__ldg(p), __ldg(p + 1), __int_as_float(__ldg(p + 2))};
+}
+// Whether the tensor cores take the query heads of key head hk: all of its operands were split without loss and the
+// products of their scales stay far inside fp32's range.  The FP32-pipe kernels take the others.
+__device__ __forceinline__ bool group_ok(const AttnArgs& a, int b, int hk) {
+  const int group = a.q_heads / a.kv_heads, kvh = b * a.kv_heads + hk;
+  const HeadInfo k = info_of(a, 1, kvh), v = info_of(a, 2, kvh);
+  bool ok = k.ok && v.ok && abs(k.e) <= 100 && abs(v.e) <= 100;
+  for (int i = 0; i < group; ++i) {
+    const int h = b * a.q_heads + hk * group + i;
+    const HeadInfo q = info_of(a, 0, h);
+    ok = ok && q.ok && abs(q.e) <= 100 && abs(q.e + k.e) <= 100;
+    if (a.backward) {
+      const HeadInfo o = info_of(a, 3, h);
+      ok = ok && o.ok && abs(o.e) <= 100 && abs(o.e + v.e) <= 100 && abs(q.e + o.e + v.e) <= 90 && abs(k.e + o.e + v.e) <= 90;
+    }
+  }
+  return ok;
+}
+// For a whole block: whether any of its work is left to the FP32 pipe.
+__device__ __forceinline__ bool any_group_left(const AttnArgs& a) {
+  int left = 0;
+  for (int i = threadIdx.x; i < a.batch * a.kv_heads; i += blockDim.x) left |= !group_ok(a, i / a.kv_heads, i % a.kv_heads);
+  return __syncthreads_or(left) != 0;
+}
+
 // 2^x with a relative error of 2^-22, 0 below the normal numbers
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -75,8 +114,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 #endif
 
+// On the FP32 pipe; with `info`, only the heads that the tensor cores have left.  Gradients: those that are not null.
 int attn_simt_fwd(Device* d, const AttnArgs& a);
-int attn_simt_bwd(Device* d, const AttnArgs& a);       // the gradients that are not null
+int attn_simt_bwd(Device* d, const AttnArgs& a);
+bool attn_tc_applicable(const AttnArgs& a);
+int attn_tc_fwd(Device* d, const AttnArgs& a);
+int attn_tc_bwd(Device* d, const AttnArgs& a);
 int attn_delta(Device* d, float* delta, const float* dout, const float* o, int64_t rows, int dim);
 
 }  // namespace lnn

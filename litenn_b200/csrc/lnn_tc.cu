@@ -2356,6 +2356,15 @@ namespace lnn {
 int64_t gemm_small_limit() { return (int64_t)knobs().gemm_small * 1000000; }
 }  // namespace lnn
 
+namespace lnn_tc {
+
+int encode_half_map(CUtensorMap* tm, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                    const uint32_t* box, const uint32_t* elem_strides) {
+  return encode_map(tm, base, 2, rank, dims, strides_bytes, box, elem_strides, 128);
+}
+
+}  // namespace lnn_tc
+
 extern "C" {
 
 int lnn_gemm_f32(int dev, uint64_t C, uint64_t A, uint64_t B, uint64_t bias, int64_t batch,

@@ -114,4 +114,8 @@ struct TcParams {
   int tap_shift[kMaxTaps];
 };
 
+// Tensor map of an fp16 tensor with the 128-byte swizzle (dims and box innermost first; rank - 1 strides in bytes).
+int encode_half_map(CUtensorMap* tm, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                    const uint32_t* box, const uint32_t* elem_strides);
+
 }  // namespace lnn_tc
