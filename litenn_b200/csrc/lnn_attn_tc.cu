@@ -15,8 +15,8 @@
 // twice) because 128 stationary rows of K and V of 128 values leave room in shared memory for two tiles of Q and one
 // of dO, not for two of both.
 //
-// A persistent CTA of 320 threads per SM: warp 0 loads (TMA), one thread of warp 1 issues the MMAs, warps 2-9 (two per
-// quarter of the TMEM lanes, half of the columns each) turn scores into weights, write them back to TMEM as the A operand
+// A persistent CTA of 576 threads per SM: warp 0 loads (TMA), one thread of warp 1 issues the MMAs, warps 2-17 (four per
+// quarter of the TMEM lanes, a fourth of the columns each) turn scores into weights, write them back to TMEM as the A operand
 // of the second product (hi and lo in the columns that the scores were in), and keep the running sums in registers.
 // The MMA stream is one step ahead: S(g + 1) runs while the weights of step g are computed.
 #include <algorithm>
@@ -32,7 +32,7 @@ using lnn::exp2_fast;
 
 enum { FWD = 0, DV = 1, DQ = 2, DK = 3 };
 
-constexpr int kComputeWarps = 8;
+constexpr int kComputeWarps = 16, kParts = kComputeWarps / 4;
 constexpr int kAttnThreads = 32 * (2 + kComputeWarps);
 constexpr int kBoxRows = 32;                     // rows of a TMA box
 constexpr int kRowsM = 128;                      // stationary rows
@@ -239,82 +239,126 @@ __device__ __forceinline__ int64_t parts_per_head(const TcArgs& t) {
   return (int64_t)t.sink_tiles * t.splits_sink + (t.splits > 1 ? (int64_t)(t.tiles - t.sink_tiles) * t.splits : 0);
 }
 
-// a tile of 128 stationary rows and the steps of its stream
-template <int MODE, int DP>
+// A tile of 128 stationary rows and the steps of its stream.  The loading warp works it out (divisions, the sequence's
+// length, the scales) and hands it to the others through shared memory, ahead of the tile's turn.
 struct Work {
-  int b, hk, h, row0, steps, first;      // h: the query head of a pass over queries
-  int len, p_hi, lowest, sink_n, sink_steps;         // queries: positions
-  int i_lo, nq, q_hi;                    // keys: first query, tiles of queries per head, position of the last query
-  int tile, split, splits;
-  int64_t part;                          // its place among the parts
-  __device__ __forceinline__ Work(const TcArgs& t, int w) {
-    using S = Shape<MODE, DP>;
-    const AttnArgs& a = t.a;
-    const int past = a.kv_len - a.q_len, group = a.q_heads / a.kv_heads;
-    first = 0;
-    if (!S::KEYS) {
-      tile = w % t.tiles;
-      const int head = w / t.tiles;
-      b = head / a.q_heads; h = head % a.q_heads; hk = h / group;
-      split = 0; splits = 1;
-      len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
-      row0 = tile * kRowsM;
-      p_hi = min(min(row0 + kRowsM, a.q_len) - 1 + past, len - 1);
-      steps = 0;
-      if (p_hi >= row0 + past) {
-        lowest = max(row0 + past - a.window + 1, 0);
-        sink_n = min(a.sinks, lowest);
-        sink_steps = (sink_n + S::BN - 1) / S::BN;
-        steps = sink_steps + (p_hi - lowest) / S::BN + 1;
-      }
+  int b, hk, h, row0, steps;
+  int p_hi, lowest, sink_n, sink_steps;  // queries: positions
+  int i_lo, nq, q_hi, hq0, q0;           // keys: first query, tiles of queries per head, position of the last query; first step
+  int split_up;                          // keys: one of several works of its rows
+  int skip;                              // the FP32 pipe's
+  int part;                              // its place among the parts
+  int ek, ev, eq, eo;                    // exponents of the scales (eq, eo: of query head h)
+  float norm_v, norm_do;
+};
+
+template <int MODE, int DP>
+__device__ __forceinline__ void make_work(Work& k, const TcArgs& t, int w, bool some_left) {
+  using S = Shape<MODE, DP>;
+  const AttnArgs& a = t.a;
+  const int past = a.kv_len - a.q_len, group = a.q_heads / a.kv_heads;
+  k.steps = 0;
+  k.split_up = 0;
+  if (!S::KEYS) {
+    const int head = w / t.tiles;
+    k.b = head / a.q_heads; k.h = head - k.b * a.q_heads; k.hk = k.h / group;
+    const int len = lnn::attn_length(a.lengths, k.b, a.kv_len, a.status);
+    k.row0 = (w - head * t.tiles) * kRowsM;
+    k.p_hi = min(min(k.row0 + kRowsM, a.q_len) - 1 + past, len - 1);
+    if (k.p_hi >= k.row0 + past) {
+      k.lowest = max(k.row0 + past - a.window + 1, 0);
+      k.sink_n = min(a.sinks, k.lowest);
+      k.sink_steps = (k.sink_n + S::BN - 1) / S::BN;
+      k.steps = k.sink_steps + (k.p_hi - k.lowest) / S::BN + 1;
+    }
+  } else {
+    const int per = t.sink_tiles * t.splits_sink + (t.tiles - t.sink_tiles) * t.splits;
+    const int head = w / per;
+    int r = w - head * per, split, splits, tile;
+    k.b = head / a.kv_heads; k.hk = head - k.b * a.kv_heads; k.h = k.hk * group;
+    k.part = (int)(head * parts_per_head(t) + r);
+    if (r < t.sink_tiles * t.splits_sink) {
+      splits = t.splits_sink; tile = r / splits; split = r - tile * splits;
     } else {
-      const int per = t.sink_tiles * t.splits_sink + (t.tiles - t.sink_tiles) * t.splits;
-      int r = w % per;
-      const int head = w / per;
-      b = head / a.kv_heads; hk = head % a.kv_heads; h = hk * group;
-      part = (int64_t)head * parts_per_head(t) + r;
-      if (r < t.sink_tiles * t.splits_sink) {
-        tile = r / t.splits_sink; split = r % t.splits_sink; splits = t.splits_sink;
-      } else {
-        r -= t.sink_tiles * t.splits_sink;
-        tile = t.sink_tiles + r / t.splits; split = r % t.splits; splits = t.splits;
-      }
-      len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
-      row0 = tile * kRowsM;
-      const lnn::QuerySpan span(row0, min(row0 + kRowsM, a.kv_len) - 1, a.window, a.sinks, past, len);
-      steps = 0;
-      if (span.hi >= span.lo) {
-        q_hi = span.hi;
-        i_lo = (span.lo - past) & ~7;                        // (the denominators are read in vectors)
-        nq = (span.hi - past - i_lo) / S::BN + 1;
-        const int all = nq * group;
-        first = (int)((int64_t)all * split / splits);
-        steps = (int)((int64_t)all * (split + 1) / splits) - first;
-      }
+      r -= t.sink_tiles * t.splits_sink;
+      splits = t.splits; tile = r / splits; split = r - tile * splits; tile += t.sink_tiles;
+    }
+    k.split_up = splits > 1;
+    const int len = lnn::attn_length(a.lengths, k.b, a.kv_len, a.status);
+    k.row0 = tile * kRowsM;
+    const lnn::QuerySpan span(k.row0, min(k.row0 + kRowsM, a.kv_len) - 1, a.window, a.sinks, past, len);
+    if (span.hi >= span.lo) {
+      k.q_hi = span.hi;
+      k.i_lo = (span.lo - past) & ~7;                        // (the denominators are read in vectors)
+      k.nq = (span.hi - past - k.i_lo) / S::BN + 1;
+      const int all = k.nq * group;
+      const int first = (int)((int64_t)all * split / splits);
+      k.steps = (int)((int64_t)all * (split + 1) / splits) - first;
+      k.hq0 = first / k.nq; k.q0 = first - k.hq0 * k.nq;
     }
   }
-  // step s: stream rows [r, r + n) of head `head` (of the stream's operands)
-  __device__ __forceinline__ void step(const TcArgs& t, int s, int& head, int& r, int& n) const {
-    using S = Shape<MODE, DP>;
-    if (!S::KEYS) {
-      head = b * t.a.kv_heads + hk;
-      if (s < sink_steps) { r = s * S::BN; n = min(S::BN, sink_n - r); }
-      else { r = lowest + (s - sink_steps) * S::BN; n = min(S::BN, p_hi + 1 - r); }
+  k.skip = some_left && !lnn::group_ok(a, k.b, k.hk);
+  const int qh = k.b * a.q_heads + k.h;
+  const HeadInfo ik = lnn::info_of(a, 1, k.b * a.kv_heads + k.hk), iv = lnn::info_of(a, 2, k.b * a.kv_heads + k.hk);
+  k.ek = ik.e; k.ev = iv.e; k.norm_v = iv.norm;
+  k.eq = lnn::info_of(a, 0, qh).e;
+  if (MODE != FWD) {
+    const HeadInfo io = lnn::info_of(a, 3, qh);
+    k.eo = io.e; k.norm_do = io.norm;
+  }
+}
+
+// The steps of a work one after another: rows [r, r + n) of head `head` of the stream.
+template <int MODE, int DP>
+struct Steps {
+  int head, r, n, s, q;
+  __device__ __forceinline__ Steps(const TcArgs& t, const Work& k) : s(0) {
+    if (!Shape<MODE, DP>::KEYS) { head = k.b * t.a.kv_heads + k.hk; q = 0; }
+    else { head = k.b * t.a.q_heads + k.h + k.hq0; q = k.q0; }
+    at(t, k);
+  }
+  __device__ __forceinline__ void at(const TcArgs& t, const Work& k) {
+    constexpr int BN = Shape<MODE, DP>::BN;
+    if (!Shape<MODE, DP>::KEYS) {
+      if (s < k.sink_steps) { r = s * BN; n = min(BN, k.sink_n - r); }
+      else { r = k.lowest + (s - k.sink_steps) * BN; n = min(BN, k.p_hi + 1 - r); }
     } else {
-      const int at = first + s, hq = at / nq;
-      head = b * t.a.q_heads + h + hq;
-      r = i_lo + (at - hq * nq) * S::BN;
-      n = min(S::BN, q_hi - (t.a.kv_len - t.a.q_len) + 1 - r);
+      r = k.i_lo + q * BN;
+      n = min(BN, k.q_hi - (t.a.kv_len - t.a.q_len) + 1 - r);
     }
+  }
+  __device__ __forceinline__ void next(const TcArgs& t, const Work& k) {
+    ++s;
+    if (Shape<MODE, DP>::KEYS && ++q == k.nq) { q = 0; ++head; }
+    at(t, k);
   }
 };
 
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+// One lane of a converged warp.  The warps that load and issue run as whole warps with this lane doing the asynchronous
+// instructions: addresses and descriptors then live in uniform registers (with a single running thread every MMA waited
+// for its descriptors to be moved there, 100 to 140 clocks an instruction).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// Descriptors as two words: the upper one is the same for all tiles of a layout.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t accum) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accum)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(accum)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(accum)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
@@ -332,24 +376,30 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, role, step));
 }
 
-// 32 weights as fp16, two to a column: 16 columns of hi, 16 of lo
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+// 16 weights as fp16, two to a column: 8 columns of hi, 8 of lo
 __device__ __forceinline__ void store_split(uint32_t at, const float* w) {
-  uint32_t hi[16], lo[16];
+  uint32_t x[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < 8; ++i) {
     const __half2 h = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
     const float2 f = __half22float2(h);
     const __half2 l = __floats2half2_rn(__fsub_rn(w[2 * i], f.x), __fsub_rn(w[2 * i + 1], f.y));
-    hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-    lo[i] = *reinterpret_cast<const uint32_t*>(&l);
+    x[i] = *reinterpret_cast<const uint32_t*>(&h);
+    x[8 + i] = *reinterpret_cast<const uint32_t*>(&l);
   }
-  tmem_st16(at, hi);
-  tmem_st16(at + 16, lo);
+  tmem_st16(at, x);
 }
-
-__device__ __forceinline__ uint32_t idesc_f16(int n, int b_major) {
-  return (1u << 4) | ((uint32_t)b_major << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
-}
+// bits 0 .. n of a word
+__device__ __forceinline__ uint32_t bits_to(int n) { return n < 0 ? 0u : (n >= 31 ? 0xffffffffu : (2u << n) - 1u); }
 
 template <int MODE, int DP>
 __global__ void __launch_bounds__(kAttnThreads, 1)
@@ -360,10 +410,13 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
   constexpr int BN = S::BN, NY = S::NY, NZ = S::NZ, NS = S::NS;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bar_x_full, bar_x_empty, bar_y_full[NY], bar_y_empty[NY], bar_z_full[NZ], bar_z_empty[NZ];
-  __shared__ uint64_t bar_s_full[NS], bar_p_full[NS], bar_o_full, bar_o_empty, bar_pair[4];
+  __shared__ uint64_t bar_s_full[NS], bar_p_full[NS], bar_o_full, bar_o_empty, bar_row[4];
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag_smem;
   __shared__ float exchange[3][kComputeWarps][32];
+  constexpr int NW = 4;                                          // works handed over
+  __shared__ uint64_t bar_w_full[NW], bar_w_empty[NW];
+  __shared__ Work works[NW];
 
   // an earlier kernel gave up: leave as a whole CTA (the decision must be uniform)
   if (threadIdx.x == 0) abort_flag_smem = (*(volatile int*)t.a.status == LNN_E_TIMEOUT) ? 2 : 0;
@@ -382,7 +435,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
     for (int i = 0; i < NY; ++i) { mbar_init(smem_u32(&bar_y_full[i]), 1); mbar_init(smem_u32(&bar_y_empty[i]), 1); }
     for (int i = 0; i < NZ; ++i) { mbar_init(smem_u32(&bar_z_full[i]), 1); mbar_init(smem_u32(&bar_z_empty[i]), 1); }
     for (int i = 0; i < NS; ++i) { mbar_init(smem_u32(&bar_s_full[i]), 1); mbar_init(smem_u32(&bar_p_full[i]), kComputeWarps); }
-    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&bar_pair[i]), 2);
+    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&bar_row[i]), kParts);
+    for (int i = 0; i < NW; ++i) { mbar_init(smem_u32(&bar_w_full[i]), 1); mbar_init(smem_u32(&bar_w_empty[i]), 1 + kComputeWarps); }
     mbar_init(smem_u32(&bar_o_full), 1);
     mbar_init(smem_u32(&bar_o_empty), kComputeWarps);
     fence_barrier_init();
@@ -394,276 +448,298 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_base_smem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base_smem, 0);
+  const bool some_left = lnn::any_group_left(t.a);               // work for the FP32 pipe
 
   if (warp == 0) {
     // ---- loads ------------------------------------------------------------------------------------
-    if (lane == 0) {
-      const int x_part = (S::KEYS ? t.a.batch * t.a.kv_heads : t.a.batch * t.a.q_heads);     // heads in front of lo
-      const int y_part = (S::KEYS ? t.a.batch * t.a.q_heads : t.a.batch * t.a.kv_heads);
-      const auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar, int part_bytes, int slab_bytes, int head,
-                            int parts, int row, int boxes) {
-        for (int p = 0; p < 2; ++p)
-          for (int s = 0; s < S::SLABS; ++s)
-            for (int i = 0; i < boxes; ++i)
-              tma_load_3d(dst + p * part_bytes + s * slab_bytes + i * (kBoxRows * 128), map, bar, s * 64, row + i * kBoxRows,
-                          head + p * parts);
-      };
-      bool ok = true;
-      int g = 0, nw = 0;
-      // what goes with a step's weights in FWD and DV is loaded one step behind the rows of its scores: the order of use
-      struct Pending { int head, r, boxes, g; bool any; } late = {0, 0, 0, 0, false};
-      const auto load_z = [&](const Pending& z) {
-        const int slot = z.g % NZ;
-        if (!mbar_wait(smem_u32(&bar_z_empty[slot]), ((z.g / NZ) & 1) ^ 1, abort_flag, status, 10, z.g)) return false;
+    const int x_part = (S::KEYS ? t.a.batch * t.a.kv_heads : t.a.batch * t.a.q_heads);     // heads in front of lo
+    const int y_part = (S::KEYS ? t.a.batch * t.a.q_heads : t.a.batch * t.a.kv_heads);
+    const auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar, uint32_t part_bytes, uint32_t slab_bytes, int head,
+                          int parts, int row, int boxes) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int s = 0; s < S::SLABS; ++s)
+          for (int i = 0; i < boxes; ++i)
+            tma_load_3d(dst + p * part_bytes + s * slab_bytes + i * (kBoxRows * 128), map, bar, s * 64, row + i * kBoxRows,
+                        head + p * parts);
+    };
+    bool ok = true;
+    int g = 0, nw = 0, nr = 0;
+    // what goes with a step's weights in FWD and DV is loaded one step behind the rows of its scores: the order of use
+    struct Pending { int head, r, boxes, g; bool any; } late = {0, 0, 0, 0, false};
+    const auto load_z = [&](const Pending& z) {
+      const int slot = z.g % NZ;
+      if (!warp_wait(smem_u32(&bar_z_empty[slot]), ((z.g / NZ) & 1) ^ 1, abort_flag, status, 10, z.g)) return false;
+      if (elect_one()) {
         const uint32_t bar = smem_u32(&bar_z_full[slot]);
         mbar_expect_tx(bar, (uint32_t)(2 * S::SLABS * z.boxes * kBoxRows * 128));
         load(&mapZ, sZ + slot * S::Y_BYTES, bar, S::Y_PART, BN * 128, z.head, y_part, z.r, z.boxes);
-        return true;
-      };
-      for (int w = blockIdx.x; ok && w < t.works; w += gridDim.x) {
-        const Work<MODE, DP> k(t, w);
-        if (k.steps == 0 || !lnn::group_ok(t.a, k.b, k.hk)) continue;
-        if (!mbar_wait(smem_u32(&bar_x_empty), (nw & 1) ^ 1, abort_flag, status, 11, w)) { ok = false; break; }
+      }
+      __syncwarp();
+      return true;
+    };
+    for (int w = blockIdx.x; ok && w < t.works; w += gridDim.x, ++nr) {
+      Work k = {};
+      make_work<MODE, DP>(k, t, w, some_left);
+      if (!warp_wait(smem_u32(&bar_w_empty[nr % NW]), ((nr / NW) & 1) ^ 1, abort_flag, status, 13, w)) { ok = false; break; }
+      if (lane == 0) {
+        works[nr % NW] = k;
+        mbar_arrive(smem_u32(&bar_w_full[nr % NW]));
+      }
+      __syncwarp();
+      if (k.steps == 0 || k.skip) continue;
+      if (!warp_wait(smem_u32(&bar_x_empty), (nw & 1) ^ 1, abort_flag, status, 11, w)) { ok = false; break; }
+      if (elect_one()) {
         const int xh = S::KEYS ? k.b * t.a.kv_heads + k.hk : k.b * t.a.q_heads + k.h;
         const uint32_t bx = smem_u32(&bar_x_full);
         mbar_expect_tx(bx, (S::TWO ? 2u : 1u) * S::X_BYTES);
         load(&mapX, sX, bx, S::X_PART, kRowsM * 128, xh, x_part, k.row0, kRowsM / kBoxRows);
         if (S::TWO) load(&mapX2, sX2, bx, S::X_PART, kRowsM * 128, xh, x_part, k.row0, kRowsM / kBoxRows);
-        for (int s = 0; s < k.steps; ++s, ++g) {
-          Pending z;
-          int n;
-          k.step(t, s, z.head, z.r, n);
-          z.boxes = (n + kBoxRows - 1) / kBoxRows;
-          z.g = g;
-          z.any = true;
-          const int slot = g % NY;
-          if (!mbar_wait(smem_u32(&bar_y_empty[slot]), ((g / NY) & 1) ^ 1, abort_flag, status, 12, g)) { ok = false; break; }
+      }
+      __syncwarp();
+      Steps<MODE, DP> step(t, k);
+      for (int s = 0; s < k.steps; ++s, ++g) {
+        const Pending z = {step.head, step.r, (step.n + kBoxRows - 1) / kBoxRows, g, true};
+        const int slot = g % NY;
+        if (!warp_wait(smem_u32(&bar_y_empty[slot]), ((g / NY) & 1) ^ 1, abort_flag, status, 12, g)) { ok = false; break; }
+        if (elect_one()) {
           const uint32_t bar = smem_u32(&bar_y_full[slot]);
           mbar_expect_tx(bar, (uint32_t)(2 * S::SLABS * z.boxes * kBoxRows * 128));
           load(&mapY, sY + slot * S::Y_BYTES, bar, S::Y_PART, BN * 128, z.head, y_part, z.r, z.boxes);
-          if (S::TWO) {
-            if (!load_z(z)) { ok = false; break; }
-          } else {
-            if (late.any && !load_z(late)) { ok = false; break; }
-            late = z;
-          }
         }
-        ++nw;
+        __syncwarp();
+        if (S::TWO) {
+          if (!load_z(z)) { ok = false; break; }
+        } else {
+          if (late.any && !load_z(late)) { ok = false; break; }
+          late = z;
+        }
+        step.next(t, k);
       }
-      if (ok && !S::TWO && late.any) load_z(late);
+      ++nw;
     }
+    if (ok && !S::TWO && late.any) load_z(late);
   } else if (warp == 1) {
     // ---- MMAs -------------------------------------------------------------------------------------
-    if (lane == 0) {
-      // K-major tiles of 128-byte rows (128-byte swizzle); the same bytes are an MN-major operand when the rows are K:
-      // 64 values of MN to a row, slabs of 64 BN rows apart
-      const uint64_t dk0 = make_smem_desc(0u, 16u, 1024u, 2u);
-      const uint64_t dm0 = make_smem_desc(0u, BN * 128u, 1024u, 2u);
-      const auto scores = [&](uint32_t d, uint32_t ax, uint32_t by, int n16) {
-        const uint32_t id = idesc_f16(n16, 0);
-        uint32_t accum = 0;
+    // K-major tiles of 128-byte rows (128-byte swizzle); the same bytes are an MN-major operand when the rows are K:
+    // 64 values of MN to a row, slabs of 64 BN rows apart.  Lower words: address and the leading offset, in 16 bytes.
+    constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+    constexpr uint32_t K_LO = 1u << 16, MN_LO = (BN * 128u >> 4) << 16;
+    const auto scores = [&](uint32_t d, uint32_t ax, uint32_t by, uint32_t id) {
+      const uint32_t a = K_LO + (ax >> 4), b = K_LO + (by >> 4);
 #pragma unroll
-        for (int pr = 0; pr < 3; ++pr) {                          // lo hi, hi lo, hi hi
-          const uint64_t a0 = dk0 + ((ax + (pr == 0 ? S::X_PART : 0u)) >> 4), b0 = dk0 + ((by + (pr == 1 ? S::Y_PART : 0u)) >> 4);
+      for (int pr = 0; pr < 3; ++pr)                            // lo hi, hi lo, hi hi
 #pragma unroll
-          for (int ks = 0; ks < DP / 16; ++ks) {
-            umma_f16(d, a0 + (ks / 4) * (kRowsM * 128 / 16) + (ks % 4) * 2, b0 + (ks / 4) * (BN * 128 / 16) + (ks % 4) * 2, id, accum);
-            accum = 1;
-          }
-        }
-      };
-      const auto weighted = [&](uint32_t d, uint32_t p, uint32_t bz, int n16) {
-        const uint32_t id = idesc_f16(DP, 1);
-        uint32_t accum = 0;
-        for (int pr = 0; pr < 3; ++pr) {
-          const uint64_t b0 = dm0 + ((bz + (pr == 1 ? S::Y_PART : 0u)) >> 4);
-          const uint32_t a0 = p + (pr == 0 ? 16 : 0);             // 32 scores became 16 columns of hi and 16 of lo
-          for (int ks = 0; ks < n16 / 16; ++ks) {
-            umma_f16_ts(d, a0 + (ks / 2) * 32 + (ks % 2) * 8, b0 + ks * (16 * 128 / 16), id, accum);
-            accum = 1;
-          }
-        }
-      };
-      bool ok = true;
-      int g = 0, nw = 0;
-      struct Pending { int g, n16; bool any; } late = {0, 0, false};
-      const auto out = [&](const Pending& q) {
-        if (!mbar_wait(smem_u32(&bar_p_full[q.g % NS]), (q.g / NS) & 1, abort_flag, status, 20, q.g)) return false;
-        if (!mbar_wait(smem_u32(&bar_o_empty), (q.g & 1) ^ 1, abort_flag, status, 21, q.g)) return false;
-        uint32_t bz = sY + (q.g % NY) * S::Y_BYTES;
-        if (!S::TWO) {
-          if (!mbar_wait(smem_u32(&bar_z_full[q.g % NZ]), (q.g / NZ) & 1, abort_flag, status, 22, q.g)) return false;
-          bz = sZ + (q.g % NZ) * S::Y_BYTES;
-        }
-        tc_fence_after();
+        for (int ks = 0; ks < DP / 16; ++ks)
+          mma_ss(d, a + (pr == 0 ? S::X_PART / 16 : 0) + (ks / 4) * (kRowsM * 128 / 16) + (ks % 4) * 2,
+                 b + (pr == 1 ? S::Y_PART / 16 : 0) + (ks / 4) * (BN * 128 / 16) + (ks % 4) * 2, DESC_HI, id, pr + ks > 0);
+    };
+    const auto weighted = [&](uint32_t d, uint32_t p, uint32_t bz, int n16) {      // 16 scores became 8 columns of hi and 8 of lo
+      constexpr uint32_t id = (1u << 4) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((128u >> 4) << 24);
+      const uint32_t b = MN_LO + (bz >> 4);
+      if (n16 == BN) {
+#pragma unroll
+        for (int pr = 0; pr < 3; ++pr)
+#pragma unroll
+          for (int ks = 0; ks < BN / 16; ++ks)
+            mma_ts(d, p + (pr == 0 ? 8 : 0) + ks * 16, b + (pr == 1 ? S::Y_PART / 16 : 0) + ks * (16 * 128 / 16), DESC_HI, id, pr + ks > 0);
+      } else {
+        for (int pr = 0; pr < 3; ++pr)
+          for (int ks = 0; ks < n16 / 16; ++ks)
+            mma_ts(d, p + (pr == 0 ? 8 : 0) + ks * 16, b + (pr == 1 ? S::Y_PART / 16 : 0) + ks * (16 * 128 / 16), DESC_HI, id, pr + ks > 0);
+      }
+    };
+    bool ok = true;
+    int g = 0, nw = 0, nr = 0;
+    struct Pending { int g, n16; bool any; } late = {0, 0, false};
+    const auto out = [&](const Pending& q) {
+      if (!warp_wait(smem_u32(&bar_p_full[q.g % NS]), (q.g / NS) & 1, abort_flag, status, 20, q.g)) return false;
+      if (!warp_wait(smem_u32(&bar_o_empty), (q.g & 1) ^ 1, abort_flag, status, 21, q.g)) return false;
+      uint32_t bz = sY + (q.g % NY) * S::Y_BYTES;
+      if (!S::TWO) {
+        if (!warp_wait(smem_u32(&bar_z_full[q.g % NZ]), (q.g / NZ) & 1, abort_flag, status, 22, q.g)) return false;
+        bz = sZ + (q.g % NZ) * S::Y_BYTES;
+      }
+      tc_fence_after();
+      if (elect_one()) {
         weighted(tmem + S::T_OUT, tmem + (q.g % NS) * BN, bz, q.n16);
         umma_commit(smem_u32(&bar_o_full));
         umma_commit(S::TWO ? smem_u32(&bar_y_empty[q.g % NY]) : smem_u32(&bar_z_empty[q.g % NZ]));
-        return true;
-      };
-      for (int w = blockIdx.x; ok && w < t.works; w += gridDim.x) {
-        const Work<MODE, DP> k(t, w);
-        if (k.steps == 0 || !lnn::group_ok(t.a, k.b, k.hk)) continue;
-        if (!mbar_wait(smem_u32(&bar_x_full), nw & 1, abort_flag, status, 23, w)) { ok = false; break; }
-        for (int s = 0; s < k.steps; ++s, ++g) {
-          int head, r, n;
-          k.step(t, s, head, r, n);
-          const int n16 = (n + 15) & ~15;
-          if (!mbar_wait(smem_u32(&bar_y_full[g % NY]), (g / NY) & 1, abort_flag, status, 24, g)) { ok = false; break; }
-          // The scores of step g - NS were in this buffer, and its weights behind them.  FWD, DV: OUT(g - 2) waited for
-          // the drain of OUT(g - 3).  DQ, DK: OUT(g - 2) has to be over, in front of dP(g - 1) in the stream.
-          if (S::TWO && g >= 2 && !mbar_wait(smem_u32(&bar_o_full), g & 1, abort_flag, status, 25, g)) { ok = false; break; }
-          tc_fence_after();
-          scores(tmem + (g % NS) * BN, sX, sY + (g % NY) * S::Y_BYTES, n16);
+      }
+      __syncwarp();
+      return true;
+    };
+    for (int w = blockIdx.x; ok && w < t.works; w += gridDim.x, ++nr) {
+      if (!warp_wait(smem_u32(&bar_w_full[nr % NW]), (nr / NW) & 1, abort_flag, status, 27, w)) { ok = false; break; }
+      const Work k = works[nr % NW];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_w_empty[nr % NW]));
+      if (k.steps == 0 || k.skip) continue;
+      if (!warp_wait(smem_u32(&bar_x_full), nw & 1, abort_flag, status, 23, w)) { ok = false; break; }
+      Steps<MODE, DP> step(t, k);
+      for (int s = 0; s < k.steps; ++s, ++g) {
+        const int n16 = (step.n + 15) & ~15;
+        const uint32_t id = (1u << 4) | ((uint32_t)(n16 >> 3) << 17) | ((128u >> 4) << 24);
+        if (!warp_wait(smem_u32(&bar_y_full[g % NY]), (g / NY) & 1, abort_flag, status, 24, g)) { ok = false; break; }
+        // The scores of step g - NS were in this buffer, and its weights behind them.  FWD, DV: OUT(g - 2) waited for
+        // the drain of OUT(g - 3).  DQ, DK: OUT(g - 2) has to be over, in front of dP(g - 1) in the stream.
+        if (S::TWO && g >= 2 && !warp_wait(smem_u32(&bar_o_full), g & 1, abort_flag, status, 25, g)) { ok = false; break; }
+        tc_fence_after();
+        if (elect_one()) {
+          scores(tmem + (g % NS) * BN, sX, sY + (g % NY) * S::Y_BYTES, id);
           if (!S::TWO) {
             umma_commit(smem_u32(&bar_s_full[g % NS]));
             umma_commit(smem_u32(&bar_y_empty[g % NY]));
             if (s == k.steps - 1) umma_commit(smem_u32(&bar_x_empty));
           }
-          if (late.any && !out(late)) { ok = false; break; }
-          late = {g, n16, true};
-          if (S::TWO) {
-            // (its buffer: the weights of step g - 1 are complete, OUT(g - 1) waited for them)
-            if (!mbar_wait(smem_u32(&bar_z_full[g % NZ]), (g / NZ) & 1, abort_flag, status, 26, g)) { ok = false; break; }
-            tc_fence_after();
-            scores(tmem + S::T_DP, sX2, sZ + (g % NZ) * S::Y_BYTES, n16);
+        }
+        __syncwarp();
+        if (late.any && !out(late)) { ok = false; break; }
+        late = {g, n16, true};
+        if (S::TWO) {
+          // (its buffer: the weights of step g - 1 are complete, OUT(g - 1) waited for them)
+          if (!warp_wait(smem_u32(&bar_z_full[g % NZ]), (g / NZ) & 1, abort_flag, status, 26, g)) { ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            scores(tmem + S::T_DP, sX2, sZ + (g % NZ) * S::Y_BYTES, id);
             umma_commit(smem_u32(&bar_s_full[g % NS]));
             umma_commit(smem_u32(&bar_z_empty[g % NZ]));
             if (s == k.steps - 1) umma_commit(smem_u32(&bar_x_empty));
           }
+          __syncwarp();
         }
-        ++nw;
+        step.next(t, k);
       }
-      if (ok && late.any) out(late);
+      ++nw;
     }
+    if (ok && late.any) out(late);
   } else {
     // ---- weights and sums -------------------------------------------------------------------------
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int quarter = warp & 3, part = (warp - 2) >> 2;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    constexpr int COLS = BN / 2, CHUNKS = COLS / 32, OUT = DP / 2;
+    constexpr int COLS = BN / kParts, OUT = DP / kParts;
     const AttnArgs& a = t.a;
     const int past = a.kv_len - a.q_len, row_in = quarter * 32 + lane;
     bool ok = true;
     int g = 0;
-    // the two warps of a quarter hold halves of the same rows: one value of each row to the other warp and back (a bounded
-    // wait, like all others: a warp that gives up must not leave its partner behind)
-    uint32_t pairs = 0;
-    const auto swapped = [&](float* buffer, float mine, float& other) {
-      buffer[(quarter + 4 * half) * 32 + lane] = mine;
+    // the warps of a quarter hold parts of the same rows: one value of each row from every warp to every other (a bounded
+    // wait, like all others: a warp that gives up must not leave its partners behind)
+    uint32_t shares = 0;
+    const auto share = [&](float (*buffer)[32], float mine, float (&all)[kParts]) {
+      buffer[quarter * kParts + part][lane] = mine;
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_pair[quarter]));
-      if (!warp_wait(smem_u32(&bar_pair[quarter]), pairs & 1u, abort_flag, status, 32, g)) return false;
-      ++pairs;
-      other = buffer[(quarter + 4 * (half ^ 1)) * 32 + lane];
+      if (lane == 0) mbar_arrive(smem_u32(&bar_row[quarter]));
+      if (!warp_wait(smem_u32(&bar_row[quarter]), shares & 1u, abort_flag, status, 32, g)) return false;
+      ++shares;
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) all[i] = buffer[quarter * kParts + i][lane];
       return true;
     };
-    for (int w = blockIdx.x; ok && w < t.works; w += gridDim.x) {
-      const Work<MODE, DP> k(t, w);
-      if (!lnn::group_ok(a, k.b, k.hk)) continue;
+    int nr = 0;
+    for (int w = blockIdx.x; ok && w < t.works; w += gridDim.x, ++nr) {
+      if (!warp_wait(smem_u32(&bar_w_full[nr % NW]), (nr / NW) & 1, abort_flag, status, 33, w)) { ok = false; break; }
+      const Work k = works[nr % NW];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_w_empty[nr % NW]));
+      if (k.skip) continue;
       const int row = k.row0 + row_in;
       const int xh = S::KEYS ? k.b * a.kv_heads + k.hk : k.b * a.q_heads + k.h;
-      const int kvh = k.b * a.kv_heads + k.hk;
       float acc[OUT];
 #pragma unroll
       for (int i = 0; i < OUT; ++i) acc[i] = 0.0f;
       float m = -CUDART_INF_F, l = 0.0f, keep_before = 1.0f;      // FWD
       float row_lse = CUDART_INF_F, row_delta = 0.0f;              // DQ
       int row_exp = 0;                                             // DQ, DK: dS is scaled by 2^row_exp
-      const int ek = lnn::info_of(a, 1, kvh).e, ev = lnn::info_of(a, 2, kvh).e;
       const int rows = S::KEYS ? a.kv_len : a.q_len;
-      float norm = 0.0f, other_norm = 0.0f;
+      float norm = 0.0f;
       if (S::TWO && row < rows) norm = __ldg(t.norms + (int64_t)xh * rows + row);
       if (MODE == DQ) {
         if (row < rows) {
           row_lse = __ldg(t.lse_p + (int64_t)xh * t.pitch + row);
           row_delta = __ldg(t.delta_p + (int64_t)xh * t.pitch + row);
         }
-        other_norm = lnn::info_of(a, 2, kvh).norm;
       }
       int cur_head = -1;
       float c = 0.0f, cdp = 0.0f, factor = 1.0f, factor_before = 1.0f;
       const auto drain = [&](int gd, float old_times, float tile_times) {
         if (!warp_wait(smem_u32(&bar_o_full), gd & 1, abort_flag, status, 30, gd)) return false;
         tc_fence_after();
+        uint32_t v[OUT];
 #pragma unroll
-        for (int q = 0; q < OUT / 32; ++q) {
-          uint32_t v[32];
-          tmem_ld32(tmem + lanes + S::T_OUT + half * OUT + q * 32, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (MODE == FWD) acc[q * 32 + i] = fmaf(acc[q * 32 + i], old_times, __uint_as_float(v[i]));
-            else acc[q * 32 + i] = fmaf(__uint_as_float(v[i]), tile_times, acc[q * 32 + i]);
-          }
-        }
+        for (int q = 0; q < OUT / 16; ++q) tmem_ld16(tmem + lanes + S::T_OUT + part * OUT + q * 16, v + q * 16);
+        tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_o_empty));
+#pragma unroll
+        for (int i = 0; i < OUT; ++i) {
+          if (MODE == FWD) acc[i] = fmaf(acc[i], old_times, __uint_as_float(v[i]));
+          else acc[i] = fmaf(__uint_as_float(v[i]), tile_times, acc[i]);
+        }
         return true;
       };
-      for (int s = 0; s < k.steps; ++s, ++g) {
-        int head, r0, n;
-        k.step(t, s, head, r0, n);
-        const int qh = S::KEYS ? head : xh;
+      Steps<MODE, DP> step(t, k);
+      for (int s = 0; s < k.steps; ++s, ++g, step.next(t, k)) {
+        const int r0 = step.r, n = step.n, qh = S::KEYS ? step.head : xh;
         if (qh != cur_head) {                                      // the scales that go with a query head
+          int eq = k.eq, eo = k.eo;
+          float norm_do = k.norm_do;
+          if (S::KEYS && (cur_head >= 0 || k.hq0 > 0)) {
+            const HeadInfo io = lnn::info_of(a, 3, qh);
+            eq = lnn::info_of(a, 0, qh).e; eo = io.e; norm_do = io.norm;
+          }
           cur_head = qh;
-          const int eq = lnn::info_of(a, 0, qh).e;
           // (2^-126 in place of 0: masked scores stay -inf)
-          c = fmaxf(__fmul_rn(__fmul_rn(fabsf(a.scale), lnn::kLog2e), pow2f_int(eq + ek)), 1.17549435e-38f);
-          if (MODE == DV) factor = pow2f_int(lnn::info_of(a, 3, qh).e - 14);
+          c = fmaxf(__fmul_rn(__fmul_rn(fabsf(a.scale), lnn::kLog2e), pow2f_int(eq + k.ek)), 1.17549435e-38f);
+          if (MODE == DV) factor = pow2f_int(eo - 14);
           if (S::TWO) {
-            const int eo = lnn::info_of(a, 3, qh).e;
-            cdp = pow2f_int(eo + ev);
-            if (MODE == DK) other_norm = lnn::info_of(a, 3, qh).norm;
+            cdp = pow2f_int(eo + k.ev);
             // |dP - delta| <= 2 |dO| |V|: below 2^15 after scaling
-            const float bound = fmaxf(2.0f * norm * other_norm, 0.0009765625f);
-            row_exp = 14 - ((int)(__float_as_uint(bound) >> 23) - 127) - (eo + ev);
+            const float bound = fmaxf(2.0f * norm * (MODE == DK ? norm_do : k.norm_v), 0.0009765625f);
+            row_exp = 14 - ((int)(__float_as_uint(bound) >> 23) - 127) - (eo + k.ev);
             if (MODE == DK) factor = pow2f_int(eq - row_exp);
           }
         }
-        // which columns of the tile this row sees: [lo, hi], or up to `always`
-        int lo, hi, always;
+        // which columns of the tile this row sees: [lo, hi], and those up to hi that are below `always`
+        const int col0 = part * COLS;
         bool all;
+        uint32_t seen = 0xffffffffu;
         if (!S::KEYS) {
           const int p = row + past;
-          lo = p - a.window + 1 - r0; hi = min(p - r0, n - 1); always = a.sinks - r0;
-          all = n == BN && r0 + BN - 1 <= k.row0 + past &&
-                (k.p_hi - r0 < a.window || r0 + BN <= a.sinks);
+          all = n == BN && r0 + BN - 1 <= k.row0 + past && (k.p_hi - r0 < a.window || r0 + BN <= a.sinks);
+          if (!all) seen = bits_to(min(p - r0, n - 1) - col0) & (~bits_to(p - a.window - r0 - col0) | bits_to(a.sinks - 1 - r0 - col0));
         } else {
-          const int last = row < a.sinks ? k.q_hi : (int)min((int64_t)row + a.window - 1, (int64_t)k.q_hi);
-          lo = row - past - r0; hi = min(last - past - r0, n - 1); always = 0;
           all = n == BN && r0 + past >= k.row0 + kRowsM - 1 &&
                 (r0 + past + BN - 1 < k.row0 + a.window || k.row0 + kRowsM <= a.sinks);
+          const int last = row < a.sinks ? k.q_hi : (int)min((int64_t)row + a.window - 1, (int64_t)k.q_hi);
+          if (!all) seen = bits_to(min(last - past - r0, n - 1) - col0) & ~bits_to(row - past - r0 - 1 - col0);
         }
         const int buf = g % NS;
-        const uint32_t ts = tmem + lanes + buf * BN + half * COLS;
-        const int col0 = half * COLS;
+        const uint32_t ts = tmem + lanes + buf * BN + col0;
         if (!warp_wait(smem_u32(&bar_s_full[buf]), (g / NS) & 1, abort_flag, status, 31, g)) { ok = false; break; }
         tc_fence_after();
+        uint32_t v[COLS];
+        if (col0 < n) {
+#pragma unroll
+          for (int q = 0; q < COLS / 16; ++q) tmem_ld16(ts + q * 16, v + q * 16);
+        }
         if (MODE == FWD) {
-          uint32_t v[COLS];
-          float sc[COLS];
           float top = -CUDART_INF_F;
           if (col0 < n) {
-#pragma unroll
-            for (int q = 0; q < CHUNKS; ++q) tmem_ld32(ts + q * 32, v + q * 32);
             tmem_ld_wait();
-            if (all) {
+            if (!all) {
 #pragma unroll
-              for (int i = 0; i < COLS; ++i) { sc[i] = __uint_as_float(v[i]); top = fmaxf(top, sc[i]); }
-            } else {
-#pragma unroll
-              for (int i = 0; i < COLS; ++i) {
-                const int col = col0 + i;
-                sc[i] = col <= hi && (col >= lo || col < always) ? __uint_as_float(v[i]) : -CUDART_INF_F;
-                top = fmaxf(top, sc[i]);
-              }
+              for (int i = 0; i < COLS; ++i)
+                if (!(seen >> i & 1u)) v[i] = 0xff800000u;
             }
+#pragma unroll
+            for (int i = 0; i < COLS; ++i) top = fmaxf(top, __uint_as_float(v[i]));
           }
-          float other;
-          if (!swapped(&exchange[g & 1][0][0], top, other)) { ok = false; break; }
-          top = fmaxf(top, other);
+          float tops[kParts];
+          if (!share(exchange[g & 1], top, tops)) { ok = false; break; }
+          top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
           const float now = fmaxf(m, __fmul_rn(top, c));
           const float at = now == -CUDART_INF_F ? 0.0f : now;
           const float keep = exp2_fast(__fsub_rn(m, at));
@@ -671,15 +747,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           float sum = 0.0f;
           if (col0 < n) {
 #pragma unroll
-            for (int q = 0; q < CHUNKS; ++q) {
-              float part = 0.0f;
+            for (int q = 0; q < COLS / 16; ++q) {
+              float wt[16];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                sc[q * 32 + i] = exp2_fast(fmaf(sc[q * 32 + i], c, shift));
-                part = __fadd_rn(part, sc[q * 32 + i]);
+              for (int i = 0; i < 16; ++i) {
+                wt[i] = exp2_fast(fmaf(__uint_as_float(v[q * 16 + i]), c, shift));
+                sum = __fadd_rn(sum, wt[i]);
               }
-              sum = __fadd_rn(sum, part);
-              store_split(ts + q * 32, sc + q * 32);
+              store_split(ts + q * 16, wt);
             }
           }
           tmem_st_wait();
@@ -692,33 +767,39 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           keep_before = keep;
         } else {
           if (col0 < n) {
+            uint32_t d[COLS];
+            if (S::TWO) {
 #pragma unroll
-            for (int q = 0; q < CHUNKS; ++q) {
-              uint32_t v[32], d[32];
-              float wt[32];
-              tmem_ld32(ts + q * 32, v);
-              if (S::TWO) tmem_ld32(tmem + lanes + S::T_DP + col0 + q * 32, d);
-              const float* cl = t.lse_p + (int64_t)qh * t.pitch + r0 + col0 + q * 32;
-              const float* cd = t.delta_p + (int64_t)qh * t.pitch + r0 + col0 + q * 32;
-              tmem_ld_wait();
+              for (int q = 0; q < COLS / 16; ++q) tmem_ld16(tmem + lanes + S::T_DP + col0 + q * 16, d + q * 16);
+            }
+            const float* cl = t.lse_p + (int64_t)qh * t.pitch + r0 + col0;
+            const float* cd = t.delta_p + (int64_t)qh * t.pitch + r0 + col0;
+            tmem_ld_wait();
+            if (!all) {
 #pragma unroll
-              for (int i0 = 0; i0 < 32; i0 += 4) {
+              for (int i = 0; i < COLS; ++i)
+                if (!(seen >> i & 1u)) v[i] = 0xff800000u;
+            }
+            const float exponent = S::TWO ? (float)row_exp : 14.0f;
+#pragma unroll
+            for (int q = 0; q < COLS / 16; ++q) {
+              float wt[16];
+#pragma unroll
+              for (int i0 = 0; i0 < 16; i0 += 4) {
                 float4 l4 = make_float4(row_lse, row_lse, row_lse, row_lse), d4 = make_float4(row_delta, row_delta, row_delta, row_delta);
                 if (S::KEYS) {
-                  l4 = __ldg(reinterpret_cast<const float4*>(cl + i0));
-                  if (S::TWO) d4 = __ldg(reinterpret_cast<const float4*>(cd + i0));
+                  l4 = __ldg(reinterpret_cast<const float4*>(cl + q * 16 + i0));
+                  if (S::TWO) d4 = __ldg(reinterpret_cast<const float4*>(cd + q * 16 + i0));
                 }
                 const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, ds[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                  const int i = i0 + u, col = col0 + q * 32 + i;
-                  const float up = (S::TWO ? (float)row_exp : 14.0f) - ls[u];
-                  float x = exp2_fast(fmaf(__uint_as_float(v[i]), c, up));
-                  if (S::TWO) x = __fmul_rn(x, fmaf(__uint_as_float(d[i]), cdp, -ds[u]));
-                  wt[i] = all || (col <= hi && (col >= lo || col < always)) ? x : 0.0f;
+                  const int i = q * 16 + i0 + u;
+                  wt[i0 + u] = exp2_fast(fmaf(__uint_as_float(v[i]), c, __fsub_rn(exponent, ls[u])));
+                  if (S::TWO) wt[i0 + u] = __fmul_rn(wt[i0 + u], fmaf(__uint_as_float(d[i]), cdp, -ds[u]));
                 }
               }
-              store_split(ts + q * 32, wt);
+              store_split(ts + q * 16, wt);
             }
           }
           tmem_st_wait();
@@ -740,13 +821,13 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       int pitch_cols = a.dim;
       if (MODE == FWD) {
         if (k.steps > 0) {
-          float other;
-          if (!swapped(&exchange[2][0][0], l, other)) { ok = false; break; }
-          l = __fadd_rn(l, other);
+          float ls[kParts];
+          if (!share(exchange[2], l, ls)) { ok = false; break; }
+          l = __fadd_rn(__fadd_rn(ls[0], ls[1]), __fadd_rn(ls[2], ls[3]));
         }
         const bool empty = k.steps == 0 || row + past > k.p_hi;
-        times = empty ? 0.0f : __fmul_rn(__fdiv_rn(1.0f, l), pow2f_int(ev));
-        if (half == 0 && row < rows)
+        times = empty ? 0.0f : __fmul_rn(__fdiv_rn(1.0f, l), pow2f_int(k.ev));
+        if (part == 0 && row < rows)
           a.lse[(int64_t)xh * rows + row] = empty ? CUDART_INF_F : __fadd_rn(m, __fsub_rn(log2f(l), 14.0f));
         if (empty) {
 #pragma unroll
@@ -754,41 +835,43 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
         }
         dst = a.o;
       } else if (MODE == DQ) {
-        times = __fmul_rn(a.scale, pow2f_int(ek - row_exp));
+        times = __fmul_rn(a.scale, pow2f_int(k.ek - row_exp));
         dst = a.dq; accumulate = a.acc_q;
       } else {
         if (MODE == DK) times = fabsf(a.scale);
         dst = MODE == DK ? a.dk : a.dv;
         accumulate = MODE == DK ? a.acc_k : a.acc_v;
-        if (k.splits > 1) {
+        if (k.split_up) {
           dst = t.parts; accumulate = 0; limit = k.row0 + kRowsM;
-          at = (k.part * kRowsM + row_in) * DP;
+          at = ((int64_t)k.part * kRowsM + row_in) * DP;
           pitch_cols = DP;
         }
       }
       if (row < limit) {
         float* to = dst + at;
-        const bool vec = pitch_cols % 4 == 0 && (((uintptr_t)dst) & 15) == 0;
+        const bool vec = pitch_cols % 8 == 0 && (((uintptr_t)dst) & 31) == 0;
 #pragma unroll
-        for (int i = 0; i < OUT; i += 4) {
-          const int col = half * OUT + i;
-          if (vec) {
-            if (col < pitch_cols) {
-              float4 x = make_float4(__fmul_rn(acc[i], times), __fmul_rn(acc[i + 1], times), __fmul_rn(acc[i + 2], times),
-                                     __fmul_rn(acc[i + 3], times));
-              if (accumulate) {
-                const float4 y = *reinterpret_cast<const float4*>(to + col);
-                x = make_float4(__fadd_rn(y.x, x.x), __fadd_rn(y.y, x.y), __fadd_rn(y.z, x.z), __fadd_rn(y.w, x.w));
-              }
-              *reinterpret_cast<float4*>(to + col) = x;
+        for (int i = 0; i < OUT; ++i) acc[i] = __fmul_rn(acc[i], times);
+        if (vec) {                                                 // whole 32-byte sectors
+#pragma unroll
+          for (int i = 0; i < OUT; i += 8) {
+            const int col = part * OUT + i;
+            if (col >= pitch_cols) break;
+            if (accumulate) {
+              const float4 y0 = *reinterpret_cast<const float4*>(to + col), y1 = *reinterpret_cast<const float4*>(to + col + 4);
+              const float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
+#pragma unroll
+              for (int u = 0; u < 8; ++u) acc[i + u] = __fadd_rn(y[u], acc[i + u]);
             }
-          } else {
+            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + col), "f"(acc[i]), "f"(acc[i + 1]),
+                         "f"(acc[i + 2]), "f"(acc[i + 3]), "f"(acc[i + 4]), "f"(acc[i + 5]), "f"(acc[i + 6]), "f"(acc[i + 7])
+                         : "memory");
+          }
+        } else {
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              if (col + u < pitch_cols) {
-                const float x = __fmul_rn(acc[i + u], times);
-                to[col + u] = accumulate ? __fadd_rn(to[col + u], x) : x;
-              }
+          for (int i = 0; i < OUT; ++i) {
+            const int col = part * OUT + i;
+            if (col < pitch_cols) to[col] = accumulate ? __fadd_rn(to[col], acc[i]) : acc[i];
           }
         }
       }
