@@ -213,6 +213,7 @@ struct TcArgs {
   const float* norms;            // DQ: of dO's rows, DK: of V's
   int pitch;
   int works;
+  const uint32_t* x2;            // DQ: dO, DK: V, split
   // DV, DK: keys below sinks take `splits_sink` works per tile of rows, the others `splits`
   int tiles, sink_tiles, splits_sink, splits;
   float* parts;                  // [part][128][DP] of the tiles that have several works
@@ -220,17 +221,18 @@ struct TcArgs {
 
 template <int MODE, int DP> struct Shape {
   static constexpr bool TWO = MODE == DQ || MODE == DK, KEYS = MODE == DV || MODE == DK;
-  static constexpr int BN = TWO && DP == 128 ? 64 : 128;
+  static constexpr int BN = TWO ? 64 : 128;
   static constexpr int SLABS = DP / 64;                          // 64 values (128 bytes) wide
   static constexpr uint32_t X_PART = kRowsM * DP * 2, X_BYTES = 2 * X_PART;
   static constexpr uint32_t Y_PART = BN * DP * 2, Y_BYTES = 2 * Y_PART;
   // ring depths: see the order of the MMAs
-  static constexpr int NY = TWO ? 2 : (DP == 128 ? 1 : 2), NZ = TWO ? 1 : (DP == 128 ? 1 : 2);
-  static constexpr int NS = TWO ? 2 : 3;                         // score buffers
-  static constexpr uint32_t SMEM = (TWO ? 2 : 1) * X_BYTES + (NY + NZ) * Y_BYTES + 1024;
-  // TMEM columns
-  static constexpr uint32_t T_DP = NS * BN, T_OUT = T_DP + (TWO ? BN : 0);
-  static_assert(T_OUT + DP <= 512, "TMEM");
+  static constexpr int NY = TWO ? 3 : (DP == 128 ? 1 : 2), NZ = TWO ? 2 : (DP == 128 ? 1 : 2);
+  static constexpr int NS = TWO ? 2 : 3;                         // score buffers (and of dP)
+  static constexpr uint32_t SMEM = X_BYTES + (NY + NZ) * Y_BYTES + 1024;
+  // TMEM columns: DQ and DK keep their second stationary operand (dO, V) there, which leaves shared memory for a third
+  // stream tile and makes its products faster (33 instead of 50 clocks for 64 columns)
+  static constexpr uint32_t T_DP = NS * BN, T_OUT = T_DP + (TWO ? NS * BN : 0), T_X2 = T_OUT + DP;
+  static_assert(T_X2 + (TWO ? DP : 0) <= 512, "TMEM");
 };
 
 // Tiles with one work only write their results themselves: their places are behind the others' and are not there where
@@ -361,6 +363,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
       ::"r"(d), "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(accum)
       : "memory");
 }
+// `bytes` (a multiple of 16, as both addresses) of global memory into shared memory
+__device__ __forceinline__ void bulk_load(uint32_t dst, const float* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+               "r"(bar)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -368,6 +376,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
       ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
         "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -385,14 +398,40 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
       : "r"(taddr)
       : "memory");
 }
+// two fp32 values to an instruction
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // 16 weights as fp16, two to a column: 8 columns of hi, 8 of lo
-__device__ __forceinline__ void store_split(uint32_t at, const float* w) {
+__device__ __forceinline__ void store_split(uint32_t at, const uint64_t* w) {
   uint32_t x[16];
+  const uint64_t minus = pack2(-1.0f, -1.0f);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const __half2 h = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
+    float a, b;
+    unpack2(w[i], a, b);
+    const __half2 h = __floats2half2_rn(a, b);
     const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(__fsub_rn(w[2 * i], f.x), __fsub_rn(w[2 * i + 1], f.y));
+    unpack2(fma2(pack2(f.x, f.y), minus, w[i]), a, b);           // (exact)
+    const __half2 l = __floats2half2_rn(a, b);
     x[i] = *reinterpret_cast<const uint32_t*>(&h);
     x[8 + i] = *reinterpret_cast<const uint32_t*>(&l);
   }
@@ -403,20 +442,24 @@ __device__ __forceinline__ uint32_t bits_to(int n) { return n < 0 ? 0u : (n >= 3
 
 template <int MODE, int DP>
 __global__ void __launch_bounds__(kAttnThreads, 1)
-attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapX2,
-               const __grid_constant__ CUtensorMap mapY, const __grid_constant__ CUtensorMap mapZ,
-               const __grid_constant__ TcArgs t) {
+attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapY,
+               const __grid_constant__ CUtensorMap mapZ, const __grid_constant__ TcArgs t) {
   using S = Shape<MODE, DP>;
   constexpr int BN = S::BN, NY = S::NY, NZ = S::NZ, NS = S::NS;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bar_x_full, bar_x_empty, bar_y_full[NY], bar_y_empty[NY], bar_z_full[NZ], bar_z_empty[NZ];
-  __shared__ uint64_t bar_s_full[NS], bar_p_full[NS], bar_o_full, bar_o_empty, bar_row[4];
+  __shared__ uint64_t bar_s_full[NS], bar_p_full[NS], bar_o_full, bar_o_empty, bar_x2_full;
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag_smem;
   __shared__ float exchange[3][kComputeWarps][32];
-  constexpr int NW = 4;                                          // works handed over
+  constexpr int NW = 2;                                          // works handed over
   __shared__ uint64_t bar_w_full[NW], bar_w_empty[NW];
   __shared__ Work works[NW];
+  // What goes with the columns of a pass over keys, loaded with the rows of their step.  A slot is free when its step's weights
+  // are complete: DK, when its Y slot is (OUT(g) is over); DV, when Y(g + 4) is loaded: S(g + 4 - NY) waited for them.
+  constexpr int NC = S::TWO ? NY : 4;
+  __shared__ uint64_t bar_c_full[NC];
+  __shared__ __align__(16) float col_lse[S::KEYS ? NC : 1][BN], col_delta[MODE == DK ? NC : 1][BN];
 
   // an earlier kernel gave up: leave as a whole CTA (the decision must be uniform)
   if (threadIdx.x == 0) abort_flag_smem = (*(volatile int*)t.a.status == LNN_E_TIMEOUT) ? 2 : 0;
@@ -427,7 +470,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
   volatile int* abort_flag = &abort_flag_smem;
   int* status = t.a.status;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t sX = base, sX2 = sX + S::X_BYTES, sY = sX2 + (S::TWO ? S::X_BYTES : 0u), sZ = sY + NY * S::Y_BYTES;
+  const uint32_t sX = base, sY = sX + S::X_BYTES, sZ = sY + NY * S::Y_BYTES;
 
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&bar_x_full), 1);
@@ -435,10 +478,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
     for (int i = 0; i < NY; ++i) { mbar_init(smem_u32(&bar_y_full[i]), 1); mbar_init(smem_u32(&bar_y_empty[i]), 1); }
     for (int i = 0; i < NZ; ++i) { mbar_init(smem_u32(&bar_z_full[i]), 1); mbar_init(smem_u32(&bar_z_empty[i]), 1); }
     for (int i = 0; i < NS; ++i) { mbar_init(smem_u32(&bar_s_full[i]), 1); mbar_init(smem_u32(&bar_p_full[i]), kComputeWarps); }
-    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&bar_row[i]), kParts);
     for (int i = 0; i < NW; ++i) { mbar_init(smem_u32(&bar_w_full[i]), 1); mbar_init(smem_u32(&bar_w_empty[i]), 1 + kComputeWarps); }
     mbar_init(smem_u32(&bar_o_full), 1);
     mbar_init(smem_u32(&bar_o_empty), kComputeWarps);
+    mbar_init(smem_u32(&bar_x2_full), kComputeWarps);
+    for (int i = 0; i < NC; ++i) mbar_init(smem_u32(&bar_c_full[i]), 1);
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -494,25 +538,30 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       if (elect_one()) {
         const int xh = S::KEYS ? k.b * t.a.kv_heads + k.hk : k.b * t.a.q_heads + k.h;
         const uint32_t bx = smem_u32(&bar_x_full);
-        mbar_expect_tx(bx, (S::TWO ? 2u : 1u) * S::X_BYTES);
+        mbar_expect_tx(bx, S::X_BYTES);
         load(&mapX, sX, bx, S::X_PART, kRowsM * 128, xh, x_part, k.row0, kRowsM / kBoxRows);
-        if (S::TWO) load(&mapX2, sX2, bx, S::X_PART, kRowsM * 128, xh, x_part, k.row0, kRowsM / kBoxRows);
       }
       __syncwarp();
       Steps<MODE, DP> step(t, k);
       for (int s = 0; s < k.steps; ++s, ++g) {
         const Pending z = {step.head, step.r, (step.n + kBoxRows - 1) / kBoxRows, g, true};
         const int slot = g % NY;
+        if (S::TWO && !load_z(z)) { ok = false; break; }
         if (!warp_wait(smem_u32(&bar_y_empty[slot]), ((g / NY) & 1) ^ 1, abort_flag, status, 12, g)) { ok = false; break; }
         if (elect_one()) {
           const uint32_t bar = smem_u32(&bar_y_full[slot]);
           mbar_expect_tx(bar, (uint32_t)(2 * S::SLABS * z.boxes * kBoxRows * 128));
           load(&mapY, sY + slot * S::Y_BYTES, bar, S::Y_PART, BN * 128, z.head, y_part, z.r, z.boxes);
+          if (S::KEYS) {
+            const int64_t at = (int64_t)z.head * t.pitch + z.r;
+            const uint32_t bc = smem_u32(&bar_c_full[g % NC]);
+            mbar_expect_tx(bc, (MODE == DK ? 2 : 1) * BN * 4);
+            bulk_load(smem_u32(&col_lse[g % NC][0]), t.lse_p + at, BN * 4, bc);
+            if (MODE == DK) bulk_load(smem_u32(&col_delta[g % NC][0]), t.delta_p + at, BN * 4, bc);
+          }
         }
         __syncwarp();
-        if (S::TWO) {
-          if (!load_z(z)) { ok = false; break; }
-        } else {
+        if (!S::TWO) {
           if (late.any && !load_z(late)) { ok = false; break; }
           late = z;
         }
@@ -535,6 +584,15 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
         for (int ks = 0; ks < DP / 16; ++ks)
           mma_ss(d, a + (pr == 0 ? S::X_PART / 16 : 0) + (ks / 4) * (kRowsM * 128 / 16) + (ks % 4) * 2,
                  b + (pr == 1 ? S::Y_PART / 16 : 0) + (ks / 4) * (BN * 128 / 16) + (ks % 4) * 2, DESC_HI, id, pr + ks > 0);
+    };
+    const auto second_scores = [&](uint32_t d, uint32_t by, uint32_t id) {      // dO or V from TMEM: DP / 2 columns of hi, then of lo
+      const uint32_t a = tmem + S::T_X2, b = K_LO + (by >> 4);
+#pragma unroll
+      for (int pr = 0; pr < 3; ++pr)
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks)
+          mma_ts(d, a + (pr == 0 ? DP / 2 : 0) + ks * 8, b + (pr == 1 ? S::Y_PART / 16 : 0) + (ks / 4) * (BN * 128 / 16) + (ks % 4) * 2,
+                 DESC_HI, id, pr + ks > 0);
     };
     const auto weighted = [&](uint32_t d, uint32_t p, uint32_t bz, int n16) {      // 16 scores became 8 columns of hi and 8 of lo
       constexpr uint32_t id = (1u << 4) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((128u >> 4) << 24);
@@ -582,34 +640,38 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       for (int s = 0; s < k.steps; ++s, ++g) {
         const int n16 = (step.n + 15) & ~15;
         const uint32_t id = (1u << 4) | ((uint32_t)(n16 >> 3) << 17) | ((128u >> 4) << 24);
+        const uint32_t at = tmem + (g % NS) * BN;
+        if (S::TWO) {
+          // dP(g), S(g), OUT(g - 1).  The last readers of these buffers: the weights of step g - 2 are complete
+          // (OUT(g - 2) waited for them), and OUT(g - 2) itself has to be over; dP(g) keeps the tensor cores busy meanwhile.
+          if (s == 0) {
+            // (whoever brings the second operand first finishes the work before: its last step cannot wait for this one)
+            if (late.any && !out(late)) { ok = false; break; }
+            late.any = false;
+            if (!warp_wait(smem_u32(&bar_x2_full), nw & 1, abort_flag, status, 28, w)) { ok = false; break; }
+          }
+          if (!warp_wait(smem_u32(&bar_z_full[g % NZ]), (g / NZ) & 1, abort_flag, status, 26, g)) { ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            second_scores(at + S::T_DP, sZ + (g % NZ) * S::Y_BYTES, id);
+            umma_commit(smem_u32(&bar_z_empty[g % NZ]));
+          }
+          __syncwarp();
+          // (a first step has nothing to wait for: the second operand came after the drain of OUT(g - 1))
+          if (s > 0 && g >= 2 && !warp_wait(smem_u32(&bar_o_full), g & 1, abort_flag, status, 25, g)) { ok = false; break; }
+        }
+        // FWD, DV: S(g), OUT(g - 1); the weights of step g - 3 were in this buffer, and OUT(g - 2) waited for the drain of OUT(g - 3)
         if (!warp_wait(smem_u32(&bar_y_full[g % NY]), (g / NY) & 1, abort_flag, status, 24, g)) { ok = false; break; }
-        // The scores of step g - NS were in this buffer, and its weights behind them.  FWD, DV: OUT(g - 2) waited for
-        // the drain of OUT(g - 3).  DQ, DK: OUT(g - 2) has to be over, in front of dP(g - 1) in the stream.
-        if (S::TWO && g >= 2 && !warp_wait(smem_u32(&bar_o_full), g & 1, abort_flag, status, 25, g)) { ok = false; break; }
         tc_fence_after();
         if (elect_one()) {
-          scores(tmem + (g % NS) * BN, sX, sY + (g % NY) * S::Y_BYTES, id);
-          if (!S::TWO) {
-            umma_commit(smem_u32(&bar_s_full[g % NS]));
-            umma_commit(smem_u32(&bar_y_empty[g % NY]));
-            if (s == k.steps - 1) umma_commit(smem_u32(&bar_x_empty));
-          }
+          scores(at, sX, sY + (g % NY) * S::Y_BYTES, id);
+          umma_commit(smem_u32(&bar_s_full[g % NS]));
+          if (!S::TWO) umma_commit(smem_u32(&bar_y_empty[g % NY]));
+          if (s == k.steps - 1) umma_commit(smem_u32(&bar_x_empty));
         }
         __syncwarp();
         if (late.any && !out(late)) { ok = false; break; }
         late = {g, n16, true};
-        if (S::TWO) {
-          // (its buffer: the weights of step g - 1 are complete, OUT(g - 1) waited for them)
-          if (!warp_wait(smem_u32(&bar_z_full[g % NZ]), (g / NZ) & 1, abort_flag, status, 26, g)) { ok = false; break; }
-          tc_fence_after();
-          if (elect_one()) {
-            scores(tmem + S::T_DP, sX2, sZ + (g % NZ) * S::Y_BYTES, id);
-            umma_commit(smem_u32(&bar_s_full[g % NS]));
-            umma_commit(smem_u32(&bar_z_empty[g % NZ]));
-            if (s == k.steps - 1) umma_commit(smem_u32(&bar_x_empty));
-          }
-          __syncwarp();
-        }
         step.next(t, k);
       }
       ++nw;
@@ -623,21 +685,20 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
     const AttnArgs& a = t.a;
     const int past = a.kv_len - a.q_len, row_in = quarter * 32 + lane;
     bool ok = true;
-    int g = 0;
-    // the warps of a quarter hold parts of the same rows: one value of each row from every warp to every other (a bounded
-    // wait, like all others: a warp that gives up must not leave its partners behind)
-    uint32_t shares = 0;
+    int g = 0, buf = 0;
+    uint32_t buf_phase = 0;
+    // The warps of a quarter hold parts of the same rows: one value of each row from every warp to every other.  The barrier
+    // itself has no limit, so a warp that gives up arrives once more on its way out (below), and those it lets go look
+    // whether somebody has given up.
     const auto share = [&](float (*buffer)[32], float mine, float (&all)[kParts]) {
       buffer[quarter * kParts + part][lane] = mine;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_row[quarter]));
-      if (!warp_wait(smem_u32(&bar_row[quarter]), shares & 1u, abort_flag, status, 32, g)) return false;
-      ++shares;
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + quarter), "n"(32 * kParts) : "memory");
+      if (__any_sync(0xffffffffu, *abort_flag)) return false;
 #pragma unroll
       for (int i = 0; i < kParts; ++i) all[i] = buffer[quarter * kParts + i][lane];
       return true;
     };
-    int nr = 0;
+    int nr = 0, nw = 0;
     for (int w = blockIdx.x; ok && w < t.works; w += gridDim.x, ++nr) {
       if (!warp_wait(smem_u32(&bar_w_full[nr % NW]), (nr / NW) & 1, abort_flag, status, 33, w)) { ok = false; break; }
       const Work k = works[nr % NW];
@@ -646,9 +707,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       if (k.skip) continue;
       const int row = k.row0 + row_in;
       const int xh = S::KEYS ? k.b * a.kv_heads + k.hk : k.b * a.q_heads + k.h;
-      float acc[OUT];
+      uint64_t sums[OUT / 2];
 #pragma unroll
-      for (int i = 0; i < OUT; ++i) acc[i] = 0.0f;
+      for (int i = 0; i < OUT / 2; ++i) sums[i] = 0;
       float m = -CUDART_INF_F, l = 0.0f, keep_before = 1.0f;      // FWD
       float row_lse = CUDART_INF_F, row_delta = 0.0f;              // DQ
       int row_exp = 0;                                             // DQ, DK: dS is scaled by 2^row_exp
@@ -661,9 +722,35 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           row_delta = __ldg(t.delta_p + (int64_t)xh * t.pitch + row);
         }
       }
+      if (S::TWO && k.steps > 0) {
+        // the second stationary operand into TMEM, once the products of the work before are over: this warp's fourth of
+        // the columns of its rows, hi and lo (what is no row of the tensor is zero)
+        if (!warp_wait(smem_u32(&bar_x_empty), (nw & 1) ^ 1, abort_flag, status, 34, w)) { ok = false; break; }
+        const int64_t lo_at = (int64_t)(S::KEYS ? a.batch * a.kv_heads : a.batch * a.q_heads) * rows * (DP / 2);
+        const uint32_t* src = t.x2 + ((int64_t)xh * rows + row) * (DP / 2) + part * (DP / 8);
+        tc_fence_after();
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          uint32_t x[DP / 8];
+#pragma unroll
+          for (int i = 0; i < DP / 8; i += 4) {
+            const uint4 v = row < rows ? __ldg(reinterpret_cast<const uint4*>(src + p * lo_at + i)) : make_uint4(0, 0, 0, 0);
+            x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+          }
+          const uint32_t to = tmem + lanes + S::T_X2 + p * (DP / 2) + part * (DP / 8);
+          if (DP == 128) tmem_st16(to, x);
+          else tmem_st8(to, x);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_x2_full));
+        ++nw;
+      }
       int cur_head = -1;
       float c = 0.0f, cdp = 0.0f, factor = 1.0f, factor_before = 1.0f;
-      const auto drain = [&](int gd, float old_times, float tile_times) {
+      // sums = sums * times + tile (FWD), or sums + tile * times
+      const auto drain = [&](int gd, float times) {
         if (!warp_wait(smem_u32(&bar_o_full), gd & 1, abort_flag, status, 30, gd)) return false;
         tc_fence_after();
         uint32_t v[OUT];
@@ -673,15 +760,16 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_o_empty));
+        const uint64_t t2 = pack2(times, times);
 #pragma unroll
-        for (int i = 0; i < OUT; ++i) {
-          if (MODE == FWD) acc[i] = fmaf(acc[i], old_times, __uint_as_float(v[i]));
-          else acc[i] = fmaf(__uint_as_float(v[i]), tile_times, acc[i]);
+        for (int i = 0; i < OUT / 2; ++i) {
+          const uint64_t x = pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+          sums[i] = MODE == FWD ? fma2(sums[i], t2, x) : fma2(x, t2, sums[i]);
         }
         return true;
       };
       Steps<MODE, DP> step(t, k);
-      for (int s = 0; s < k.steps; ++s, ++g, step.next(t, k)) {
+      for (int s = 0; s < k.steps; ++s, ++g, buf_phase ^= buf == NS - 1, buf = buf == NS - 1 ? 0 : buf + 1, step.next(t, k)) {
         const int r0 = step.r, n = step.n, qh = S::KEYS ? step.head : xh;
         if (qh != cur_head) {                                      // the scales that go with a query head
           int eq = k.eq, eo = k.eo;
@@ -716,26 +804,27 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           const int last = row < a.sinks ? k.q_hi : (int)min((int64_t)row + a.window - 1, (int64_t)k.q_hi);
           if (!all) seen = bits_to(min(last - past - r0, n - 1) - col0) & ~bits_to(row - past - r0 - 1 - col0);
         }
-        const int buf = g % NS;
         const uint32_t ts = tmem + lanes + buf * BN + col0;
-        if (!warp_wait(smem_u32(&bar_s_full[buf]), (g / NS) & 1, abort_flag, status, 31, g)) { ok = false; break; }
+        if (S::KEYS && !warp_wait(smem_u32(&bar_c_full[g % NC]), (g / NC) & 1, abort_flag, status, 35, g)) { ok = false; break; }
+        if (!warp_wait(smem_u32(&bar_s_full[buf]), buf_phase, abort_flag, status, 31, g)) { ok = false; break; }
         tc_fence_after();
-        uint32_t v[COLS];
-        if (col0 < n) {
-#pragma unroll
-          for (int q = 0; q < COLS / 16; ++q) tmem_ld16(ts + q * 16, v + q * 16);
-        }
         if (MODE == FWD) {
+          // (the scores are read twice, 16 at a time: registers)
           float top = -CUDART_INF_F;
           if (col0 < n) {
-            tmem_ld_wait();
-            if (!all) {
 #pragma unroll
-              for (int i = 0; i < COLS; ++i)
-                if (!(seen >> i & 1u)) v[i] = 0xff800000u;
+            for (int q = 0; q < COLS / 16; ++q) {
+              uint32_t v[16];
+              tmem_ld16(ts + q * 16, v);
+              tmem_ld_wait();
+              if (!all) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                  if (!(seen >> (q * 16 + i) & 1u)) v[i] = 0xff800000u;
+              }
+#pragma unroll
+              for (int i = 0; i < 16; ++i) top = fmaxf(top, __uint_as_float(v[i]));
             }
-#pragma unroll
-            for (int i = 0; i < COLS; ++i) top = fmaxf(top, __uint_as_float(v[i]));
           }
           float tops[kParts];
           if (!share(exchange[g & 1], top, tops)) { ok = false; break; }
@@ -743,16 +832,26 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           const float now = fmaxf(m, __fmul_rn(top, c));
           const float at = now == -CUDART_INF_F ? 0.0f : now;
           const float keep = exp2_fast(__fsub_rn(m, at));
-          const float shift = 14.0f - at;
-          float sum = 0.0f;
+          const uint64_t c2 = pack2(c, c), shift = pack2(14.0f - at, 14.0f - at);
+          uint64_t sum = 0;
           if (col0 < n) {
 #pragma unroll
             for (int q = 0; q < COLS / 16; ++q) {
-              float wt[16];
+              uint32_t v[16];
+              uint64_t wt[8];
+              tmem_ld16(ts + q * 16, v);
+              tmem_ld_wait();
+              if (!all) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                wt[i] = exp2_fast(fmaf(__uint_as_float(v[q * 16 + i]), c, shift));
-                sum = __fadd_rn(sum, wt[i]);
+                for (int i = 0; i < 16; ++i)
+                  if (!(seen >> (q * 16 + i) & 1u)) v[i] = 0xff800000u;
+              }
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                float x, y;
+                unpack2(fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), c2, shift), x, y);
+                wt[i] = pack2(exp2_fast(x), exp2_fast(y));
+                sum = add2(sum, wt[i]);
               }
               store_split(ts + q * 16, wt);
             }
@@ -761,43 +860,46 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&bar_p_full[buf]));
-          l = fmaf(l, keep, sum);
+          float s0, s1;
+          unpack2(sum, s0, s1);
+          l = fmaf(l, keep, __fadd_rn(s0, s1));
           m = now;
-          if (s > 0 && !drain(g - 1, keep_before, 1.0f)) { ok = false; break; }
+          if (s > 0 && !drain(g - 1, keep_before)) { ok = false; break; }
           keep_before = keep;
         } else {
           if (col0 < n) {
-            uint32_t d[COLS];
-            if (S::TWO) {
-#pragma unroll
-              for (int q = 0; q < COLS / 16; ++q) tmem_ld16(tmem + lanes + S::T_DP + col0 + q * 16, d + q * 16);
-            }
-            const float* cl = t.lse_p + (int64_t)qh * t.pitch + r0 + col0;
-            const float* cd = t.delta_p + (int64_t)qh * t.pitch + r0 + col0;
-            tmem_ld_wait();
-            if (!all) {
-#pragma unroll
-              for (int i = 0; i < COLS; ++i)
-                if (!(seen >> i & 1u)) v[i] = 0xff800000u;
-            }
             const float exponent = S::TWO ? (float)row_exp : 14.0f;
+            const uint64_t c2 = pack2(c, c), cdp2 = pack2(cdp, cdp), e2 = pack2(exponent, exponent), minus = pack2(-1.0f, -1.0f);
+            uint64_t up = pack2(exponent - row_lse, exponent - row_lse), less = pack2(-row_delta, -row_delta);
+            const float* cl = &col_lse[S::KEYS ? g % NC : 0][S::KEYS ? col0 : 0];
+            const float* cd = &col_delta[MODE == DK ? g % NC : 0][MODE == DK ? col0 : 0];
 #pragma unroll
             for (int q = 0; q < COLS / 16; ++q) {
-              float wt[16];
+              uint32_t v[16], d[16];
+              uint64_t wt[8];
+              tmem_ld16(ts + q * 16, v);
+              if (S::TWO) tmem_ld16(ts + S::T_DP + q * 16, d);
+              tmem_ld_wait();
+              if (!all) {
 #pragma unroll
-              for (int i0 = 0; i0 < 16; i0 += 4) {
-                float4 l4 = make_float4(row_lse, row_lse, row_lse, row_lse), d4 = make_float4(row_delta, row_delta, row_delta, row_delta);
-                if (S::KEYS) {
-                  l4 = __ldg(reinterpret_cast<const float4*>(cl + q * 16 + i0));
-                  if (S::TWO) d4 = __ldg(reinterpret_cast<const float4*>(cd + q * 16 + i0));
-                }
-                const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, ds[4] = {d4.x, d4.y, d4.z, d4.w};
+                for (int i = 0; i < 16; ++i)
+                  if (!(seen >> (q * 16 + i) & 1u)) v[i] = 0xff800000u;
+              }
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                  const int i = q * 16 + i0 + u;
-                  wt[i0 + u] = exp2_fast(fmaf(__uint_as_float(v[i]), c, __fsub_rn(exponent, ls[u])));
-                  if (S::TWO) wt[i0 + u] = __fmul_rn(wt[i0 + u], fmaf(__uint_as_float(d[i]), cdp, -ds[u]));
+              for (int i = 0; i < 8; ++i) {
+                if (S::KEYS) {                                     // (a warp reads one address)
+                  const float2 l2 = *reinterpret_cast<const float2*>(cl + q * 16 + 2 * i);
+                  up = fma2(pack2(l2.x, l2.y), minus, e2);
+                  if (S::TWO) {
+                    const float2 d2 = *reinterpret_cast<const float2*>(cd + q * 16 + 2 * i);
+                    less = pack2(-d2.x, -d2.y);
+                  }
                 }
+                float x, y;
+                unpack2(fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), c2, up), x, y);
+                wt[i] = pack2(exp2_fast(x), exp2_fast(y));
+                if (S::TWO)
+                  wt[i] = mul2(wt[i], fma2(pack2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), cdp2, less));
               }
               store_split(ts + q * 16, wt);
             }
@@ -806,12 +908,15 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&bar_p_full[buf]));
-          if (s > 0 && !drain(g - 1, 1.0f, factor_before)) { ok = false; break; }
+          if (s > 0 && !drain(g - 1, factor_before)) { ok = false; break; }
           factor_before = factor;
         }
       }
       if (!ok) break;
-      if (k.steps > 0 && !drain(g - 1, keep_before, factor_before)) { ok = false; break; }
+      if (k.steps > 0 && !drain(g - 1, MODE == FWD ? keep_before : factor_before)) { ok = false; break; }
+      float acc[OUT];
+#pragma unroll
+      for (int i = 0; i < OUT / 2; ++i) unpack2(sums[i], acc[2 * i], acc[2 * i + 1]);
 
       // ---- results ----
       float* dst;
@@ -876,6 +981,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
         }
       }
     }
+    if (!ok) asm volatile("bar.arrive %0, %1;" ::"r"(1 + quarter), "n"(32 * kParts) : "memory");
   }
 
   // ---- tear-down ------------------------------------------------------------------------------------
@@ -929,11 +1035,11 @@ int operand_map(CUtensorMap* tm, const void* base, int dp, int rows, int64_t hea
 }
 
 template <int MODE, int DP>
-int launch_pass(lnn::Device* d, const CUtensorMap* x, const CUtensorMap* x2, const CUtensorMap* y, const CUtensorMap* z, const TcArgs& t) {
+int launch_pass(lnn::Device* d, const CUtensorMap* x, const CUtensorMap* y, const CUtensorMap* z, const TcArgs& t) {
   using S = Shape<MODE, DP>;
   static_assert(S::SMEM + 2048 <= 227 * 1024, "shared memory");
   LNN_CUDA(cudaFuncSetAttribute(attn_tc_kernel<MODE, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
-  attn_tc_kernel<MODE, DP><<<std::min(t.works, d->sm_count), kAttnThreads, S::SMEM, d->stream>>>(*x, *x2, *y, *z, t);
+  attn_tc_kernel<MODE, DP><<<std::min(t.works, d->sm_count), kAttnThreads, S::SMEM, d->stream>>>(*x, *y, *z, t);
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
 }
@@ -1014,7 +1120,7 @@ int tc_fwd(lnn::Device* d, AttnArgs a) {
   t.a = a;
   t.tiles = (a.q_len + kRowsM - 1) / kRowsM;
   t.works = a.batch * a.q_heads * t.tiles;
-  rc = launch_pass<FWD, DP>(d, &op.map[0], &op.map[0], &op.map[1], &op.map[2], t);
+  rc = launch_pass<FWD, DP>(d, &op.map[0], &op.map[1], &op.map[2], t);
   return rc ? rc : lnn::attn_simt_fwd(d, a);                     // the heads that were marked
 }
 
@@ -1030,7 +1136,7 @@ int keys_pass(lnn::Device* d, TcArgs t, Operands& op, float* dst, int accumulate
     if (rc) return rc;
     t.parts = parts.as<float>();
   }
-  int rc = launch_pass<MODE, DP>(d, &op.map[1], &op.map[2], &op.map[0], &op.map[3], t);
+  int rc = launch_pass<MODE, DP>(d, &op.map[1], &op.map[0], &op.map[3], t);
   if (rc || !cut) return rc;
   attn_parts_kernel<DP><<<dim3((unsigned)t.tiles, (unsigned)t.a.kv_heads, (unsigned)t.a.batch), 256, 0, d->stream>>>(
       dst, t.parts, t, accumulate);
@@ -1049,9 +1155,10 @@ int tc_bwd(lnn::Device* d, AttnArgs a) {
   if (a.dq) {
     TcArgs q = t;
     q.norms = op.p.t[3].norms;
+    q.x2 = (const uint32_t*)op.p.t[3].hi;
     q.tiles = (a.q_len + kRowsM - 1) / kRowsM;
     q.works = a.batch * a.q_heads * q.tiles;
-    rc = launch_pass<DQ, DP>(d, &op.map[0], &op.map[3], &op.map[1], &op.map[2], q);
+    rc = launch_pass<DQ, DP>(d, &op.map[0], &op.map[1], &op.map[2], q);
     if (rc) return rc;
   }
   if (a.dv) {
@@ -1060,6 +1167,7 @@ int tc_bwd(lnn::Device* d, AttnArgs a) {
   }
   if (a.dk) {
     t.norms = op.p.t[2].norms;
+    t.x2 = (const uint32_t*)op.p.t[2].hi;
     rc = keys_pass<DK, DP>(d, t, op, a.dk, a.acc_k);
     if (rc) return rc;
   }

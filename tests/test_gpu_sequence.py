@@ -307,6 +307,9 @@ CASES = [
     (1, 2, 2, 520, 520, 64, 130, 130, None),
     (1, 1, 1, 700, 700, 17, 64, 3, (640,)),
     (2, 4, 2, 384, 384, 128, 128, 4, (384, 383)),
+    # more tiles of 128 rows than the device has SMs
+    (3, 16, 8, 500, 530, 24, 90, 2, (530, 77, 400)),
+    (2, 24, 12, 900, 900, 66, 300, 6, None),
 ]
 
 
