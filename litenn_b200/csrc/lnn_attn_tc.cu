@@ -228,6 +228,7 @@ template <int MODE, int DP> struct Shape {
   // ring depths: see the order of the MMAs
   static constexpr int NY = TWO ? 3 : (DP == 128 ? 1 : 2), NZ = TWO ? 2 : (DP == 128 ? 1 : 2);
   static constexpr int NS = TWO ? 2 : 3;                         // score buffers (and of dP)
+  static constexpr int NO = TWO ? NY : NZ;                       // steps that a completed result is told apart over
   static constexpr uint32_t SMEM = X_BYTES + (NY + NZ) * Y_BYTES + 1024;
   // TMEM columns: DQ and DK keep their second stationary operand (dO, V) there, which leaves shared memory for a third
   // stream tile and makes its products faster (33 instead of 50 clocks for 64 columns)
@@ -386,6 +387,7 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 
 // A whole warp's wait: all lanes go on or all give up (what follows is done by whole warps).
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int role, int step) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, role, step));
 }
 
@@ -445,10 +447,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapY,
                const __grid_constant__ CUtensorMap mapZ, const __grid_constant__ TcArgs t) {
   using S = Shape<MODE, DP>;
-  constexpr int BN = S::BN, NY = S::NY, NZ = S::NZ, NS = S::NS;
+  constexpr int BN = S::BN, NY = S::NY, NZ = S::NZ, NS = S::NS, NO = S::NO;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bar_x_full, bar_x_empty, bar_y_full[NY], bar_y_empty[NY], bar_z_full[NZ], bar_z_empty[NZ];
-  __shared__ uint64_t bar_s_full[NS], bar_p_full[NS], bar_o_full, bar_o_empty, bar_x2_full;
+  __shared__ uint64_t bar_x_full, bar_x_empty, bar_y_full[NY], bar_z_full[NZ];
+  __shared__ uint64_t bar_s_full[NS], bar_p_full[NS], bar_o_full[NO], bar_x2_full;
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag_smem;
   __shared__ float exchange[3][kComputeWarps][32];
@@ -475,12 +477,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&bar_x_full), 1);
     mbar_init(smem_u32(&bar_x_empty), 1);
-    for (int i = 0; i < NY; ++i) { mbar_init(smem_u32(&bar_y_full[i]), 1); mbar_init(smem_u32(&bar_y_empty[i]), 1); }
-    for (int i = 0; i < NZ; ++i) { mbar_init(smem_u32(&bar_z_full[i]), 1); mbar_init(smem_u32(&bar_z_empty[i]), 1); }
+    for (int i = 0; i < NY; ++i) mbar_init(smem_u32(&bar_y_full[i]), 1);
+    for (int i = 0; i < NZ; ++i) mbar_init(smem_u32(&bar_z_full[i]), 1);
     for (int i = 0; i < NS; ++i) { mbar_init(smem_u32(&bar_s_full[i]), 1); mbar_init(smem_u32(&bar_p_full[i]), kComputeWarps); }
     for (int i = 0; i < NW; ++i) { mbar_init(smem_u32(&bar_w_full[i]), 1); mbar_init(smem_u32(&bar_w_empty[i]), 1 + kComputeWarps); }
-    mbar_init(smem_u32(&bar_o_full), 1);
-    mbar_init(smem_u32(&bar_o_empty), kComputeWarps);
+    for (int i = 0; i < NO; ++i) mbar_init(smem_u32(&bar_o_full[i]), 1);
     mbar_init(smem_u32(&bar_x2_full), kComputeWarps);
     for (int i = 0; i < NC; ++i) mbar_init(smem_u32(&bar_c_full[i]), 1);
     fence_barrier_init();
@@ -511,14 +512,22 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
     };
     bool ok = true;
     int g = 0, nw = 0, nr = 0;
-    // what goes with a step's weights in FWD and DV is loaded one step behind the rows of its scores: the order of use
+    // What goes with a step's weights in FWD and DV is loaded one step behind the rows of its scores: the order of use.
+    // A slot is free when the products of the step that used it are over, which the barriers of their results tell (each
+    // batch of MMAs has one commit: a second one cost 50 clocks of a stream that has few to spare).
     struct Pending { int head, r, boxes, g; bool any; } late = {0, 0, 0, 0, false};
     const auto load_z = [&](const Pending& z) {
       const int slot = z.g % NZ;
-      if (!warp_wait(smem_u32(&bar_z_empty[slot]), ((z.g / NZ) & 1) ^ 1, abort_flag, status, 10, z.g)) return false;
+      // its last reader: OUT(g - NZ) (FWD, DV); dP(g - NZ), complete with S(g - NZ) (DQ, DK)
+      if (z.g >= NZ) {
+        const int before = z.g - NZ;
+        if (!warp_wait(S::TWO ? smem_u32(&bar_s_full[before % NS]) : smem_u32(&bar_o_full[before % NO]),
+                       (before / (S::TWO ? NS : NO)) & 1, abort_flag, status, 10, z.g)) return false;
+      }
       if (elect_one()) {
-        const uint32_t bar = smem_u32(&bar_z_full[slot]);
-        mbar_expect_tx(bar, (uint32_t)(2 * S::SLABS * z.boxes * kBoxRows * 128));
+        // DQ, DK: Y and Z of a step are waited for together
+        const uint32_t bar = S::TWO ? smem_u32(&bar_y_full[z.g % NY]) : smem_u32(&bar_z_full[slot]);
+        if (!S::TWO) mbar_expect_tx(bar, (uint32_t)(2 * S::SLABS * z.boxes * kBoxRows * 128));
         load(&mapZ, sZ + slot * S::Y_BYTES, bar, S::Y_PART, BN * 128, z.head, y_part, z.r, z.boxes);
       }
       __syncwarp();
@@ -546,11 +555,15 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       for (int s = 0; s < k.steps; ++s, ++g) {
         const Pending z = {step.head, step.r, (step.n + kBoxRows - 1) / kBoxRows, g, true};
         const int slot = g % NY;
-        if (S::TWO && !load_z(z)) { ok = false; break; }
-        if (!warp_wait(smem_u32(&bar_y_empty[slot]), ((g / NY) & 1) ^ 1, abort_flag, status, 12, g)) { ok = false; break; }
+        // its last reader: S(g - NY) (FWD, DV), OUT(g - NY) (DQ, DK)
+        if (g >= NY) {
+          const int before = g - NY;
+          if (!warp_wait(S::TWO ? smem_u32(&bar_o_full[before % NO]) : smem_u32(&bar_s_full[before % NS]),
+                         (before / (S::TWO ? NO : NS)) & 1, abort_flag, status, 12, g)) { ok = false; break; }
+        }
         if (elect_one()) {
           const uint32_t bar = smem_u32(&bar_y_full[slot]);
-          mbar_expect_tx(bar, (uint32_t)(2 * S::SLABS * z.boxes * kBoxRows * 128));
+          mbar_expect_tx(bar, (uint32_t)((S::TWO ? 4 : 2) * S::SLABS * z.boxes * kBoxRows * 128));
           load(&mapY, sY + slot * S::Y_BYTES, bar, S::Y_PART, BN * 128, z.head, y_part, z.r, z.boxes);
           if (S::KEYS) {
             const int64_t at = (int64_t)z.head * t.pitch + z.r;
@@ -561,7 +574,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           }
         }
         __syncwarp();
-        if (!S::TWO) {
+        if (S::TWO) {
+          if (!load_z(z)) { ok = false; break; }
+        } else {
           if (late.any && !load_z(late)) { ok = false; break; }
           late = z;
         }
@@ -614,7 +629,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
     struct Pending { int g, n16; bool any; } late = {0, 0, false};
     const auto out = [&](const Pending& q) {
       if (!warp_wait(smem_u32(&bar_p_full[q.g % NS]), (q.g / NS) & 1, abort_flag, status, 20, q.g)) return false;
-      if (!warp_wait(smem_u32(&bar_o_empty), (q.g & 1) ^ 1, abort_flag, status, 21, q.g)) return false;
       uint32_t bz = sY + (q.g % NY) * S::Y_BYTES;
       if (!S::TWO) {
         if (!warp_wait(smem_u32(&bar_z_full[q.g % NZ]), (q.g / NZ) & 1, abort_flag, status, 22, q.g)) return false;
@@ -623,8 +637,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       tc_fence_after();
       if (elect_one()) {
         weighted(tmem + S::T_OUT, tmem + (q.g % NS) * BN, bz, q.n16);
-        umma_commit(smem_u32(&bar_o_full));
-        umma_commit(S::TWO ? smem_u32(&bar_y_empty[q.g % NY]) : smem_u32(&bar_z_empty[q.g % NZ]));
+        umma_commit(smem_u32(&bar_o_full[q.g % NO]));
       }
       __syncwarp();
       return true;
@@ -637,10 +650,12 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       if (k.steps == 0 || k.skip) continue;
       if (!warp_wait(smem_u32(&bar_x_full), nw & 1, abort_flag, status, 23, w)) { ok = false; break; }
       Steps<MODE, DP> step(t, k);
-      for (int s = 0; s < k.steps; ++s, ++g) {
-        const int n16 = (step.n + 15) & ~15;
+      int n16 = (step.n + 15) & ~15;
+      const int steps = k.steps;
+      for (int s = 0; s < steps; ++s, ++g) {
         const uint32_t id = (1u << 4) | ((uint32_t)(n16 >> 3) << 17) | ((128u >> 4) << 24);
         const uint32_t at = tmem + (g % NS) * BN;
+        const uint32_t y = sY + (g % NY) * S::Y_BYTES, z = sZ + (g % NZ) * S::Y_BYTES;
         if (S::TWO) {
           // dP(g), S(g), OUT(g - 1).  The last readers of these buffers: the weights of step g - 2 are complete
           // (OUT(g - 2) waited for them), and OUT(g - 2) itself has to be over; dP(g) keeps the tensor cores busy meanwhile.
@@ -650,29 +665,28 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
             late.any = false;
             if (!warp_wait(smem_u32(&bar_x2_full), nw & 1, abort_flag, status, 28, w)) { ok = false; break; }
           }
-          if (!warp_wait(smem_u32(&bar_z_full[g % NZ]), (g / NZ) & 1, abort_flag, status, 26, g)) { ok = false; break; }
+          if (!warp_wait(smem_u32(&bar_y_full[g % NY]), (g / NY) & 1, abort_flag, status, 26, g)) { ok = false; break; }
           tc_fence_after();
-          if (elect_one()) {
-            second_scores(at + S::T_DP, sZ + (g % NZ) * S::Y_BYTES, id);
-            umma_commit(smem_u32(&bar_z_empty[g % NZ]));
-          }
+          if (elect_one()) second_scores(at + S::T_DP, z, id);
           __syncwarp();
-          // (a first step has nothing to wait for: the second operand came after the drain of OUT(g - 1))
-          if (s > 0 && g >= 2 && !warp_wait(smem_u32(&bar_o_full), g & 1, abort_flag, status, 25, g)) { ok = false; break; }
+          // (a first step has nothing to wait for: the second operand came after OUT(g - 1) had been read)
+          if (s > 0 && g >= 2 && !warp_wait(smem_u32(&bar_o_full[(g - 2) % NO]), ((g - 2) / NO) & 1, abort_flag, status, 25, g)) { ok = false; break; }
+        } else {
+          // S(g), OUT(g - 1); the weights of step g - 3 were in this buffer, and OUT(g - 2) waited until OUT(g - 3) was read
+          if (!warp_wait(smem_u32(&bar_y_full[g % NY]), (g / NY) & 1, abort_flag, status, 24, g)) { ok = false; break; }
         }
-        // FWD, DV: S(g), OUT(g - 1); the weights of step g - 3 were in this buffer, and OUT(g - 2) waited for the drain of OUT(g - 3)
-        if (!warp_wait(smem_u32(&bar_y_full[g % NY]), (g / NY) & 1, abort_flag, status, 24, g)) { ok = false; break; }
         tc_fence_after();
         if (elect_one()) {
-          scores(at, sX, sY + (g % NY) * S::Y_BYTES, id);
+          scores(at, sX, y, id);
           umma_commit(smem_u32(&bar_s_full[g % NS]));
-          if (!S::TWO) umma_commit(smem_u32(&bar_y_empty[g % NY]));
-          if (s == k.steps - 1) umma_commit(smem_u32(&bar_x_empty));
+          if (s == steps - 1) umma_commit(smem_u32(&bar_x_empty));
         }
         __syncwarp();
+        const Pending now = {g, n16, true};
+        step.next(t, k);                                         // while the scores run
+        n16 = (step.n + 15) & ~15;
         if (late.any && !out(late)) { ok = false; break; }
-        late = {g, n16, true};
-        step.next(t, k);
+        late = now;
       }
       ++nw;
     }
@@ -751,15 +765,12 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       float c = 0.0f, cdp = 0.0f, factor = 1.0f, factor_before = 1.0f;
       // sums = sums * times + tile (FWD), or sums + tile * times
       const auto drain = [&](int gd, float times) {
-        if (!warp_wait(smem_u32(&bar_o_full), gd & 1, abort_flag, status, 30, gd)) return false;
+        if (!warp_wait(smem_u32(&bar_o_full[gd % NO]), (gd / NO) & 1, abort_flag, status, 30, gd)) return false;
         tc_fence_after();
         uint32_t v[OUT];
 #pragma unroll
         for (int q = 0; q < OUT / 16; ++q) tmem_ld16(tmem + lanes + S::T_OUT + part * OUT + q * 16, v + q * 16);
         tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_o_empty));
         const uint64_t t2 = pack2(times, times);
 #pragma unroll
         for (int i = 0; i < OUT / 2; ++i) {
@@ -856,10 +867,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
               store_split(ts + q * 16, wt);
             }
           }
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&bar_p_full[buf]));
           float s0, s1;
           unpack2(sum, s0, s1);
           l = fmaf(l, keep, __fadd_rn(s0, s1));
@@ -904,13 +911,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
               store_split(ts + q * 16, wt);
             }
           }
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&bar_p_full[buf]));
           if (s > 0 && !drain(g - 1, factor_before)) { ok = false; break; }
           factor_before = factor;
         }
+        // the weights are there, and OUT(g - 1) has been read: OUT(g) may start
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_p_full[buf]));
       }
       if (!ok) break;
       if (k.steps > 0 && !drain(g - 1, MODE == FWD ? keep_before : factor_before)) { ok = false; break; }
