@@ -75,11 +75,12 @@ struct PrepArgs {
 template <int DP>
 __global__ void __launch_bounds__(kPrepThreads)
 attn_prep_kernel(const __grid_constant__ PrepArgs a) {
-  constexpr int E = DP / 32;                                    // elements per lane
-  __shared__ uint32_t red[kPrepThreads / 32];
-  __shared__ float redn[kPrepThreads / 32];
+  constexpr int LANES = DP / 4, ROWS = 32 / LANES;              // four values per lane; rows that a warp takes at once
+  constexpr int kWarps = kPrepThreads / 32, BATCH = kPrepRows / (kWarps * ROWS) < 4 ? kPrepRows / (kWarps * ROWS) : 4;
+  __shared__ uint32_t red[kWarps];
+  __shared__ float redn[kWarps];
   __shared__ int last_block;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES, c = lane % LANES * 4;
   int head = blockIdx.y, ti = 0;
   while (head >= a.t[ti].heads) head -= a.t[ti++].heads;
   const PrepTensor& t = a.t[ti];
@@ -88,33 +89,37 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
   const int len = lnn::attn_length(a.lengths, head / t.per_batch, a.kv_len, a.status);
   const int end = min(t.rows, len - t.past), dim = a.dim;        // rows from here on are padding
   const float* src = t.src + (int64_t)head * t.rows * dim;
-  const bool vec = E == 4 && dim == DP && (((uintptr_t)t.src) & 15) == 0;
-  const auto load = [&](const float* base, int r, float (&x)[E]) {
-    const float* p = base + (int64_t)r * dim + lane * E;
-    if (vec) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(p));
-      x[0] = v.x; x[1] = v.y; x[E - 2] = v.z; x[E - 1] = v.w;
-    } else {
+  const bool is_do = a.o != nullptr && ti == a.tensors - 1;
+  const bool vec = dim % 4 == 0 && (((uintptr_t)t.src | (is_do ? (uintptr_t)a.o : 0)) & 15) == 0;
+  const auto load = [&](const float* base, int r) {
+    const float* p = base + (int64_t)r * dim + c;
+    if (vec) return c < dim ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    return make_float4(c < dim ? __ldg(p) : 0.0f, c + 1 < dim ? __ldg(p + 1) : 0.0f, c + 2 < dim ? __ldg(p + 2) : 0.0f,
+                       c + 3 < dim ? __ldg(p + 3) : 0.0f);
+  };
+  const auto largest = [&](float4 v) {
+    return max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
+               max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
+  };
+  const auto row_total = [&](float v) {                          // over the lanes of a row
 #pragma unroll
-      for (int i = 0; i < E; ++i) x[i] = lane * E + i < dim ? __ldg(p + i) : 0.0f;
-    }
+    for (int s = LANES / 2; s > 0; s >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, s));
+    return v;
   };
   // the scale, from rows spread over those that are real (the same ones in every block of the head)
   uint32_t m = 0;
   const int span = end - t.first;
-  if (span > 0)
-    for (int i = warp; i < kSampleRows; i += kPrepThreads / 32) {
-      float x[E];
-      load(src, t.first + (int)((int64_t)i * span / kSampleRows), x);
+  if (span > 0) {
 #pragma unroll
-      for (int k = 0; k < E; ++k) m = max(m, __float_as_uint(x[k]) & 0x7fffffffu);
-    }
+    for (int i = warp * ROWS + sub; i < kSampleRows; i += kWarps * ROWS)
+      m = max(m, largest(load(src, t.first + (int)((int64_t)i * span / kSampleRows))));
+  }
   m = __reduce_max_sync(0xffffffffu, m);
   if (lane == 0) red[warp] = m;
   __syncthreads();
   m = red[0];
 #pragma unroll
-  for (int w = 1; w < kPrepThreads / 32; ++w) m = max(m, red[w]);
+  for (int w = 1; w < kWarps; ++w) m = max(m, red[w]);
   const int ebits = (int)(m >> 23);
   const int e = m == 0u || ebits == 255 ? 0 : max(ebits, 1) - 127 - 8;
   const Pow2Scale scale(-e);
@@ -122,53 +127,48 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
 
   __half* hi = t.hi + (int64_t)head * t.rows * DP;
   __half* lo = hi + (int64_t)t.heads * t.rows * DP;
-  const bool is_do = a.o != nullptr && ti == a.tensors - 1;
   uint32_t top = 0;
   float top_norm = 0.0f;
   const int r_end = min((int)(blockIdx.x + 1) * kPrepRows, t.rows);
-  for (int r = blockIdx.x * kPrepRows + warp; r < r_end; r += kPrepThreads / 32) {
-    const bool real = r < end && (r >= t.first || r < t.sinks);
-    float x[E];
+  for (int r0 = blockIdx.x * kPrepRows + warp * ROWS + sub; r0 < (int)(blockIdx.x + 1) * kPrepRows; r0 += BATCH * kWarps * ROWS) {
+    float4 x[BATCH], y[BATCH];
 #pragma unroll
-    for (int k = 0; k < E; ++k) x[k] = 0.0f;
-    if (real) load(src, r, x);
-    float delta = 0.0f;
-    if (is_do) {
-      if (real) {
-        float y[E];
-        load(a.o + (int64_t)head * t.rows * dim, r, y);
+    for (int u = 0; u < BATCH; ++u) {
+      const int r = r0 + u * kWarps * ROWS;
+      const bool real = r < end && (r >= t.first || r < t.sinks);
+      x[u] = real ? load(src, r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (is_do) y[u] = real ? load(a.o + (int64_t)head * t.rows * dim, r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
 #pragma unroll
-        for (int k = 0; k < E; ++k) delta = fmaf(x[k], y[k], delta);
+    for (int u = 0; u < BATCH; ++u) {
+      const int r = r0 + u * kWarps * ROWS;
+      const bool in = r < r_end;
+      const float v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+      if (is_do) {
+        const float delta = row_total(fmaf(x[u].w, y[u].w, fmaf(x[u].z, y[u].z, fmaf(x[u].y, y[u].y, __fmul_rn(x[u].x, y[u].x)))));
+        if (c == 0 && in) {
+          a.delta_p[(int64_t)head * a.pitch + r] = delta;
+          a.lse_p[(int64_t)head * a.pitch + r] = r < end ? a.lse[(int64_t)head * t.rows + r] : CUDART_INF_F;
+        }
       }
+      __half h[4], l[4];
+      float norm = 0.0f;
 #pragma unroll
-      for (int s = 16; s > 0; s >>= 1) delta = __fadd_rn(delta, __shfl_xor_sync(0xffffffffu, delta, s));
-      if (lane == 0) {
-        a.delta_p[(int64_t)head * a.pitch + r] = delta;
-        a.lse_p[(int64_t)head * a.pitch + r] = real ? a.lse[(int64_t)head * t.rows + r] : CUDART_INF_F;
+      for (int k = 0; k < 4; ++k) {
+        const float xs = scale(__fmul_rn(v[k], t.sign));
+        top = max(top, __float_as_uint(xs) & 0x7fffffffu);
+        norm = fmaf(xs, xs, norm);
+        split_half(xs, h[k], l[k]);
       }
-    }
-    __half h[E], l[E];
-    float norm = 0.0f;
-#pragma unroll
-    for (int k = 0; k < E; ++k) {
-      const float xs = scale(__fmul_rn(x[k], t.sign));
-      top = max(top, __float_as_uint(xs) & 0x7fffffffu);
-      norm = fmaf(xs, xs, norm);
-      split_half(xs, h[k], l[k]);
-    }
-    if (E == 4) {
-      reinterpret_cast<uint2*>(hi + (int64_t)r * DP)[lane] = *reinterpret_cast<uint2*>(h);
-      reinterpret_cast<uint2*>(lo + (int64_t)r * DP)[lane] = *reinterpret_cast<uint2*>(l);
-    } else {
-      reinterpret_cast<uint32_t*>(hi + (int64_t)r * DP)[lane] = *reinterpret_cast<uint32_t*>(h);
-      reinterpret_cast<uint32_t*>(lo + (int64_t)r * DP)[lane] = *reinterpret_cast<uint32_t*>(l);
-    }
-    if (t.norms) {
-#pragma unroll
-      for (int s = 16; s > 0; s >>= 1) norm = __fadd_rn(norm, __shfl_xor_sync(0xffffffffu, norm, s));
-      norm = sqrtf(norm);
-      top_norm = fmaxf(top_norm, norm);
-      if (lane == 0) t.norms[(int64_t)head * t.rows + r] = norm;
+      if (in) {
+        *reinterpret_cast<uint2*>(hi + (int64_t)r * DP + c) = *reinterpret_cast<uint2*>(h);
+        *reinterpret_cast<uint2*>(lo + (int64_t)r * DP + c) = *reinterpret_cast<uint2*>(l);
+      }
+      if (t.norms) {
+        norm = sqrtf(row_total(norm));
+        top_norm = fmaxf(top_norm, norm);
+        if (c == 0 && in) t.norms[(int64_t)head * t.rows + r] = norm;
+      }
     }
   }
   if (is_do && (int)blockIdx.x == blocks - 1)                    // columns that exist in no head
@@ -176,6 +176,8 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
       a.delta_p[(int64_t)head * a.pitch + r] = 0.0f;
       a.lse_p[(int64_t)head * a.pitch + r] = CUDART_INF_F;
     }
+#pragma unroll
+  for (int s = 16; s >= LANES; s >>= 1) top_norm = fmaxf(top_norm, __shfl_xor_sync(0xffffffffu, top_norm, s));
   top = __reduce_max_sync(0xffffffffu, top);
   if (lane == 0) { red[warp] = top; redn[warp] = top_norm; }
   __syncthreads();
@@ -454,7 +456,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag_smem;
   __shared__ float exchange[3][kComputeWarps][32];
-  constexpr int NW = 2;                                          // works handed over
+  constexpr int NW = 3;                                          // works handed over
   __shared__ uint64_t bar_w_full[NW], bar_w_empty[NW];
   __shared__ Work works[NW];
   // What goes with the columns of a pass over keys, loaded with the rows of their step.  A slot is free when its step's weights
@@ -669,7 +671,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           tc_fence_after();
           if (elect_one()) second_scores(at + S::T_DP, z, id);
           __syncwarp();
-          // (a first step has nothing to wait for: the second operand came after OUT(g - 1) had been read)
+          // (a first step has nothing to wait for: OUT(g - 1), in front of it, waited until OUT(g - 2) had been read)
           if (s > 0 && g >= 2 && !warp_wait(smem_u32(&bar_o_full[(g - 2) % NO]), ((g - 2) / NO) & 1, abort_flag, status, 25, g)) { ok = false; break; }
         } else {
           // S(g), OUT(g - 1); the weights of step g - 3 were in this buffer, and OUT(g - 2) waited until OUT(g - 3) was read
@@ -712,33 +714,138 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       for (int i = 0; i < kParts; ++i) all[i] = buffer[quarter * kParts + i][lane];
       return true;
     };
-    int nr = 0, nw = 0;
-    for (int w = blockIdx.x; ok && w < t.works; w += gridDim.x, ++nr) {
-      if (!warp_wait(smem_u32(&bar_w_full[nr % NW]), (nr / NW) & 1, abort_flag, status, 33, w)) { ok = false; break; }
-      const Work k = works[nr % NW];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_w_empty[nr % NW]));
-      if (k.skip) continue;
-      const int row = k.row0 + row_in;
-      const int xh = S::KEYS ? k.b * a.kv_heads + k.hk : k.b * a.q_heads + k.h;
-      uint64_t sums[OUT / 2];
+    // The running sums of a tile are finished during the first step of the next one: its first weights are computed (and the
+    // second product of this tile started) before this tile's results are stored.
+    uint64_t sums[OUT / 2];
+    float m = -CUDART_INF_F, l = 0.0f, times = 1.0f;             // FWD: maximum and sum; DQ: what the sums are multiplied by
+    float keep_before = 1.0f, factor_before = 1.0f;
+    int pending = -1;                                              // the slot of the work that is not finished
 #pragma unroll
-      for (int i = 0; i < OUT / 2; ++i) sums[i] = 0;
-      float m = -CUDART_INF_F, l = 0.0f, keep_before = 1.0f;      // FWD
-      float row_lse = CUDART_INF_F, row_delta = 0.0f;              // DQ
-      int row_exp = 0;                                             // DQ, DK: dS is scaled by 2^row_exp
-      const int rows = S::KEYS ? a.kv_len : a.q_len;
-      float norm = 0.0f;
-      if (S::TWO && row < rows) norm = __ldg(t.norms + (int64_t)xh * rows + row);
-      if (MODE == DQ) {
-        if (row < rows) {
-          row_lse = __ldg(t.lse_p + (int64_t)xh * t.pitch + row);
-          row_delta = __ldg(t.delta_p + (int64_t)xh * t.pitch + row);
+    for (int i = 0; i < OUT / 2; ++i) sums[i] = 0;
+    const int rows = S::KEYS ? a.kv_len : a.q_len;
+    // sums = sums * keep + tile (FWD), or sums + tile * factor, with what belonged to step gd
+    const auto drain = [&](int gd) {
+      if (!warp_wait(smem_u32(&bar_o_full[gd % NO]), (gd / NO) & 1, abort_flag, status, 30, gd)) return false;
+      tc_fence_after();
+      uint32_t v[OUT];
+#pragma unroll
+      for (int q = 0; q < OUT / 16; ++q) tmem_ld16(tmem + lanes + S::T_OUT + part * OUT + q * 16, v + q * 16);
+      tmem_ld_wait();
+      const float f = MODE == FWD ? keep_before : factor_before;
+      const uint64_t f2 = pack2(f, f);
+#pragma unroll
+      for (int i = 0; i < OUT / 2; ++i) {
+        const uint64_t x = pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+        sums[i] = MODE == FWD ? fma2(sums[i], f2, x) : fma2(x, f2, sums[i]);
+      }
+      return true;
+    };
+    // The results of the work in `slot`, whose maximum, sum and factor are given; the sums are zero after it.
+    const auto finish = [&](int slot, float top, float sum, float factor_of) {
+      const Work& k = works[slot];
+      const int row = k.row0 + row_in, steps = k.steps;
+      const int xh = S::KEYS ? k.b * a.kv_heads + k.hk : k.b * a.q_heads + k.h;
+      float* dst;
+      int accumulate = 0, limit = rows, pitch_cols = a.dim;
+      float mul = 1.0f;
+      bool empty = false;
+      int64_t at = ((int64_t)xh * rows + row) * a.dim;
+      if (MODE == FWD) {
+        if (steps > 0) {
+          float all[kParts];
+          if (!share(exchange[2], sum, all)) return false;
+          sum = __fadd_rn(__fadd_rn(all[0], all[1]), __fadd_rn(all[2], all[3]));
+        }
+        empty = steps == 0 || row + past > k.p_hi;
+        mul = __fmul_rn(__fdiv_rn(1.0f, sum), pow2f_int(k.ev));
+        if (part == 0 && row < rows)
+          a.lse[(int64_t)xh * rows + row] = empty ? CUDART_INF_F : __fadd_rn(top, __fsub_rn(log2f(sum), 14.0f));
+        dst = a.o;
+      } else if (MODE == DQ) {
+        mul = factor_of;
+        dst = a.dq; accumulate = a.acc_q;
+      } else {
+        if (MODE == DK) mul = fabsf(a.scale);
+        dst = MODE == DK ? a.dk : a.dv;
+        accumulate = MODE == DK ? a.acc_k : a.acc_v;
+        if (k.split_up) {
+          dst = t.parts; accumulate = 0; limit = k.row0 + kRowsM;
+          at = ((int64_t)k.part * kRowsM + row_in) * DP;
+          pitch_cols = DP;
         }
       }
-      if (S::TWO && k.steps > 0) {
-        // the second stationary operand into TMEM, once the products of the work before are over: this warp's fourth of
-        // the columns of its rows, hi and lo (what is no row of the tensor is zero)
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_w_empty[slot]));
+      const uint64_t mul2x = pack2(mul, mul);
+      float* to = dst + at + part * OUT;
+      const int cols = row < limit ? pitch_cols - part * OUT : 0;  // of this warp's part
+      const bool vec = pitch_cols % 8 == 0 && (((uintptr_t)dst) & 31) == 0;
+#pragma unroll
+      for (int i = 0; i < OUT; i += 8) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; u += 2) {
+          unpack2(mul2(sums[(i + u) / 2], mul2x), x[u], x[u + 1]);
+          sums[(i + u) / 2] = 0;
+        }
+        if (MODE == FWD && empty) {
+#pragma unroll
+          for (int u = 0; u < 8; ++u) x[u] = 0.0f;
+        }
+        if (vec) {                                                 // whole 32-byte sectors
+          if (i < cols) {
+            if (MODE != FWD && accumulate) {
+              const float4 y0 = *reinterpret_cast<const float4*>(to + i), y1 = *reinterpret_cast<const float4*>(to + i + 4);
+              const float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
+#pragma unroll
+              for (int u = 0; u < 8; ++u) x[u] = __fadd_rn(y[u], x[u]);
+            }
+            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + i), "f"(x[0]), "f"(x[1]), "f"(x[2]),
+                         "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+                         : "memory");
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            if (i + u < cols) to[i + u] = MODE != FWD && accumulate ? __fadd_rn(to[i + u], x[u]) : x[u];
+        }
+      }
+      return true;
+    };
+    int nr = 0, nw = 0;
+    for (int w = blockIdx.x; ok && w < t.works; w += gridDim.x, ++nr) {
+      const int slot = nr % NW;
+      if (!warp_wait(smem_u32(&bar_w_full[slot]), (nr / NW) & 1, abort_flag, status, 33, w)) { ok = false; break; }
+      const Work& k = works[slot];
+      const int steps = k.steps, row0 = k.row0;
+      if (k.skip || steps == 0) {
+        if (!k.skip) {
+          // nothing is seen: zeros (behind the results that are still to be stored)
+          if (pending >= 0 && (!drain(g - 1) || !finish(pending, m, l, times))) { ok = false; break; }
+          pending = -1;
+          if (!finish(slot, 0.0f, 1.0f, 1.0f)) { ok = false; break; }
+        } else {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&bar_w_empty[slot]));
+        }
+        continue;
+      }
+      const int row = row0 + row_in;
+      const int xh = S::KEYS ? k.b * a.kv_heads + k.hk : k.b * a.q_heads + k.h;
+      const float m_old = m, l_old = l, times_old = times;
+      m = -CUDART_INF_F;
+      l = 0.0f;
+      float row_lse = CUDART_INF_F, row_delta = 0.0f;              // DQ
+      int row_exp = 0;                                             // DQ, DK: dS is scaled by 2^row_exp
+      float norm = 0.0f;
+      if (S::TWO && row < rows) norm = __ldg(t.norms + (int64_t)xh * rows + row);
+      if (MODE == DQ && row < rows) {
+        row_lse = __ldg(t.lse_p + (int64_t)xh * t.pitch + row);
+        row_delta = __ldg(t.delta_p + (int64_t)xh * t.pitch + row);
+      }
+      if (S::TWO) {
+        // The second stationary operand into TMEM, once the products of the work before are over: this warp's fourth of
+        // the columns of its rows, hi and lo (what is no row of the tensor is zero).
         if (!warp_wait(smem_u32(&bar_x_empty), (nw & 1) ^ 1, abort_flag, status, 34, w)) { ok = false; break; }
         const int64_t lo_at = (int64_t)(S::KEYS ? a.batch * a.kv_heads : a.batch * a.q_heads) * rows * (DP / 2);
         const uint32_t* src = t.x2 + ((int64_t)xh * rows + row) * (DP / 2) + part * (DP / 8);
@@ -762,25 +869,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
         ++nw;
       }
       int cur_head = -1;
-      float c = 0.0f, cdp = 0.0f, factor = 1.0f, factor_before = 1.0f;
-      // sums = sums * times + tile (FWD), or sums + tile * times
-      const auto drain = [&](int gd, float times) {
-        if (!warp_wait(smem_u32(&bar_o_full[gd % NO]), (gd / NO) & 1, abort_flag, status, 30, gd)) return false;
-        tc_fence_after();
-        uint32_t v[OUT];
-#pragma unroll
-        for (int q = 0; q < OUT / 16; ++q) tmem_ld16(tmem + lanes + S::T_OUT + part * OUT + q * 16, v + q * 16);
-        tmem_ld_wait();
-        const uint64_t t2 = pack2(times, times);
-#pragma unroll
-        for (int i = 0; i < OUT / 2; ++i) {
-          const uint64_t x = pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-          sums[i] = MODE == FWD ? fma2(sums[i], t2, x) : fma2(x, t2, sums[i]);
-        }
-        return true;
-      };
+      float c = 0.0f, cdp = 0.0f, factor = 1.0f;
       Steps<MODE, DP> step(t, k);
-      for (int s = 0; s < k.steps; ++s, ++g, buf_phase ^= buf == NS - 1, buf = buf == NS - 1 ? 0 : buf + 1, step.next(t, k)) {
+      for (int s = 0; s < steps; ++s, ++g, buf_phase ^= buf == NS - 1, buf = buf == NS - 1 ? 0 : buf + 1, step.next(t, k)) {
         const int r0 = step.r, n = step.n, qh = S::KEYS ? step.head : xh;
         if (qh != cur_head) {                                      // the scales that go with a query head
           int eq = k.eq, eo = k.eo;
@@ -807,11 +898,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
         uint32_t seen = 0xffffffffu;
         if (!S::KEYS) {
           const int p = row + past;
-          all = n == BN && r0 + BN - 1 <= k.row0 + past && (k.p_hi - r0 < a.window || r0 + BN <= a.sinks);
+          all = n == BN && r0 + BN - 1 <= row0 + past && (k.p_hi - r0 < a.window || r0 + BN <= a.sinks);
           if (!all) seen = bits_to(min(p - r0, n - 1) - col0) & (~bits_to(p - a.window - r0 - col0) | bits_to(a.sinks - 1 - r0 - col0));
         } else {
-          all = n == BN && r0 + past >= k.row0 + kRowsM - 1 &&
-                (r0 + past + BN - 1 < k.row0 + a.window || k.row0 + kRowsM <= a.sinks);
+          all = n == BN && r0 + past >= row0 + kRowsM - 1 &&
+                (r0 + past + BN - 1 < row0 + a.window || row0 + kRowsM <= a.sinks);
           const int last = row < a.sinks ? k.q_hi : (int)min((int64_t)row + a.window - 1, (int64_t)k.q_hi);
           if (!all) seen = bits_to(min(last - past - r0, n - 1) - col0) & ~bits_to(row - past - r0 - 1 - col0);
         }
@@ -871,7 +962,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           unpack2(sum, s0, s1);
           l = fmaf(l, keep, __fadd_rn(s0, s1));
           m = now;
-          if (s > 0 && !drain(g - 1, keep_before)) { ok = false; break; }
+          if ((s > 0 || pending >= 0) && !drain(g - 1)) { ok = false; break; }
           keep_before = keep;
         } else {
           if (col0 < n) {
@@ -911,7 +1002,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
               store_split(ts + q * 16, wt);
             }
           }
-          if (s > 0 && !drain(g - 1, factor_before)) { ok = false; break; }
+          if ((s > 0 || pending >= 0) && !drain(g - 1)) { ok = false; break; }
           factor_before = factor;
         }
         // the weights are there, and OUT(g - 1) has been read: OUT(g) may start
@@ -919,76 +1010,16 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&bar_p_full[buf]));
+        if (pending >= 0) {
+          if (!finish(pending, m_old, l_old, times_old)) { ok = false; break; }
+          pending = -1;
+        }
       }
       if (!ok) break;
-      if (k.steps > 0 && !drain(g - 1, MODE == FWD ? keep_before : factor_before)) { ok = false; break; }
-      float acc[OUT];
-#pragma unroll
-      for (int i = 0; i < OUT / 2; ++i) unpack2(sums[i], acc[2 * i], acc[2 * i + 1]);
-
-      // ---- results ----
-      float* dst;
-      int accumulate = 0, limit = rows;
-      float times = 1.0f;
-      int64_t at = ((int64_t)xh * rows + row) * a.dim;
-      int pitch_cols = a.dim;
-      if (MODE == FWD) {
-        if (k.steps > 0) {
-          float ls[kParts];
-          if (!share(exchange[2], l, ls)) { ok = false; break; }
-          l = __fadd_rn(__fadd_rn(ls[0], ls[1]), __fadd_rn(ls[2], ls[3]));
-        }
-        const bool empty = k.steps == 0 || row + past > k.p_hi;
-        times = empty ? 0.0f : __fmul_rn(__fdiv_rn(1.0f, l), pow2f_int(k.ev));
-        if (part == 0 && row < rows)
-          a.lse[(int64_t)xh * rows + row] = empty ? CUDART_INF_F : __fadd_rn(m, __fsub_rn(log2f(l), 14.0f));
-        if (empty) {
-#pragma unroll
-          for (int i = 0; i < OUT; ++i) acc[i] = 0.0f;
-        }
-        dst = a.o;
-      } else if (MODE == DQ) {
-        times = __fmul_rn(a.scale, pow2f_int(k.ek - row_exp));
-        dst = a.dq; accumulate = a.acc_q;
-      } else {
-        if (MODE == DK) times = fabsf(a.scale);
-        dst = MODE == DK ? a.dk : a.dv;
-        accumulate = MODE == DK ? a.acc_k : a.acc_v;
-        if (k.split_up) {
-          dst = t.parts; accumulate = 0; limit = k.row0 + kRowsM;
-          at = ((int64_t)k.part * kRowsM + row_in) * DP;
-          pitch_cols = DP;
-        }
-      }
-      if (row < limit) {
-        float* to = dst + at;
-        const bool vec = pitch_cols % 8 == 0 && (((uintptr_t)dst) & 31) == 0;
-#pragma unroll
-        for (int i = 0; i < OUT; ++i) acc[i] = __fmul_rn(acc[i], times);
-        if (vec) {                                                 // whole 32-byte sectors
-#pragma unroll
-          for (int i = 0; i < OUT; i += 8) {
-            const int col = part * OUT + i;
-            if (col >= pitch_cols) break;
-            if (accumulate) {
-              const float4 y0 = *reinterpret_cast<const float4*>(to + col), y1 = *reinterpret_cast<const float4*>(to + col + 4);
-              const float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
-#pragma unroll
-              for (int u = 0; u < 8; ++u) acc[i + u] = __fadd_rn(y[u], acc[i + u]);
-            }
-            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + col), "f"(acc[i]), "f"(acc[i + 1]),
-                         "f"(acc[i + 2]), "f"(acc[i + 3]), "f"(acc[i + 4]), "f"(acc[i + 5]), "f"(acc[i + 6]), "f"(acc[i + 7])
-                         : "memory");
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < OUT; ++i) {
-            const int col = part * OUT + i;
-            if (col < pitch_cols) to[col] = accumulate ? __fadd_rn(to[col], acc[i]) : acc[i];
-          }
-        }
-      }
+      if (MODE == DQ) times = __fmul_rn(a.scale, pow2f_int(k.ek - row_exp));
+      pending = slot;
     }
+    if (ok && pending >= 0) ok = drain(g - 1) && finish(pending, m, l, times);
     if (!ok) asm volatile("bar.arrive %0, %1;" ::"r"(1 + quarter), "n"(32 * kParts) : "memory");
   }
 
@@ -1008,21 +1039,25 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
 }
 
 // dK or dV of the tiles that several works shared: their parts in order.
+constexpr int kPartBlocks = 8;                   // blocks per tile
 template <int DP>
 __global__ void __launch_bounds__(256)
 attn_parts_kernel(float* __restrict__ dst, const float* __restrict__ parts, const TcArgs t, int accumulate) {
   const AttnArgs& a = t.a;
-  const int tile = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  constexpr int ROWS = kRowsM / kPartBlocks;
+  const int tile = blockIdx.x / kPartBlocks, first = blockIdx.x % kPartBlocks * ROWS, hk = blockIdx.y, b = blockIdx.z;
   const int splits = tile < t.sink_tiles ? t.splits_sink : t.splits;
   if (splits == 1 || !lnn::group_ok(a, b, hk)) return;
   const int64_t w0 = (int64_t)(b * a.kv_heads + hk) * parts_per_head(t) +
                      (tile < t.sink_tiles ? tile * t.splits_sink : t.sink_tiles * t.splits_sink + (tile - t.sink_tiles) * t.splits);
-  for (int i = threadIdx.x; i < kRowsM * DP / 4; i += 256) {
-    const int row = tile * kRowsM + i / (DP / 4), col = i % (DP / 4) * 4;
+  for (int i = threadIdx.x; i < ROWS * DP / 4; i += 256) {
+    const int row = tile * kRowsM + first + i / (DP / 4), col = i % (DP / 4) * 4;
     if (row >= a.kv_len || col >= a.dim) continue;
-    float4 s = __ldg(reinterpret_cast<const float4*>(parts + w0 * kRowsM * DP) + i);
+    const float4* from = reinterpret_cast<const float4*>(parts + w0 * kRowsM * DP + first * DP) + i;
+    float4 s = __ldg(from);
+#pragma unroll 4
     for (int k = 1; k < splits; ++k) {
-      const float4 x = __ldg(reinterpret_cast<const float4*>(parts + (w0 + k) * kRowsM * DP) + i);
+      const float4 x = __ldg(from + (int64_t)k * (kRowsM * DP / 4));
       s = make_float4(__fadd_rn(s.x, x.x), __fadd_rn(s.y, x.y), __fadd_rn(s.z, x.z), __fadd_rn(s.w, x.w));
     }
     float* to = dst + ((int64_t)(b * a.kv_heads + hk) * a.kv_len + row) * a.dim + col;
@@ -1146,7 +1181,7 @@ int keys_pass(lnn::Device* d, TcArgs t, Operands& op, float* dst, int accumulate
   }
   int rc = launch_pass<MODE, DP>(d, &op.map[1], &op.map[0], &op.map[3], t);
   if (rc || !cut) return rc;
-  attn_parts_kernel<DP><<<dim3((unsigned)t.tiles, (unsigned)t.a.kv_heads, (unsigned)t.a.batch), 256, 0, d->stream>>>(
+  attn_parts_kernel<DP><<<dim3((unsigned)t.tiles * kPartBlocks, (unsigned)t.a.kv_heads, (unsigned)t.a.batch), 256, 0, d->stream>>>(
       dst, t.parts, t, accumulate);
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
