@@ -7,6 +7,7 @@
 #include <float.h>
 #include <algorithm>
 #include "lnn_attn.cuh"
+#include "lnn_tc_dev.cuh"
 
 namespace {
 
@@ -368,6 +369,8 @@ cache_store_kernel(float* __restrict__ ck, float* __restrict__ cv, float* __rest
   }
 }
 
+constexpr int kMaxStages = 8;
+
 struct StepArgs {
   float* o;
   const float *q, *k, *v;                // [batch][q_heads][dim], [batch][kv_heads][dim]
@@ -375,118 +378,102 @@ struct StepArgs {
   const float* lengths;
   float* lengths_out;
   int batch, q_heads, kv_heads, dim, window, sinks, splits, group_chunks;
+  int stage_slots, stages;
   float scale;
   int* status;
 };
 
-// Eight lanes share a key: each holds 4 NV of its values, and of the queries and outputs of GC heads.  A warp takes
-// four keys at a time, and every group of eight lanes has a softmax of its own, which meet at the end: within the warp
-// by shuffles, in the block through shared memory and over the blocks of a cluster (the slots of one sequence and head,
-// cut into contiguous shares) through distributed shared memory.  The new key and value are read from the arguments
-// while one block writes them into the cache.
-template <int GC, int NV, bool VEC>
-__global__ void __launch_bounds__(kThreads)
-step_kernel(const StepArgs a) {
-  extern __shared__ __align__(16) float smem[];
-  constexpr int kWarps = kThreads / 32;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane & 7, sub = lane >> 3;
-  const int rank = blockIdx.x;                                    // the cluster runs along x
-  const int hk = blockIdx.y / a.group_chunks, chunk = blockIdx.y % a.group_chunks, b = blockIdx.z;
-  const int group = a.q_heads / a.kv_heads, dim = a.dim, slots = a.window + a.sinks;
-  const int h0 = hk * group + chunk * GC, heads = min(GC, group - chunk * GC);
-  const int len = cache_length(__ldg(a.lengths + b), b, a.status);
-  if (rank == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.lengths_out[b] = len < 0 ? a.lengths[b] : (float)(len + 1);
-  const int64_t oq = ((int64_t)b * a.q_heads + h0) * dim, okv = ((int64_t)b * a.kv_heads + hk) * dim, oc = okv * slots;
-  if (len < 0) {                                                  // the same for the whole cluster
-    if (rank == 0)
-      for (int i = threadIdx.x; i < heads * dim; i += kThreads) a.o[oq + i] = 0.0f;
-    return;
-  }
-  const int fresh = len < a.sinks ? len : a.sinks + (len - a.sinks) % a.window;
-  const int n = min(len + 1, slots);
-  const int per = ((n + a.splits - 1) / a.splits + 31) / 32 * 32;
-  const int begin = min(rank * per, n), end = min(begin + per, n);
+// Eight lanes share a key: each holds 4 NV of its values, and of the outputs of GC heads.  A warp takes four keys at a time,
+// and every group of eight lanes has a softmax of its own, which meet at the end: within the warp by shuffles, in the
+// block through shared memory and over the blocks of a cluster (the slots of one sequence and head, cut into contiguous
+// shares) through distributed shared memory.  The new key and value are read from the arguments while one block writes
+// them into the cache.
+constexpr int kStepWarps = kThreads / 32;
+template <int NV> constexpr int kStepRow = NV * 32 + 2;        // values, maximum and sum of a partial result
 
-  const auto load = [&](const float* row, int u) {
-    const int c = u * 32 + part * 4;
-    if (VEC) return c < dim ? __ldg(reinterpret_cast<const float4*>(row + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    return make_float4(c < dim ? __ldg(row + c) : 0.0f, c + 1 < dim ? __ldg(row + c + 1) : 0.0f,
-                       c + 2 < dim ? __ldg(row + c + 2) : 0.0f, c + 3 < dim ? __ldg(row + c + 3) : 0.0f);
-  };
-  float4 q[GC][NV], o[GC][NV];
-  float m[GC], l[GC];
-  const float factor = a.scale * lnn::kLog2e;
-#pragma unroll
-  for (int g = 0; g < GC; ++g) {
-    m[g] = -FLT_MAX;
-    l[g] = 0.0f;
-#pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      o[g][u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      q[g][u] = g < heads ? load(a.q + oq + g * dim, u) : o[g][u];
-      q[g][u].x *= factor; q[g][u].y *= factor; q[g][u].z *= factor; q[g][u].w *= factor;
+struct StepPlace {
+  int rank, hk, chunk, b, h0, heads, len, fresh, n, begin, end;
+  int64_t oq, okv, oc;
+  bool idle;
+  __device__ __forceinline__ StepPlace(const StepArgs& a, int gc) {
+    rank = blockIdx.x;                                            // the cluster runs along x
+    hk = blockIdx.y / a.group_chunks; chunk = blockIdx.y % a.group_chunks; b = blockIdx.z;
+    const int group = a.q_heads / a.kv_heads, slots = a.window + a.sinks;
+    h0 = hk * group + chunk * gc;
+    heads = min(gc, group - chunk * gc);
+    const float length = __ldg(a.lengths + b);
+    len = cache_length(length, b, a.status);
+    if (rank == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.lengths_out[b] = len < 0 ? length : (float)(len + 1);
+    oq = ((int64_t)b * a.q_heads + h0) * a.dim;
+    okv = ((int64_t)b * a.kv_heads + hk) * a.dim;
+    oc = okv * slots;
+    idle = len < 0;                                               // the same for the whole cluster
+    if (idle) {
+      if (rank == 0)
+        for (int i = threadIdx.x; i < heads * a.dim; i += kThreads) a.o[oq + i] = 0.0f;
+      return;
     }
+    fresh = len < a.sinks ? len : a.sinks + (len - a.sinks) % a.window;
+    n = min(len + 1, slots);
+    const int per = ((n + a.splits - 1) / a.splits + 31) / 32 * 32;
+    begin = min(rank * per, n);
+    end = min(begin + per, n);
   }
-  for (int s0 = begin; s0 < end; s0 += 4 * kWarps) {
-    const int slot = s0 + warp * 4 + sub;
-    const bool in = slot < end;
-    const float* krow = slot == fresh ? a.k + okv : a.ck + oc + (int64_t)slot * dim;
-    const float* vrow = slot == fresh ? a.v + okv : a.cv + oc + (int64_t)slot * dim;
-    float4 k[NV], v[NV];
-#pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      k[u] = in ? load(krow, u) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      v[u] = in ? load(vrow, u) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
+};
+
+// The softmax of a group of eight lanes over the keys it has seen, for GC heads.
+template <int GC, int NV>
+struct StepSums {
+  float4 o[GC][NV];
+  float m[GC], l[GC];
+  __device__ __forceinline__ StepSums() {
 #pragma unroll
     for (int g = 0; g < GC; ++g) {
-      float s = 0.0f;
+      m[g] = -FLT_MAX;
+      l[g] = 0.0f;
 #pragma unroll
-      for (int u = 0; u < NV; ++u)
-        s = fmaf(q[g][u].w, k[u].w, fmaf(q[g][u].z, k[u].z, fmaf(q[g][u].y, k[u].y, fmaf(q[g][u].x, k[u].x, s))));
-#pragma unroll
-      for (int x = 4; x > 0; x >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, x));
-      if (in) {
-        if (s > m[g]) {
-          const float keep = exp2_fast(__fsub_rn(m[g], s));
-          l[g] = __fmul_rn(l[g], keep);
-#pragma unroll
-          for (int u = 0; u < NV; ++u) {
-            o[g][u].x *= keep; o[g][u].y *= keep; o[g][u].z *= keep; o[g][u].w *= keep;
-          }
-          m[g] = s;
-        }
-        const float e = exp2_fast(__fsub_rn(s, m[g]));
-        l[g] = __fadd_rn(l[g], e);
-#pragma unroll
-        for (int u = 0; u < NV; ++u) {
-          o[g][u].x = fmaf(e, v[u].x, o[g][u].x); o[g][u].y = fmaf(e, v[u].y, o[g][u].y);
-          o[g][u].z = fmaf(e, v[u].z, o[g][u].z); o[g][u].w = fmaf(e, v[u].w, o[g][u].w);
-        }
-      }
+      for (int u = 0; u < NV; ++u) o[g][u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
   }
-  // one share per cluster and head writes the new row: nobody reads it from the cache in this launch
-  if (rank == 0 && chunk == 0)
-    for (int i = threadIdx.x; i < dim; i += kThreads) {
-      a.ck[oc + (int64_t)fresh * dim + i] = a.k[okv + i];
-      a.cv[oc + (int64_t)fresh * dim + i] = a.v[okv + i];
+  // the next key's score (the same in all eight lanes) and value
+  __device__ __forceinline__ void take(int g, float s, const float4 (&v)[NV]) {
+    if (s > m[g]) {
+      const float keep = exp2_fast(__fsub_rn(m[g], s));
+      l[g] = __fmul_rn(l[g], keep);
+#pragma unroll
+      for (int u = 0; u < NV; ++u) {
+        o[g][u].x *= keep; o[g][u].y *= keep; o[g][u].z *= keep; o[g][u].w *= keep;
+      }
+      m[g] = s;
     }
-  // shared memory: per warp GC heads of {values, m, l}; then the block's own
-  constexpr int kRow = NV * 32 + 2;
+    const float e = exp2_fast(__fsub_rn(s, m[g]));
+    l[g] = __fadd_rn(l[g], e);
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      o[g][u].x = fmaf(e, v[u].x, o[g][u].x); o[g][u].y = fmaf(e, v[u].y, o[g][u].y);
+      o[g][u].z = fmaf(e, v[u].z, o[g][u].z); o[g][u].w = fmaf(e, v[u].w, o[g][u].w);
+    }
+  }
+};
+
+// The sums of all threads of the cluster into the output.  smem: (kStepWarps + 1) * GC * kStepRow floats.
+template <int GC, int NV>
+__device__ __forceinline__ void step_finish(const StepArgs& a, const StepPlace& p, StepSums<GC, NV>& t, float* smem) {
+  constexpr int kRow = kStepRow<NV>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane & 7, sub = lane >> 3;
   float* mine = smem + warp * GC * kRow;
-  float* block = smem + kWarps * GC * kRow;
+  float* block = smem + kStepWarps * GC * kRow;
 #pragma unroll
   for (int g = 0; g < GC; ++g) {
-    float top = fmaxf(m[g], __shfl_xor_sync(0xffffffffu, m[g], 8));
+    float top = fmaxf(t.m[g], __shfl_xor_sync(0xffffffffu, t.m[g], 8));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-    const float w = exp2_fast(__fsub_rn(m[g], top));
-    float sum = __fmul_rn(l[g], w);
+    const float w = exp2_fast(__fsub_rn(t.m[g], top));
+    float sum = __fmul_rn(t.l[g], w);
     sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, 8));
     sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, 16));
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      float x[4] = {o[g][u].x, o[g][u].y, o[g][u].z, o[g][u].w};
+      float x[4] = {t.o[g][u].x, t.o[g][u].y, t.o[g][u].z, t.o[g][u].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         x[i] = __fmul_rn(x[i], w);
@@ -501,7 +488,7 @@ step_kernel(const StepArgs a) {
     }
   }
   __syncthreads();
-  // {values, m, l} of `count` partial results `stride` floats apart; column NV * 32 + 1 gives the sum of the l
+  // column c of `count` partial results: values, or (NV * 32 + 1) the sums; and their maximum
   const auto join = [&](auto&& from, int count, int g, int c) {
     float top = from(0)[g * kRow + NV * 32];
     for (int w = 1; w < count; ++w) top = fmaxf(top, from(w)[g * kRow + NV * 32]);
@@ -512,7 +499,7 @@ step_kernel(const StepArgs a) {
   const auto of_warp = [&](int w) { return smem + w * GC * kRow; };
   for (int i = threadIdx.x; i < GC * (NV * 32 + 1); i += kThreads) {
     const int g = i / (NV * 32 + 1), c = i % (NV * 32 + 1);
-    const float2 r = join(of_warp, kWarps, g, c < NV * 32 ? c : NV * 32 + 1);
+    const float2 r = join(of_warp, kStepWarps, g, c < NV * 32 ? c : NV * 32 + 1);
     if (c < NV * 32) block[g * kRow + c] = r.x;
     else { block[g * kRow + NV * 32] = r.y; block[g * kRow + NV * 32 + 1] = r.x; }
   }
@@ -520,33 +507,198 @@ step_kernel(const StepArgs a) {
   if (a.splits > 1) cluster.sync();
   else __syncthreads();
   const auto of_rank = [&](int r) { return a.splits > 1 ? cluster.map_shared_rank(block, r) : block; };
-  for (int i = rank * kThreads + threadIdx.x; i < heads * dim; i += a.splits * kThreads) {
-    const int g = i / dim, c = i % dim;
+  for (int i = p.rank * kThreads + threadIdx.x; i < p.heads * a.dim; i += a.splits * kThreads) {
+    const int g = i / a.dim, c = i % a.dim;
     const float sum = join(of_rank, a.splits, g, NV * 32 + 1).x;
-    a.o[oq + i] = __fdiv_rn(join(of_rank, a.splits, g, c).x, sum);
+    a.o[p.oq + i] = __fdiv_rn(join(of_rank, a.splits, g, c).x, sum);
   }
   if (a.splits > 1) cluster.sync();                      // nobody leaves while its shared memory is being read
+}
+// One block per cluster and key head writes the new row: nobody reads it from the cache in this launch.
+__device__ __forceinline__ void step_append(const StepArgs& a, const StepPlace& p) {
+  if (p.rank == 0 && p.chunk == 0)
+    for (int i = threadIdx.x; i < a.dim; i += kThreads) {
+      a.ck[p.oc + (int64_t)p.fresh * a.dim + i] = a.k[p.okv + i];
+      a.cv[p.oc + (int64_t)p.fresh * a.dim + i] = a.v[p.okv + i];
+    }
+}
+
+// Rows of any alignment, straight from global memory.
+template <int GC, int NV>
+__global__ void __launch_bounds__(kThreads)
+step_kernel(const StepArgs a) {
+  extern __shared__ __align__(16) float smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane & 7, sub = lane >> 3, dim = a.dim;
+  const StepPlace p(a, GC);
+  if (p.idle) return;
+  const auto load = [&](const float* row, int u) {
+    const int c = u * 32 + part * 4;
+    return make_float4(c < dim ? __ldg(row + c) : 0.0f, c + 1 < dim ? __ldg(row + c + 1) : 0.0f,
+                       c + 2 < dim ? __ldg(row + c + 2) : 0.0f, c + 3 < dim ? __ldg(row + c + 3) : 0.0f);
+  };
+  const float factor = a.scale * lnn::kLog2e;
+  float4 q[GC][NV];
+#pragma unroll
+  for (int g = 0; g < GC; ++g)
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      q[g][u] = g < p.heads ? load(a.q + p.oq + g * dim, u) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      q[g][u].x *= factor; q[g][u].y *= factor; q[g][u].z *= factor; q[g][u].w *= factor;
+    }
+  StepSums<GC, NV> t;
+  for (int s0 = p.begin; s0 < p.end; s0 += 4 * kStepWarps) {
+    const int slot = s0 + warp * 4 + sub;
+    const bool in = slot < p.end;
+    const float* krow = slot == p.fresh ? a.k + p.okv : a.ck + p.oc + (int64_t)slot * dim;
+    const float* vrow = slot == p.fresh ? a.v + p.okv : a.cv + p.oc + (int64_t)slot * dim;
+    float4 k[NV], v[NV];
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      k[u] = in ? load(krow, u) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      v[u] = in ? load(vrow, u) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+#pragma unroll
+    for (int g = 0; g < GC; ++g) {
+      float s = 0.0f;
+#pragma unroll
+      for (int u = 0; u < NV; ++u)
+        s = fmaf(q[g][u].w, k[u].w, fmaf(q[g][u].z, k[u].z, fmaf(q[g][u].y, k[u].y, fmaf(q[g][u].x, k[u].x, s))));
+#pragma unroll
+      for (int x = 4; x > 0; x >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, x));
+      if (in) t.take(g, s, v);
+    }
+  }
+  step_append(a, p);
+  step_finish(a, p, t, smem);
+}
+
+// Rows of 16-byte units: the slots of a share are one piece of memory, which bulk copies bring into a ring of stages in
+// shared memory; two blocks per SM have up to 192 KB on the way.  The queries are in shared memory too (eight lanes
+// read 128 bytes, the other groups the same ones): in registers they would leave room for one block.
+template <int GC, int NV>
+__global__ void __launch_bounds__(kThreads, 2)
+step_bulk_kernel(const StepArgs a) {
+  extern __shared__ __align__(16) float smem[];
+  __shared__ uint64_t full[kMaxStages];
+  __shared__ __align__(16) float queries[GC][NV * 32];
+  __shared__ int abort_flag_smem;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane & 7, sub = lane >> 3, dim = a.dim;
+  const StepPlace p(a, GC);
+  if (p.idle) return;
+  const int per_stage = a.stage_slots, steps = (p.end - p.begin + per_stage - 1) / per_stage;
+  const int64_t stage_floats = 2ll * per_stage * dim;
+  const auto fetch = [&](int i) {                                // by one thread: K and V of step i
+    const int first = p.begin + i * per_stage, count = min(per_stage, p.end - first);
+    const uint32_t bar = lnn_tc::smem_u32(&full[i % a.stages]), bytes = (uint32_t)(count * dim * 4);
+    const uint32_t dst = lnn_tc::smem_u32(smem + (i % a.stages) * stage_floats);
+    lnn_tc::mbar_expect_tx(bar, 2 * bytes);
+    lnn_tc::bulk_load(dst, a.ck + p.oc + (int64_t)first * dim, bytes, bar);
+    lnn_tc::bulk_load(dst + per_stage * dim * 4, a.cv + p.oc + (int64_t)first * dim, bytes, bar);
+  };
+  if (threadIdx.x == 0) {
+    abort_flag_smem = 0;
+    for (int i = 0; i < a.stages; ++i) lnn_tc::mbar_init(lnn_tc::smem_u32(&full[i]), 1);
+    lnn_tc::fence_barrier_init();
+    for (int i = 0; i < min(a.stages, steps); ++i) fetch(i);
+  }
+  const float factor = a.scale * lnn::kLog2e;
+  for (int i = threadIdx.x; i < GC * NV * 32; i += kThreads) {
+    const int g = i / (NV * 32), c = i % (NV * 32);
+    queries[g][c] = g < p.heads && c < dim ? __fmul_rn(__ldg(a.q + p.oq + g * dim + c), factor) : 0.0f;
+  }
+  __syncthreads();
+  StepSums<GC, NV> t;
+  for (int i = 0; i < steps; ++i) {
+    const int first = p.begin + i * per_stage;
+    float* K = smem + (i % a.stages) * stage_floats;
+    float* V = K + per_stage * dim;
+    bool ok = lnn_tc::mbar_wait(lnn_tc::smem_u32(&full[i % a.stages]), (i / a.stages) & 1, &abort_flag_smem, a.status, 40, i);
+    if (p.fresh >= first && p.fresh < first + per_stage) {        // its place in the cache is being written
+      for (int c = threadIdx.x; c < dim; c += kThreads) {
+        K[(p.fresh - first) * dim + c] = __ldg(a.k + p.okv + c);
+        V[(p.fresh - first) * dim + c] = __ldg(a.v + p.okv + c);
+      }
+      ok = !__syncthreads_or(!ok);
+    }
+    if (ok)
+      for (int at = warp * 4 + sub; at < per_stage; at += 4 * kStepWarps) {
+        const bool in = first + at < p.end;
+        if (!__any_sync(0xffffffffu, in)) break;
+        float4 k[NV], v[NV];
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+          const int c = u * 32 + part * 4;
+          const bool on = in && c < dim;
+          k[u] = on ? *reinterpret_cast<const float4*>(K + at * dim + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          v[u] = on ? *reinterpret_cast<const float4*>(V + at * dim + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        float s[GC];
+#pragma unroll
+        for (int g = 0; g < GC; ++g) {
+          s[g] = 0.0f;
+#pragma unroll
+          for (int u = 0; u < NV; ++u) {
+            const float4 q = *reinterpret_cast<const float4*>(&queries[g][u * 32 + part * 4]);
+            s[g] = fmaf(q.w, k[u].w, fmaf(q.z, k[u].z, fmaf(q.y, k[u].y, fmaf(q.x, k[u].x, s[g]))));
+          }
+        }
+#pragma unroll
+        for (int x = 4; x > 0; x >>= 1)
+#pragma unroll
+          for (int g = 0; g < GC; ++g) s[g] = __fadd_rn(s[g], __shfl_xor_sync(0xffffffffu, s[g], x));
+#pragma unroll
+        for (int g = 0; g < GC; ++g)
+          if (in) t.take(g, s[g], v);
+      }
+    if (__syncthreads_or(!ok)) {
+      // copies that are still on their way must not land in what comes next
+      const long long t0 = clock64();
+      while (clock64() - t0 < lnn_tc::kAbortDelay) { }
+      break;
+    }
+    if (threadIdx.x == 0 && i + a.stages < steps) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (the new row was written by ordinary stores)
+      fetch(i + a.stages);
+    }
+  }
+  __syncthreads();
+  step_append(a, p);
+  step_finish(a, p, t, smem);
 }
 
 template <int GC, int NV>
 int launch_step(lnn::Device* d, StepArgs& a, bool vec) {
-  const int group = a.q_heads / a.kv_heads;
+  const int group = a.q_heads / a.kv_heads, slots = a.window + a.sinks;
   a.group_chunks = (group + GC - 1) / GC;
   const int64_t clusters = (int64_t)a.batch * a.kv_heads * a.group_chunks;
   a.splits = 1;
-  while (a.splits < 8 && clusters * a.splits < 2 * d->sm_count && a.window + a.sinks >= a.splits * 2 * 64) a.splits *= 2;
+  while (a.splits < 8 && clusters * a.splits < 8 * d->sm_count && slots >= a.splits * 2 * 64) a.splits *= 2;
   LNN_REQUIRE((int64_t)a.kv_heads * a.group_chunks < 65536, "too many heads");
+  const size_t join = (size_t)(kStepWarps + 1) * GC * kStepRow<NV> * 4;
+  size_t bytes = join;
+  if (vec) {
+    // stages of about 32 KB, as many as two blocks per SM have room for or the share has slots for
+    const int share = (slots + a.splits - 1) / a.splits;
+    a.stage_slots = 32;
+    while (a.stage_slots * 2 * a.dim * 8 <= 32768 && a.stage_slots < share) a.stage_slots *= 2;
+    const int stage = a.stage_slots * a.dim * 8;
+    a.stages = std::max(1, std::min({kMaxStages, (104 * 1024 - GC * NV * 128) / stage, (share + a.stage_slots - 1) / a.stage_slots}));
+    bytes = std::max(join, (size_t)a.stages * stage);
+    LNN_CUDA(cudaFuncSetAttribute(step_bulk_kernel<GC, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  } else if (bytes > 48 * 1024) {
+    LNN_CUDA(cudaFuncSetAttribute(step_kernel<GC, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.splits, (unsigned)(a.kv_heads * a.group_chunks), (unsigned)a.batch);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)(kThreads / 32 + 1) * GC * (NV * 32 + 2) * 4;
+  cfg.dynamicSmemBytes = bytes;
   cfg.stream = d->stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)a.splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = a.splits > 1 ? 1 : 0;
-  LNN_CUDA(vec ? cudaLaunchKernelEx(&cfg, step_kernel<GC, NV, true>, a) : cudaLaunchKernelEx(&cfg, step_kernel<GC, NV, false>, a));
+  LNN_CUDA(vec ? cudaLaunchKernelEx(&cfg, step_bulk_kernel<GC, NV>, a) : cudaLaunchKernelEx(&cfg, step_kernel<GC, NV>, a));
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
 }
@@ -554,8 +706,10 @@ template <int NV>
 int launch_step(lnn::Device* d, StepArgs& a, bool vec) {
   const int group = a.q_heads / a.kv_heads;
   if (group == 1) return launch_step<1, NV>(d, a, vec);
-  if (group == 2 || NV > 4) return launch_step<2, NV>(d, a, vec);
-  return launch_step<4, NV>(d, a, vec);
+  if constexpr (NV <= 4) {                                       // (four heads of 256 values do not fit the registers)
+    if (group > 2) return launch_step<4, NV>(d, a, vec);
+  }
+  return launch_step<2, NV>(d, a, vec);
 }
 
 const float* in(uint64_t p) { return (const float*)(uintptr_t)p; }
