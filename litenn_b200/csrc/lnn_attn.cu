@@ -389,6 +389,11 @@ struct StepArgs {
 // shares) through distributed shared memory.  The new key and value are read from the arguments while one block writes
 // them into the cache.
 constexpr int kStepWarps = kThreads / 32;
+// A warp has two heads at most (their queries and sums in registers; one of more than 128 values): where a block has
+// more, its warps are teams.
+template <int GC, int NV> constexpr int kStepHeads = GC > 1 && NV <= 4 ? 2 : 1;
+template <int GC, int NV> constexpr int kStepTeams = GC / kStepHeads<GC, NV>;
+template <int GC, int NV> constexpr int kStepKeys = kStepHeads<GC, NV> * NV <= 8 && NV <= 4 ? 2 : 1;      // that a group of lanes takes at a time
 template <int NV> constexpr int kStepRow = NV * 32 + 2;        // values, maximum and sum of a partial result
 
 struct StepPlace {
@@ -421,10 +426,12 @@ struct StepPlace {
   }
 };
 
-// The softmax of a group of eight lanes over the keys it has seen, for GC heads.
+// The softmax of a group of eight lanes over the keys it has seen, for GC heads.  m is no maximum but a score that no other
+// is more than kSlack above: a weight of 2^kSlack costs fp32 nothing, and short streams would move a maximum all the time.
+constexpr float kSlack = 30.0f;
 template <int GC, int NV>
 struct StepSums {
-  float4 o[GC][NV];
+  uint64_t o[GC][2 * NV];                                        // pairs of values
   float m[GC], l[GC];
   __device__ __forceinline__ StepSums() {
 #pragma unroll
@@ -432,39 +439,63 @@ struct StepSums {
       m[g] = -FLT_MAX;
       l[g] = 0.0f;
 #pragma unroll
-      for (int u = 0; u < NV; ++u) o[g][u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int u = 0; u < 2 * NV; ++u) o[g][u] = 0;
     }
   }
-  // the next key's score (the same in all eight lanes) and value
-  __device__ __forceinline__ void take(int g, float s, const float4 (&v)[NV]) {
-    if (s > m[g]) {
-      const float keep = exp2_fast(__fsub_rn(m[g], s));
-      l[g] = __fmul_rn(l[g], keep);
+  // scores s[g][k] (the same in all eight lanes) of KEYS keys, of which the first `real` are there, and their values
+  template <int KEYS>
+  __device__ __forceinline__ void take(const float (&s)[GC][KEYS], int real, const uint64_t (&v)[KEYS][2 * NV]) {
+    bool far = false;
 #pragma unroll
-      for (int u = 0; u < NV; ++u) {
-        o[g][u].x *= keep; o[g][u].y *= keep; o[g][u].z *= keep; o[g][u].w *= keep;
+    for (int g = 0; g < GC; ++g)
+#pragma unroll
+      for (int k = 0; k < KEYS; ++k) far = far || (k < real && s[g][k] > m[g] + kSlack);
+    if (__any_sync(0xffffffffu, far)) {
+#pragma unroll
+      for (int g = 0; g < GC; ++g) {
+        float top = m[g];
+#pragma unroll
+        for (int k = 0; k < KEYS; ++k) top = k < real ? fmaxf(top, s[g][k]) : top;
+        const float keep = exp2_fast(__fsub_rn(m[g], top));
+        const uint64_t keep2 = lnn_tc::pack2(keep, keep);
+        m[g] = top;
+        l[g] = __fmul_rn(l[g], keep);
+#pragma unroll
+        for (int u = 0; u < 2 * NV; ++u) o[g][u] = lnn_tc::mul2(o[g][u], keep2);
       }
-      m[g] = s;
     }
-    const float e = exp2_fast(__fsub_rn(s, m[g]));
-    l[g] = __fadd_rn(l[g], e);
 #pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      o[g][u].x = fmaf(e, v[u].x, o[g][u].x); o[g][u].y = fmaf(e, v[u].y, o[g][u].y);
-      o[g][u].z = fmaf(e, v[u].z, o[g][u].z); o[g][u].w = fmaf(e, v[u].w, o[g][u].w);
-    }
+    for (int g = 0; g < GC; ++g)
+#pragma unroll
+      for (int k = 0; k < KEYS; ++k) {
+        const float e = k < real ? exp2_fast(__fsub_rn(s[g][k], m[g])) : 0.0f;
+        const uint64_t e2 = lnn_tc::pack2(e, e);
+        l[g] = __fadd_rn(l[g], e);
+#pragma unroll
+        for (int u = 0; u < 2 * NV; ++u) o[g][u] = lnn_tc::fma2(e2, v[k][u], o[g][u]);
+      }
   }
 };
-
-// The sums of all threads of the cluster into the output.  smem: (kStepWarps + 1) * GC * kStepRow floats.
-template <int GC, int NV>
-__device__ __forceinline__ void step_finish(const StepArgs& a, const StepPlace& p, StepSums<GC, NV>& t, float* smem) {
-  constexpr int kRow = kStepRow<NV>;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane & 7, sub = lane >> 3;
-  float* mine = smem + warp * GC * kRow;
-  float* block = smem + kStepWarps * GC * kRow;
+// this lane's share of q . k
+template <int NV>
+__device__ __forceinline__ float step_dot(const uint64_t (&q)[2 * NV], const uint64_t (&k)[2 * NV]) {
+  uint64_t s = 0;
 #pragma unroll
-  for (int g = 0; g < GC; ++g) {
+  for (int u = 0; u < 2 * NV; ++u) s = lnn_tc::fma2(q[u], k[u], s);
+  float x, y;
+  lnn_tc::unpack2(s, x, y);
+  return __fadd_rn(x, y);
+}
+
+// The sums of all threads of the cluster into the output.  smem: kStepWarps * kStepHeads + GC rows.
+template <int GC, int NV>
+__device__ __forceinline__ void step_finish(const StepArgs& a, const StepPlace& p, StepSums<kStepHeads<GC, NV>, NV>& t, float* smem) {
+  constexpr int kRow = kStepRow<NV>, TEAMS = kStepTeams<GC, NV>, HEADS = kStepHeads<GC, NV>, WARPS = kStepWarps / TEAMS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane & 7, sub = lane >> 3;
+  float* mine = smem + warp * HEADS * kRow;
+  float* block = smem + kStepWarps * HEADS * kRow;
+#pragma unroll
+  for (int g = 0; g < HEADS; ++g) {
     float top = fmaxf(t.m[g], __shfl_xor_sync(0xffffffffu, t.m[g], 8));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
     const float w = exp2_fast(__fsub_rn(t.m[g], top));
@@ -473,7 +504,9 @@ __device__ __forceinline__ void step_finish(const StepArgs& a, const StepPlace& 
     sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, 16));
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      float x[4] = {t.o[g][u].x, t.o[g][u].y, t.o[g][u].z, t.o[g][u].w};
+      float x[4];
+      lnn_tc::unpack2(t.o[g][2 * u], x[0], x[1]);
+      lnn_tc::unpack2(t.o[g][2 * u + 1], x[2], x[3]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         x[i] = __fmul_rn(x[i], w);
@@ -489,28 +522,28 @@ __device__ __forceinline__ void step_finish(const StepArgs& a, const StepPlace& 
   }
   __syncthreads();
   // column c of `count` partial results: values, or (NV * 32 + 1) the sums; and their maximum
-  const auto join = [&](auto&& from, int count, int g, int c) {
-    float top = from(0)[g * kRow + NV * 32];
-    for (int w = 1; w < count; ++w) top = fmaxf(top, from(w)[g * kRow + NV * 32]);
+  const auto join = [&](auto&& from, int count, int c) {
+    float top = from(0)[NV * 32];
+    for (int w = 1; w < count; ++w) top = fmaxf(top, from(w)[NV * 32]);
     float sum = 0.0f;
-    for (int w = 0; w < count; ++w) sum = fmaf(exp2_fast(__fsub_rn(from(w)[g * kRow + NV * 32], top)), from(w)[g * kRow + c], sum);
+    for (int w = 0; w < count; ++w) sum = fmaf(exp2_fast(__fsub_rn(from(w)[NV * 32], top)), from(w)[c], sum);
     return make_float2(sum, top);
   };
-  const auto of_warp = [&](int w) { return smem + w * GC * kRow; };
   for (int i = threadIdx.x; i < GC * (NV * 32 + 1); i += kThreads) {
     const int g = i / (NV * 32 + 1), c = i % (NV * 32 + 1);
-    const float2 r = join(of_warp, kStepWarps, g, c < NV * 32 ? c : NV * 32 + 1);
+    const auto of_warp = [&](int w) { return smem + ((g / HEADS * WARPS + w) * HEADS + g % HEADS) * kRow; };
+    const float2 r = join(of_warp, WARPS, c < NV * 32 ? c : NV * 32 + 1);
     if (c < NV * 32) block[g * kRow + c] = r.x;
     else { block[g * kRow + NV * 32] = r.y; block[g * kRow + NV * 32 + 1] = r.x; }
   }
   cg::cluster_group cluster = cg::this_cluster();
   if (a.splits > 1) cluster.sync();
   else __syncthreads();
-  const auto of_rank = [&](int r) { return a.splits > 1 ? cluster.map_shared_rank(block, r) : block; };
   for (int i = p.rank * kThreads + threadIdx.x; i < p.heads * a.dim; i += a.splits * kThreads) {
     const int g = i / a.dim, c = i % a.dim;
-    const float sum = join(of_rank, a.splits, g, NV * 32 + 1).x;
-    a.o[p.oq + i] = __fdiv_rn(join(of_rank, a.splits, g, c).x, sum);
+    const auto of_rank = [&](int r) { return (a.splits > 1 ? cluster.map_shared_rank(block, r) : block) + g * kRow; };
+    const float sum = join(of_rank, a.splits, NV * 32 + 1).x;
+    a.o[p.oq + i] = __fdiv_rn(join(of_rank, a.splits, c).x, sum);
   }
   if (a.splits > 1) cluster.sync();                      // nobody leaves while its shared memory is being read
 }
@@ -531,139 +564,152 @@ step_kernel(const StepArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane & 7, sub = lane >> 3, dim = a.dim;
   const StepPlace p(a, GC);
   if (p.idle) return;
-  const auto load = [&](const float* row, int u) {
-    const int c = u * 32 + part * 4;
-    return make_float4(c < dim ? __ldg(row + c) : 0.0f, c + 1 < dim ? __ldg(row + c + 1) : 0.0f,
-                       c + 2 < dim ? __ldg(row + c + 2) : 0.0f, c + 3 < dim ? __ldg(row + c + 3) : 0.0f);
+  const auto load = [&](const float* row, uint64_t (&x)[2 * NV], float times) {
+#pragma unroll
+    for (int u = 0; u < 2 * NV; ++u) {
+      const int c = u / 2 * 32 + part * 4 + u % 2 * 2;
+      x[u] = lnn_tc::pack2(c < dim ? __fmul_rn(__ldg(row + c), times) : 0.0f, c + 1 < dim ? __fmul_rn(__ldg(row + c + 1), times) : 0.0f);
+    }
   };
-  const float factor = a.scale * lnn::kLog2e;
-  float4 q[GC][NV];
+  constexpr int HEADS = kStepHeads<GC, NV>, WARPS = kStepWarps / kStepTeams<GC, NV>;
+  const int team = warp / WARPS, turn = warp % WARPS;
+  uint64_t q[HEADS][2 * NV];
 #pragma unroll
-  for (int g = 0; g < GC; ++g)
+  for (int g = 0; g < HEADS; ++g) load(a.q + p.oq + min(team * HEADS + g, p.heads - 1) * dim, q[g], a.scale * lnn::kLog2e);
+  StepSums<HEADS, NV> t;
+  for (int s0 = p.begin; s0 < p.end; s0 += 4 * WARPS) {
+    const int slot = s0 + turn * 4 + sub, from = min(slot, p.end - 1);
+    uint64_t k[2 * NV], v[1][2 * NV];
+    load(from == p.fresh ? a.k + p.okv : a.ck + p.oc + (int64_t)from * dim, k, 1.0f);
+    load(from == p.fresh ? a.v + p.okv : a.cv + p.oc + (int64_t)from * dim, v[0], 1.0f);
+    float s[HEADS][1];
 #pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      q[g][u] = g < p.heads ? load(a.q + p.oq + g * dim, u) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      q[g][u].x *= factor; q[g][u].y *= factor; q[g][u].z *= factor; q[g][u].w *= factor;
+    for (int g = 0; g < HEADS; ++g) {
+      s[g][0] = step_dot<NV>(q[g], k);
+#pragma unroll
+      for (int x = 4; x > 0; x >>= 1) s[g][0] = __fadd_rn(s[g][0], __shfl_xor_sync(0xffffffffu, s[g][0], x));
     }
-  StepSums<GC, NV> t;
-  for (int s0 = p.begin; s0 < p.end; s0 += 4 * kStepWarps) {
-    const int slot = s0 + warp * 4 + sub;
-    const bool in = slot < p.end;
-    const float* krow = slot == p.fresh ? a.k + p.okv : a.ck + p.oc + (int64_t)slot * dim;
-    const float* vrow = slot == p.fresh ? a.v + p.okv : a.cv + p.oc + (int64_t)slot * dim;
-    float4 k[NV], v[NV];
-#pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      k[u] = in ? load(krow, u) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      v[u] = in ? load(vrow, u) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
-#pragma unroll
-    for (int g = 0; g < GC; ++g) {
-      float s = 0.0f;
-#pragma unroll
-      for (int u = 0; u < NV; ++u)
-        s = fmaf(q[g][u].w, k[u].w, fmaf(q[g][u].z, k[u].z, fmaf(q[g][u].y, k[u].y, fmaf(q[g][u].x, k[u].x, s))));
-#pragma unroll
-      for (int x = 4; x > 0; x >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, x));
-      if (in) t.take(g, s, v);
-    }
+    t.template take<1>(s, slot < p.end ? 1 : 0, v);
   }
   step_append(a, p);
-  step_finish(a, p, t, smem);
+  step_finish<GC, NV>(a, p, t, smem);
 }
 
 // Rows of 16-byte units: the slots of a share are one piece of memory, which bulk copies bring into a ring of stages in
-// shared memory; two blocks per SM have up to 192 KB on the way.  The queries are in shared memory too (eight lanes
-// read 128 bytes, the other groups the same ones): in registers they would leave room for one block.
-template <int GC, int NV>
+// shared memory; two blocks per SM have up to 192 KB on the way.  FULL: dim = 32 NV.
+template <int GC, int NV, bool FULL>
 __global__ void __launch_bounds__(kThreads, 2)
 step_bulk_kernel(const StepArgs a) {
   extern __shared__ __align__(16) float smem[];
-  __shared__ uint64_t full[kMaxStages];
-  __shared__ __align__(16) float queries[GC][NV * 32];
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages];
   __shared__ int abort_flag_smem;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane & 7, sub = lane >> 3, dim = a.dim;
+  constexpr int HEADS = kStepHeads<GC, NV>, WARPS = kStepWarps / kStepTeams<GC, NV>, KEYS = kStepKeys<GC, NV>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane & 7, sub = lane >> 3;
+  const int team = warp / WARPS, turn = warp % WARPS, dim = FULL ? NV * 32 : a.dim;
   const StepPlace p(a, GC);
   if (p.idle) return;
   const int per_stage = a.stage_slots, steps = (p.end - p.begin + per_stage - 1) / per_stage;
-  const int64_t stage_floats = 2ll * per_stage * dim;
-  const auto fetch = [&](int i) {                                // by one thread: K and V of step i
+  const int stage_floats = 2 * per_stage * dim;
+  const auto fetch = [&](int i, int stage) {                     // by one thread: K and V of step i
     const int first = p.begin + i * per_stage, count = min(per_stage, p.end - first);
-    const uint32_t bar = lnn_tc::smem_u32(&full[i % a.stages]), bytes = (uint32_t)(count * dim * 4);
-    const uint32_t dst = lnn_tc::smem_u32(smem + (i % a.stages) * stage_floats);
+    const uint32_t bar = lnn_tc::smem_u32(&full[stage]), bytes = (uint32_t)(count * dim * 4);
+    const uint32_t dst = lnn_tc::smem_u32(smem + stage * stage_floats);
     lnn_tc::mbar_expect_tx(bar, 2 * bytes);
     lnn_tc::bulk_load(dst, a.ck + p.oc + (int64_t)first * dim, bytes, bar);
     lnn_tc::bulk_load(dst + per_stage * dim * 4, a.cv + p.oc + (int64_t)first * dim, bytes, bar);
   };
   if (threadIdx.x == 0) {
     abort_flag_smem = 0;
-    for (int i = 0; i < a.stages; ++i) lnn_tc::mbar_init(lnn_tc::smem_u32(&full[i]), 1);
+    for (int i = 0; i < a.stages; ++i) {
+      lnn_tc::mbar_init(lnn_tc::smem_u32(&full[i]), 1);
+      lnn_tc::mbar_init(lnn_tc::smem_u32(&empty[i]), kStepWarps);
+    }
     lnn_tc::fence_barrier_init();
-    for (int i = 0; i < min(a.stages, steps); ++i) fetch(i);
+    for (int i = 0; i < min(a.stages, steps); ++i) fetch(i, i);
   }
   const float factor = a.scale * lnn::kLog2e;
-  for (int i = threadIdx.x; i < GC * NV * 32; i += kThreads) {
-    const int g = i / (NV * 32), c = i % (NV * 32);
-    queries[g][c] = g < p.heads && c < dim ? __fmul_rn(__ldg(a.q + p.oq + g * dim + c), factor) : 0.0f;
+  uint64_t q[HEADS][2 * NV];
+#pragma unroll
+  for (int g = 0; g < HEADS; ++g) {
+    const float* from = a.q + p.oq + min(team * HEADS + g, p.heads - 1) * dim + part * 4;      // (a head too many is not stored)
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const float4 v = FULL || u * 32 + part * 4 < dim ? __ldg(reinterpret_cast<const float4*>(from + u * 32)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      q[g][2 * u] = lnn_tc::pack2(v.x * factor, v.y * factor);
+      q[g][2 * u + 1] = lnn_tc::pack2(v.z * factor, v.w * factor);
+    }
   }
   __syncthreads();
-  StepSums<GC, NV> t;
+  StepSums<HEADS, NV> t;
+  bool ok = true;
+  int stage = 0, before = 0;
+  uint32_t phase = 0, phase_before = 0;
   for (int i = 0; i < steps; ++i) {
-    const int first = p.begin + i * per_stage;
-    float* K = smem + (i % a.stages) * stage_floats;
-    float* V = K + per_stage * dim;
-    bool ok = lnn_tc::mbar_wait(lnn_tc::smem_u32(&full[i % a.stages]), (i / a.stages) & 1, &abort_flag_smem, a.status, 40, i);
-    if (p.fresh >= first && p.fresh < first + per_stage) {        // its place in the cache is being written
-      for (int c = threadIdx.x; c < dim; c += kThreads) {
-        K[(p.fresh - first) * dim + c] = __ldg(a.k + p.okv + c);
-        V[(p.fresh - first) * dim + c] = __ldg(a.v + p.okv + c);
+    const int first = p.begin + i * per_stage, count = min(per_stage, p.end - first), fresh = p.fresh - first;
+    if (warp == 0 && i > 0 && i - 1 + a.stages < steps) {         // the stage before this one is filled again
+      ok = lnn_tc::mbar_wait(lnn_tc::smem_u32(&empty[before]), phase_before, &abort_flag_smem, a.status, 41, i);
+      if (ok && lane == 0) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (a new row was written by ordinary stores)
+        fetch(i - 1 + a.stages, before);
       }
-      ok = !__syncthreads_or(!ok);
     }
-    if (ok)
-      for (int at = warp * 4 + sub; at < per_stage; at += 4 * kStepWarps) {
-        const bool in = first + at < p.end;
-        if (!__any_sync(0xffffffffu, in)) break;
-        float4 k[NV], v[NV];
-#pragma unroll
-        for (int u = 0; u < NV; ++u) {
-          const int c = u * 32 + part * 4;
-          const bool on = in && c < dim;
-          k[u] = on ? *reinterpret_cast<const float4*>(K + at * dim + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          v[u] = on ? *reinterpret_cast<const float4*>(V + at * dim + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float* K = smem + stage * stage_floats;
+    float* V = K + per_stage * dim;
+    ok = ok && lnn_tc::mbar_wait(lnn_tc::smem_u32(&full[stage]), phase, &abort_flag_smem, a.status, 40, i);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) break;
+    // KEYS keys of a group at a time, 4 apart: the warps of a team take pieces of 4 KEYS slots
+    for (int base = turn * 4 * KEYS; base < count; base += 4 * KEYS * WARPS) {
+      const int at = base + sub, real = KEYS == 2 && at + 4 < count ? 2 : (at < count ? 1 : 0);
+      if (fresh >= base && fresh < base + 4 * KEYS) {             // the row's place in the cache is being written
+        for (int c = lane; c < dim; c += 32) {
+          K[fresh * dim + c] = __ldg(a.k + p.okv + c);           // (each team writes it: the same values)
+          V[fresh * dim + c] = __ldg(a.v + p.okv + c);
         }
-        float s[GC];
+        __syncwarp();
+      }
+      // (what is not there is read from the last slot that is, and has no weight)
+      uint64_t x[KEYS][2 * NV];
+      const auto load = [&](const float* rows) {
 #pragma unroll
-        for (int g = 0; g < GC; ++g) {
-          s[g] = 0.0f;
+        for (int k = 0; k < KEYS; ++k) {
+          const float* r = rows + min(at + 4 * k, count - 1) * dim + part * 4;
 #pragma unroll
           for (int u = 0; u < NV; ++u) {
-            const float4 q = *reinterpret_cast<const float4*>(&queries[g][u * 32 + part * 4]);
-            s[g] = fmaf(q.w, k[u].w, fmaf(q.z, k[u].z, fmaf(q.y, k[u].y, fmaf(q.x, k[u].x, s[g]))));
+            const ulonglong2 v = FULL || u * 32 + part * 4 < dim ? *reinterpret_cast<const ulonglong2*>(r + u * 32) : make_ulonglong2(0, 0);
+            x[k][2 * u] = v.x; x[k][2 * u + 1] = v.y;
           }
         }
+      };
+      load(K);
+      float s[HEADS][KEYS];
 #pragma unroll
-        for (int x = 4; x > 0; x >>= 1)
+      for (int g = 0; g < HEADS; ++g)
 #pragma unroll
-          for (int g = 0; g < GC; ++g) s[g] = __fadd_rn(s[g], __shfl_xor_sync(0xffffffffu, s[g], x));
+        for (int k = 0; k < KEYS; ++k) s[g][k] = step_dot<NV>(q[g], x[k]);
+      load(V);
 #pragma unroll
-        for (int g = 0; g < GC; ++g)
-          if (in) t.take(g, s[g], v);
-      }
-    if (__syncthreads_or(!ok)) {
-      // copies that are still on their way must not land in what comes next
-      const long long t0 = clock64();
-      while (clock64() - t0 < lnn_tc::kAbortDelay) { }
-      break;
+      for (int y = 4; y > 0; y >>= 1)
+#pragma unroll
+        for (int g = 0; g < HEADS; ++g)
+#pragma unroll
+          for (int k = 0; k < KEYS; ++k) s[g][k] = __fadd_rn(s[g][k], __shfl_xor_sync(0xffffffffu, s[g][k], y));
+      t.template take<KEYS>(s, real, x);
     }
-    if (threadIdx.x == 0 && i + a.stages < steps) {
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (the new row was written by ordinary stores)
-      fetch(i + a.stages);
-    }
+    __syncwarp();
+    if (lane == 0) lnn_tc::mbar_arrive(lnn_tc::smem_u32(&empty[stage]));
+    before = stage;
+    phase_before = phase;
+    if (++stage == a.stages) { stage = 0; phase ^= 1u; }
+  }
+  if (__syncthreads_or(!ok)) {
+    // copies that are still on their way must not land in what comes next
+    const long long t0 = clock64();
+    while (clock64() - t0 < lnn_tc::kAbortDelay) { }
   }
   __syncthreads();
   step_append(a, p);
-  step_finish(a, p, t, smem);
+  step_finish<GC, NV>(a, p, t, smem);
 }
 
 template <int GC, int NV>
@@ -672,22 +718,22 @@ int launch_step(lnn::Device* d, StepArgs& a, bool vec) {
   a.group_chunks = (group + GC - 1) / GC;
   const int64_t clusters = (int64_t)a.batch * a.kv_heads * a.group_chunks;
   a.splits = 1;
-  while (a.splits < 8 && clusters * a.splits < 8 * d->sm_count && slots >= a.splits * 2 * 64) a.splits *= 2;
+  while (a.splits < 8 && clusters * a.splits < 2 * d->sm_count && slots >= a.splits * 2 * 64) a.splits *= 2;
   LNN_REQUIRE((int64_t)a.kv_heads * a.group_chunks < 65536, "too many heads");
-  const size_t join = (size_t)(kStepWarps + 1) * GC * kStepRow<NV> * 4;
+  const size_t join = (size_t)(kStepWarps * kStepHeads<GC, NV> + GC) * kStepRow<NV> * 4;
   size_t bytes = join;
+  void (*kernel)(const StepArgs) = step_kernel<GC, NV>;
   if (vec) {
-    // stages of about 32 KB, as many as two blocks per SM have room for or the share has slots for
+    // stages of 32 KB or less, a turn of a team's warps at least, as many as two blocks per SM have room for or the share has slots for
     const int share = (slots + a.splits - 1) / a.splits;
-    a.stage_slots = 32;
+    a.stage_slots = 4 * kStepKeys<GC, NV> * kStepWarps / kStepTeams<GC, NV>;
     while (a.stage_slots * 2 * a.dim * 8 <= 32768 && a.stage_slots < share) a.stage_slots *= 2;
     const int stage = a.stage_slots * a.dim * 8;
-    a.stages = std::max(1, std::min({kMaxStages, (104 * 1024 - GC * NV * 128) / stage, (share + a.stage_slots - 1) / a.stage_slots}));
+    a.stages = std::max(1, std::min({kMaxStages, 104 * 1024 / stage, (share + a.stage_slots - 1) / a.stage_slots}));
     bytes = std::max(join, (size_t)a.stages * stage);
-    LNN_CUDA(cudaFuncSetAttribute(step_bulk_kernel<GC, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  } else if (bytes > 48 * 1024) {
-    LNN_CUDA(cudaFuncSetAttribute(step_kernel<GC, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    kernel = a.dim == NV * 32 ? step_bulk_kernel<GC, NV, true> : step_bulk_kernel<GC, NV, false>;
   }
+  if (bytes > 48 * 1024) LNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.splits, (unsigned)(a.kv_heads * a.group_chunks), (unsigned)a.batch);
   cfg.blockDim = dim3(kThreads);
@@ -698,7 +744,7 @@ int launch_step(lnn::Device* d, StepArgs& a, bool vec) {
   attr[0].val.clusterDim.x = (unsigned)a.splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = a.splits > 1 ? 1 : 0;
-  LNN_CUDA(vec ? cudaLaunchKernelEx(&cfg, step_bulk_kernel<GC, NV>, a) : cudaLaunchKernelEx(&cfg, step_kernel<GC, NV>, a));
+  LNN_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
 }
@@ -706,10 +752,8 @@ template <int NV>
 int launch_step(lnn::Device* d, StepArgs& a, bool vec) {
   const int group = a.q_heads / a.kv_heads;
   if (group == 1) return launch_step<1, NV>(d, a, vec);
-  if constexpr (NV <= 4) {                                       // (four heads of 256 values do not fit the registers)
-    if (group > 2) return launch_step<4, NV>(d, a, vec);
-  }
-  return launch_step<2, NV>(d, a, vec);
+  if (group == 2) return launch_step<2, NV>(d, a, vec);
+  return launch_step<4, NV>(d, a, vec);
 }
 
 const float* in(uint64_t p) { return (const float*)(uintptr_t)p; }
