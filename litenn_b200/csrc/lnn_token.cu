@@ -62,65 +62,111 @@ embedding_fwd_kernel(T* __restrict__ Y, const T* __restrict__ table, const float
 // of the tokens whatever the launch looks like: no atomics on values.
 constexpr int kSortWarps = kThreads / 32;
 constexpr int kMaxSortBlocks = 64;
+constexpr int kSortKeys = 4;                       // per lane at a time
 
-struct SortSpan { int64_t begin, end; };
-// the share of a block, cut into one contiguous strip per warp
-__device__ __forceinline__ SortSpan sort_strip(int64_t n) {
-  const int64_t per = ((n + gridDim.x - 1) / gridDim.x + kThreads - 1) / kThreads * 32;      // tokens per warp
-  const int64_t begin = ((int64_t)blockIdx.x * kSortWarps + (threadIdx.x >> 5)) * per;
-  return {min(begin, n), min(begin + per, n)};
+// Sorting is a chain of short dependent steps; rows without tokens have to become zero.  Blocks behind the first
+// `sort_blocks` of every launch write a share of the zeros meanwhile.
+struct SortArgs {
+  const float* ids;                                // the first pass reads these, the later ones keys and at
+  const uint32_t *keys, *at;
+  uint32_t *out_keys, *out_at, *hist;              // hist [sort_blocks][256]
+  int64_t n;
+  int vocab, shift, sort_blocks;
+  float4* zeros;                                   // [zero_begin, zero_end) of the table in 16-byte units, and its odd floats
+  int64_t zero_begin, zero_end;
+  float* odd;
+  int odds;
+  int* status;
+};
+__device__ __forceinline__ void write_zeros(const SortArgs& a) {
+  const int64_t stride = (int64_t)(gridDim.x - a.sort_blocks) * kThreads;
+  const int64_t first = (int64_t)(blockIdx.x - a.sort_blocks) * kThreads + threadIdx.x;
+  for (int64_t i = a.zero_begin + first; i < a.zero_end; i += stride) a.zeros[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (first < a.odds) a.odd[first] = 0.0f;
 }
-__device__ __forceinline__ uint32_t sort_key(const float* ids, const uint32_t* keys, int64_t i, int vocab, int* status) {
-  if (keys) return keys[i];
-  const int row = token_row(ids[i], vocab, i, 2, status);
-  return row < 0 ? (uint32_t)vocab : (uint32_t)row;           // padding comes last
+
+// The share of a block, cut into one contiguous strip per warp, which takes kSortKeys * 32 tokens of it at a time.
+struct SortStrip {
+  int64_t begin, end;
+  __device__ __forceinline__ explicit SortStrip(const SortArgs& a) {
+    const int64_t per = ((a.n + a.sort_blocks - 1) / a.sort_blocks + kThreads - 1) / kThreads * 32;      // tokens per warp
+    begin = min(((int64_t)blockIdx.x * kSortWarps + (threadIdx.x >> 5)) * per, a.n);
+    end = min(begin + per, a.n);
+  }
+};
+constexpr uint32_t kNoKey = 0xffffffffu;
+__device__ __forceinline__ void load_keys(const SortArgs& a, int64_t i0, int64_t end, uint32_t (&key)[kSortKeys]) {
+#pragma unroll
+  for (int u = 0; u < kSortKeys; ++u) {
+    const int64_t i = i0 + u * 32 + (threadIdx.x & 31);
+    key[u] = kNoKey;
+    if (i < end) {
+      if (a.keys) {
+        key[u] = __ldg(a.keys + i);
+      } else {
+        const int row = token_row(__ldg(a.ids + i), a.vocab, i, 2, a.status);
+        key[u] = row < 0 ? (uint32_t)a.vocab : (uint32_t)row;    // padding comes last
+      }
+    }
+  }
 }
-// counts of the digits of a warp's strip in its line of `count`
-__device__ __forceinline__ void count_digits(uint32_t* count, const float* ids, const uint32_t* keys, SortSpan s,
-                                             int vocab, int shift, int* status) {
-  const int lane = threadIdx.x & 31;
-  for (int64_t i0 = s.begin; i0 < s.end; i0 += 32) {
-    const bool in = i0 + lane < s.end;
-    const uint32_t digit = in ? (sort_key(ids, keys, i0 + lane, vocab, status) >> shift) & 255u : 256u;
+__device__ __forceinline__ uint32_t digit_of(uint32_t key, int shift) { return key == kNoKey ? 256u : (key >> shift) & 255u; }
+__device__ __forceinline__ void count_digits(uint32_t* count, const uint32_t (&key)[kSortKeys], int shift) {
+#pragma unroll
+  for (int u = 0; u < kSortKeys; ++u) {
+    const uint32_t digit = digit_of(key[u], shift);
     const uint32_t same = __match_any_sync(0xffffffffu, digit);
-    if (in && lane == __ffs(same) - 1) count[digit] += __popc(same);
+    if (digit < 256u && (threadIdx.x & 31) == __ffs(same) - 1) count[digit] += __popc(same);
     __syncwarp();
   }
 }
 
 __global__ void __launch_bounds__(kThreads)
-sort_count_kernel(uint32_t* __restrict__ hist, const float* __restrict__ ids, const uint32_t* __restrict__ keys, int64_t n,
-                  int vocab, int shift, int* status) {
+sort_count_kernel(const __grid_constant__ SortArgs a) {
   __shared__ uint32_t count[kSortWarps][256];
+  if ((int)blockIdx.x >= a.sort_blocks) { write_zeros(a); return; }
   for (int i = threadIdx.x; i < kSortWarps * 256; i += kThreads) (&count[0][0])[i] = 0;
+  const SortStrip s(a);
+  uint32_t key[kSortKeys];
+  load_keys(a, s.begin, s.end, key);
   __syncthreads();
-  count_digits(count[threadIdx.x >> 5], ids, keys, sort_strip(n), vocab, shift, status);
+  for (int64_t i0 = s.begin; i0 < s.end; i0 += kSortKeys * 32) {
+    if (i0 > s.begin) load_keys(a, i0, s.end, key);
+    count_digits(count[threadIdx.x >> 5], key, a.shift);
+  }
   __syncthreads();
   uint32_t total = 0;
+#pragma unroll
   for (int w = 0; w < kSortWarps; ++w) total += count[w][threadIdx.x];
-  hist[blockIdx.x * 256 + threadIdx.x] = total;
+  a.hist[blockIdx.x * 256 + threadIdx.x] = total;
 }
 
 __global__ void __launch_bounds__(kThreads)
-sort_scatter_kernel(uint32_t* __restrict__ out_keys, uint32_t* __restrict__ out_at, const uint32_t* __restrict__ hist,
-                    const float* __restrict__ ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ at,
-                    int64_t n, int vocab, int shift, int* status) {
+sort_scatter_kernel(const __grid_constant__ SortArgs a) {
   __shared__ uint32_t count[kSortWarps][256];
   __shared__ uint32_t warp_total[kSortWarps];
+  if ((int)blockIdx.x >= a.sort_blocks) { write_zeros(a); return; }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int i = threadIdx.x; i < kSortWarps * 256; i += kThreads) (&count[0][0])[i] = 0;
-  __syncthreads();
-  const SortSpan s = sort_strip(n);
-  count_digits(count[warp], ids, keys, s, vocab, shift, status);
-  __syncthreads();
+  const SortStrip s(a);
+  const bool once = s.end - s.begin <= kSortKeys * 32;           // the strip's keys stay in registers
+  uint32_t key[kSortKeys];
+  load_keys(a, s.begin, s.end, key);
   // where this block's tokens of digit threadIdx.x begin: all smaller digits, then the blocks before this one
   uint32_t before = 0, total = 0;
-  for (unsigned b = 0; b < gridDim.x; ++b) {
-    const uint32_t c = hist[b * 256 + threadIdx.x];
-    if (b < blockIdx.x) before += c;
+#pragma unroll 16
+  for (int b = 0; b < a.sort_blocks; ++b) {
+    const uint32_t c = __ldg(a.hist + b * 256 + threadIdx.x);
+    if (b < (int)blockIdx.x) before += c;
     total += c;
   }
+  __syncthreads();
+  for (int64_t i0 = s.begin; i0 < s.end; i0 += kSortKeys * 32) {
+    if (i0 > s.begin) load_keys(a, i0, s.end, key);
+    count_digits(count[warp], key, a.shift);
+  }
   uint32_t scan = total;
+#pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const uint32_t v = __shfl_up_sync(0xffffffffu, scan, o);
     if (lane >= o) scan += v;
@@ -129,27 +175,30 @@ sort_scatter_kernel(uint32_t* __restrict__ out_keys, uint32_t* __restrict__ out_
   __syncthreads();
   for (int w = 0; w < warp; ++w) scan += warp_total[w];
   uint32_t base = scan - total + before;
+#pragma unroll
   for (int w = 0; w < kSortWarps; ++w) {
     const uint32_t c = count[w][threadIdx.x];
     count[w][threadIdx.x] = base;
     base += c;
   }
   __syncthreads();
-  for (int64_t i0 = s.begin; i0 < s.end; i0 += 32) {
-    const int64_t i = i0 + lane;
-    const bool in = i < s.end;
-    const uint32_t key = in ? sort_key(ids, keys, i, vocab, status) : 0u;
-    const uint32_t digit = in ? (key >> shift) & 255u : 256u;
-    const uint32_t same = __match_any_sync(0xffffffffu, digit);
-    uint32_t to = 0;
-    if (in) to = count[warp][digit] + __popc(same & ((1u << lane) - 1u));
-    __syncwarp();
-    if (in) {
-      if (lane == __ffs(same) - 1) count[warp][digit] += __popc(same);
-      out_keys[to] = key;
-      out_at[to] = at ? at[i] : (uint32_t)i;
+  for (int64_t i0 = s.begin; i0 < s.end; i0 += kSortKeys * 32) {
+    if (!once) load_keys(a, i0, s.end, key);
+#pragma unroll
+    for (int u = 0; u < kSortKeys; ++u) {
+      const int64_t i = i0 + u * 32 + lane;
+      const uint32_t digit = digit_of(key[u], a.shift);
+      const uint32_t same = __match_any_sync(0xffffffffu, digit);
+      uint32_t to = 0;
+      if (digit < 256u) to = count[warp][digit] + __popc(same & ((1u << lane) - 1u));
+      __syncwarp();
+      if (digit < 256u) {
+        if (lane == __ffs(same) - 1) count[warp][digit] += __popc(same);
+        a.out_keys[to] = key[u];
+        a.out_at[to] = a.at ? __ldg(a.at + i) : (uint32_t)i;
+      }
+      __syncwarp();
     }
-    __syncwarp();
   }
 }
 
@@ -221,11 +270,16 @@ table_join_kernel(T* __restrict__ dtable, const uint32_t* __restrict__ keys, con
   const uint32_t row = keys[hi - 1];
   if (row >= (uint32_t)vocab || keys[hi] != row) return;                    // nothing goes on behind this piece
   if (keys[lo] == row && lo > 0 && keys[lo - 1] == row) return;             // it began earlier
-  int64_t last = piece + 1;                                                 // the last piece that has some of the row
-  while ((last + 1) * kPiece < tokens && keys[(last + 1) * kPiece] == row) ++last;
+  // the last piece that has some of the row: it begins with it (steps that double, then halve)
+  const auto begins = [&](int64_t p) { return p < pieces && __ldg(keys + p * kPiece) == row; };
+  int64_t last = piece + 1, step = 1;
+  while (begins(last + step)) { last += step; step *= 2; }
+  for (; step > 0; step >>= 1)
+    if (begins(last + step)) last += step;
   for (int64_t c = threadIdx.x + (int64_t)blockIdx.y * blockDim.x; c < units; c += (int64_t)gridDim.y * blockDim.x) {
     T sum = tail[piece * units + c];
-    for (int64_t p = piece + 1; p <= last; ++p) sum = plus(sum, head[p * units + c]);
+#pragma unroll 8
+    for (int64_t p = piece + 1; p <= last; ++p) sum = plus(sum, __ldg(head + p * units + c));
     T* o = dtable + row * units + c;
     *o = accumulate ? plus(*o, scaled(sum, scale)) : scaled(sum, scale);
   }
@@ -245,27 +299,50 @@ bool aligned16(const void* a, const void* b, int64_t cols) {
 template <class T>
 int embedding_bwd(lnn::Device* d, T* dtable, const T* dy, const float* ids, int64_t tokens, int vocab, int64_t units,
                   float scale, int accumulate) {
-  if (!accumulate) LNN_CUDA(cudaMemsetAsync(dtable, 0, (size_t)vocab * units * sizeof(T), d->stream));
   const int64_t pieces = lnn_ceil_div(tokens, kPiece);
   lnn::Scratch keys(d), parts(d);
-  const int blocks = (int)std::min<int64_t>(kMaxSortBlocks, lnn_ceil_div(tokens, 4 * kThreads));
+  SortArgs a = {};
+  a.sort_blocks = (int)std::min<int64_t>(kMaxSortBlocks, lnn_ceil_div(tokens, kSortKeys * kThreads));
   const int64_t pad = (tokens + 3) / 4 * 4;
-  int rc = keys.get((uint64_t)(4 * pad + blocks * 256) * 4);
+  int rc = keys.get((uint64_t)(4 * pad + a.sort_blocks * 256) * 4);
   if (!rc) rc = parts.get((uint64_t)pieces * units * sizeof(T) * 2);
   if (rc) return rc;
   uint32_t* buf = keys.as<uint32_t>();
-  uint32_t *k[2] = {buf, buf + pad}, *at[2] = {buf + 2 * pad, buf + 3 * pad}, *hist = buf + 4 * pad;
-  const uint32_t *src_k = nullptr, *src_at = nullptr;
-  int to = 0;
-  for (int shift = 0; shift == 0 || (vocab >> shift) != 0; shift += 8) {       // (keys go up to vocab)
-    sort_count_kernel<<<blocks, kThreads, 0, d->stream>>>(hist, ids, src_k, tokens, vocab, shift, d->status_dev);
+  uint32_t *k[2] = {buf, buf + pad}, *at[2] = {buf + 2 * pad, buf + 3 * pad};
+  a.hist = buf + 4 * pad;
+  a.ids = ids; a.n = tokens; a.vocab = vocab; a.status = d->status_dev;
+  int passes = 1;
+  while ((vocab >> (8 * passes)) != 0) ++passes;                 // (keys go up to vocab)
+  // the zeros, a share with each launch
+  const int64_t floats = accumulate ? 0 : (int64_t)vocab * units * (int64_t)(sizeof(T) / 4);
+  float* table = reinterpret_cast<float*>(dtable);
+  const int64_t lead = std::min<int64_t>((4 - (((uintptr_t)table >> 2) & 3)) & 3, floats), quads = (floats - lead) / 4;
+  a.zeros = reinterpret_cast<float4*>(table + lead);
+  const int64_t fill_blocks = std::min<int64_t>((int64_t)d->sm_count * 4, lnn_ceil_div(quads, 2 * passes * kThreads * 4));
+  int launch = 0;
+  const auto next = [&]() {                                      // a share of the zeros for the next launch; its grid
+    a.zero_begin = quads * launch / (2 * passes);
+    a.zero_end = quads * (launch + 1) / (2 * passes);
+    a.odds = 0;
+    if (launch == 0) { a.odd = table; a.odds = (int)lead; }
+    if (launch == 1) { a.odd = table + lead + quads * 4; a.odds = (int)(floats - lead - quads * 4); }
+    ++launch;
+    return (unsigned)(a.sort_blocks + std::max<int64_t>(fill_blocks, a.odds > 0));
+  };
+  for (int pass = 0; pass < passes; ++pass) {
+    a.shift = 8 * pass;
+    a.keys = pass ? k[(pass - 1) & 1] : nullptr;
+    a.at = pass ? at[(pass - 1) & 1] : nullptr;
+    a.out_keys = k[pass & 1];
+    a.out_at = at[pass & 1];
+    unsigned blocks = next();
+    sort_count_kernel<<<blocks, kThreads, 0, d->stream>>>(a);
     LNN_CHECK_LAUNCH(d);
-    sort_scatter_kernel<<<blocks, kThreads, 0, d->stream>>>(k[to], at[to], hist, ids, src_k, src_at, tokens, vocab, shift,
-                                                            d->status_dev);
+    blocks = next();
+    sort_scatter_kernel<<<blocks, kThreads, 0, d->stream>>>(a);
     LNN_CHECK_LAUNCH(d);
-    src_k = k[to]; src_at = at[to];
-    to ^= 1;
   }
+  const uint32_t *src_k = a.out_keys, *src_at = a.out_at;
   const dim3 block = row_block(units);
   const dim3 grid((unsigned)lnn_ceil_div(pieces, block.y), (unsigned)std::min<int64_t>(lnn_ceil_div(units, block.x), 64));
   T *head = parts.as<T>(), *tail = head + pieces * units;
@@ -303,6 +380,7 @@ struct PolicyArgs {
   float low, high, kl;
 };
 
+constexpr int kLogitQuads = 4;                      // loads of a thread at a time
 // out[row] = log p(id) or the policy loss; stats[row] = {max, 1 / sum, d out / d log p}
 __global__ void __launch_bounds__(kThreads)
 token_logit_kernel(float* __restrict__ out, float* __restrict__ stats, const float* __restrict__ logits,
@@ -325,9 +403,16 @@ token_logit_kernel(float* __restrict__ out, float* __restrict__ stats, const flo
   const int64_t quads = (vocab - lead) >> 2;
   const float4* z4 = reinterpret_cast<const float4*>(z + lead);
   const int64_t begin = quads * rank / splits, end = quads * (rank + 1) / splits;
-  for (int64_t i = begin + threadIdx.x; i < end; i += kThreads) {
-    const float4 v = __ldg(z4 + i);
-    take(t, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), v.x, v.y, v.z, v.w);
+  for (int64_t i = begin + threadIdx.x; i < end; i += kThreads * kLogitQuads) {
+    float4 v[kLogitQuads];
+#pragma unroll
+    for (int u = 0; u < kLogitQuads; ++u)
+      v[u] = i + u * kThreads < end ? __ldg(z4 + i + u * kThreads) : make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
+    float top = -CUDART_INF_F;
+#pragma unroll
+    for (int u = 0; u < kLogitQuads; ++u) top = fmaxf(top, fmaxf(fmaxf(v[u].x, v[u].y), fmaxf(v[u].z, v[u].w)));
+#pragma unroll
+    for (int u = 0; u < kLogitQuads; ++u) take(t, top, v[u].x, v[u].y, v[u].z, v[u].w);
   }
   if (rank == 0 && threadIdx.x < 8) {                         // up to three values in front, up to three behind
     const int64_t j = threadIdx.x < 4 ? (int64_t)threadIdx.x : lead + (quads << 2) + threadIdx.x - 4;

@@ -6,7 +6,7 @@ one C-ABI call per current device does the work.  Token numbers and lengths are 
 exact up to 2^24.  A token below zero marks a padded place.  A number that is no row of the table, or no length, is taken
 for padding and raises LnnError (E_INVALID) when a result is next read.
 """
-from functools import partial
+from functools import lru_cache, partial
 
 import numpy as np
 
@@ -25,10 +25,15 @@ _out = ops._out
 _each_device = ops._each_device
 
 
-def _tensors(**named):
-    for name, t in named.items():
+def _tensors(names, *tensors):
+    for name, t in zip(names.split(), tensors):
         if not isinstance(t, Tensor):
             raise ValueError(f"{name} must be a Tensor, got {t.__class__}")
+
+
+@lru_cache(maxsize=4096)
+def _shape(*dims):
+    return TensorShape(dims)
 
 
 def _whole(name, value, lowest):
@@ -46,15 +51,15 @@ def embedding(ids_t, table_t, scale=1.0):
 
     The gradient of the table adds the terms of a row in the order of the tokens (they are sorted by row first), so that
     it is the same from run to run."""
-    _tensors(ids_t=ids_t, table_t=table_t)
+    _tensors("ids_t table_t", ids_t, table_t)
     if table_t.shape.rank != 2:
         raise ValueError(f"table_t must be (tokens, dim), got {table_t.shape}")
-    vocab, dim = table_t.shape
+    vocab, dim = table_t.shape.shape
     if vocab > MAX_NUMBER:
         raise ValueError(f"a table of {vocab} rows: token numbers are exact in fp32 up to {MAX_NUMBER}")
     scale = float(scale)
     n = ids_t.shape.size
-    output_t = _out(tuple(ids_t.shape.shape) + (dim,), "embedding")
+    output_t = _out(_shape(*ids_t.shape.shape, dim), "embedding")
 
     def grad(O_t, dO_t):
         g, acc = table_t._grad_to_write()
@@ -70,19 +75,20 @@ def embedding(ids_t, table_t, scale=1.0):
 # =============================================================================================
 # probabilities of tokens
 # =============================================================================================
-def _logit_rows(logits_t, ids_t, **rows_of):
-    """(rows, vocab, result shape) after the checks"""
-    _tensors(logits_t=logits_t, ids_t=ids_t, **{k: t for k, t in rows_of.items() if t is not None})
-    if logits_t.shape.rank < 2:
+def _logit_rows(logits_t, names, *of_rows):
+    """(rows, vocab, result shape) after the checks; of_rows: the tensors with one element per row, or None"""
+    _tensors("logits_t " + names, logits_t, *of_rows)
+    dims = logits_t.shape.shape
+    if len(dims) < 2:
         raise ValueError(f"logits_t must be (..., vocabulary) of rank 2 or more, got {logits_t.shape}")
-    vocab = logits_t.shape[-1]
+    vocab = dims[-1]
     if vocab > MAX_NUMBER:
         raise ValueError(f"a vocabulary of {vocab}: token numbers are exact in fp32 up to {MAX_NUMBER}")
     rows = logits_t.shape.size // vocab
-    for name, t in dict(rows_of, ids_t=ids_t).items():
-        if t is not None and t.shape.size != rows:
+    for name, t in zip(names.split(), of_rows):
+        if t.shape.size != rows:
             raise ValueError(f"{name} must have {rows} elements, one per row of logits_t, got {t.shape}")
-    return rows, vocab, TensorShape(logits_t.shape[:-1])
+    return rows, vocab, _shape(*dims[:-1])
 
 
 def _logit_grad(logits_t, ids_t, stats_t, rows, vocab, O_t, dO_t):
@@ -94,8 +100,8 @@ def _logit_grad(logits_t, ids_t, stats_t, rows, vocab, O_t, dO_t):
 def token_log_prob(logits_t, ids_t):
     """log(softmax(logits)[id]) of each row, with the maximum subtracted: logits (..., V), one id per row -> (...).
     Rows with an id below zero give 0 and no gradient."""
-    rows, vocab, shape = _logit_rows(logits_t, ids_t)
-    output_t, stats_t = _out(shape, "token_log_prob"), _out((rows, 3))
+    rows, vocab, shape = _logit_rows(logits_t, "ids_t", ids_t)
+    output_t, stats_t = _out(shape, "token_log_prob"), _out(_shape(rows, 3))
     output_t._assign_gradfn(logits_t, partial(_logit_grad, logits_t, ids_t, stats_t, rows, vocab))
     for i, dev in _each_device():
         _call.lnn_token_log_prob_fwd(i, dev, output_t, stats_t, logits_t, ids_t, rows, vocab)
@@ -112,9 +118,10 @@ def policy_loss(logits_t, ids_t, old_t, advantage_t, ref_t=None, clip_low=0.2, c
     logits (..., V) -> (...); ids, old, advantage and ref have one element per row.  old and ref are logarithms as
     token_log_prob gives them.  The gradient goes to the logits; the other arguments are constants.  Rows with an id
     below zero give 0 and no gradient."""
-    rows, vocab, shape = _logit_rows(logits_t, ids_t, old_t=old_t, advantage_t=advantage_t, ref_t=ref_t)
-    if old_t is None or advantage_t is None:
-        raise ValueError("old_t and advantage_t are needed")
+    if ref_t is None:
+        rows, vocab, shape = _logit_rows(logits_t, "ids_t old_t advantage_t", ids_t, old_t, advantage_t)
+    else:
+        rows, vocab, shape = _logit_rows(logits_t, "ids_t old_t advantage_t ref_t", ids_t, old_t, advantage_t, ref_t)
     clip_low, clip_high, kl = float(clip_low), float(clip_high), float(kl)
     if not 0.0 <= clip_low <= 1.0 or not 0.0 <= clip_high < float("inf"):
         raise ValueError(f"the ratio cannot be clipped to 1 - {clip_low} .. 1 + {clip_high}")
@@ -124,7 +131,7 @@ def policy_loss(logits_t, ids_t, old_t, advantage_t, ref_t=None, clip_low=0.2, c
         raise ValueError("a KL term needs ref_t")
     if kl == 0.0:
         ref_t = None
-    output_t, stats_t = _out(shape, "policy_loss"), _out((rows, 3))
+    output_t, stats_t = _out(shape, "policy_loss"), _out(_shape(rows, 3))
     output_t._assign_gradfn(logits_t, partial(_logit_grad, logits_t, ids_t, stats_t, rows, vocab))
     for i, dev in _each_device():
         _call.lnn_policy_loss_fwd(i, dev, output_t, stats_t, logits_t, ids_t, old_t, advantage_t, ref_t, rows, vocab,
@@ -190,12 +197,13 @@ def sink_attention(q_t, k_t, v_t, window, sinks=0, scale=None, lengths_t=None):
     (p - j < window or j < sinks).  scale is D ** -0.5 unless given.  lengths_t, of B elements, says how many of the S
     keys of each sequence are real: the rest is padding behind it, whose rows give zeros and neither get nor pass on a
     gradient.  All three inputs have gradients."""
-    _tensors(q_t=q_t, k_t=k_t, v_t=v_t)
-    if q_t.shape.rank != 4 or k_t.shape.rank != 4 or v_t.shape != k_t.shape:
+    _tensors("q_t k_t v_t", q_t, k_t, v_t)
+    q_dims, k_dims = q_t.shape.shape, k_t.shape.shape
+    if len(q_dims) != 4 or len(k_dims) != 4 or v_t.shape.shape != k_dims:
         raise ValueError(f"expected q (B, Hq, T, D) and k, v (B, Hkv, S, D), got {q_t.shape}, {k_t.shape}, {v_t.shape}")
-    B, Hq, T, D = q_t.shape
-    Hkv, S = k_t.shape[1], k_t.shape[2]
-    if k_t.shape[0] != B or k_t.shape[3] != D or Hq % Hkv != 0:
+    B, Hq, T, D = q_dims
+    Hkv, S = k_dims[1], k_dims[2]
+    if k_dims[0] != B or k_dims[3] != D or Hq % Hkv != 0:
         raise ValueError(f"q {q_t.shape} does not go with k and v {k_t.shape}")
     if T > S:
         raise ValueError(f"{T} queries over {S} keys: the last key belongs to the last query")
@@ -204,11 +212,11 @@ def sink_attention(q_t, k_t, v_t, window, sinks=0, scale=None, lengths_t=None):
     window, sinks = _span(window, sinks)
     scale = _scale(scale, D)
     if lengths_t is not None:
-        _tensors(lengths_t=lengths_t)
+        _tensors("lengths_t", lengths_t)
         if lengths_t.shape.size != B:
             raise ValueError(f"lengths_t must have {B} elements, one per sequence, got {lengths_t.shape}")
     geom = _lib.AttnGeom(B, Hq, Hkv, T, S, D, min(window, S), min(sinks, S), scale)
-    output_t, lse_t = _out(q_t.shape, "sink_attention"), _out((B, Hq, T))
+    output_t, lse_t = _out(q_t.shape, "sink_attention"), _out(_shape(B, Hq, T))
     output_t._gradfns = _AttentionGrad(q_t, k_t, v_t, lengths_t, lse_t, geom)
     for i, dev in _each_device():
         _call.lnn_sink_attn_fwd(i, dev, output_t, lse_t, q_t, k_t, v_t, lengths_t, geom.address)
@@ -232,6 +240,7 @@ class SinkCache:
         if self.window + self.sinks > MAX_NUMBER:
             raise ValueError(f"{self.window + self.sinks} slots: at most {MAX_NUMBER}")
         shape = (self.batch, self.heads, self.sinks + self.window, self.dim)
+        self._token_shape = (self.batch, self.heads, self.dim)
         self.k, self.v = Tensor(shape), Tensor(shape)
         self._lengths = [Tensor((self.batch,)), Tensor((self.batch,))]
 
@@ -255,14 +264,15 @@ class SinkCache:
         """Fill the cache from a prompt: k and v (batch, heads, S, dim), of which lengths_t (S everywhere unless given) are
         real.  Slots that no position of the prompt falls into stay as they are, and so does the place of a sequence
         whose length is below zero."""
-        _tensors(k_t=k_t, v_t=v_t)
-        if k_t.shape.rank != 4 or v_t.shape != k_t.shape or (k_t.shape[0], k_t.shape[1], k_t.shape[3]) != (self.batch, self.heads, self.dim):
+        _tensors("k_t v_t", k_t, v_t)
+        dims = k_t.shape.shape
+        if len(dims) != 4 or v_t.shape.shape != dims or (dims[0], dims[1], dims[3]) != self._token_shape:
             raise ValueError(f"expected k and v ({self.batch}, {self.heads}, S, {self.dim}), got {k_t.shape}, {v_t.shape}")
-        S = k_t.shape[2]
+        S = dims[2]
         if S > MAX_NUMBER:
             raise ValueError(f"{S} keys: lengths are exact in fp32 up to {MAX_NUMBER}")
         if lengths_t is not None:
-            _tensors(lengths_t=lengths_t)
+            _tensors("lengths_t", lengths_t)
             if lengths_t.shape.size != self.batch:
                 raise ValueError(f"lengths_t must have {self.batch} elements, one per sequence, got {lengths_t.shape}")
         sources = [t._get_top_reference_source() for t in (k_t, v_t, lengths_t) if t is not None]
@@ -277,21 +287,23 @@ def sink_attention_step(q_t, k_t, v_t, cache, scale=None):
     """One more token of each sequence: its key and value (batch, heads, dim) go into the cache, and its query
     (batch, Hq, dim) attends over what sink_attention would see -> (batch, Hq, dim).  Hq is a multiple of the cache's
     heads.  Places of a length below zero give zeros and stay as they are.  Forward only: no grad functions."""
-    _tensors(q_t=q_t, k_t=k_t, v_t=v_t)
+    _tensors("q_t k_t v_t", q_t, k_t, v_t)
     if not isinstance(cache, SinkCache):
         raise ValueError(f"cache must be a SinkCache, got {cache.__class__}")
-    kv_shape = (cache.batch, cache.heads, cache.dim)
-    if tuple(k_t.shape.shape) != kv_shape or tuple(v_t.shape.shape) != kv_shape:
-        raise ValueError(f"expected k and v {kv_shape}, got {k_t.shape}, {v_t.shape}")
-    if q_t.shape.rank != 3 or (q_t.shape[0], q_t.shape[2]) != (cache.batch, cache.dim) or q_t.shape[1] % cache.heads != 0:
-        raise ValueError(f"q {q_t.shape} does not go with a cache of {kv_shape}")
-    if any(t._get_top_reference_source() in (cache.k, cache.v) for t in (q_t, k_t, v_t)):
-        raise ValueError("the token cannot be part of the cache's own memory")
-    scale = _scale(scale, cache.dim)
+    dims = q_t.shape.shape
+    if k_t.shape.shape != cache._token_shape or v_t.shape.shape != cache._token_shape:
+        raise ValueError(f"expected k and v {cache._token_shape}, got {k_t.shape}, {v_t.shape}")
+    if len(dims) != 3 or dims[0] != cache.batch or dims[2] != cache.dim or dims[1] % cache.heads != 0:
+        raise ValueError(f"q {q_t.shape} does not go with a cache of {cache._token_shape}")
+    for t in (q_t, k_t, v_t):
+        source = t._get_top_reference_source()
+        if source is cache.k or source is cache.v:
+            raise ValueError("the token cannot be part of the cache's own memory")
+    scale = cache.dim ** -0.5 if scale is None else float(scale)
     output_t = _out(q_t.shape, "sink_attention_step")
     now, after = cache._lengths
     for i, dev in _each_device():
-        _call.lnn_sink_attn_step(i, dev, output_t, q_t, k_t, v_t, cache.k, cache.v, now, after, cache.batch, q_t.shape[1],
+        _call.lnn_sink_attn_step(i, dev, output_t, q_t, k_t, v_t, cache.k, cache.v, now, after, cache.batch, dims[1],
                                  cache.heads, cache.dim, cache.window, cache.sinks, scale)
     if devices._shallow == 0:
         cache._lengths = [after, now]

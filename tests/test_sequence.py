@@ -39,7 +39,7 @@ def test_refusals_of_the_losses(fake):
     refused("old_t must have", nn.policy_loss, z, n, T(2), n)
     refused("advantage_t must have", nn.policy_loss, z, n, n, T(7))
     refused("ref_t must have", nn.policy_loss, z, n, n, n, T(1), kl=0.1)
-    refused("are needed", nn.policy_loss, z, n, None, n)
+    refused("old_t must be a Tensor", nn.policy_loss, z, n, None, n)
     refused("needs ref_t", nn.policy_loss, z, n, n, n, kl=0.1)
     refused("negative", nn.policy_loss, z, n, n, n, n, kl=-0.1)
     refused("negative", nn.policy_loss, z, n, n, n, n, kl=float("nan"))
