@@ -6,6 +6,7 @@
 #include <math_constants.h>
 #include <float.h>
 #include <algorithm>
+#include <type_traits>
 #include "lnn_attn.cuh"
 #include "lnn_tc_dev.cuh"
 
@@ -81,6 +82,7 @@ simt_fwd_kernel(const AttnArgs a) {
   extern __shared__ __align__(16) float smem[];
   float *Q = smem, *K = Q + B * PITCH, *V = K + B * PITCH, *P = V + B * PITCH;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  lnn::wait_for_previous();
   if (a.info && !lnn::any_group_left(a)) return;
   const int tiles_q = (a.q_len + B - 1) / B, past = a.kv_len - a.q_len;
   for (int64_t work = blockIdx.x; work < (int64_t)tiles_q * a.q_heads * a.batch; work += gridDim.x) {
@@ -164,6 +166,7 @@ simt_dq_kernel(const AttnArgs a) {
   extern __shared__ __align__(16) float smem[];
   float *Q = smem, *D = Q + B * PITCH, *K = D + B * PITCH, *V = K + B * PITCH, *S = V + B * PITCH;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  lnn::wait_for_previous();
   if (a.info && !lnn::any_group_left(a)) return;
   const int tiles_q = (a.q_len + B - 1) / B, past = a.kv_len - a.q_len;
   for (int64_t work = blockIdx.x; work < (int64_t)tiles_q * a.q_heads * a.batch; work += gridDim.x) {
@@ -230,6 +233,7 @@ simt_dkv_kernel(const AttnArgs a) {
   extern __shared__ __align__(16) float smem[];
   float *Q = smem, *D = Q + B * PITCH, *K = D + B * PITCH, *V = K + B * PITCH, *P = V + B * PITCH, *S = P + B * (B + 1);
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  lnn::wait_for_previous();
   if (a.info && !lnn::any_group_left(a)) return;
   const int tiles_k = (a.kv_len + B - 1) / B, past = a.kv_len - a.q_len, group = a.q_heads / a.kv_heads;
   for (int64_t work = blockIdx.x; work < (int64_t)tiles_k * a.kv_heads * a.batch; work += gridDim.x) {
@@ -297,6 +301,7 @@ simt_dkv_kernel(const AttnArgs a) {
 // one warp per row
 __global__ void __launch_bounds__(kThreads)
 attn_delta_kernel(float* __restrict__ delta, const float* __restrict__ dout, const float* __restrict__ o, int64_t rows, int dim) {
+  lnn::wait_for_previous();
   const int64_t row = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   if (row >= rows) return;
   float s = 0.0f;
@@ -307,11 +312,11 @@ attn_delta_kernel(float* __restrict__ delta, const float* __restrict__ dout, con
 }
 
 template <int B, int DP, class Kernel>
-int launch_simt(lnn::Device* d, Kernel kernel, int matrices, int tiles, int64_t works, const AttnArgs& a) {
+int launch_simt(lnn::Device* d, Kernel* kernel, int matrices, int tiles, int64_t works, const AttnArgs& a) {
   const unsigned grid = (unsigned)std::min<int64_t>(works, a.info ? d->sm_count : 1 << 30);
   const size_t bytes = (size_t)(matrices * B * (DP + 4) + tiles * B * (B + 1)) * 4;
   LNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  kernel<<<grid, kThreads, bytes, d->stream>>>(a);
+  LNN_CUDA(lnn::launch_chained(d, kernel, grid, kThreads, bytes, a));
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
 }
@@ -353,6 +358,7 @@ __global__ void __launch_bounds__(kThreads)
 cache_store_kernel(float* __restrict__ ck, float* __restrict__ cv, float* __restrict__ lengths_out, const float* __restrict__ k,
                    const float* __restrict__ v, const float* __restrict__ lengths, int heads, int kv_len, int dim, int window,
                    int sinks, int* status) {
+  lnn::wait_for_previous();
   const int b = blockIdx.z, h = blockIdx.y, slots = window + sinks;
   if (lengths && __ldg(lengths + b) < 0.0f) return;               // this slot of the batch stays as it is
   const int len = lnn::attn_length(lengths, b, kv_len, status);
@@ -369,7 +375,7 @@ cache_store_kernel(float* __restrict__ ck, float* __restrict__ cv, float* __rest
   }
 }
 
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 8, kMaxSplits = 8;
 
 struct StepArgs {
   float* o;
@@ -521,18 +527,27 @@ __device__ __forceinline__ void step_finish(const StepArgs& a, const StepPlace& 
     }
   }
   __syncthreads();
-  // column c of `count` partial results: values, or (NV * 32 + 1) the sums; and their maximum
-  const auto join = [&](auto&& from, int count, int c) {
-    float top = from(0)[NV * 32];
-    for (int w = 1; w < count; ++w) top = fmaxf(top, from(w)[NV * 32]);
+  // column c of COUNT partial results (those from `count` on have no weight), or with c = NV * 32 + 1 the sum of the sums;
+  // and their maximum.  All are loaded at once: the ones of other blocks are far away.
+  const auto join = [&](auto&& from, auto most, int count, int c) {
+    constexpr int COUNT = decltype(most)::value;
+    float top = -FLT_MAX, m[COUNT], x[COUNT];
+#pragma unroll
+    for (int w = 0; w < COUNT; ++w) {
+      m[w] = w < count ? from(w)[NV * 32] : -FLT_MAX;
+      x[w] = w < count ? from(w)[c] : 0.0f;
+    }
+#pragma unroll
+    for (int w = 0; w < COUNT; ++w) top = fmaxf(top, m[w]);
     float sum = 0.0f;
-    for (int w = 0; w < count; ++w) sum = fmaf(exp2_fast(__fsub_rn(from(w)[NV * 32], top)), from(w)[c], sum);
+#pragma unroll
+    for (int w = 0; w < COUNT; ++w) sum = fmaf(exp2_fast(__fsub_rn(m[w], top)), x[w], sum);
     return make_float2(sum, top);
   };
   for (int i = threadIdx.x; i < GC * (NV * 32 + 1); i += kThreads) {
     const int g = i / (NV * 32 + 1), c = i % (NV * 32 + 1);
     const auto of_warp = [&](int w) { return smem + ((g / HEADS * WARPS + w) * HEADS + g % HEADS) * kRow; };
-    const float2 r = join(of_warp, WARPS, c < NV * 32 ? c : NV * 32 + 1);
+    const float2 r = join(of_warp, std::integral_constant<int, WARPS>(), WARPS, c < NV * 32 ? c : NV * 32 + 1);
     if (c < NV * 32) block[g * kRow + c] = r.x;
     else { block[g * kRow + NV * 32] = r.y; block[g * kRow + NV * 32 + 1] = r.x; }
   }
@@ -542,8 +557,9 @@ __device__ __forceinline__ void step_finish(const StepArgs& a, const StepPlace& 
   for (int i = p.rank * kThreads + threadIdx.x; i < p.heads * a.dim; i += a.splits * kThreads) {
     const int g = i / a.dim, c = i % a.dim;
     const auto of_rank = [&](int r) { return (a.splits > 1 ? cluster.map_shared_rank(block, r) : block) + g * kRow; };
-    const float sum = join(of_rank, a.splits, NV * 32 + 1).x;
-    a.o[p.oq + i] = __fdiv_rn(join(of_rank, a.splits, c).x, sum);
+    constexpr std::integral_constant<int, kMaxSplits> most{};
+    const float sum = join(of_rank, most, a.splits, NV * 32 + 1).x;
+    a.o[p.oq + i] = __fdiv_rn(join(of_rank, most, a.splits, c).x, sum);
   }
   if (a.splits > 1) cluster.sync();                      // nobody leaves while its shared memory is being read
 }
@@ -562,6 +578,7 @@ __global__ void __launch_bounds__(kThreads)
 step_kernel(const StepArgs a) {
   extern __shared__ __align__(16) float smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane & 7, sub = lane >> 3, dim = a.dim;
+  lnn::wait_for_previous();
   const StepPlace p(a, GC);
   if (p.idle) return;
   const auto load = [&](const float* row, uint64_t (&x)[2 * NV], float times) {
@@ -606,6 +623,7 @@ step_bulk_kernel(const StepArgs a) {
   constexpr int HEADS = kStepHeads<GC, NV>, WARPS = kStepWarps / kStepTeams<GC, NV>, KEYS = kStepKeys<GC, NV>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane & 7, sub = lane >> 3;
   const int team = warp / WARPS, turn = warp % WARPS, dim = FULL ? NV * 32 : a.dim;
+  lnn::wait_for_previous();
   const StepPlace p(a, GC);
   if (p.idle) return;
   const int per_stage = a.stage_slots, steps = (p.end - p.begin + per_stage - 1) / per_stage;
@@ -718,7 +736,7 @@ int launch_step(lnn::Device* d, StepArgs& a, bool vec) {
   a.group_chunks = (group + GC - 1) / GC;
   const int64_t clusters = (int64_t)a.batch * a.kv_heads * a.group_chunks;
   a.splits = 1;
-  while (a.splits < 8 && clusters * a.splits < 2 * d->sm_count && slots >= a.splits * 2 * 64) a.splits *= 2;
+  while (a.splits < kMaxSplits && clusters * a.splits < 2 * d->sm_count && slots >= a.splits * 2 * 64) a.splits *= 2;
   LNN_REQUIRE((int64_t)a.kv_heads * a.group_chunks < 65536, "too many heads");
   const size_t join = (size_t)(kStepWarps * kStepHeads<GC, NV> + GC) * kStepRow<NV> * 4;
   size_t bytes = join;
@@ -739,11 +757,13 @@ int launch_step(lnn::Device* d, StepArgs& a, bool vec) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = d->stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)a.splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)a.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = a.splits > 1 ? 1 : 0;
+  cfg.numAttrs = a.splits > 1 ? 2 : 1;
   LNN_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
@@ -799,7 +819,7 @@ int attn_simt_bwd(Device* d, const AttnArgs& a) {
 }
 
 int attn_delta(Device* d, float* delta, const float* dout, const float* o, int64_t rows, int dim) {
-  attn_delta_kernel<<<(unsigned)lnn_ceil_div(rows, kThreads / 32), kThreads, 0, d->stream>>>(delta, dout, o, rows, dim);
+  LNN_CUDA(launch_chained(d, attn_delta_kernel, (unsigned)lnn_ceil_div(rows, kThreads / 32), kThreads, 0, delta, dout, o, rows, dim));
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
 }
@@ -815,7 +835,7 @@ int lnn_sink_attn_fwd(int dev, uint64_t O, uint64_t LSE, uint64_t Q, uint64_t K,
   LNN_REQUIRE(O && LSE && Q && K && V, "bad arguments");
   AttnArgs a = attn_args(d, g, Q, K, V, LEN);
   a.o = out(O); a.lse = out(LSE);
-  return lnn::attn_tc_applicable(a) ? lnn::attn_tc_fwd(d, a) : lnn::attn_simt_fwd(d, a);
+  return lnn::attn_tc_applicable(a, false) ? lnn::attn_tc_fwd(d, a) : lnn::attn_simt_fwd(d, a);
 }
 
 int lnn_sink_attn_bwd(int dev, uint64_t dQ, uint64_t dK, uint64_t dV, uint64_t Q, uint64_t K, uint64_t V, uint64_t O, uint64_t LSE,
@@ -828,7 +848,7 @@ int lnn_sink_attn_bwd(int dev, uint64_t dQ, uint64_t dK, uint64_t dV, uint64_t Q
   a.o = out(O); a.lse = out(LSE); a.dout = in(dO);
   a.dq = out(dQ); a.dk = out(dK); a.dv = out(dV);
   a.acc_q = acc_q; a.acc_k = acc_k; a.acc_v = acc_v;
-  if (lnn::attn_tc_applicable(a)) return lnn::attn_tc_bwd(d, a);
+  if (lnn::attn_tc_applicable(a, true)) return lnn::attn_tc_bwd(d, a);
   const int64_t rows = (int64_t)g->batch * g->q_heads * g->q_len;
   lnn::Scratch delta(d);
   rc = delta.get((uint64_t)rows * 4);
@@ -847,8 +867,8 @@ int lnn_sink_cache_store(int dev, uint64_t CK, uint64_t CV, uint64_t LEN_OUT, ui
   const int64_t elements = (int64_t)std::min(kv_len, window + sinks) * dim;
   const int64_t blocks = std::min<int64_t>(lnn_ceil_div(elements, kThreads),
                                            std::max<int64_t>(1, (int64_t)d->sm_count * 16 / ((int64_t)batch * heads)));
-  cache_store_kernel<<<dim3((unsigned)blocks, (unsigned)heads, (unsigned)batch), kThreads, 0, d->stream>>>(
-      out(CK), out(CV), out(LEN_OUT), in(K), in(V), in(LEN), heads, kv_len, dim, window, sinks, d->status_dev);
+  LNN_CUDA(lnn::launch_chained(d, cache_store_kernel, dim3((unsigned)blocks, (unsigned)heads, (unsigned)batch), kThreads, 0, out(CK),
+                               out(CV), out(LEN_OUT), in(K), in(V), in(LEN), heads, kv_len, dim, window, sinks, d->status_dev));
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
 }

@@ -80,6 +80,7 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
   __shared__ uint32_t red[kWarps];
   __shared__ float redn[kWarps];
   __shared__ int last_block;
+  lnn::wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES, c = lane % LANES * 4;
   int head = blockIdx.y, ti = 0;
   while (head >= a.t[ti].heads) head -= a.t[ti++].heads;
@@ -437,11 +438,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
   __shared__ uint64_t bar_c_full[NC];
   __shared__ __align__(16) float col_lse[S::KEYS ? NC : 1][BN], col_delta[MODE == DK ? NC : 1][BN];
 
-  // an earlier kernel gave up: leave as a whole CTA (the decision must be uniform)
-  if (threadIdx.x == 0) abort_flag_smem = (*(volatile int*)t.a.status == LNN_E_TIMEOUT) ? 2 : 0;
-  __syncthreads();
-  if (abort_flag_smem == 2) return;
-
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &abort_flag_smem;
   int* status = t.a.status;
@@ -464,9 +460,16 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
     tmem_alloc(smem_u32(&tmem_base_smem), 512);
     tmem_relinquish();
   }
+  lnn::wait_for_previous();
+  // an earlier kernel gave up: leave as a whole CTA (the decision must be uniform)
+  if (threadIdx.x == 0) abort_flag_smem = (*(volatile int*)status == LNN_E_TIMEOUT) ? 2 : 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (abort_flag_smem == 2) {
+    if (warp == 1) tmem_dealloc(tmem_base_smem, 512);
+    return;
+  }
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base_smem, 0);
   const bool some_left = lnn::any_group_left(t.a);               // work for the FP32 pipe
 
@@ -1016,6 +1019,7 @@ template <int DP>
 __global__ void __launch_bounds__(256)
 attn_parts_kernel(float* __restrict__ dst, const float* __restrict__ parts, const TcArgs t, int accumulate) {
   const AttnArgs& a = t.a;
+  lnn::wait_for_previous();
   constexpr int ROWS = kRowsM / kPartBlocks;
   const int tile = blockIdx.x / kPartBlocks, first = blockIdx.x % kPartBlocks * ROWS, hk = blockIdx.y, b = blockIdx.z;
   const int splits = tile < t.sink_tiles ? t.splits_sink : t.splits;
@@ -1054,7 +1058,7 @@ int launch_pass(lnn::Device* d, const CUtensorMap* x, const CUtensorMap* y, cons
   using S = Shape<MODE, DP>;
   static_assert(S::SMEM + 2048 <= 227 * 1024, "shared memory");
   LNN_CUDA(cudaFuncSetAttribute(attn_tc_kernel<MODE, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
-  attn_tc_kernel<MODE, DP><<<std::min(t.works, d->sm_count), kAttnThreads, S::SMEM, d->stream>>>(*x, *y, *z, t);
+  LNN_CUDA(lnn::launch_chained(d, attn_tc_kernel<MODE, DP>, std::min(t.works, d->sm_count), kAttnThreads, S::SMEM, *x, *y, *z, t));
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
 }
@@ -1121,7 +1125,7 @@ int prepare(lnn::Device* d, AttnArgs& a, Operands& op, bool backward) {
     rc = operand_map(&op.map[i], at[i], DP, p.t[i].rows, p.t[i].heads);
     if (rc) return rc;
   }
-  attn_prep_kernel<DP><<<dim3((unsigned)p.blocks, (unsigned)heads), kPrepThreads, 0, d->stream>>>(p);
+  LNN_CUDA(lnn::launch_chained(d, attn_prep_kernel<DP>, dim3((unsigned)p.blocks, (unsigned)heads), kPrepThreads, 0, p));
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
 }
@@ -1153,8 +1157,9 @@ int keys_pass(lnn::Device* d, TcArgs t, Operands& op, float* dst, int accumulate
   }
   int rc = launch_pass<MODE, DP>(d, &op.map[1], &op.map[0], &op.map[3], t);
   if (rc || !cut) return rc;
-  attn_parts_kernel<DP><<<dim3((unsigned)t.tiles * kPartBlocks, (unsigned)t.a.kv_heads, (unsigned)t.a.batch), 256, 0, d->stream>>>(
-      dst, t.parts, t, accumulate);
+  LNN_CUDA(lnn::launch_chained(d, attn_parts_kernel<DP>,
+                               dim3((unsigned)t.tiles * kPartBlocks, (unsigned)t.a.kv_heads, (unsigned)t.a.batch), 256, 0, dst, t.parts,
+                               t, accumulate));
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
 }
@@ -1195,8 +1200,12 @@ int tc_bwd(lnn::Device* d, AttnArgs a) {
 
 namespace lnn {
 
-bool attn_tc_applicable(const AttnArgs& a) {
+// Sequences of one tile of the FP32-pipe kernels' 64 keys are theirs: one launch in place of three or six, and a tile of 128
+// rows would be half empty (us for 32 heads, FP32 pipe / tensor cores, cache filled too: 64 positions of 64 values 18.8 / 25.0,
+// of 128 29.0 / 31.1, 100 of 64 28.0 / 29.6; with gradients 55.9 / 69.5, but 88.5 / 83.5 for 128 values and 86.5 / 79.1 for 100).
+bool attn_tc_applicable(const AttnArgs& a, bool backward) {
   const int64_t heads = 2ll * a.batch * (a.q_heads + a.kv_heads);
+  if (a.kv_len <= 64 && (a.dim <= 64 || !backward)) return false;
   return a.dim <= 128 && heads <= kTileCounters && heads < 65536;
 }
 int attn_tc_fwd(Device* d, const AttnArgs& a) { return a.dim <= 64 ? tc_fwd<64>(d, a) : tc_fwd<128>(d, a); }

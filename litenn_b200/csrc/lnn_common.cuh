@@ -79,6 +79,31 @@ struct Scratch {
   template <class T> T* as() { return reinterpret_cast<T*>(p); }
 };
 
+// Launch of a kernel that begins with wait_for_previous(): its blocks are set up while the kernel in front of it in the
+// stream still runs (programmatic dependent launch), which hides one to two microseconds of every link of a chain of
+// short kernels.
+template <class... Params, class... Args>
+cudaError_t launch_chained(Device* d, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = d->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+#ifdef __CUDACC__
+// Before a kernel's first access to global memory: all of the kernels in front of it are over and their writes visible.
+// The kernel behind it may be set up from here on.
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
+}
+#endif
+
 // matrix products too small for the tensor cores, on the FP32 pipe (lnn_small.cu)
 int64_t gemm_small_limit();           // multiply-adds up to which they are
 bool gemm_small_applicable(int64_t batch, int64_t m, int64_t n, int64_t k);

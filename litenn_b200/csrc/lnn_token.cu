@@ -50,6 +50,7 @@ template <class T>
 __global__ void __launch_bounds__(kThreads)
 embedding_fwd_kernel(T* __restrict__ Y, const T* __restrict__ table, const float* __restrict__ ids, int64_t tokens,
                      int vocab, int64_t units, float scale, int* status) {
+  lnn::wait_for_previous();
   for (int64_t n = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; n < tokens; n += (int64_t)gridDim.x * blockDim.y) {
     const int row = token_row(__ldg(ids + n), vocab, n, 1, status);
     for (int64_t c = threadIdx.x; c < units; c += blockDim.x)
@@ -124,6 +125,7 @@ __device__ __forceinline__ void count_digits(uint32_t* count, const uint32_t (&k
 __global__ void __launch_bounds__(kThreads)
 sort_count_kernel(const __grid_constant__ SortArgs a) {
   __shared__ uint32_t count[kSortWarps][256];
+  lnn::wait_for_previous();
   if ((int)blockIdx.x >= a.sort_blocks) { write_zeros(a); return; }
   for (int i = threadIdx.x; i < kSortWarps * 256; i += kThreads) (&count[0][0])[i] = 0;
   const SortStrip s(a);
@@ -145,6 +147,7 @@ __global__ void __launch_bounds__(kThreads)
 sort_scatter_kernel(const __grid_constant__ SortArgs a) {
   __shared__ uint32_t count[kSortWarps][256];
   __shared__ uint32_t warp_total[kSortWarps];
+  lnn::wait_for_previous();
   if ((int)blockIdx.x >= a.sort_blocks) { write_zeros(a); return; }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int i = threadIdx.x; i < kSortWarps * 256; i += kThreads) (&count[0][0])[i] = 0;
@@ -211,6 +214,7 @@ __global__ void __launch_bounds__(kThreads)
 table_grad_kernel(T* __restrict__ dtable, const T* __restrict__ dy, const uint32_t* __restrict__ keys,
                   const uint32_t* __restrict__ at, T* __restrict__ head, T* __restrict__ tail, int64_t tokens, int vocab,
                   int64_t units, float scale, int accumulate) {
+  lnn::wait_for_previous();
   const int64_t pieces = (tokens + kPiece - 1) / kPiece;
   const int64_t piece = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (piece >= pieces) return;
@@ -263,6 +267,7 @@ template <class T>
 __global__ void __launch_bounds__(kThreads)
 table_join_kernel(T* __restrict__ dtable, const uint32_t* __restrict__ keys, const T* __restrict__ head,
                   const T* __restrict__ tail, int64_t tokens, int vocab, int64_t units, float scale, int accumulate) {
+  lnn::wait_for_previous();
   const int64_t pieces = (tokens + kPiece - 1) / kPiece;
   const int64_t piece = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (piece + 1 >= pieces) return;
@@ -336,20 +341,20 @@ int embedding_bwd(lnn::Device* d, T* dtable, const T* dy, const float* ids, int6
     a.out_keys = k[pass & 1];
     a.out_at = at[pass & 1];
     unsigned blocks = next();
-    sort_count_kernel<<<blocks, kThreads, 0, d->stream>>>(a);
+    LNN_CUDA(lnn::launch_chained(d, sort_count_kernel, blocks, kThreads, 0, a));
     LNN_CHECK_LAUNCH(d);
     blocks = next();
-    sort_scatter_kernel<<<blocks, kThreads, 0, d->stream>>>(a);
+    LNN_CUDA(lnn::launch_chained(d, sort_scatter_kernel, blocks, kThreads, 0, a));
     LNN_CHECK_LAUNCH(d);
   }
   const uint32_t *src_k = a.out_keys, *src_at = a.out_at;
   const dim3 block = row_block(units);
   const dim3 grid((unsigned)lnn_ceil_div(pieces, block.y), (unsigned)std::min<int64_t>(lnn_ceil_div(units, block.x), 64));
   T *head = parts.as<T>(), *tail = head + pieces * units;
-  table_grad_kernel<T><<<grid, block, 0, d->stream>>>(dtable, dy, src_k, src_at, head, tail, tokens, vocab, units, scale, accumulate);
+  LNN_CUDA(lnn::launch_chained(d, table_grad_kernel<T>, grid, block, 0, dtable, dy, src_k, src_at, head, tail, tokens, vocab, units, scale, accumulate));
   LNN_CHECK_LAUNCH(d);
   if (pieces > 1) {
-    table_join_kernel<T><<<grid, block, 0, d->stream>>>(dtable, src_k, head, tail, tokens, vocab, units, scale, accumulate);
+    LNN_CUDA(lnn::launch_chained(d, table_join_kernel<T>, grid, block, 0, dtable, src_k, head, tail, tokens, vocab, units, scale, accumulate));
     LNN_CHECK_LAUNCH(d);
   }
   return LNN_OK;
@@ -385,6 +390,7 @@ constexpr int kLogitQuads = 4;                      // loads of a thread at a ti
 __global__ void __launch_bounds__(kThreads)
 token_logit_kernel(float* __restrict__ out, float* __restrict__ stats, const float* __restrict__ logits,
                    const float* __restrict__ ids, int64_t vocab, int splits, PolicyArgs a, int* status) {
+  lnn::wait_for_previous();
   const int64_t row = blockIdx.x / (unsigned)splits;
   const int rank = (int)(blockIdx.x - row * splits);
   const float* z = logits + row * vocab;
@@ -425,15 +431,28 @@ token_logit_kernel(float* __restrict__ out, float* __restrict__ stats, const flo
   }
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = t;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kThreads / 32; ++w) t = joined(t, part[w]);
-    block_part = t;
+  // the first lanes hold the parts of the warps, then those of the blocks of the cluster
+  const auto of_lanes = [&](MaxSum x) {
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+      const MaxSum b = {__shfl_xor_sync(0xffffffffu, x.m, o), __shfl_xor_sync(0xffffffffu, x.s, o)};
+      x = joined(x, b);
+    }
+    return x;
+  };
+  if (threadIdx.x < 32) {
+    t = of_lanes(part[threadIdx.x & 7]);
+    if (threadIdx.x == 0) block_part = t;
   }
   if (splits > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    if (rank == 0 && threadIdx.x == 0)
-      for (int r = 1; r < splits; ++r) t = joined(t, *cluster.map_shared_rank(&block_part, r));
+    if (rank == 0 && threadIdx.x < 32) {
+      const int r = threadIdx.x & 7;
+      t = MaxSum{-CUDART_INF_F, 0.0f};
+      if (r < splits) t = *cluster.map_shared_rank(&block_part, r);
+      t = of_lanes(t);
+    }
     cluster.sync();
   }
   if (rank == 0 && threadIdx.x == 0) {
@@ -463,6 +482,7 @@ __global__ void __launch_bounds__(kThreads)
 token_logit_grad_kernel(float* __restrict__ dlogits, const float* __restrict__ logits, const float* __restrict__ stats,
                         const float* __restrict__ ids, const float* __restrict__ dout, int64_t vocab, int chunks,
                         int accumulate) {
+  lnn::wait_for_previous();
   const int64_t row = blockIdx.x / (unsigned)chunks;
   const int chunk = (int)(blockIdx.x - row * chunks);
   const float m = __ldg(stats + row * 3), inv = __ldg(stats + row * 3 + 1);
@@ -520,16 +540,19 @@ int token_logit(int dev, uint64_t OUT, uint64_t STATS, uint64_t X, uint64_t IDS,
   LNN_REQUIRE(rows <= (1 << 27), "too many rows");
   // a row goes over a cluster of blocks where the rows alone do not fill the device
   int splits = 1;
+  static_assert(kThreads / 32 == 8, "parts of a block, blocks of a cluster: eight");
   while (splits < 8 && rows * splits < 4 * d->sm_count && vocab >= (int64_t)splits * 2 * kThreads * 16) splits *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * splits));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = d->stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = splits > 1 ? 1 : 0;
+  cfg.numAttrs = splits > 1 ? 2 : 1;
   LNN_CUDA(cudaLaunchKernelEx(&cfg, token_logit_kernel, out(OUT), out(STATS), in(X), in(IDS), vocab, splits, a, d->status_dev));
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
@@ -549,11 +572,11 @@ int lnn_embedding_fwd(int dev, uint64_t Y, uint64_t TABLE, uint64_t IDS, int64_t
   const dim3 block = row_block(units);
   const unsigned grid = (unsigned)std::min<int64_t>(lnn_ceil_div(tokens, block.y), (int64_t)d->sm_count * 64);
   if (vec)
-    embedding_fwd_kernel<float4><<<grid, block, 0, d->stream>>>((float4*)out(Y), (const float4*)in(TABLE), in(IDS), tokens,
-                                                                (int)vocab, units, scale, d->status_dev);
+    LNN_CUDA(lnn::launch_chained(d, embedding_fwd_kernel<float4>, grid, block, 0, (float4*)out(Y), (const float4*)in(TABLE), in(IDS),
+                                 tokens, (int)vocab, units, scale, d->status_dev));
   else
-    embedding_fwd_kernel<float><<<grid, block, 0, d->stream>>>(out(Y), in(TABLE), in(IDS), tokens, (int)vocab, units, scale,
-                                                               d->status_dev);
+    LNN_CUDA(lnn::launch_chained(d, embedding_fwd_kernel<float>, grid, block, 0, out(Y), in(TABLE), in(IDS), tokens, (int)vocab, units,
+                                 scale, d->status_dev));
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
 }
@@ -587,8 +610,8 @@ int lnn_token_logit_bwd_acc(int dev, uint64_t dX, uint64_t X, uint64_t STATS, ui
   LNN_REQUIRE(dX && X && STATS && IDS && dOUT && rows > 0 && vocab > 0 && vocab <= (1 << 24), "bad arguments");
   const int64_t chunks = lnn_ceil_div(vocab, kThreads * kGradQuads * 4);
   LNN_REQUIRE(rows * chunks < (1ll << 31), "too many rows");
-  token_logit_grad_kernel<<<(unsigned)(rows * chunks), kThreads, 0, d->stream>>>(out(dX), in(X), in(STATS), in(IDS), in(dOUT),
-                                                                                vocab, (int)chunks, accumulate);
+  LNN_CUDA(lnn::launch_chained(d, token_logit_grad_kernel, (unsigned)(rows * chunks), kThreads, 0, out(dX), in(X), in(STATS), in(IDS),
+                               in(dOUT), vocab, (int)chunks, accumulate));
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
 }
