@@ -48,7 +48,7 @@ constexpr int kSampleRows = 32;
 
 struct PrepTensor {
   const float* src;
-  __half* hi;                    // [heads][rows][DP]; lo behind all heads
+  __half* hi;                    // [heads][rows][width]; lo behind all heads
   float* norms;                  // [heads][rows], or null
   int heads, per_batch, rows;
   int first, sinks;              // keys: rows below `first` that are no sinks are seen by no query
@@ -57,7 +57,7 @@ struct PrepTensor {
 };
 struct PrepArgs {
   PrepTensor t[4];
-  int tensors, dim, batch;
+  int tensors, dim, width, batch;        // width: dim rounded up to the 16 values of an MMA
   const float* lengths;
   int kv_len;
   HeadInfo* info;                // [all heads of all tensors]
@@ -107,6 +107,18 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
     for (int s = LANES / 2; s > 0; s >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, s));
     return v;
   };
+  float4 x[BATCH], y[BATCH];
+  const auto fetch = [&](int r0) {
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const int r = r0 + u * kWarps * ROWS;
+      const bool real = r < end && (r >= t.first || r < t.sinks);
+      x[u] = real ? load(src, r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (is_do) y[u] = real ? load(a.o + (int64_t)head * t.rows * dim, r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+  };
+  const int r_first = blockIdx.x * kPrepRows + warp * ROWS + sub;
+  fetch(r_first);
   // the scale, from rows spread over those that are real (the same ones in every block of the head)
   uint32_t m = 0;
   const int span = end - t.first;
@@ -126,20 +138,13 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
   const Pow2Scale scale(-e);
   __syncthreads();
 
-  __half* hi = t.hi + (int64_t)head * t.rows * DP;
-  __half* lo = hi + (int64_t)t.heads * t.rows * DP;
+  __half* hi = t.hi + (int64_t)head * t.rows * a.width;
+  __half* lo = hi + (int64_t)t.heads * t.rows * a.width;
   uint32_t top = 0;
   float top_norm = 0.0f;
   const int r_end = min((int)(blockIdx.x + 1) * kPrepRows, t.rows);
-  for (int r0 = blockIdx.x * kPrepRows + warp * ROWS + sub; r0 < (int)(blockIdx.x + 1) * kPrepRows; r0 += BATCH * kWarps * ROWS) {
-    float4 x[BATCH], y[BATCH];
-#pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      const int r = r0 + u * kWarps * ROWS;
-      const bool real = r < end && (r >= t.first || r < t.sinks);
-      x[u] = real ? load(src, r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (is_do) y[u] = real ? load(a.o + (int64_t)head * t.rows * dim, r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
+  for (int r0 = r_first; r0 < (int)(blockIdx.x + 1) * kPrepRows; r0 += BATCH * kWarps * ROWS) {
+    if (r0 != r_first) fetch(r0);
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
       const int r = r0 + u * kWarps * ROWS;
@@ -161,9 +166,9 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
         norm = fmaf(xs, xs, norm);
         split_half(xs, h[k], l[k]);
       }
-      if (in) {
-        *reinterpret_cast<uint2*>(hi + (int64_t)r * DP + c) = *reinterpret_cast<uint2*>(h);
-        *reinterpret_cast<uint2*>(lo + (int64_t)r * DP + c) = *reinterpret_cast<uint2*>(l);
+      if (in && c < a.width) {
+        *reinterpret_cast<uint2*>(hi + (int64_t)r * a.width + c) = *reinterpret_cast<uint2*>(h);
+        *reinterpret_cast<uint2*>(lo + (int64_t)r * a.width + c) = *reinterpret_cast<uint2*>(l);
       }
       if (t.norms) {
         norm = sqrtf(row_total(norm));
@@ -214,7 +219,7 @@ struct TcArgs {
   AttnArgs a;
   const float *lse_p, *delta_p;  // [q head][pitch]
   const float* norms;            // DQ: of dO's rows, DK: of V's
-  int pitch;
+  int pitch, width;
   int works;
   const uint32_t* x2;            // DQ: dO, DK: V, split
   // DV, DK: keys below sinks take `splits_sink` works per tile of rows, the others `splits`
@@ -266,10 +271,11 @@ __device__ __forceinline__ void make_work(Work& k, const TcArgs& t, int w, bool 
   k.steps = 0;
   k.split_up = 0;
   if (!S::KEYS) {
-    const int head = w / t.tiles;
+    // the last tiles first: they see most, and the short ones fill up what is left
+    const int heads = a.batch * a.q_heads, turn = w / heads, head = w - turn * heads;
     k.b = head / a.q_heads; k.h = head - k.b * a.q_heads; k.hk = k.h / group;
     const int len = lnn::attn_length(a.lengths, k.b, a.kv_len, a.status);
-    k.row0 = (w - head * t.tiles) * kRowsM;
+    k.row0 = (t.tiles - 1 - turn) * kRowsM;
     k.p_hi = min(min(k.row0 + kRowsM, a.q_len) - 1 + past, len - 1);
     if (k.p_hi >= k.row0 + past) {
       k.lowest = max(k.row0 + past - a.window + 1, 0);
@@ -278,9 +284,10 @@ __device__ __forceinline__ void make_work(Work& k, const TcArgs& t, int w, bool 
       k.steps = k.sink_steps + (k.p_hi - k.lowest) / S::BN + 1;
     }
   } else {
-    const int per = t.sink_tiles * t.splits_sink + (t.tiles - t.sink_tiles) * t.splits;
-    const int head = w / per;
-    int r = w - head * per, split, splits, tile;
+    // the first tiles first: most queries see them
+    const int heads = a.batch * a.kv_heads;
+    int r = w / heads, split, splits, tile;
+    const int head = w - r * heads;
     k.b = head / a.kv_heads; k.hk = head - k.b * a.kv_heads; k.h = k.hk * group;
     k.part = (int)(head * parts_per_head(t) + r);
     if (r < t.sink_tiles * t.splits_sink) {
@@ -568,13 +575,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
     // 64 values of MN to a row, slabs of 64 BN rows apart.  Lower words: address and the leading offset, in 16 bytes.
     constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
     constexpr uint32_t K_LO = 1u << 16, MN_LO = (BN * 128u >> 4) << 16;
+    const int ksteps = t.width / 16;
     const auto scores = [&](uint32_t d, uint32_t ax, uint32_t by, uint32_t id) {
       const uint32_t a = K_LO + (ax >> 4), b = K_LO + (by >> 4);
 #pragma unroll
       for (int pr = 0; pr < 3; ++pr)                            // lo hi, hi lo, hi hi
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks)
-          mma_ss(d, a + (pr == 0 ? S::X_PART / 16 : 0) + (ks / 4) * (kRowsM * 128 / 16) + (ks % 4) * 2,
+          if (ks < ksteps) mma_ss(d, a + (pr == 0 ? S::X_PART / 16 : 0) + (ks / 4) * (kRowsM * 128 / 16) + (ks % 4) * 2,
                  b + (pr == 1 ? S::Y_PART / 16 : 0) + (ks / 4) * (BN * 128 / 16) + (ks % 4) * 2, DESC_HI, id, pr + ks > 0);
     };
     const auto second_scores = [&](uint32_t d, uint32_t by, uint32_t id) {      // dO or V from TMEM: DP / 2 columns of hi, then of lo
@@ -583,11 +591,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       for (int pr = 0; pr < 3; ++pr)
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks)
-          mma_ts(d, a + (pr == 0 ? DP / 2 : 0) + ks * 8, b + (pr == 1 ? S::Y_PART / 16 : 0) + (ks / 4) * (BN * 128 / 16) + (ks % 4) * 2,
+          if (ks < ksteps) mma_ts(d, a + (pr == 0 ? DP / 2 : 0) + ks * 8, b + (pr == 1 ? S::Y_PART / 16 : 0) + (ks / 4) * (BN * 128 / 16) + (ks % 4) * 2,
                  DESC_HI, id, pr + ks > 0);
     };
     const auto weighted = [&](uint32_t d, uint32_t p, uint32_t bz, int n16) {      // 16 scores became 8 columns of hi and 8 of lo
-      constexpr uint32_t id = (1u << 4) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((128u >> 4) << 24);
+      const uint32_t id = (1u << 4) | (1u << 16) | ((uint32_t)(t.width >> 3) << 17) | ((128u >> 4) << 24);
       const uint32_t b = MN_LO + (bz >> 4);
       if (n16 == BN) {
 #pragma unroll
@@ -822,15 +830,15 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
         // The second stationary operand into TMEM, once the products of the work before are over: this warp's fourth of
         // the columns of its rows, hi and lo (what is no row of the tensor is zero).
         if (!warp_wait(smem_u32(&bar_x_empty), (nw & 1) ^ 1, abort_flag, status, 34, w)) { ok = false; break; }
-        const int64_t lo_at = (int64_t)(S::KEYS ? a.batch * a.kv_heads : a.batch * a.q_heads) * rows * (DP / 2);
-        const uint32_t* src = t.x2 + ((int64_t)xh * rows + row) * (DP / 2) + part * (DP / 8);
+        const int64_t lo_at = (int64_t)(S::KEYS ? a.batch * a.kv_heads : a.batch * a.q_heads) * rows * (t.width / 2);
+        const uint32_t* src = t.x2 + ((int64_t)xh * rows + row) * (t.width / 2) + part * (DP / 8);
         tc_fence_after();
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           uint32_t x[DP / 8];
 #pragma unroll
           for (int i = 0; i < DP / 8; i += 4) {
-            const uint4 v = row < rows ? __ldg(reinterpret_cast<const uint4*>(src + p * lo_at + i)) : make_uint4(0, 0, 0, 0);
+            const uint4 v = row < rows && part * (DP / 8) + i < t.width / 2 ? __ldg(reinterpret_cast<const uint4*>(src + p * lo_at + i)) : make_uint4(0, 0, 0, 0);
             x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
           }
           const uint32_t to = tmem + lanes + S::T_X2 + p * (DP / 2) + part * (DP / 8);
@@ -1045,10 +1053,10 @@ attn_parts_kernel(float* __restrict__ dst, const float* __restrict__ parts, cons
 }
 
 // ---- host ------------------------------------------------------------------------------------------------
-// [2 heads][rows][DP] fp16: lo behind hi
-int operand_map(CUtensorMap* tm, const void* base, int dp, int rows, int64_t heads) {
-  const uint64_t dims[3] = {(uint64_t)dp, (uint64_t)rows, (uint64_t)(2 * heads)};
-  const uint64_t strides[2] = {(uint64_t)dp * 2, (uint64_t)rows * dp * 2};
+// [2 heads][rows][width] fp16: lo behind hi; the boxes are 64 wide (zeros behind the width)
+int operand_map(CUtensorMap* tm, const void* base, int width, int rows, int64_t heads) {
+  const uint64_t dims[3] = {(uint64_t)width, (uint64_t)rows, (uint64_t)(2 * heads)};
+  const uint64_t strides[2] = {(uint64_t)width * 2, (uint64_t)rows * width * 2};
   const uint32_t box[3] = {64, kBoxRows, 1}, es[3] = {1, 1, 1};
   return lnn_tc::encode_half_map(tm, base, 3, dims, strides, box, es);
 }
@@ -1093,7 +1101,8 @@ int prepare(lnn::Device* d, AttnArgs& a, Operands& op, bool backward) {
   PrepArgs& p = op.p;
   const int past = a.kv_len - a.q_len, first = std::max(0, past - a.window + 1);
   const int64_t nq = (int64_t)a.batch * a.q_heads, nk = (int64_t)a.batch * a.kv_heads;
-  const int64_t sq = nq * a.q_len * DP, sk = nk * a.kv_len * DP;
+  p.width = (a.dim + 15) / 16 * 16;
+  const int64_t sq = nq * a.q_len * p.width, sk = nk * a.kv_len * p.width;
   int rc = op.halves.get((uint64_t)(2 * (sq + 2 * sk + (backward ? sq : 0))) * 2);
   if (rc) return rc;
   __half* h = op.halves.as<__half>();
@@ -1122,7 +1131,7 @@ int prepare(lnn::Device* d, AttnArgs& a, Operands& op, bool backward) {
   a.info = p.info;
   a.backward = backward;
   for (int i = 0; i < p.tensors; ++i) {
-    rc = operand_map(&op.map[i], at[i], DP, p.t[i].rows, p.t[i].heads);
+    rc = operand_map(&op.map[i], at[i], p.width, p.t[i].rows, p.t[i].heads);
     if (rc) return rc;
   }
   LNN_CUDA(lnn::launch_chained(d, attn_prep_kernel<DP>, dim3((unsigned)p.blocks, (unsigned)heads), kPrepThreads, 0, p));
@@ -1137,6 +1146,7 @@ int tc_fwd(lnn::Device* d, AttnArgs a) {
   if (rc) return rc;
   TcArgs t = {};
   t.a = a;
+  t.width = op.p.width;
   t.tiles = (a.q_len + kRowsM - 1) / kRowsM;
   t.works = a.batch * a.q_heads * t.tiles;
   rc = launch_pass<FWD, DP>(d, &op.map[0], &op.map[1], &op.map[2], t);
@@ -1171,7 +1181,7 @@ int tc_bwd(lnn::Device* d, AttnArgs a) {
   if (rc) return rc;
   TcArgs t = {};
   t.a = a;
-  t.lse_p = op.p.lse_p; t.delta_p = op.p.delta_p; t.pitch = op.p.pitch;
+  t.lse_p = op.p.lse_p; t.delta_p = op.p.delta_p; t.pitch = op.p.pitch; t.width = op.p.width;
   if (a.dq) {
     TcArgs q = t;
     q.norms = op.p.t[3].norms;
