@@ -43,13 +43,14 @@ constexpr int kRowsM = 128;                      // stationary rows
 // [2^8, 2^9); the true maximum may be 2^7 times that before fp16 overflows.  A head beyond it, or with values that are
 // not finite, is marked and goes to the FP32-pipe kernels.
 constexpr int kPrepThreads = 256;
-constexpr int kPrepRows = 64;
+constexpr int kPrepRows = 64;                    // a block takes a multiple of them
+constexpr int kPrepBlocksPerSm = 4;
 constexpr int kSampleRows = 32;
 
 struct PrepTensor {
   const float* src;
   __half* hi;                    // [heads][rows][width]; lo behind all heads
-  float* norms;                  // [heads][rows], or null
+  float* norms;                  // [heads][rows]: squares of the rows' norms after scaling, or null
   int heads, per_batch, rows;
   int first, sinks;              // keys: rows below `first` that are no sinks are seen by no query
   int past;                      // queries: row i is at position i + past
@@ -61,9 +62,9 @@ struct PrepArgs {
   const float* lengths;
   int kv_len;
   HeadInfo* info;                // [all heads of all tensors]
-  uint32_t* block_max;           // [head][blocks]: largest magnitudes after scaling
+  float* block_max;              // [head][blocks]: largest magnitudes after scaling, +inf: not finite
   float* block_norm;
-  int blocks;                    // row blocks of the longest tensor
+  int blocks, block_rows;        // row blocks of the longest tensor, rows of a block
   unsigned int* counters;        // one per head, zero between launches
   // the last tensor is dO
   const float *o, *lse;
@@ -73,122 +74,133 @@ struct PrepArgs {
 };
 
 template <int DP>
-__global__ void __launch_bounds__(kPrepThreads)
+__global__ void __launch_bounds__(kPrepThreads, kPrepBlocksPerSm)
 attn_prep_kernel(const __grid_constant__ PrepArgs a) {
   constexpr int LANES = DP / 4, ROWS = 32 / LANES;              // four values per lane; rows that a warp takes at once
-  constexpr int kWarps = kPrepThreads / 32, BATCH = kPrepRows / (kWarps * ROWS) < 4 ? kPrepRows / (kWarps * ROWS) : 4;
-  __shared__ uint32_t red[kWarps];
-  __shared__ float redn[kWarps];
+  constexpr int kWarps = kPrepThreads / 32, STRIDE = kWarps * ROWS, BATCH = kPrepRows / STRIDE < 4 ? kPrepRows / STRIDE : 4;
+  __shared__ float red[kWarps], red_norm[kWarps];
   __shared__ int last_block;
   lnn::wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES, c = lane % LANES * 4;
   int head = blockIdx.y, ti = 0;
   while (head >= a.t[ti].heads) head -= a.t[ti++].heads;
   const PrepTensor& t = a.t[ti];
-  const int blocks = (t.rows + kPrepRows - 1) / kPrepRows;
+  const int blocks = (t.rows + a.block_rows - 1) / a.block_rows;
   if ((int)blockIdx.x >= blocks) return;
   const int len = lnn::attn_length(a.lengths, head / t.per_batch, a.kv_len, a.status);
-  const int end = min(t.rows, len - t.past), dim = a.dim;        // rows from here on are padding
-  const float* src = t.src + (int64_t)head * t.rows * dim;
-  const bool is_do = a.o != nullptr && ti == a.tensors - 1;
+  const int end = min(t.rows, len - t.past), dim = a.dim, first = t.first, sinks = t.sinks;      // rows from `end` on are padding
+  const bool is_do = a.o != nullptr && ti == a.tensors - 1, with_norms = t.norms != nullptr;
   const bool vec = dim % 4 == 0 && (((uintptr_t)t.src | (is_do ? (uintptr_t)a.o : 0)) & 15) == 0;
-  const auto load = [&](const float* base, int r) {
-    const float* p = base + (int64_t)r * dim + c;
+  const float* src = t.src + (int64_t)head * t.rows * dim + c;
+  const float* src_o = a.o + (int64_t)head * t.rows * dim + c;
+  const auto load = [&](const float* p) {                        // (p: this lane's four values)
     if (vec) return c < dim ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     return make_float4(c < dim ? __ldg(p) : 0.0f, c + 1 < dim ? __ldg(p + 1) : 0.0f, c + 2 < dim ? __ldg(p + 2) : 0.0f,
                        c + 3 < dim ? __ldg(p + 3) : 0.0f);
-  };
-  const auto largest = [&](float4 v) {
-    return max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
-               max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
   };
   const auto row_total = [&](float v) {                          // over the lanes of a row
 #pragma unroll
     for (int s = LANES / 2; s > 0; s >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, s));
     return v;
   };
+  const auto warp_max = [&](float v) {
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, s));
+    return v;
+  };
   float4 x[BATCH], y[BATCH];
   const auto fetch = [&](int r0) {
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
-      const int r = r0 + u * kWarps * ROWS;
-      const bool real = r < end && (r >= t.first || r < t.sinks);
-      x[u] = real ? load(src, r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (is_do) y[u] = real ? load(a.o + (int64_t)head * t.rows * dim, r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const int r = r0 + u * STRIDE;
+      const bool real = r < end && (r >= first || r < sinks);
+      x[u] = y[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (real) x[u] = load(src + (int64_t)r * dim);
+      if (is_do && real) y[u] = load(src_o + (int64_t)r * dim);
     }
   };
-  const int r_first = blockIdx.x * kPrepRows + warp * ROWS + sub;
+  const int r_first = blockIdx.x * a.block_rows + warp * ROWS + sub, r_end = min((int)(blockIdx.x + 1) * a.block_rows, t.rows);
   fetch(r_first);
-  // the scale, from rows spread over those that are real (the same ones in every block of the head)
-  uint32_t m = 0;
-  const int span = end - t.first;
+  // the scale, from rows spread over those that are real (the same ones in every block of the head; what is not a number is
+  // left out here and found below)
+  float top = 0.0f;
+  const int span = end - first;
   if (span > 0) {
 #pragma unroll
-    for (int i = warp * ROWS + sub; i < kSampleRows; i += kWarps * ROWS)
-      m = max(m, largest(load(src, t.first + (int)((int64_t)i * span / kSampleRows))));
+    for (int i = warp * ROWS + sub; i < kSampleRows; i += STRIDE) {
+      const float4 v = load(src + (int64_t)(first + (int)((int64_t)i * span / kSampleRows)) * dim);
+      top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+    }
   }
-  m = __reduce_max_sync(0xffffffffu, m);
-  if (lane == 0) red[warp] = m;
+  top = warp_max(top);
+  if (lane == 0) red[warp] = top;
   __syncthreads();
-  m = red[0];
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) m = max(m, red[w]);
-  const int ebits = (int)(m >> 23);
-  const int e = m == 0u || ebits == 255 ? 0 : max(ebits, 1) - 127 - 8;
-  const Pow2Scale scale(-e);
+  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, red[w]);
+  const int ebits = (int)(__float_as_uint(top) >> 23);
+  const int e = top == 0.0f || ebits == 255 ? 0 : ebits - 127 - 8;
+  const float factor = t.sign * pow2f_int(max(-126, min(127, -e)));       // (|e| > 100 is not taken anyway)
+  const uint64_t factor2 = pack2(factor, factor), minus = pack2(-1.0f, -1.0f);
   __syncthreads();
 
-  __half* hi = t.hi + (int64_t)head * t.rows * a.width;
+  __half* hi = t.hi + (int64_t)head * t.rows * a.width + c;
   __half* lo = hi + (int64_t)t.heads * t.rows * a.width;
-  uint32_t top = 0;
   float top_norm = 0.0f;
-  const int r_end = min((int)(blockIdx.x + 1) * kPrepRows, t.rows);
-  for (int r0 = r_first; r0 < (int)(blockIdx.x + 1) * kPrepRows; r0 += BATCH * kWarps * ROWS) {
+  bool finite = true;
+  top = 0.0f;
+  for (int r0 = r_first; r0 - sub < r_end; r0 += BATCH * STRIDE) {      // (the same turns for both rows of a warp)
     if (r0 != r_first) fetch(r0);
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
-      const int r = r0 + u * kWarps * ROWS;
+      const int r = r0 + u * STRIDE;
       const bool in = r < r_end;
-      const float v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
       if (is_do) {
         const float delta = row_total(fmaf(x[u].w, y[u].w, fmaf(x[u].z, y[u].z, fmaf(x[u].y, y[u].y, __fmul_rn(x[u].x, y[u].x)))));
-        if (c == 0 && in) {
-          a.delta_p[(int64_t)head * a.pitch + r] = delta;
-          a.lse_p[(int64_t)head * a.pitch + r] = r < end ? a.lse[(int64_t)head * t.rows + r] : CUDART_INF_F;
-        }
+        if (c == 0 && in) a.delta_p[(int64_t)head * a.pitch + r] = delta;
       }
-      __half h[4], l[4];
+      uint32_t h[2], l[2];
       float norm = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float xs = scale(__fmul_rn(v[k], t.sign));
-        top = max(top, __float_as_uint(xs) & 0x7fffffffu);
-        norm = fmaf(xs, xs, norm);
-        split_half(xs, h[k], l[k]);
+      for (int k = 0; k < 2; ++k) {
+        const uint64_t v = mul2(k ? pack2(x[u].z, x[u].w) : pack2(x[u].x, x[u].y), factor2);
+        float p, q;
+        unpack2(v, p, q);
+        top = fmaxf(top, fmaxf(fabsf(p), fabsf(q)));
+        norm = fmaf(q, q, fmaf(p, p, norm));
+        const __half2 hh = __floats2half2_rn(p, q);
+        const float2 f = __half22float2(hh);
+        unpack2(fma2(pack2(f.x, f.y), minus, v), p, q);
+        const __half2 ll = __floats2half2_rn(p, q);
+        h[k] = *reinterpret_cast<const uint32_t*>(&hh);
+        l[k] = *reinterpret_cast<const uint32_t*>(&ll);
       }
+      finite = finite && norm <= 3.0e38f;                         // (false for what is not a number)
       if (in && c < a.width) {
-        *reinterpret_cast<uint2*>(hi + (int64_t)r * a.width + c) = *reinterpret_cast<uint2*>(h);
-        *reinterpret_cast<uint2*>(lo + (int64_t)r * a.width + c) = *reinterpret_cast<uint2*>(l);
+        *reinterpret_cast<uint2*>(hi + (int64_t)r * a.width) = make_uint2(h[0], h[1]);
+        *reinterpret_cast<uint2*>(lo + (int64_t)r * a.width) = make_uint2(l[0], l[1]);
       }
-      if (t.norms) {
-        norm = sqrtf(row_total(norm));
+      if (with_norms) {
+        norm = row_total(norm);
         top_norm = fmaxf(top_norm, norm);
         if (c == 0 && in) t.norms[(int64_t)head * t.rows + r] = norm;
       }
     }
   }
-  if (is_do && (int)blockIdx.x == blocks - 1)                    // columns that exist in no head
-    for (int r = t.rows + threadIdx.x; r < a.pitch; r += kPrepThreads) {
-      a.delta_p[(int64_t)head * a.pitch + r] = 0.0f;
-      a.lse_p[(int64_t)head * a.pitch + r] = CUDART_INF_F;
-    }
-#pragma unroll
-  for (int s = 16; s >= LANES; s >>= 1) top_norm = fmaxf(top_norm, __shfl_xor_sync(0xffffffffu, top_norm, s));
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0) { red[warp] = top; redn[warp] = top_norm; }
+  if (is_do) {
+    for (int r = blockIdx.x * a.block_rows + threadIdx.x; r < r_end; r += kPrepThreads)
+      a.lse_p[(int64_t)head * a.pitch + r] = r < end ? __ldg(a.lse + (int64_t)head * t.rows + r) : CUDART_INF_F;
+    if ((int)blockIdx.x == blocks - 1)                           // columns that exist in no head
+      for (int r = t.rows + threadIdx.x; r < a.pitch; r += kPrepThreads) {
+        a.delta_p[(int64_t)head * a.pitch + r] = 0.0f;
+        a.lse_p[(int64_t)head * a.pitch + r] = CUDART_INF_F;
+      }
+  }
+  top = __all_sync(0xffffffffu, finite) ? warp_max(top) : CUDART_INF_F;
+  top_norm = warp_max(top_norm);
+  if (lane == 0) { red[warp] = top; red_norm[warp] = top_norm; }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kPrepThreads / 32; ++w) { top = max(top, red[w]); top_norm = fmaxf(top_norm, redn[w]); }
+    for (int w = 1; w < kWarps; ++w) { top = fmaxf(top, red[w]); top_norm = fmaxf(top_norm, red_norm[w]); }
     const int64_t at = (int64_t)blockIdx.y * a.blocks;
     __stcg(a.block_max + at + blockIdx.x, top);
     __stcg(a.block_norm + at + blockIdx.x, top_norm);
@@ -198,18 +210,16 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
   __syncthreads();
   if (!last_block || warp != 0) return;
   __threadfence();
-  top = 0;
+  top = 0.0f;
   top_norm = 0.0f;
   for (int i = lane; i < blocks; i += 32) {
-    top = max(top, __ldcg(a.block_max + (int64_t)blockIdx.y * a.blocks + i));
+    top = fmaxf(top, __ldcg(a.block_max + (int64_t)blockIdx.y * a.blocks + i));
     top_norm = fmaxf(top_norm, __ldcg(a.block_norm + (int64_t)blockIdx.y * a.blocks + i));
   }
-  top = __reduce_max_sync(0xffffffffu, top);
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) top_norm = fmaxf(top_norm, __shfl_xor_sync(0xffffffffu, top_norm, s));
+  top = warp_max(top);
+  top_norm = warp_max(top_norm);
   if (lane == 0) {
-    const float largest = __uint_as_float(top);
-    a.info[blockIdx.y] = HeadInfo{e, top == 0u || (largest >= 4.0f && largest < 65000.0f), top_norm};
+    a.info[blockIdx.y] = HeadInfo{e, top == 0.0f || (top >= 4.0f && top < 65000.0f), sqrtf(top_norm)};
     a.counters[blockIdx.y] = 0;
   }
 }
@@ -218,7 +228,7 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
 struct TcArgs {
   AttnArgs a;
   const float *lse_p, *delta_p;  // [q head][pitch]
-  const float* norms;            // DQ: of dO's rows, DK: of V's
+  const float* norms;            // squares, DQ: of dO's rows, DK: of V's
   int pitch, width;
   int works;
   const uint32_t* x2;            // DQ: dO, DK: V, split
@@ -821,7 +831,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       float row_lse = CUDART_INF_F, row_delta = 0.0f;              // DQ
       int row_exp = 0;                                             // DQ, DK: dS is scaled by 2^row_exp
       float norm = 0.0f;
-      if (S::TWO && row < rows) norm = __ldg(t.norms + (int64_t)xh * rows + row);
+      if (S::TWO && row < rows) norm = sqrtf(__ldg(t.norms + (int64_t)xh * rows + row));
       if (MODE == DQ && row < rows) {
         row_lse = __ldg(t.lse_p + (int64_t)xh * t.pitch + row);
         row_delta = __ldg(t.delta_p + (int64_t)xh * t.pitch + row);
@@ -1109,7 +1119,12 @@ int prepare(lnn::Device* d, AttnArgs& a, Operands& op, bool backward) {
   __half* at[4] = {h, h + 2 * sq, h + 2 * sq + 2 * sk, h + 2 * sq + 4 * sk};
   p.tensors = backward ? 4 : 3;
   p.dim = a.dim; p.batch = a.batch; p.lengths = a.lengths; p.kv_len = a.kv_len; p.status = a.status;
-  p.blocks = (a.kv_len + kPrepRows - 1) / kPrepRows;
+  // one round of blocks: each has about 5 us of latencies (the sample, the last block's turn) to hide behind its rows
+  const auto row_blocks = [&](int rows) { return ((int64_t)rows + p.block_rows - 1) / p.block_rows; };
+  p.block_rows = kPrepRows;
+  while ((backward ? 2 : 1) * nq * row_blocks(a.q_len) + 2 * nk * row_blocks(a.kv_len) > kPrepBlocksPerSm * d->sm_count && p.block_rows < 1024)
+    p.block_rows += kPrepRows;
+  p.blocks = (int)row_blocks(a.kv_len);
   p.pitch = (a.q_len + 7) / 8 * 8 + kRowsM;
   const int64_t heads = 2 * nk + (backward ? 2 : 1) * nq;
   const int64_t norm_words = backward ? nk * a.kv_len + nq * a.q_len : 0, col_words = backward ? 2 * nq * p.pitch : 0;
@@ -1119,7 +1134,7 @@ int prepare(lnn::Device* d, AttnArgs& a, Operands& op, bool backward) {
   float* s = op.small.as<float>();
   p.info = (HeadInfo*)s; s += info_words;
   p.lse_p = s; p.delta_p = s + col_words / 2; s += (col_words + 3) / 4 * 4;       // (16-byte aligned: the pitch is a multiple of 8)
-  p.block_max = (uint32_t*)s; s += heads * p.blocks;
+  p.block_max = s; s += heads * p.blocks;
   p.block_norm = s; s += heads * p.blocks;
   float *norm_v = backward ? s : nullptr, *norm_do = backward ? s + nk * a.kv_len : nullptr;
   p.counters = d->tile_counters;
