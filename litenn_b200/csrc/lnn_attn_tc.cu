@@ -232,6 +232,9 @@ struct TcArgs {
   int pitch, width;
   int works;
   const uint32_t* x2;            // DQ: dO, DK: V, split
+  // FWD, DQ: the works from `whole` on are cut into `splits` each (few tiles, or few in the last round of the SMs)
+  int whole;
+  float2* stats;                 // FWD: [part][128] maximum and sum of a row
   // DV, DK: keys below sinks take `splits_sink` works per tile of rows, the others `splits`
   int tiles, sink_tiles, splits_sink, splits;
   float* parts;                  // [part][128][DP] of the tiles that have several works
@@ -265,8 +268,9 @@ __device__ __forceinline__ int64_t parts_per_head(const TcArgs& t) {
 struct Work {
   int b, hk, h, row0, steps;
   int p_hi, lowest, sink_n, sink_steps;  // queries: positions
+  int s0;                                // queries: first step
   int i_lo, nq, q_hi, hq0, q0;           // keys: first query, tiles of queries per head, position of the last query; first step
-  int split_up;                          // keys: one of several works of its rows
+  int split_up;                          // one of several works of its rows
   int skip;                              // the FP32 pipe's
   int part;                              // its place among the parts
   int ek, ev, eq, eo;                    // exponents of the scales (eq, eo: of query head h)
@@ -282,6 +286,13 @@ __device__ __forceinline__ void make_work(Work& k, const TcArgs& t, int w, bool 
   k.split_up = 0;
   if (!S::KEYS) {
     // the last tiles first: they see most, and the short ones fill up what is left
+    int split = 0, splits = 1;
+    k.part = w - t.whole;
+    if (w >= t.whole) {
+      splits = t.splits;
+      split = k.part % splits;
+      w = t.whole + k.part / splits;
+    }
     const int heads = a.batch * a.q_heads, turn = w / heads, head = w - turn * heads;
     k.b = head / a.q_heads; k.h = head - k.b * a.q_heads; k.hk = k.h / group;
     const int len = lnn::attn_length(a.lengths, k.b, a.kv_len, a.status);
@@ -291,8 +302,11 @@ __device__ __forceinline__ void make_work(Work& k, const TcArgs& t, int w, bool 
       k.lowest = max(k.row0 + past - a.window + 1, 0);
       k.sink_n = min(a.sinks, k.lowest);
       k.sink_steps = (k.sink_n + S::BN - 1) / S::BN;
-      k.steps = k.sink_steps + (k.p_hi - k.lowest) / S::BN + 1;
+      const int all = k.sink_steps + (k.p_hi - k.lowest) / S::BN + 1;
+      k.s0 = (int)((int64_t)all * split / splits);
+      k.steps = (int)((int64_t)all * (split + 1) / splits) - k.s0;
     }
+    k.split_up = splits > 1;
   } else {
     // the first tiles first: most queries see them
     const int heads = a.batch * a.kv_heads;
@@ -336,7 +350,7 @@ template <int MODE, int DP>
 struct Steps {
   int head, r, n, s, q;
   __device__ __forceinline__ Steps(const TcArgs& t, const Work& k) : s(0) {
-    if (!Shape<MODE, DP>::KEYS) { head = k.b * t.a.kv_heads + k.hk; q = 0; }
+    if (!Shape<MODE, DP>::KEYS) { head = k.b * t.a.kv_heads + k.hk; q = 0; s = k.s0; }
     else { head = k.b * t.a.q_heads + k.h + k.hq0; q = k.q0; }
     at(t, k);
   }
@@ -751,7 +765,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
         }
         empty = steps == 0 || row + past > k.p_hi;
         mul = __fmul_rn(__fdiv_rn(1.0f, sum), pow2f_int(k.ev));
-        if (part == 0 && row < rows)
+        if (k.split_up) {
+          mul = 1.0f;
+          if (part == 0) t.stats[(int64_t)k.part * kRowsM + row_in] = make_float2(empty ? -CUDART_INF_F : top, empty ? 0.0f : sum);
+        } else if (part == 0 && row < rows)
           a.lse[(int64_t)xh * rows + row] = empty ? CUDART_INF_F : __fadd_rn(top, __fsub_rn(log2f(sum), 14.0f));
         dst = a.o;
       } else if (MODE == DQ) {
@@ -761,11 +778,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
         if (MODE == DK) mul = fabsf(a.scale);
         dst = MODE == DK ? a.dk : a.dv;
         accumulate = MODE == DK ? a.acc_k : a.acc_v;
-        if (k.split_up) {
-          dst = t.parts; accumulate = 0; limit = k.row0 + kRowsM;
-          at = ((int64_t)k.part * kRowsM + row_in) * DP;
-          pitch_cols = DP;
-        }
+      }
+      if (k.split_up) {
+        dst = t.parts; accumulate = 0; limit = k.row0 + kRowsM;
+        at = ((int64_t)k.part * kRowsM + row_in) * DP;
+        pitch_cols = DP;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bar_w_empty[slot]));
@@ -1062,6 +1079,57 @@ attn_parts_kernel(float* __restrict__ dst, const float* __restrict__ parts, cons
   }
 }
 
+// O or dQ of the tiles of queries that several works shared.
+template <int MODE, int DP>
+__global__ void __launch_bounds__(256)
+attn_merge_kernel(const __grid_constant__ TcArgs t) {
+  lnn::wait_for_previous();
+  constexpr int ROWS = kRowsM / kPartBlocks;
+  const AttnArgs& a = t.a;
+  const int work = blockIdx.x / kPartBlocks, first = blockIdx.x % kPartBlocks * ROWS;
+  const int heads = a.batch * a.q_heads, w = t.whole + work, turn = w / heads, head = w - turn * heads;
+  const int b = head / a.q_heads, hk = (head - b * a.q_heads) / (a.q_heads / a.kv_heads), row0 = (t.tiles - 1 - turn) * kRowsM;
+  if (!lnn::group_ok(a, b, hk)) return;
+  const int past = a.kv_len - a.q_len, len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
+  const float scale_v = MODE == FWD ? pow2f_int(lnn::info_of(a, 2, b * a.kv_heads + hk).e) : 1.0f;
+  const int64_t part0 = (int64_t)work * t.splits;
+  for (int i = threadIdx.x; i < ROWS * DP / 4; i += 256) {
+    const int r = first + i / (DP / 4), col = i % (DP / 4) * 4, row = row0 + r;
+    if (row >= a.q_len || col >= a.dim) continue;
+    const float4* from = reinterpret_cast<const float4*>(t.parts + (part0 * kRowsM + r) * DP + col);
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float top = -CUDART_INF_F, total = 0.0f;
+    if (MODE == FWD)
+      for (int k = 0; k < t.splits; ++k) top = fmaxf(top, __ldg(t.stats + (part0 + k) * kRowsM + r).x);
+    const float base = top == -CUDART_INF_F ? 0.0f : top;
+#pragma unroll 4
+    for (int k = 0; k < t.splits; ++k) {
+      const float4 x = __ldg(from + (int64_t)k * (kRowsM * DP / 4));
+      float f = 1.0f;
+      if (MODE == FWD) {
+        const float2 st = __ldg(t.stats + (part0 + k) * kRowsM + r);
+        f = exp2_fast(__fsub_rn(st.x, base));
+        total = fmaf(f, st.y, total);
+      }
+      s = make_float4(fmaf(x.x, f, s.x), fmaf(x.y, f, s.y), fmaf(x.z, f, s.z), fmaf(x.w, f, s.w));
+    }
+    const int64_t at = ((int64_t)head * a.q_len + row) * a.dim + col;
+    float v[4] = {s.x, s.y, s.z, s.w};
+    if (MODE == FWD) {
+      const bool empty = row + past >= len;
+      const float mul = empty ? 0.0f : __fmul_rn(__fdiv_rn(1.0f, total), scale_v);
+      if (col == 0) a.lse[(int64_t)head * a.q_len + row] = empty ? CUDART_INF_F : __fadd_rn(top, __fsub_rn(log2f(total), 14.0f));
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (col + u < a.dim) a.o[at + u] = empty ? 0.0f : __fmul_rn(v[u], mul);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (col + u < a.dim) a.dq[at + u] = a.acc_q ? __fadd_rn(a.dq[at + u], v[u]) : v[u];
+    }
+  }
+}
+
 // ---- host ------------------------------------------------------------------------------------------------
 // [2 heads][rows][width] fp16: lo behind hi; the boxes are 64 wide (zeros behind the width)
 int operand_map(CUtensorMap* tm, const void* base, int width, int rows, int64_t heads) {
@@ -1081,7 +1149,10 @@ int launch_pass(lnn::Device* d, const CUtensorMap* x, const CUtensorMap* y, cons
   return LNN_OK;
 }
 
-// Works of a pass over keys: a tile's steps are cut so that there are about three works per SM and none is longer than that.
+// What a work costs beside its steps (its first loads, its results), in steps; the traffic of one part; a launch.
+constexpr double kWorkCost = 3.0, kPartCost = 0.011, kMergeCost = 1.5;
+
+// Works of a pass over keys: how often a tile's steps are cut, so that the rounds of the SMs come out even.
 template <int MODE, int DP>
 void plan_keys(const lnn::Device* d, TcArgs& t) {
   constexpr int BN = Shape<MODE, DP>::BN;
@@ -1089,13 +1160,42 @@ void plan_keys(const lnn::Device* d, TcArgs& t) {
   const int64_t group = a.q_heads / a.kv_heads, heads = (int64_t)a.batch * a.kv_heads;
   t.tiles = (a.kv_len + kRowsM - 1) / kRowsM;
   t.sink_tiles = std::min(t.tiles, (a.sinks + kRowsM - 1) / kRowsM);
-  const int64_t most = group * ((a.q_len + BN - 1) / BN + 1);
+  const int64_t most = group * ((a.q_len + BN - 1) / BN + 1);                      // steps of a tile that sees all queries
   const int64_t some = std::min<int64_t>(most, group * ((std::min<int64_t>((int64_t)a.window + kRowsM, a.q_len) + BN - 1) / BN + 1));
-  const int64_t total = heads * (t.sink_tiles * most + (t.tiles - t.sink_tiles) * some);
-  const int64_t length = std::max<int64_t>(6, total / (d->sm_count * 3));
-  t.splits_sink = (int)std::min<int64_t>(64, (most + length - 1) / length);
-  t.splits = (int)std::min<int64_t>(64, (some + length - 1) / length);
-  t.works = (int)(heads * (t.sink_tiles * t.splits_sink + (t.tiles - t.sink_tiles) * t.splits));
+  double best = 0.0;
+  for (int splits = 1; splits <= 32 && splits <= some; ++splits) {
+    const int64_t length = (some + splits - 1) / splits, sink = std::min<int64_t>(64, (most + length - 1) / length);
+    const int64_t works = heads * (t.sink_tiles * sink + (t.tiles - t.sink_tiles) * splits);
+    const int64_t parts = heads * ((sink > 1 ? t.sink_tiles * sink : 0) + (splits > 1 ? (t.tiles - t.sink_tiles) * splits : 0));
+    const double cost = (double)((works + d->sm_count - 1) / d->sm_count) * (double)(std::max(length, (most + sink - 1) / sink) + kWorkCost) +
+                        kPartCost * (double)parts + (parts ? kMergeCost : 0.0);
+    if (splits == 1 || cost < best) {
+      best = cost;
+      t.splits = splits; t.splits_sink = (int)sink; t.works = (int)works;
+    }
+  }
+}
+
+// Works of a pass over queries: those of the last round of the SMs, or all where they are few, may be cut.
+template <int MODE, int DP>
+void plan_queries(const lnn::Device* d, TcArgs& t) {
+  constexpr int BN = Shape<MODE, DP>::BN;
+  const AttnArgs& a = t.a;
+  t.tiles = (a.q_len + kRowsM - 1) / kRowsM;
+  const int64_t all = (int64_t)a.batch * a.q_heads * t.tiles, full = all / d->sm_count, rest = all - full * d->sm_count;
+  // steps of the first work of the last round, the longest of them
+  const int64_t row0 = (t.tiles - 1 - full * d->sm_count / ((int64_t)a.batch * a.q_heads)) * kRowsM, past = a.kv_len - a.q_len;
+  const int64_t p_hi = std::min<int64_t>(row0 + kRowsM, a.q_len) - 1 + past, lowest = std::max<int64_t>(row0 + past - a.window + 1, 0);
+  const int64_t steps = rest > 0 ? (std::min<int64_t>(a.sinks, lowest) + BN - 1) / BN + (p_hi - lowest) / BN + 1 : 0;
+  double best = (rest > 0 ? 1.0 : 0.0) * ((double)steps + kWorkCost);
+  t.splits = 1;
+  for (int splits = 2; splits <= 32 && splits <= steps && rest > 0; ++splits) {
+    const double cost = (double)((rest * splits + d->sm_count - 1) / d->sm_count) * ((double)((steps + splits - 1) / splits) + kWorkCost) +
+                        kPartCost * (double)(rest * splits) + kMergeCost;
+    if (cost < best) { best = cost; t.splits = splits; }
+  }
+  t.whole = t.splits > 1 ? (int)(full * d->sm_count) : (int)all;
+  t.works = t.whole + (int)(t.splits > 1 ? rest * t.splits : 0);
 }
 
 struct Operands {
@@ -1154,6 +1254,24 @@ int prepare(lnn::Device* d, AttnArgs& a, Operands& op, bool backward) {
   return LNN_OK;
 }
 
+template <int MODE, int DP>
+int queries_pass(lnn::Device* d, TcArgs t, const CUtensorMap* x, const CUtensorMap* y, const CUtensorMap* z) {
+  plan_queries<MODE, DP>(d, t);
+  lnn::Scratch parts(d);
+  const int64_t n = t.works - t.whole;
+  if (n > 0) {
+    int rc = parts.get((uint64_t)n * kRowsM * (DP * 4 + (MODE == FWD ? 8 : 0)));
+    if (rc) return rc;
+    t.parts = parts.as<float>();
+    t.stats = reinterpret_cast<float2*>(t.parts + n * kRowsM * DP);
+  }
+  int rc = launch_pass<MODE, DP>(d, x, y, z, t);
+  if (rc || n == 0) return rc;
+  LNN_CUDA(lnn::launch_chained(d, attn_merge_kernel<MODE, DP>, (unsigned)(n / t.splits * kPartBlocks), 256, 0, t));
+  LNN_CHECK_LAUNCH(d);
+  return LNN_OK;
+}
+
 template <int DP>
 int tc_fwd(lnn::Device* d, AttnArgs a) {
   Operands op(d);
@@ -1162,9 +1280,7 @@ int tc_fwd(lnn::Device* d, AttnArgs a) {
   TcArgs t = {};
   t.a = a;
   t.width = op.p.width;
-  t.tiles = (a.q_len + kRowsM - 1) / kRowsM;
-  t.works = a.batch * a.q_heads * t.tiles;
-  rc = launch_pass<FWD, DP>(d, &op.map[0], &op.map[1], &op.map[2], t);
+  rc = queries_pass<FWD, DP>(d, t, &op.map[0], &op.map[1], &op.map[2]);
   return rc ? rc : lnn::attn_simt_fwd(d, a);                     // the heads that were marked
 }
 
@@ -1201,9 +1317,7 @@ int tc_bwd(lnn::Device* d, AttnArgs a) {
     TcArgs q = t;
     q.norms = op.p.t[3].norms;
     q.x2 = (const uint32_t*)op.p.t[3].hi;
-    q.tiles = (a.q_len + kRowsM - 1) / kRowsM;
-    q.works = a.batch * a.q_heads * q.tiles;
-    rc = launch_pass<DQ, DP>(d, &op.map[0], &op.map[1], &op.map[2], q);
+    rc = queries_pass<DQ, DP>(d, q, &op.map[0], &op.map[1], &op.map[2]);
     if (rc) return rc;
   }
   if (a.dv) {
