@@ -60,148 +60,150 @@ embedding_fwd_kernel(T* __restrict__ Y, const T* __restrict__ table, const float
 
 // ---- gradient of the table ---------------------------------------------------------------------
 // Tokens are sorted by row, stably (radix sort, 8 bits a pass), so that the terms of a row are added in the order
-// of the tokens whatever the launch looks like: no atomics on values.
-constexpr int kSortWarps = kThreads / 32;
-constexpr int kMaxSortBlocks = 64;
+// of the tokens whatever the launch looks like: no atomics on values.  One cluster of eight blocks sorts: its passes are
+// short chains of dependent steps, which meet in distributed shared memory instead of at the ends of kernels (16384 tokens of
+// 50001 rows: four launches took 32 us), and the other clusters write the zeros of the rows without tokens meanwhile.
+constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kSortBlocks = 8;
 constexpr int kSortKeys = 4;                       // per lane at a time
 
-// Sorting is a chain of short dependent steps; rows without tokens have to become zero.  Blocks behind the first
-// `sort_blocks` of every launch write a share of the zeros meanwhile.
 struct SortArgs {
-  const float* ids;                                // the first pass reads these, the later ones keys and at
-  const uint32_t *keys, *at;
-  uint32_t *out_keys, *out_at, *hist;              // hist [sort_blocks][256]
+  const float* ids;
+  uint32_t *keys[2], *at[2];                       // by turns; the last pass leaves its result in keys[(passes - 1) & 1]
   int64_t n;
-  int vocab, shift, sort_blocks;
-  float4* zeros;                                   // [zero_begin, zero_end) of the table in 16-byte units, and its odd floats
-  int64_t zero_begin, zero_end;
-  float* odd;
-  int odds;
+  int vocab, passes;
+  float4* zeros;                                   // the table in 16-byte units, and the floats in front and behind
+  int64_t quads;
+  float *lead, *tail;
+  int leads, tails;
   int* status;
 };
-__device__ __forceinline__ void write_zeros(const SortArgs& a) {
-  const int64_t stride = (int64_t)(gridDim.x - a.sort_blocks) * kThreads;
-  const int64_t first = (int64_t)(blockIdx.x - a.sort_blocks) * kThreads + threadIdx.x;
-  for (int64_t i = a.zero_begin + first; i < a.zero_end; i += stride) a.zeros[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (first < a.odds) a.odd[first] = 0.0f;
-}
-
-// The share of a block, cut into one contiguous strip per warp, which takes kSortKeys * 32 tokens of it at a time.
-struct SortStrip {
-  int64_t begin, end;
-  __device__ __forceinline__ explicit SortStrip(const SortArgs& a) {
-    const int64_t per = ((a.n + a.sort_blocks - 1) / a.sort_blocks + kThreads - 1) / kThreads * 32;      // tokens per warp
-    begin = min(((int64_t)blockIdx.x * kSortWarps + (threadIdx.x >> 5)) * per, a.n);
-    end = min(begin + per, a.n);
-  }
-};
 constexpr uint32_t kNoKey = 0xffffffffu;
-__device__ __forceinline__ void load_keys(const SortArgs& a, int64_t i0, int64_t end, uint32_t (&key)[kSortKeys]) {
+
+// The lanes whose key has this lane's digit; none for a lane without a key.  Eight votes take a fraction of the time of one
+// __match_any_sync.
+__device__ __forceinline__ uint32_t same_digit(uint32_t key, int shift) {
+  uint32_t same = __ballot_sync(0xffffffffu, key != kNoKey);
 #pragma unroll
-  for (int u = 0; u < kSortKeys; ++u) {
-    const int64_t i = i0 + u * 32 + (threadIdx.x & 31);
-    key[u] = kNoKey;
-    if (i < end) {
-      if (a.keys) {
-        key[u] = __ldg(a.keys + i);
-      } else {
-        const int row = token_row(__ldg(a.ids + i), a.vocab, i, 2, a.status);
-        key[u] = row < 0 ? (uint32_t)a.vocab : (uint32_t)row;    // padding comes last
-      }
-    }
+  for (int bit = 0; bit < 8; ++bit) {
+    const bool one = (key >> (shift + bit)) & 1u;
+    const uint32_t ones = __ballot_sync(0xffffffffu, one);
+    same &= one ? ones : ~ones;
   }
-}
-__device__ __forceinline__ uint32_t digit_of(uint32_t key, int shift) { return key == kNoKey ? 256u : (key >> shift) & 255u; }
-__device__ __forceinline__ void count_digits(uint32_t* count, const uint32_t (&key)[kSortKeys], int shift) {
-#pragma unroll
-  for (int u = 0; u < kSortKeys; ++u) {
-    const uint32_t digit = digit_of(key[u], shift);
-    const uint32_t same = __match_any_sync(0xffffffffu, digit);
-    if (digit < 256u && (threadIdx.x & 31) == __ffs(same) - 1) count[digit] += __popc(same);
-    __syncwarp();
-  }
+  return key == kNoKey ? 0u : same;
 }
 
-__global__ void __launch_bounds__(kThreads)
-sort_count_kernel(const __grid_constant__ SortArgs a) {
+__global__ void __launch_bounds__(kSortThreads, 2) __cluster_dims__(kSortBlocks, 1, 1)
+sort_tokens_kernel(const __grid_constant__ SortArgs a) {
   __shared__ uint32_t count[kSortWarps][256];
+  __shared__ uint32_t hist[256], warp_total[8];
   lnn::wait_for_previous();
-  if ((int)blockIdx.x >= a.sort_blocks) { write_zeros(a); return; }
-  for (int i = threadIdx.x; i < kSortWarps * 256; i += kThreads) (&count[0][0])[i] = 0;
-  const SortStrip s(a);
-  uint32_t key[kSortKeys];
-  load_keys(a, s.begin, s.end, key);
-  __syncthreads();
-  for (int64_t i0 = s.begin; i0 < s.end; i0 += kSortKeys * 32) {
-    if (i0 > s.begin) load_keys(a, i0, s.end, key);
-    count_digits(count[threadIdx.x >> 5], key, a.shift);
+  if (blockIdx.x >= kSortBlocks) {
+    const int64_t first = (int64_t)(blockIdx.x - kSortBlocks) * kSortThreads + threadIdx.x;
+    const int64_t stride = (int64_t)(gridDim.x - kSortBlocks) * kSortThreads;
+    for (int64_t i = first; i < a.quads; i += stride) a.zeros[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (first < a.leads) a.lead[first] = 0.0f;
+    if (first < a.tails) a.tail[first] = 0.0f;
+    return;
   }
-  __syncthreads();
-  uint32_t total = 0;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, block = blockIdx.x;
+  // a contiguous strip of the tokens per warp, in the order of the warps
+  const int64_t per = ((a.n + kSortBlocks * kSortWarps - 1) / (kSortBlocks * kSortWarps) + 31) / 32 * 32;
+  const int64_t begin = min((int64_t)(block * kSortWarps + warp) * per, a.n), end = min(begin + per, a.n);
+  const bool once = per <= kSortKeys * 32;                       // a strip's keys stay in registers
+  uint32_t key[kSortKeys], same[kSortKeys];
+  for (int pass = 0; pass < a.passes; ++pass) {
+    const uint32_t *keys = a.keys[(pass + 1) & 1], *from = a.at[(pass + 1) & 1];
+    uint32_t *out_keys = a.keys[pass & 1], *out_at = a.at[pass & 1];
+    const int shift = 8 * pass;
+    const auto load = [&](int64_t i0) {
 #pragma unroll
-  for (int w = 0; w < kSortWarps; ++w) total += count[w][threadIdx.x];
-  a.hist[blockIdx.x * 256 + threadIdx.x] = total;
-}
-
-__global__ void __launch_bounds__(kThreads)
-sort_scatter_kernel(const __grid_constant__ SortArgs a) {
-  __shared__ uint32_t count[kSortWarps][256];
-  __shared__ uint32_t warp_total[kSortWarps];
-  lnn::wait_for_previous();
-  if ((int)blockIdx.x >= a.sort_blocks) { write_zeros(a); return; }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < kSortWarps * 256; i += kThreads) (&count[0][0])[i] = 0;
-  const SortStrip s(a);
-  const bool once = s.end - s.begin <= kSortKeys * 32;           // the strip's keys stay in registers
-  uint32_t key[kSortKeys];
-  load_keys(a, s.begin, s.end, key);
-  // where this block's tokens of digit threadIdx.x begin: all smaller digits, then the blocks before this one
-  uint32_t before = 0, total = 0;
-#pragma unroll 16
-  for (int b = 0; b < a.sort_blocks; ++b) {
-    const uint32_t c = __ldg(a.hist + b * 256 + threadIdx.x);
-    if (b < (int)blockIdx.x) before += c;
-    total += c;
-  }
-  __syncthreads();
-  for (int64_t i0 = s.begin; i0 < s.end; i0 += kSortKeys * 32) {
-    if (i0 > s.begin) load_keys(a, i0, s.end, key);
-    count_digits(count[warp], key, a.shift);
-  }
-  uint32_t scan = total;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t v = __shfl_up_sync(0xffffffffu, scan, o);
-    if (lane >= o) scan += v;
-  }
-  if (lane == 31) warp_total[warp] = scan;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) scan += warp_total[w];
-  uint32_t base = scan - total + before;
-#pragma unroll
-  for (int w = 0; w < kSortWarps; ++w) {
-    const uint32_t c = count[w][threadIdx.x];
-    count[w][threadIdx.x] = base;
-    base += c;
-  }
-  __syncthreads();
-  for (int64_t i0 = s.begin; i0 < s.end; i0 += kSortKeys * 32) {
-    if (!once) load_keys(a, i0, s.end, key);
-#pragma unroll
-    for (int u = 0; u < kSortKeys; ++u) {
-      const int64_t i = i0 + u * 32 + lane;
-      const uint32_t digit = digit_of(key[u], a.shift);
-      const uint32_t same = __match_any_sync(0xffffffffu, digit);
-      uint32_t to = 0;
-      if (digit < 256u) to = count[warp][digit] + __popc(same & ((1u << lane) - 1u));
-      __syncwarp();
-      if (digit < 256u) {
-        if (lane == __ffs(same) - 1) count[warp][digit] += __popc(same);
-        a.out_keys[to] = key[u];
-        a.out_at[to] = a.at ? __ldg(a.at + i) : (uint32_t)i;
+      for (int u = 0; u < kSortKeys; ++u) {
+        const int64_t i = i0 + u * 32 + lane;
+        key[u] = kNoKey;
+        if (i < end) {
+          if (pass > 0) {
+            key[u] = __ldcg(keys + i);                           // (written by other blocks of this kernel)
+          } else {
+            const int row = token_row(__ldg(a.ids + i), a.vocab, i, 2, a.status);
+            key[u] = row < 0 ? (uint32_t)a.vocab : (uint32_t)row;      // padding comes last
+          }
+        }
       }
-      __syncwarp();
+    };
+    for (int i = threadIdx.x; i < kSortWarps * 256; i += kSortThreads) (&count[0][0])[i] = 0;
+    load(begin);
+    __syncthreads();
+    for (int64_t i0 = begin; i0 < end; i0 += kSortKeys * 32) {
+      if (i0 > begin) load(i0);
+#pragma unroll
+      for (int u = 0; u < kSortKeys; ++u) {
+        if (i0 + u * 32 >= end) break;
+        same[u] = same_digit(key[u], shift);
+        if (lane == __ffs(same[u]) - 1) count[warp][(key[u] >> shift) & 255u] += __popc(same[u]);
+        __syncwarp();
+      }
     }
+    __syncthreads();
+    if (threadIdx.x < 256) {
+      uint32_t total = 0;
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) total += count[w][threadIdx.x];
+      hist[threadIdx.x] = total;
+    }
+    cluster.sync();
+    // where this block's tokens of digit threadIdx.x begin: all smaller digits, then the blocks before this one
+    uint32_t before = 0, total = 0, scan = 0;
+    if (threadIdx.x < 256) {
+      uint32_t h[kSortBlocks];
+#pragma unroll
+      for (int b = 0; b < kSortBlocks; ++b) h[b] = cluster.map_shared_rank(hist, b)[threadIdx.x];
+#pragma unroll
+      for (int b = 0; b < kSortBlocks; ++b) {
+        if (b < block) before += h[b];
+        total += h[b];
+      }
+      scan = total;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += v;
+      }
+      if (lane == 31) warp_total[warp] = scan;
+    }
+    __syncthreads();
+    if (threadIdx.x < 256) {
+      for (int w = 0; w < warp; ++w) scan += warp_total[w];
+      uint32_t base = scan - total + before;
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t c = count[w][threadIdx.x];
+        count[w][threadIdx.x] = base;
+        base += c;
+      }
+    }
+    __syncthreads();
+    for (int64_t i0 = begin; i0 < end; i0 += kSortKeys * 32) {
+      if (!once) load(i0);
+#pragma unroll
+      for (int u = 0; u < kSortKeys; ++u) {
+        if (i0 + u * 32 >= end) break;
+        const int64_t i = i0 + u * 32 + lane;
+        const uint32_t digit = (key[u] >> shift) & 255u;
+        if (!once) same[u] = same_digit(key[u], shift);
+        uint32_t to = 0;
+        if (same[u]) to = count[warp][digit] + __popc(same[u] & ((1u << lane) - 1u));
+        __syncwarp();
+        if (same[u]) {
+          if (lane == __ffs(same[u]) - 1) count[warp][digit] += __popc(same[u]);
+          __stcg(out_keys + to, key[u]);
+          __stcg(out_at + to, pass > 0 ? __ldcg(from + i) : (uint32_t)i);
+        }
+        __syncwarp();
+      }
+    }
+    __threadfence();
+    cluster.sync();                                              // the next pass reads what all have written; hist is free
   }
 }
 
@@ -214,27 +216,42 @@ __global__ void __launch_bounds__(kThreads)
 table_grad_kernel(T* __restrict__ dtable, const T* __restrict__ dy, const uint32_t* __restrict__ keys,
                   const uint32_t* __restrict__ at, T* __restrict__ head, T* __restrict__ tail, int64_t tokens, int vocab,
                   int64_t units, float scale, int accumulate) {
+  // the block's sorted tokens, read once: the sums then wait for one load, not for three that depend on one another
+  __shared__ uint32_t key_of[kThreads / 32 * kPiece], token_of[kThreads / 32 * kPiece];
   lnn::wait_for_previous();
   const int64_t pieces = (tokens + kPiece - 1) / kPiece;
   const int64_t piece = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (piece >= pieces) return;
   const int64_t lo = piece * kPiece, hi = min(lo + kPiece, tokens);
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x;
+  for (int i = tid; i < (int)blockDim.y * kPiece; i += kThreads) {
+    const int64_t e = (int64_t)blockIdx.x * blockDim.y * kPiece + i;
+    if (e < tokens) {
+      key_of[i] = __ldg(keys + e);
+      token_of[i] = __ldg(at + e);
+    }
+  }
+  const uint32_t before = lo > 0 && lo < tokens ? __ldg(keys + lo - 1) : (uint32_t)vocab;
+  const uint32_t behind = hi < tokens ? __ldg(keys + hi) : (uint32_t)vocab;
+  __syncthreads();
+  if (piece >= pieces) return;
+  const uint32_t *key = key_of + threadIdx.y * kPiece, *token = token_of + threadIdx.y * kPiece;
+  const int n = (int)(hi - lo);
   for (int64_t c = threadIdx.x + (int64_t)blockIdx.y * blockDim.x; c < units; c += (int64_t)gridDim.y * blockDim.x) {
-    uint32_t cur = keys[lo];
-    bool continued = lo > 0 && keys[lo - 1] == cur;
+    uint32_t cur = key[0];
+    bool continued = before == cur;
     T sum = nothing<T>();
-    for (int64_t e0 = lo; e0 < hi; e0 += 8) {
+    for (int e0 = 0; e0 < n; e0 += 8) {
       T v[8];
       uint32_t k[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const bool in = e0 + u < hi;
-        k[u] = in ? keys[e0 + u] : cur;
-        v[u] = in && k[u] < (uint32_t)vocab ? __ldg(dy + at[e0 + u] * units + c) : nothing<T>();
+        const bool in = e0 + u < n;
+        k[u] = in ? key[e0 + u] : cur;
+        v[u] = in && k[u] < (uint32_t)vocab ? __ldg(dy + (int64_t)token[e0 + u] * units + c) : nothing<T>();
       }
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        if (e0 + u < hi) {
+        if (e0 + u < n) {
           if (k[u] != cur) {
             if (continued) {
               head[piece * units + c] = sum;
@@ -254,7 +271,7 @@ table_grad_kernel(T* __restrict__ dtable, const T* __restrict__ dy, const uint32
     if (cur >= (uint32_t)vocab) continue;
     if (continued) {
       head[piece * units + c] = sum;
-    } else if (hi < tokens && keys[hi] == cur) {
+    } else if (behind == cur) {
       tail[piece * units + c] = sum;
     } else {
       T* o = dtable + cur * units + c;
@@ -275,24 +292,37 @@ table_join_kernel(T* __restrict__ dtable, const uint32_t* __restrict__ keys, con
   const uint32_t row = keys[hi - 1];
   if (row >= (uint32_t)vocab || keys[hi] != row) return;                    // nothing goes on behind this piece
   if (keys[lo] == row && lo > 0 && keys[lo - 1] == row) return;             // it began earlier
-  // the last piece that has some of the row: it begins with it (steps that double, then halve)
-  const auto begins = [&](int64_t p) { return p < pieces && __ldg(keys + p * kPiece) == row; };
+  // the last piece that has some of the row: it begins with it.  Eight pieces are looked at at once, further apart each time.
   int64_t last = piece + 1, step = 1;
-  while (begins(last + step)) { last += step; step *= 2; }
-  for (; step > 0; step >>= 1)
-    if (begins(last + step)) last += step;
+  const auto advance = [&]() {
+    int found = 0;
+#pragma unroll
+    for (int u = 1; u <= 8; ++u) {
+      const int64_t p = last + u * step;
+      found += p < pieces && __ldg(keys + p * kPiece) == row ? 1 : 0;
+    }
+    last += found * step;
+    return found;
+  };
+  while (advance() == 8) step *= 8;
+  for (step /= 8; step > 0; step /= 8) advance();
   for (int64_t c = threadIdx.x + (int64_t)blockIdx.y * blockDim.x; c < units; c += (int64_t)gridDim.y * blockDim.x) {
     T sum = tail[piece * units + c];
-#pragma unroll 8
-    for (int64_t p = piece + 1; p <= last; ++p) sum = plus(sum, __ldg(head + p * units + c));
+    for (int64_t p0 = piece + 1; p0 <= last; p0 += 16) {
+      T v[16];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) v[u] = p0 + u <= last ? __ldg(head + (p0 + u) * units + c) : nothing<T>();
+#pragma unroll
+      for (int u = 0; u < 16; ++u)
+        if (p0 + u <= last) sum = plus(sum, v[u]);
+    }
     T* o = dtable + row * units + c;
     *o = accumulate ? plus(*o, scaled(sum, scale)) : scaled(sum, scale);
   }
 }
 
 // Threads along the columns of a row and rows per block.
-dim3 row_block(int64_t units) {
-  unsigned x = 1;
+dim3 row_block(int64_t units, unsigned x = 1) {
   while (x < kThreads && x < units) x *= 2;
   return dim3(x, kThreads / x);
 }
@@ -306,49 +336,32 @@ int embedding_bwd(lnn::Device* d, T* dtable, const T* dy, const float* ids, int6
                   float scale, int accumulate) {
   const int64_t pieces = lnn_ceil_div(tokens, kPiece);
   lnn::Scratch keys(d), parts(d);
-  SortArgs a = {};
-  a.sort_blocks = (int)std::min<int64_t>(kMaxSortBlocks, lnn_ceil_div(tokens, kSortKeys * kThreads));
   const int64_t pad = (tokens + 3) / 4 * 4;
-  int rc = keys.get((uint64_t)(4 * pad + a.sort_blocks * 256) * 4);
-  if (!rc) rc = parts.get((uint64_t)pieces * units * sizeof(T) * 2);
+  int rc = keys.get((uint64_t)(4 * pad) * 4);
+  if (!rc && pieces > 1) rc = parts.get((uint64_t)pieces * units * sizeof(T) * 2);
   if (rc) return rc;
   uint32_t* buf = keys.as<uint32_t>();
-  uint32_t *k[2] = {buf, buf + pad}, *at[2] = {buf + 2 * pad, buf + 3 * pad};
-  a.hist = buf + 4 * pad;
+  SortArgs a = {};
+  for (int i = 0; i < 2; ++i) { a.keys[i] = buf + i * pad; a.at[i] = buf + (2 + i) * pad; }
   a.ids = ids; a.n = tokens; a.vocab = vocab; a.status = d->status_dev;
-  int passes = 1;
-  while ((vocab >> (8 * passes)) != 0) ++passes;                 // (keys go up to vocab)
-  // the zeros, a share with each launch
+  a.passes = 1;
+  while ((vocab >> (8 * a.passes)) != 0) ++a.passes;             // (keys go up to vocab)
   const int64_t floats = accumulate ? 0 : (int64_t)vocab * units * (int64_t)(sizeof(T) / 4);
   float* table = reinterpret_cast<float*>(dtable);
-  const int64_t lead = std::min<int64_t>((4 - (((uintptr_t)table >> 2) & 3)) & 3, floats), quads = (floats - lead) / 4;
-  a.zeros = reinterpret_cast<float4*>(table + lead);
-  const int64_t fill_blocks = std::min<int64_t>((int64_t)d->sm_count * 4, lnn_ceil_div(quads, 2 * passes * kThreads * 4));
-  int launch = 0;
-  const auto next = [&]() {                                      // a share of the zeros for the next launch; its grid
-    a.zero_begin = quads * launch / (2 * passes);
-    a.zero_end = quads * (launch + 1) / (2 * passes);
-    a.odds = 0;
-    if (launch == 0) { a.odd = table; a.odds = (int)lead; }
-    if (launch == 1) { a.odd = table + lead + quads * 4; a.odds = (int)(floats - lead - quads * 4); }
-    ++launch;
-    return (unsigned)(a.sort_blocks + std::max<int64_t>(fill_blocks, a.odds > 0));
-  };
-  for (int pass = 0; pass < passes; ++pass) {
-    a.shift = 8 * pass;
-    a.keys = pass ? k[(pass - 1) & 1] : nullptr;
-    a.at = pass ? at[(pass - 1) & 1] : nullptr;
-    a.out_keys = k[pass & 1];
-    a.out_at = at[pass & 1];
-    unsigned blocks = next();
-    LNN_CUDA(lnn::launch_chained(d, sort_count_kernel, blocks, kThreads, 0, a));
-    LNN_CHECK_LAUNCH(d);
-    blocks = next();
-    LNN_CUDA(lnn::launch_chained(d, sort_scatter_kernel, blocks, kThreads, 0, a));
-    LNN_CHECK_LAUNCH(d);
-  }
-  const uint32_t *src_k = a.out_keys, *src_at = a.out_at;
-  const dim3 block = row_block(units);
+  a.lead = table;
+  a.leads = (int)std::min<int64_t>((4 - (((uintptr_t)table >> 2) & 3)) & 3, floats);
+  a.zeros = reinterpret_cast<float4*>(table + a.leads);
+  a.quads = (floats - a.leads) / 4;
+  a.tail = table + a.leads + a.quads * 4;
+  a.tails = (int)(floats - a.leads - a.quads * 4);
+  // a block writes 64 KB of zeros: small enough to even out over SMs of which a cluster of eight leaves some free (as many blocks as
+  // SMs: 39 us for 154 MB, small ones: 30)
+  const int64_t fill = lnn_ceil_div(floats, kSortThreads * 32);
+  const unsigned blocks = (unsigned)(kSortBlocks + lnn_ceil_div(fill, kSortBlocks) * kSortBlocks);
+  LNN_CUDA(lnn::launch_chained(d, sort_tokens_kernel, blocks, kSortThreads, 0, a));
+  LNN_CHECK_LAUNCH(d);
+  const uint32_t *src_k = a.keys[(a.passes - 1) & 1], *src_at = a.at[(a.passes - 1) & 1];
+  const dim3 block = row_block(units, 32);
   const dim3 grid((unsigned)lnn_ceil_div(pieces, block.y), (unsigned)std::min<int64_t>(lnn_ceil_div(units, block.x), 64));
   T *head = parts.as<T>(), *tail = head + pieces * units;
   LNN_CUDA(lnn::launch_chained(d, table_grad_kernel<T>, grid, block, 0, dtable, dy, src_k, src_at, head, tail, tokens, vocab, units, scale, accumulate));
