@@ -73,15 +73,18 @@ struct PrepArgs {
   int* status;
 };
 
-template <int DP>
+struct Eight { float4 a, b; };
+
+// VEC: rows of whole, aligned quads
+template <int DP, bool VEC>
 __global__ void __launch_bounds__(kPrepThreads, kPrepBlocksPerSm)
 attn_prep_kernel(const __grid_constant__ PrepArgs a) {
-  constexpr int LANES = DP / 4, ROWS = 32 / LANES;              // four values per lane; rows that a warp takes at once
-  constexpr int kWarps = kPrepThreads / 32, STRIDE = kWarps * ROWS, BATCH = kPrepRows / STRIDE < 4 ? kPrepRows / STRIDE : 4;
+  constexpr int LANES = DP / 8, ROWS = 32 / LANES;              // eight values per lane; rows that a warp takes at once
+  constexpr int kWarps = kPrepThreads / 32, STRIDE = kWarps * ROWS, BATCH = 2;
   __shared__ float red[kWarps], red_norm[kWarps];
   __shared__ int last_block;
   lnn::wait_for_previous();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES, c = lane % LANES * 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES, c = lane % LANES * 8;
   int head = blockIdx.y, ti = 0;
   while (head >= a.t[ti].heads) head -= a.t[ti++].heads;
   const PrepTensor& t = a.t[ti];
@@ -90,14 +93,14 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
   const int len = lnn::attn_length(a.lengths, head / t.per_batch, a.kv_len, a.status);
   const int end = min(t.rows, len - t.past), dim = a.dim, first = t.first, sinks = t.sinks;      // rows from `end` on are padding
   const bool is_do = a.o != nullptr && ti == a.tensors - 1, with_norms = t.norms != nullptr;
-  const bool vec = dim % 4 == 0 && (((uintptr_t)t.src | (is_do ? (uintptr_t)a.o : 0)) & 15) == 0;
   const float* src = t.src + (int64_t)head * t.rows * dim + c;
   const float* src_o = a.o + (int64_t)head * t.rows * dim + c;
-  const auto load = [&](const float* p) {                        // (p: this lane's four values)
-    if (vec) return c < dim ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const auto quad = [&](const float* p, int c) {
+    if (VEC) return c < dim ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     return make_float4(c < dim ? __ldg(p) : 0.0f, c + 1 < dim ? __ldg(p + 1) : 0.0f, c + 2 < dim ? __ldg(p + 2) : 0.0f,
                        c + 3 < dim ? __ldg(p + 3) : 0.0f);
   };
+  const auto load = [&](const float* p) { return Eight{quad(p, c), quad(p + 4, c + 4)}; };      // (p: this lane's values)
   const auto row_total = [&](float v) {                          // over the lanes of a row
 #pragma unroll
     for (int s = LANES / 2; s > 0; s >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, s));
@@ -108,13 +111,13 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
     for (int s = 16; s > 0; s >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, s));
     return v;
   };
-  float4 x[BATCH], y[BATCH];
+  Eight x[BATCH], y[BATCH];
   const auto fetch = [&](int r0) {
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
       const int r = r0 + u * STRIDE;
       const bool real = r < end && (r >= first || r < sinks);
-      x[u] = y[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      x[u].a = x[u].b = y[u].a = y[u].b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (real) x[u] = load(src + (int64_t)r * dim);
       if (is_do && real) y[u] = load(src_o + (int64_t)r * dim);
     }
@@ -128,8 +131,9 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
   if (span > 0) {
 #pragma unroll
     for (int i = warp * ROWS + sub; i < kSampleRows; i += STRIDE) {
-      const float4 v = load(src + (int64_t)(first + (int)((int64_t)i * span / kSampleRows)) * dim);
-      top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+      const Eight v = load(src + (int64_t)(first + (int)((int64_t)i * span / kSampleRows)) * dim);
+      top = fmaxf(fmaxf(top, fmaxf(fabsf(v.a.x), fabsf(v.a.y))), fmaxf(fabsf(v.a.z), fabsf(v.a.w)));
+      top = fmaxf(fmaxf(top, fmaxf(fabsf(v.b.x), fabsf(v.b.y))), fmaxf(fabsf(v.b.z), fabsf(v.b.w)));
     }
   }
   top = warp_max(top);
@@ -155,14 +159,16 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
       const int r = r0 + u * STRIDE;
       const bool in = r < r_end;
       if (is_do) {
-        const float delta = row_total(fmaf(x[u].w, y[u].w, fmaf(x[u].z, y[u].z, fmaf(x[u].y, y[u].y, __fmul_rn(x[u].x, y[u].x)))));
+        const float half = fmaf(x[u].a.w, y[u].a.w, fmaf(x[u].a.z, y[u].a.z, fmaf(x[u].a.y, y[u].a.y, __fmul_rn(x[u].a.x, y[u].a.x))));
+        const float delta = row_total(fmaf(x[u].b.w, y[u].b.w, fmaf(x[u].b.z, y[u].b.z, fmaf(x[u].b.y, y[u].b.y, fmaf(x[u].b.x, y[u].b.x, half)))));
         if (c == 0 && in) a.delta_p[(int64_t)head * a.pitch + r] = delta;
       }
-      uint32_t h[2], l[2];
+      uint32_t h[4], l[4];
       float norm = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint64_t v = mul2(k ? pack2(x[u].z, x[u].w) : pack2(x[u].x, x[u].y), factor2);
+      for (int k = 0; k < 4; ++k) {
+        const float4& w = k < 2 ? x[u].a : x[u].b;
+        const uint64_t v = mul2(k & 1 ? pack2(w.z, w.w) : pack2(w.x, w.y), factor2);
         float p, q;
         unpack2(v, p, q);
         top = fmaxf(top, fmaxf(fabsf(p), fabsf(q)));
@@ -176,8 +182,8 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
       }
       finite = finite && norm <= 3.0e38f;                         // (false for what is not a number)
       if (in && c < a.width) {
-        *reinterpret_cast<uint2*>(hi + (int64_t)r * a.width) = make_uint2(h[0], h[1]);
-        *reinterpret_cast<uint2*>(lo + (int64_t)r * a.width) = make_uint2(l[0], l[1]);
+        *reinterpret_cast<uint4*>(hi + (int64_t)r * a.width) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(lo + (int64_t)r * a.width) = make_uint4(l[0], l[1], l[2], l[3]);
       }
       if (with_norms) {
         norm = row_total(norm);
@@ -1249,7 +1255,10 @@ int prepare(lnn::Device* d, AttnArgs& a, Operands& op, bool backward) {
     rc = operand_map(&op.map[i], at[i], p.width, p.t[i].rows, p.t[i].heads);
     if (rc) return rc;
   }
-  LNN_CUDA(lnn::launch_chained(d, attn_prep_kernel<DP>, dim3((unsigned)p.blocks, (unsigned)heads), kPrepThreads, 0, p));
+  const bool vec = a.dim % 4 == 0 && (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (backward ? (uintptr_t)a.dout | (uintptr_t)a.o : 0)) & 15) == 0;
+  const dim3 grid((unsigned)p.blocks, (unsigned)heads);
+  if (vec) LNN_CUDA(lnn::launch_chained(d, attn_prep_kernel<DP, true>, grid, kPrepThreads, 0, p));
+  else LNN_CUDA(lnn::launch_chained(d, attn_prep_kernel<DP, false>, grid, kPrepThreads, 0, p));
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
 }
