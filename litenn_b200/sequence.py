@@ -149,7 +149,10 @@ def _span(window, sinks):
 def _scale(scale, dim):
     if not 0 < dim <= MAX_HEAD_DIM:
         raise ValueError(f"heads of {dim} values: at most {MAX_HEAD_DIM}")
-    return dim ** -0.5 if scale is None else float(scale)
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not abs(scale) < float("inf"):
+        raise ValueError(f"scale {scale} must be finite")
+    return scale
 
 
 class _AttentionGrad(_deferred.JointGrad):
@@ -299,7 +302,7 @@ def sink_attention_step(q_t, k_t, v_t, cache, scale=None):
         source = t._get_top_reference_source()
         if source is cache.k or source is cache.v:
             raise ValueError("the token cannot be part of the cache's own memory")
-    scale = cache.dim ** -0.5 if scale is None else float(scale)
+    scale = _scale(scale, cache.dim)
     output_t = _out(q_t.shape, "sink_attention_step")
     now, after = cache._lengths
     for i, dev in _each_device():

@@ -91,6 +91,22 @@ def test_embedding_many_tokens_and_shapes(nn_gpu):
     close(table_t.get_grad().np(), sums, 200 * U * size, "gradient")         # (about 150 terms a row)
 
 
+def test_embedding_in_a_table_of_more_than_2_32_values(nn_gpu):
+    """Rows 2^32 values apart keep their own gradients, and are found again in the gradient."""
+    nn = nn_gpu
+    far, dim = 1 << 23, 516                                # (far * 512 = 2^32)
+    ids = np.array([far + 1, 1, far, far + 1, 0, far * 512 // dim, far + 2], np.float32)
+    dy = np.random.default_rng(11).standard_normal((7, dim)).astype(np.float32)
+    table_t = nn.Tensor((far + 3, dim))
+    trainable(nn, table_t)
+    nn.backward({nn.embedding(nn.Tensor_from_value(ids), table_t): nn.Tensor_from_value(dy)})
+    look = np.concatenate([ids, [far - 1, 2, far * 512 // dim + 1]]).astype(np.float32)
+    got = nn.embedding(nn.Tensor_from_value(look), table_t.get_grad()).np()
+    want = np.concatenate([dy, np.zeros((3, dim), np.float32)])
+    want[0] = want[3] = dy[0] + dy[3]                      # (two terms: one rounding)
+    assert_bit_exact(got, want)
+
+
 @pytest.mark.parametrize("bad", [float("nan"), 7.0, 0.5, 3e9, float("inf")])
 def test_bad_token_numbers_raise_at_the_next_read(nn_gpu, bad):
     nn = nn_gpu
@@ -178,6 +194,23 @@ def test_token_log_prob_of_odd_rows(nn_gpu):
     g = z_t.get_grad().np()
     assert np.isnan(g[0]).all() and np.isnan(g[1, 0]).all()
     close(g[1, 1], np.where(np.arange(9) == 3, 1.0, 0.0) - 1 / 9, 40 * U)
+
+
+def test_logits_of_more_than_2_32_values(nn_gpu):
+    nn = nn_gpu
+    rows, vocab = 258, (1 << 24) - 1
+    ids = np.arange(rows).astype(np.float32) * 50000
+    z_t, ids_t = nn.Tensor((rows, vocab)), nn.Tensor_from_value(ids)
+    z_t.fill(0.0)
+    trainable(nn, z_t)
+    y = nn.token_log_prob(z_t, ids_t)
+    # a thread adds vocab / 8192 / 4 groups of ones, exactly; the rest is 16 roundings
+    close(y.np(), np.full(rows, -math.log(vocab)), 40 * U)
+    y.backward()
+    # the gradient is 1 - 1 / vocab at the token and -1 / vocab elsewhere
+    close(nn.token_log_prob(z_t.get_grad(), ids_t).np(), np.full(rows, 1 - math.log(vocab - 1 + math.e)), 60 * U)
+    other = nn.Tensor_from_value((ids + 1).astype(np.float32))
+    close(nn.token_log_prob(z_t.get_grad(), other).np(), np.full(rows, -math.log(vocab - 1 + math.e)), 60 * U)
 
 
 @pytest.mark.parametrize("rows,vocab,kl,ref", [(1, 5, 0.0, False), (37, 1003, 0.05, True), (64, 300, 0.3, True), (9, 20000, 0.0, True),
@@ -310,6 +343,15 @@ CASES = [
     # more tiles of 128 rows than the device has SMs
     (3, 16, 8, 500, 530, 24, 90, 2, (530, 77, 400)),
     (2, 24, 12, 900, 900, 66, 300, 6, None),
+    # few tiles that see many keys: cut over several works, the parts merged
+    (1, 1, 1, 1500, 1500, 64, 1500, 0, None),
+    (2, 1, 1, 700, 1100, 96, 2000, 0, (1100, 650)),
+    (1, 2, 1, 129, 4000, 128, 3900, 130, None),
+    (1, 4, 4, 1, 5000, 64, 4000, 3, None),
+    # a sequence of which no query is real
+    (2, 2, 2, 50, 200, 64, 30, 2, (150, 200)),
+    # more heads than the tensor-core kernels have counters for
+    (2100, 4, 2, 66, 66, 4, 20, 1, None),
 ]
 
 
@@ -413,6 +455,51 @@ def test_sink_attention_one_tensor_in_three_places(nn_gpu):
     assert np.linalg.norm(t.get_grad().np().reshape(x.shape) - r.grad.numpy()) <= 1e-5 * float(r.grad.norm())
 
 
+def test_sink_attention_with_a_negative_scale(nn_gpu):
+    nn = nn_gpu
+    (q, k, v, do), lens = attention_inputs((1, 2, 1, 150, 150, 64, 60, 4, None))
+    seen = visible(150, 150, 60, 4, lens)
+    r = [torch.tensor(x, dtype=torch.float64, requires_grad=True) for x in (-q, k, v)]
+    o = plain_attention(*r, seen, 0.3)
+    d64 = torch.tensor(do, dtype=torch.float64)
+    o.backward(d64)
+    bounds = attention_bounds(*[x.detach() for x in r], d64, seen, 0.3)
+    t = [nn.Tensor_from_value(x) for x in (q, k, v)]
+    trainable(nn, *t)
+    y = nn.sink_attention(*t, 60, 4, scale=-0.3)
+    nn.backward({y: nn.Tensor_from_value(do)})
+    for name, g, w, b in zip(("o", "dq", "dk", "dv"), [y] + [x.get_grad() for x in t], [o.detach(), -r[0].grad, r[1].grad, r[2].grad],
+                             bounds):
+        close(g.np(), w.numpy(), b.detach().numpy() + 1e-30, name)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), 0.5, 2000.0])
+def test_bad_lengths_of_long_sequences(nn_gpu, bad):
+    """Kernels in tiles end early; the next call is right again."""
+    nn = nn_gpu
+    case = (2, 2, 1, 300, 300, 64, 120, 4, None)
+    (q, k, v, do), _ = attention_inputs(case)
+    t = [nn.Tensor_from_value(x) for x in (q, k, v)]
+    trainable(nn, *t)
+    do_t = nn.Tensor_from_value(do)
+    want = nn.sink_attention(*t, 120, 4)
+    nn.backward({want: do_t})
+    want, grads = want.np(), [x.get_grad().np() for x in t]
+    for x in t:
+        x.zero_grad()
+    y = nn.sink_attention(*t, 120, 4, lengths_t=nn.Tensor_from_value(np.array([300, bad], np.float32)))
+    nn.backward({y: do_t})
+    with pytest.raises(nn.LnnError, match="length of a sequence"):
+        y.np()
+    for x in t:
+        x.zero_grad()
+    y = nn.sink_attention(*t, 120, 4)
+    nn.backward({y: do_t})
+    assert_bit_exact(y.np(), want)
+    for x, g in zip(t, grads):
+        assert_bit_exact(x.get_grad().np(), g)
+
+
 def test_sink_attention_only_some_gradients(nn_gpu):
     nn = nn_gpu
     (q, k, v, do), _ = attention_inputs((1, 2, 1, 70, 70, 64, 30, 4, None))
@@ -498,6 +585,28 @@ def test_step_over_a_long_cache(nn_gpu):
         r = [torch.tensor(x, dtype=torch.float64) for x in (q1[:, :, None], k[:, :, :n], v[:, :, :n])]
         want = plain_attention(*r, torch.ones(1, 1, 1, n, dtype=torch.bool), D ** -0.5).numpy()[:, :, 0]
         close(y.np(), want, 5 * (72 * 2.0 ** -22 * 10 + 2.0 ** -20 + n * U), f"length {length}")
+
+
+def test_step_over_a_cache_of_more_than_2_32_values(nn_gpu):
+    """All old keys and values are zero: n of them and the new ones share the weights 1 : exp(s)."""
+    nn = nn_gpu
+    slots, D = 1 << 24, 160
+    cache = nn.SinkCache(2, 1, slots - 5, 5, D)
+    cache.k.fill(0.0)
+    cache.v.fill(0.0)
+    lengths = np.array([10, slots - 3])
+    cache.set_lengths(lengths)
+    one = np.ones((2, 1, D), np.float32)
+    score = np.log([10, 2.0 ** 24]).astype(np.float32)             # half of the weight for the first new key
+    key = one * (score[:, None, None] / D)
+    value = np.random.default_rng(12).standard_normal((2, 2, 1, D)).astype(np.float32)
+    for step in range(2):
+        y = nn.sink_attention_step(*[nn.Tensor_from_value(x) for x in (one, key, value[step])], cache, scale=1.0).np()
+        w = np.exp(np.float64(D) * key[:, :, :1])
+        want = value[:step + 1].astype(np.float64).sum(0) * w / (lengths[:, None, None] + w * (step + 1))
+        # the score is off by D + 8 roundings, the weight by that, a sum of whole numbers up to 2^24 by 16 roundings
+        close(y, want, np.abs(value).max() * 2 * ((D + 8) * U * 17 + 16 * U), f"step {step}")
+    assert cache.lengths.np().tolist() == (lengths + 2).tolist()
 
 
 def test_places_that_are_not_in_use_stay_as_they_are(nn_gpu):

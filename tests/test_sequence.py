@@ -61,6 +61,7 @@ def test_refusals_of_attention(fake):
     refused("window", f, q, k, k, 0)
     refused("window", f, q, k, k, 2.5)
     refused("sinks", f, q, k, k, 3, -1)
+    refused("must be finite", f, q, k, k, 3, scale=float("inf"))
     refused("at most 256", f, T(1, 1, 1, 257), T(1, 1, 1, 257), T(1, 1, 1, 257), 3)
     refused("2 elements", f, q, k, k, 3, lengths_t=T(3))
     refused("must be a Tensor", f, q, k, k, 3, lengths_t=[9, 9])
@@ -76,6 +77,7 @@ def test_refusals_of_the_cache(fake):
     refused("expected k and v", nn.sink_attention_step, T(2, 3, 8), T(2, 3, 4), kv, c)
     refused("does not go with", nn.sink_attention_step, T(2, 4, 8), kv, kv, c)
     refused("does not go with", nn.sink_attention_step, T(1, 3, 8), kv, kv, c)
+    refused("must be finite", nn.sink_attention_step, T(2, 3, 8), kv, kv, c, scale=float("nan"))
     refused("SinkCache", nn.sink_attention_step, T(2, 3, 8), kv, kv, None)
     refused("expected k and v", c.store, T(2, 3, 4), T(2, 3, 4))
     refused("2 elements", c.store, T(2, 3, 4, 8), T(2, 3, 4, 8), T(3))
