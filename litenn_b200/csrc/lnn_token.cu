@@ -473,16 +473,16 @@ token_logit_kernel(float* __restrict__ out, float* __restrict__ stats, const flo
     const double logp = (double)z[id] - (double)t.m - log((double)t.s);
     double value = logp, slope = 1.0;
     if (a.old) {
-      const double adv = a.adv[row], r = exp(logp - (double)a.old[row]);
+      const double adv = a.adv[row], r = exp(logp - (double)a.old[row]), plain = r * adv;
       const double lo = 1.0 - (double)a.low, hi = 1.0 + (double)a.high;
-      value = -fmin(r * adv, fmin(fmax(r, lo), hi) * adv);
-      slope = (adv >= 0.0 ? r <= hi : r >= lo) ? -adv * r : 0.0;
+      value = -fmin(plain, fmin(fmax(r, lo), hi) * adv);
+      slope = (adv >= 0.0 ? r <= hi : r >= lo) ? -plain : 0.0;
+      if (plain != plain) value = slope = plain;           // (fmin and comparisons drop a NaN)
       if (a.ref) {
         const double u = (double)a.ref[row] - logp, e = exp(u);
         value += (double)a.kl * (e - u - 1.0);
         slope += (double)a.kl * (1.0 - e);
       }
-      if (logp != logp) value = slope = logp;              // (fmin and comparisons drop a NaN)
     }
     out[row] = (float)value;
     if (stats) { stats[row * 3] = t.m; stats[row * 3 + 1] = (float)(1.0 / (double)t.s); stats[row * 3 + 2] = (float)slope; }

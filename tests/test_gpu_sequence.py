@@ -258,6 +258,25 @@ def test_policy_loss(nn_gpu, rows, vocab, kl, ref):
         assert not z_t.get_grad().np()[3].any() and y.np()[3] == 0
 
 
+def test_policy_loss_of_numbers_that_are_none(nn_gpu):
+    """A row whose old logarithm, advantage or reference is NaN has a loss and a gradient of NaN; the others have not."""
+    nn = nn_gpu
+    z = np.random.default_rng(7).standard_normal((5, 33)).astype(np.float32)
+    make = lambda *x: nn.Tensor_from_value(np.array(x, np.float32))      # noqa: E731
+    nan = math.nan
+    z_t = nn.Tensor_from_value(z)
+    trainable(nn, z_t)
+    y = nn.policy_loss(z_t, make(1, 2, 3, -1, 4), make(nan, -3, -3, nan, -3), make(0.5, nan, 0.5, nan, -0.5),
+                       make(-3, -3, nan, nan, -3), kl=0.1)
+    got = y.np()
+    assert np.isnan(got[:3]).all() and got[3] == 0 and np.isfinite(got[4])
+    y.backward()
+    g = z_t.get_grad().np()
+    assert np.isnan(g[:3]).all() and not g[3].any() and np.isfinite(g[4]).all() and g[4].any()
+    # no probability before and no advantage: 0 times infinity
+    assert np.isnan(nn.policy_loss(nn.Tensor_from_value(z[:1]), make(1), make(-math.inf), make(0)).np()).all()
+
+
 def test_policy_loss_gradient_against_differences(nn_gpu):
     nn = nn_gpu
     rng = np.random.default_rng(8)
