@@ -82,10 +82,11 @@ simt_fwd_kernel(const AttnArgs a) {
   extern __shared__ __align__(16) float smem[];
   float *Q = smem, *K = Q + B * PITCH, *V = K + B * PITCH, *P = V + B * PITCH;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  lnn::wait_for_previous();
-  if (a.info && !lnn::any_group_left(a)) return;
+  if (a.beside) lnn::start_next();
+  else lnn::wait_for_previous();
+  const bool left = !a.info || lnn::any_group_left(a);
   const int tiles_q = (a.q_len + B - 1) / B, past = a.kv_len - a.q_len;
-  for (int64_t work = blockIdx.x; work < (int64_t)tiles_q * a.q_heads * a.batch; work += gridDim.x) {
+  for (int64_t work = blockIdx.x; left && work < (int64_t)tiles_q * a.q_heads * a.batch; work += gridDim.x) {
   const int h = (int)(work / tiles_q % a.q_heads), b = (int)(work / tiles_q / a.q_heads);
   const int i0 = (int)(work % tiles_q) * B;
   if (a.info && lnn::group_ok(a, b, h / (a.q_heads / a.kv_heads))) continue;
@@ -156,6 +157,7 @@ simt_fwd_kernel(const AttnArgs a) {
     if (tx == 0) a.lse[head * a.q_len + i] = empty ? CUDART_INF_F : __fadd_rn(m[r], log2f(l[r]));
   }
   }
+  if (a.beside) lnn::wait_at_end();
 }
 
 // P = 2^(factor S - lse) and dS = scale P (dP - delta) of a tile: rows are queries (KEYS false) or keys (true)
@@ -166,10 +168,11 @@ simt_dq_kernel(const AttnArgs a) {
   extern __shared__ __align__(16) float smem[];
   float *Q = smem, *D = Q + B * PITCH, *K = D + B * PITCH, *V = K + B * PITCH, *S = V + B * PITCH;
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  lnn::wait_for_previous();
-  if (a.info && !lnn::any_group_left(a)) return;
+  if (a.beside) lnn::start_next();
+  else lnn::wait_for_previous();
+  const bool left = !a.info || lnn::any_group_left(a);
   const int tiles_q = (a.q_len + B - 1) / B, past = a.kv_len - a.q_len;
-  for (int64_t work = blockIdx.x; work < (int64_t)tiles_q * a.q_heads * a.batch; work += gridDim.x) {
+  for (int64_t work = blockIdx.x; left && work < (int64_t)tiles_q * a.q_heads * a.batch; work += gridDim.x) {
   const int h = (int)(work / tiles_q % a.q_heads), b = (int)(work / tiles_q / a.q_heads);
   const int i0 = (int)(work % tiles_q) * B;
   if (a.info && lnn::group_ok(a, b, h / (a.q_heads / a.kv_heads))) continue;
@@ -224,6 +227,7 @@ simt_dq_kernel(const AttnArgs a) {
       if (tx + 16 * u < a.dim) to[tx + 16 * u] = a.acc_q ? __fadd_rn(to[tx + 16 * u], g[r][u]) : g[r][u];
   }
   }
+  if (a.beside) lnn::wait_at_end();
 }
 
 template <int B, int DP>
@@ -233,10 +237,11 @@ simt_dkv_kernel(const AttnArgs a) {
   extern __shared__ __align__(16) float smem[];
   float *Q = smem, *D = Q + B * PITCH, *K = D + B * PITCH, *V = K + B * PITCH, *P = V + B * PITCH, *S = P + B * (B + 1);
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  lnn::wait_for_previous();
-  if (a.info && !lnn::any_group_left(a)) return;
+  if (a.beside) lnn::start_next();
+  else lnn::wait_for_previous();
+  const bool left = !a.info || lnn::any_group_left(a);
   const int tiles_k = (a.kv_len + B - 1) / B, past = a.kv_len - a.q_len, group = a.q_heads / a.kv_heads;
-  for (int64_t work = blockIdx.x; work < (int64_t)tiles_k * a.kv_heads * a.batch; work += gridDim.x) {
+  for (int64_t work = blockIdx.x; left && work < (int64_t)tiles_k * a.kv_heads * a.batch; work += gridDim.x) {
   const int hk = (int)(work / tiles_k % a.kv_heads), b = (int)(work / tiles_k / a.kv_heads);
   const int j0 = (int)(work % tiles_k) * B;
   if (a.info && lnn::group_ok(a, b, hk)) continue;
@@ -296,6 +301,7 @@ simt_dkv_kernel(const AttnArgs a) {
     }
   }
   }
+  if (a.beside) lnn::wait_at_end();
 }
 
 // one warp per row
@@ -327,11 +333,12 @@ int simt_fwd(lnn::Device* d, const AttnArgs& a) {
                             lnn_ceil_div(a.q_len, B) * a.q_heads * a.batch, a);
 }
 template <int B, int DP>
-int simt_bwd(lnn::Device* d, const AttnArgs& a) {
+int simt_bwd(lnn::Device* d, AttnArgs a) {
   int rc = LNN_OK;
   if (a.dq)
     rc = launch_simt<B, DP>(d, simt_dq_kernel<B, DP>, 4, 1,
                             lnn_ceil_div(a.q_len, B) * a.q_heads * a.batch, a);
+  a.beside = a.beside || a.dq;
   if (!rc && (a.dk || a.dv))
     rc = launch_simt<B, DP>(d, simt_dkv_kernel<B, DP>, 4, 2,
                             lnn_ceil_div(a.kv_len, B) * a.kv_heads * a.batch, a);

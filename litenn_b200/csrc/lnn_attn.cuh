@@ -32,6 +32,7 @@ struct AttnArgs {
   int* status;
   const HeadInfo* info;          // of q's, k's, v's and (backward) dout's heads, or null: see group_ok
   int backward;
+  int beside;                    // FP32 pipe: runs beside the kernel in front of it, which shares only operands with it
 };
 
 constexpr float kLog2e = 1.4426950408889634f;

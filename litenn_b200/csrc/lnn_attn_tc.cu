@@ -237,6 +237,7 @@ struct TcArgs {
   const float* norms;            // squares, DQ: of dO's rows, DK: of V's
   int pitch, width;
   int works;
+  int beside;                    // runs beside the pass in front of it, which shares only operands with it
   const uint32_t* x2;            // DQ: dO, DK: V, split
   // FWD, DQ: the works from `whole` on are cut into `splits` each (few tiles, or few in the last round of the SMs)
   int whole;
@@ -497,7 +498,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
     tmem_alloc(smem_u32(&tmem_base_smem), 512);
     tmem_relinquish();
   }
-  lnn::wait_for_previous();
+  if (t.beside) lnn::start_next();
+  else lnn::wait_for_previous();
   // an earlier kernel gave up: leave as a whole CTA (the decision must be uniform)
   if (threadIdx.x == 0) abort_flag_smem = (*(volatile int*)status == LNN_E_TIMEOUT) ? 2 : 0;
   tc_fence_before();
@@ -505,6 +507,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
   tc_fence_after();
   if (abort_flag_smem == 2) {
     if (warp == 1) tmem_dealloc(tmem_base_smem, 512);
+    if (t.beside) lnn::wait_at_end();
     return;
   }
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base_smem, 0);
@@ -1052,19 +1055,26 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (t.beside) lnn::wait_at_end();
 }
 
-// dK or dV of the tiles that several works shared: their parts in order.
+// dK and dV of the tiles that several works shared: their parts in order.
 constexpr int kPartBlocks = 8;                   // blocks per tile
 template <int DP>
 __global__ void __launch_bounds__(256)
-attn_parts_kernel(float* __restrict__ dst, const float* __restrict__ parts, const TcArgs t, int accumulate) {
-  const AttnArgs& a = t.a;
+attn_parts_kernel(const __grid_constant__ TcArgs tk, const __grid_constant__ TcArgs tv, int blocks_k) {
   lnn::wait_for_previous();
+  const bool values = (int)blockIdx.x >= blocks_k;               // blocks of dK first, if any
+  const TcArgs& t = values ? tv : tk;
+  const AttnArgs& a = t.a;
   constexpr int ROWS = kRowsM / kPartBlocks;
-  const int tile = blockIdx.x / kPartBlocks, first = blockIdx.x % kPartBlocks * ROWS, hk = blockIdx.y, b = blockIdx.z;
+  const int block = values ? blockIdx.x - blocks_k : blockIdx.x;
+  const int tile = block / kPartBlocks, first = block % kPartBlocks * ROWS, hk = blockIdx.y, b = blockIdx.z;
   const int splits = tile < t.sink_tiles ? t.splits_sink : t.splits;
   if (splits == 1 || !lnn::group_ok(a, b, hk)) return;
+  float* __restrict__ dst = values ? a.dv : a.dk;
+  const float* __restrict__ parts = t.parts;
+  const bool accumulate = values ? a.acc_v : a.acc_k;
   const int64_t w0 = (int64_t)(b * a.kv_heads + hk) * parts_per_head(t) +
                      (tile < t.sink_tiles ? tile * t.splits_sink : t.sink_tiles * t.splits_sink + (tile - t.sink_tiles) * t.splits);
   for (int i = threadIdx.x; i < ROWS * DP / 4; i += 256) {
@@ -1263,23 +1273,31 @@ int prepare(lnn::Device* d, AttnArgs& a, Operands& op, bool backward) {
   return LNN_OK;
 }
 
+// A pass over queries, and the launch that joins its parts.
 template <int MODE, int DP>
-int queries_pass(lnn::Device* d, TcArgs t, const CUtensorMap* x, const CUtensorMap* y, const CUtensorMap* z) {
-  plan_queries<MODE, DP>(d, t);
-  lnn::Scratch parts(d);
-  const int64_t n = t.works - t.whole;
-  if (n > 0) {
-    int rc = parts.get((uint64_t)n * kRowsM * (DP * 4 + (MODE == FWD ? 8 : 0)));
-    if (rc) return rc;
-    t.parts = parts.as<float>();
-    t.stats = reinterpret_cast<float2*>(t.parts + n * kRowsM * DP);
+struct QueriesPass {
+  lnn::Scratch parts;
+  TcArgs t;
+  int64_t n = 0;
+  QueriesPass(lnn::Device* d, const TcArgs& args) : parts(d), t(args) {}
+  int run(lnn::Device* d, const Operands& op) {
+    plan_queries<MODE, DP>(d, t);
+    n = t.works - t.whole;
+    if (n > 0) {
+      const int rc = parts.get((uint64_t)n * kRowsM * (DP * 4 + (MODE == FWD ? 8 : 0)));
+      if (rc) return rc;
+      t.parts = parts.as<float>();
+      t.stats = reinterpret_cast<float2*>(t.parts + n * kRowsM * DP);
+    }
+    return launch_pass<MODE, DP>(d, &op.map[0], &op.map[1], &op.map[2], t);
   }
-  int rc = launch_pass<MODE, DP>(d, x, y, z, t);
-  if (rc || n == 0) return rc;
-  LNN_CUDA(lnn::launch_chained(d, attn_merge_kernel<MODE, DP>, (unsigned)(n / t.splits * kPartBlocks), 256, 0, t));
-  LNN_CHECK_LAUNCH(d);
-  return LNN_OK;
-}
+  int join(lnn::Device* d) {
+    if (n == 0) return LNN_OK;
+    LNN_CUDA(lnn::launch_chained(d, attn_merge_kernel<MODE, DP>, (unsigned)(n / t.splits * kPartBlocks), 256, 0, t));
+    LNN_CHECK_LAUNCH(d);
+    return LNN_OK;
+  }
+};
 
 template <int DP>
 int tc_fwd(lnn::Device* d, AttnArgs a) {
@@ -1289,31 +1307,31 @@ int tc_fwd(lnn::Device* d, AttnArgs a) {
   TcArgs t = {};
   t.a = a;
   t.width = op.p.width;
-  rc = queries_pass<FWD, DP>(d, t, &op.map[0], &op.map[1], &op.map[2]);
-  return rc ? rc : lnn::attn_simt_fwd(d, a);                     // the heads that were marked
+  QueriesPass<FWD, DP> pass(d, t);
+  a.beside = 1;
+  if ((rc = pass.run(d, op)) || (rc = lnn::attn_simt_fwd(d, a))) return rc;      // (the latter: the heads that were marked)
+  return pass.join(d);
 }
 
 template <int MODE, int DP>
-int keys_pass(lnn::Device* d, TcArgs t, Operands& op, float* dst, int accumulate) {
-  plan_keys<MODE, DP>(d, t);
-  lnn::Scratch parts(d);
-  const bool cut = t.splits > 1 || t.splits_sink > 1;
-  if (cut) {
-    const int64_t n = (int64_t)t.a.batch * t.a.kv_heads *
-                      ((int64_t)t.sink_tiles * t.splits_sink + (t.splits > 1 ? (int64_t)(t.tiles - t.sink_tiles) * t.splits : 0));
-    int rc = n ? parts.get((uint64_t)n * kRowsM * DP * 4) : LNN_OK;
+struct KeysPass {
+  lnn::Scratch parts;
+  TcArgs t;
+  bool cut = false;
+  KeysPass(lnn::Device* d, const TcArgs& args) : parts(d), t(args) {}
+  int run(lnn::Device* d, const Operands& op) {
+    plan_keys<MODE, DP>(d, t);
+    cut = t.splits > 1 || t.splits_sink > 1;
+    const int64_t n = cut ? (int64_t)t.a.batch * t.a.kv_heads * ((int64_t)t.sink_tiles * t.splits_sink +
+                                                                 (t.splits > 1 ? (int64_t)(t.tiles - t.sink_tiles) * t.splits : 0)) : 0;
+    const int rc = n ? parts.get((uint64_t)n * kRowsM * DP * 4) : LNN_OK;
     if (rc) return rc;
     t.parts = parts.as<float>();
+    return launch_pass<MODE, DP>(d, &op.map[1], &op.map[0], &op.map[3], t);
   }
-  int rc = launch_pass<MODE, DP>(d, &op.map[1], &op.map[0], &op.map[3], t);
-  if (rc || !cut) return rc;
-  LNN_CUDA(lnn::launch_chained(d, attn_parts_kernel<DP>,
-                               dim3((unsigned)t.tiles * kPartBlocks, (unsigned)t.a.kv_heads, (unsigned)t.a.batch), 256, 0, dst, t.parts,
-                               t, accumulate));
-  LNN_CHECK_LAUNCH(d);
-  return LNN_OK;
-}
+};
 
+// The three passes read the same operands and write memory of their own: the SMs that are done with one begin the next.
 template <int DP>
 int tc_bwd(lnn::Device* d, AttnArgs a) {
   Operands op(d);
@@ -1322,26 +1340,29 @@ int tc_bwd(lnn::Device* d, AttnArgs a) {
   TcArgs t = {};
   t.a = a;
   t.lse_p = op.p.lse_p; t.delta_p = op.p.delta_p; t.pitch = op.p.pitch; t.width = op.p.width;
-  if (a.dq) {
-    TcArgs q = t;
-    q.norms = op.p.t[3].norms;
-    q.x2 = (const uint32_t*)op.p.t[3].hi;
-    rc = queries_pass<DQ, DP>(d, q, &op.map[0], &op.map[1], &op.map[2]);
-    if (rc) return rc;
-  }
-  if (a.dv) {
-    rc = keys_pass<DV, DP>(d, t, op, a.dv, a.acc_v);
-    if (rc) return rc;
-  }
-  if (a.dk) {
-    t.norms = op.p.t[2].norms;
-    t.x2 = (const uint32_t*)op.p.t[2].hi;
-    rc = keys_pass<DK, DP>(d, t, op, a.dk, a.acc_k);
-    if (rc) return rc;
-  }
+  QueriesPass<DQ, DP> q(d, t);
+  KeysPass<DV, DP> v(d, t);
+  KeysPass<DK, DP> k(d, t);
+  q.t.norms = op.p.t[3].norms;
+  q.t.x2 = (const uint32_t*)op.p.t[3].hi;
+  k.t.norms = op.p.t[2].norms;
+  k.t.x2 = (const uint32_t*)op.p.t[2].hi;
+  v.t.beside = a.dq != nullptr;
+  k.t.beside = a.dq || a.dv;
+  if (a.dq && (rc = q.run(d, op))) return rc;
+  if (a.dv && (rc = v.run(d, op))) return rc;
+  if (a.dk && (rc = k.run(d, op))) return rc;
   a.delta = op.p.delta_p;
   a.delta_pitch = op.p.pitch;
-  return lnn::attn_simt_bwd(d, a);
+  a.beside = 1;
+  if ((rc = lnn::attn_simt_bwd(d, a)) || (rc = q.join(d))) return rc;
+  if (k.cut || v.cut) {
+    const int tiles = (a.kv_len + kRowsM - 1) / kRowsM, blocks_k = k.cut ? tiles * kPartBlocks : 0, blocks_v = v.cut ? tiles * kPartBlocks : 0;
+    LNN_CUDA(lnn::launch_chained(d, attn_parts_kernel<DP>,
+                                 dim3((unsigned)(blocks_k + blocks_v), (unsigned)a.kv_heads, (unsigned)a.batch), 256, 0, k.t, v.t, blocks_k));
+    LNN_CHECK_LAUNCH(d);
+  }
+  return LNN_OK;
 }
 
 }  // namespace

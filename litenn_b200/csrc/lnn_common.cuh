@@ -102,6 +102,11 @@ cudaError_t launch_chained(Device* d, void (*kernel)(Params...), dim3 grid, dim3
 __device__ __forceinline__ void wait_for_previous() {
   asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
 }
+// For a kernel that reads nothing of what the one in front of it writes, and writes nothing that one touches, where that one
+// began with wait_for_previous(): what lies before both is over when its blocks start, and it need not wait for more
+// before it ends (its end then means the end of all before it, as the others take for granted).
+__device__ __forceinline__ void start_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_at_end() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 #endif
 
 // matrix products too small for the tensor cores, on the FP32 pipe (lnn_small.cu)
