@@ -550,16 +550,22 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       __syncwarp();
       return true;
     };
+    // A work is made out while the one before it is loaded: its rows are asked for the moment that their place is free.
+    Work k = {}, ahead = {};
+    if (blockIdx.x < t.works) make_work<MODE, DP>(ahead, t, blockIdx.x, some_left);
     for (int w = blockIdx.x; ok && w < t.works; w += gridDim.x, ++nr) {
-      Work k = {};
-      make_work<MODE, DP>(k, t, w, some_left);
+      const int following = w + gridDim.x;
+      k = ahead;
       if (!warp_wait(smem_u32(&bar_w_empty[nr % NW]), ((nr / NW) & 1) ^ 1, abort_flag, status, 13, w)) { ok = false; break; }
       if (lane == 0) {
         works[nr % NW] = k;
         mbar_arrive(smem_u32(&bar_w_full[nr % NW]));
       }
       __syncwarp();
-      if (k.steps == 0 || k.skip) continue;
+      if (k.steps == 0 || k.skip) {
+        if (following < t.works) make_work<MODE, DP>(ahead, t, following, some_left);
+        continue;
+      }
       if (!warp_wait(smem_u32(&bar_x_empty), (nw & 1) ^ 1, abort_flag, status, 11, w)) { ok = false; break; }
       if (elect_one()) {
         const int xh = S::KEYS ? k.b * t.a.kv_heads + k.hk : k.b * t.a.q_heads + k.h;
@@ -598,6 +604,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           late = z;
         }
         step.next(t, k);
+        if (s == 0 && following < t.works) make_work<MODE, DP>(ahead, t, following, some_left);
       }
       ++nw;
     }
