@@ -5,6 +5,7 @@
 //
 // All of them are bound by HBM.
 #include <cooperative_groups.h>
+#include <float.h>
 #include <math_constants.h>
 #include <algorithm>
 #include "lnn_common.cuh"
@@ -44,6 +45,25 @@ template <> __device__ __forceinline__ float4 plus(float4 a, float4 b) {
 template <class T> __device__ __forceinline__ T nothing();
 template <> __device__ __forceinline__ float nothing() { return 0.0f; }
 template <> __device__ __forceinline__ float4 nothing() { return make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+
+// A sum of values T with what its additions have rounded off beside it (Knuth's two-sum): a frequent token's row has
+// thousands of terms in pieces.
+template <class T> struct Sum;
+template <> struct Sum<float> {
+  float v = 0.0f, rest = 0.0f;
+  __device__ __forceinline__ void add(float x) {
+    const float s = __fadd_rn(v, x), b = __fsub_rn(s, v);
+    rest = __fadd_rn(rest, __fadd_rn(__fsub_rn(v, __fsub_rn(s, b)), __fsub_rn(x, b)));
+    v = s;
+  }
+  // (a sum that is not finite leaves nothing to add)
+  __device__ __forceinline__ float rounded(float scale) const { return __fmul_rn(fabsf(v) <= FLT_MAX ? __fadd_rn(v, rest) : v, scale); }
+};
+template <> struct Sum<float4> {
+  Sum<float> x, y, z, w;
+  __device__ __forceinline__ void add(float4 v) { x.add(v.x); y.add(v.y); z.add(v.z); w.add(v.w); }
+  __device__ __forceinline__ float4 rounded(float s) const { return make_float4(x.rounded(s), y.rounded(s), z.rounded(s), w.rounded(s)); }
+};
 
 // One row of threads (blockDim.x) per token, columns in units of T.
 template <class T>
@@ -249,6 +269,10 @@ table_grad_kernel(T* __restrict__ dtable, const T* __restrict__ dy, const uint32
         k[u] = in ? key[e0 + u] : cur;
         v[u] = in && k[u] < (uint32_t)vocab ? __ldg(dy + (int64_t)token[e0 + u] * units + c) : nothing<T>();
       }
+      if (e0 + 8 <= n && k[0] == cur && k[7] == cur) {            // (sorted: all eight) pairs of pairs: fewer roundings
+        sum = plus(sum, plus(plus(plus(v[0], v[1]), plus(v[2], v[3])), plus(plus(v[4], v[5]), plus(v[6], v[7]))));
+        continue;
+      }
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         if (e0 + u < n) {
@@ -307,17 +331,18 @@ table_join_kernel(T* __restrict__ dtable, const uint32_t* __restrict__ keys, con
   while (advance() == 8) step *= 8;
   for (step /= 8; step > 0; step /= 8) advance();
   for (int64_t c = threadIdx.x + (int64_t)blockIdx.y * blockDim.x; c < units; c += (int64_t)gridDim.y * blockDim.x) {
-    T sum = tail[piece * units + c];
+    Sum<T> sum;
+    sum.add(tail[piece * units + c]);
     for (int64_t p0 = piece + 1; p0 <= last; p0 += 16) {
       T v[16];
 #pragma unroll
       for (int u = 0; u < 16; ++u) v[u] = p0 + u <= last ? __ldg(head + (p0 + u) * units + c) : nothing<T>();
 #pragma unroll
       for (int u = 0; u < 16; ++u)
-        if (p0 + u <= last) sum = plus(sum, v[u]);
+        if (p0 + u <= last) sum.add(v[u]);
     }
     T* o = dtable + row * units + c;
-    *o = accumulate ? plus(*o, scaled(sum, scale)) : scaled(sum, scale);
+    *o = accumulate ? plus(*o, sum.rounded(scale)) : sum.rounded(scale);
   }
 }
 
