@@ -142,6 +142,9 @@ def policy_loss(logits_t, ids_t, old_t, advantage_t, ref_t=None, clip_low=0.2, c
 # =============================================================================================
 # attention
 # =============================================================================================
+_geom = lru_cache(maxsize=4096)(_lib.AttnGeom)           # (read only)
+
+
 def _span(window, sinks):
     return _whole("window", window, 1), _whole("sinks", sinks, 0)
 
@@ -161,7 +164,7 @@ class _AttentionGrad(_deferred.JointGrad):
     def __init__(self, q_t, k_t, v_t, lengths_t, lse_t, geom):
         self.roles = (q_t, k_t, v_t)
         self.lengths_t, self.lse_t, self.geom = lengths_t, lse_t, geom
-        super().__init__((t, []) for t in self.roles)
+        self[q_t], self[k_t], self[v_t] = [], [], []
 
     def joint(self, O_t, dO_t, inputs):
         targets, flags, later, seen = [], [], [], set()
@@ -218,7 +221,7 @@ def sink_attention(q_t, k_t, v_t, window, sinks=0, scale=None, lengths_t=None):
         _tensors("lengths_t", lengths_t)
         if lengths_t.shape.size != B:
             raise ValueError(f"lengths_t must have {B} elements, one per sequence, got {lengths_t.shape}")
-    geom = _lib.AttnGeom(B, Hq, Hkv, T, S, D, min(window, S), min(sinks, S), scale)
+    geom = _geom(B, Hq, Hkv, T, S, D, min(window, S), min(sinks, S), scale)
     output_t, lse_t = _out(q_t.shape, "sink_attention"), _out(_shape(B, Hq, T))
     output_t._gradfns = _AttentionGrad(q_t, k_t, v_t, lengths_t, lse_t, geom)
     for i, dev in _each_device():
