@@ -15,6 +15,12 @@
 // twice) because 128 stationary rows of K and V of 128 values leave room in shared memory for two tiles of Q and one
 // of dO, not for two of both.
 //
+// What bounds it, for heads of 128 values: FWD and DV the way of the stream from L2 to shared memory (128 KB for a tile of 128 x
+// 128, about 3800 clocks where the products take 3120; with a quarter of the loads 3200), DQ and DK the gaps between the products
+// (3500 clocks for 128 x 64, 2780 of them products), and the turn from one tile of rows to the next (its first loads, 64 KB of
+// results: two to three steps).  Under load the SMs run at 1.6 of their 1.9 GHz.  8192 positions, 16 heads, window 1024: 206 us,
+// 314 TFLOP/s (three products each: 551 is the most); 8 heads over 2, window 2048: FWD 171, DQ 306, DV 186, DK 337 us.
+//
 // A persistent CTA of 576 threads per SM: warp 0 loads (TMA), one thread of warp 1 issues the MMAs, warps 2-17 (four per
 // quarter of the TMEM lanes, a fourth of the columns each) turn scores into weights, write them back to TMEM as the A operand
 // of the second product (hi and lo in the columns that the scores were in), and keep the running sums in registers.
@@ -39,7 +45,8 @@ constexpr int kRowsM = 128;                      // stationary rows
 
 // ---- preparation -----------------------------------------------------------------------------------
 // One pass over each operand: split, row norms (what bounds dS), and for dO the rows of dO * O and the denominators
-// with a padded pitch.  The scale of a head is guessed from 32 of its rows, so that the largest value of them is in
+// with a padded pitch.  Bound by HBM, with about 5 us of dependent latencies in front and behind (24 heads of 8192 rows of 128
+// values, 200 MB: 35 us).  Eight values to a lane: half the address arithmetic and shuffles of four.  The scale of a head is guessed from 32 of its rows, so that the largest value of them is in
 // [2^8, 2^9); the true maximum may be 2^7 times that before fp16 overflows.  A head beyond it, or with values that are
 // not finite, is marked and goes to the FP32-pipe kernels.
 constexpr int kPrepThreads = 256;
@@ -1400,12 +1407,13 @@ int tc_bwd(lnn::Device* d, AttnArgs a) {
 
 namespace lnn {
 
-// Sequences of one tile of the FP32-pipe kernels' 64 keys are theirs: one launch in place of three or six, and a tile of 128
-// rows would be half empty (us for 32 heads, FP32 pipe / tensor cores, cache filled too: 64 positions of 64 values 18.8 / 25.0,
-// of 128 29.0 / 31.1, 100 of 64 28.0 / 29.6; with gradients 55.9 / 69.5, but 88.5 / 83.5 for 128 values and 86.5 / 79.1 for 100).
+// Short sequences are the FP32-pipe kernels': one launch in place of three, or three in place of five, and a tile of 128 rows would
+// be half empty.  us for 32 heads, FP32 pipe / tensor cores: of 64 values, 64 positions 10.3 / 15.2, 96 positions 17.5 / 15.5, with
+// gradients 32.5 / 40.0 and 46.5 / 39.6; of 128 values, 32 positions 9.9 / 16.8, 64 positions 16.5 / 18.2, 96 positions 22.8 / 19.4,
+// with gradients (theirs always here) 37.7 / 41.1, 53.6 / 45.9 and 78.8 / 49.4.
 bool attn_tc_applicable(const AttnArgs& a, bool backward) {
   const int64_t heads = 2ll * a.batch * (a.q_heads + a.kv_heads);
-  if (a.kv_len <= 64 && (a.dim <= 64 || !backward)) return false;
+  if (a.dim <= 64 ? a.kv_len <= 64 : a.kv_len <= 32 && !backward) return false;
   return a.dim <= 128 && heads <= kTileCounters && heads < 65536;
 }
 int attn_tc_fwd(Device* d, const AttnArgs& a) { return a.dim <= 64 ? tc_fwd<64>(d, a) : tc_fwd<128>(d, a); }
