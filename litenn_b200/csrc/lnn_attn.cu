@@ -93,75 +93,75 @@ simt_fwd_kernel(const AttnArgs a) {
   const bool left = !a.info || lnn::any_group_left(a);
   const int tiles_q = (a.q_len + B - 1) / B, past = a.kv_len - a.q_len;
   for (int64_t work = blockIdx.x; left && work < (int64_t)tiles_q * a.q_heads * a.batch; work += gridDim.x) {
-  const int h = (int)(work / tiles_q % a.q_heads), b = (int)(work / tiles_q / a.q_heads);
-  const int i0 = (int)(work % tiles_q) * B;
-  if (a.info && lnn::group_ok(a, b, h / (a.q_heads / a.kv_heads))) continue;
-  __syncthreads();
-  const int len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
-  const int64_t head = (int64_t)b * a.q_heads + h;
-  const int64_t kv = ((int64_t)b * a.kv_heads + h / (a.q_heads / a.kv_heads)) * a.kv_len * a.dim;
-  const float factor = a.scale * lnn::kLog2e;
-  float o[R][DP / 16], m[R], l[R];
+    const int h = (int)(work / tiles_q % a.q_heads), b = (int)(work / tiles_q / a.q_heads);
+    const int i0 = (int)(work % tiles_q) * B;
+    if (a.info && lnn::group_ok(a, b, h / (a.q_heads / a.kv_heads))) continue;
+    __syncthreads();
+    const int len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
+    const int64_t head = (int64_t)b * a.q_heads + h;
+    const int64_t kv = ((int64_t)b * a.kv_heads + h / (a.q_heads / a.kv_heads)) * a.kv_len * a.dim;
+    const float factor = a.scale * lnn::kLog2e;
+    float o[R][DP / 16], m[R], l[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    m[r] = -CUDART_INF_F;
-    l[r] = 0.0f;
+    for (int r = 0; r < R; ++r) {
+      m[r] = -CUDART_INF_F;
+      l[r] = 0.0f;
 #pragma unroll
-    for (int u = 0; u < DP / 16; ++u) o[r][u] = 0.0f;
-  }
-  const int p_hi = min(min(i0 + B, a.q_len) - 1 + past, len - 1);
-  if (p_hi >= i0 + past) {
-    load_rows<B, DP>(Q, a.q + head * a.q_len * a.dim, i0, a.q_len, a.dim);
-    const lnn::KeyTiles tiles(i0 + past, p_hi, a.window, a.sinks, B);
-    for (int t = 0; t < tiles.count; ++t) {
-      const int j0 = tiles.at(t) * B;
-      __syncthreads();
-      load_rows<B, DP>(K, a.k + kv, j0, a.kv_len, a.dim);
-      load_rows<B, DP>(V, a.v + kv, j0, a.kv_len, a.dim);
-      __syncthreads();
-      float s[R][R];
-      tile_product<B, DP>(s, Q, K, ty, tx);
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int p = i0 + ty + 16 * r + past;
-        float top = -CUDART_INF_F;
-#pragma unroll
-        for (int c = 0; c < R; ++c) {
-          s[r][c] = p <= p_hi && lnn::attn_visible(p, j0 + tx + 16 * c, a.window, a.sinks) ? __fmul_rn(s[r][c], factor)
-                                                                                            : -CUDART_INF_F;
-          top = fmaxf(top, s[r][c]);
-        }
-        top = fmaxf(m[r], row_max(top));
-        const float base = top == -CUDART_INF_F ? 0.0f : top;
-        const float keep = exp2_fast(__fsub_rn(m[r], base));
-        float sum = 0.0f;
-#pragma unroll
-        for (int c = 0; c < R; ++c) {
-          const float e = exp2_fast(__fsub_rn(s[r][c], base));
-          sum = __fadd_rn(sum, e);
-          P[(ty + 16 * r) * (B + 1) + tx + 16 * c] = e;
-        }
-        l[r] = __fadd_rn(__fmul_rn(l[r], keep), row_sum(sum));
-        m[r] = top;
-#pragma unroll
-        for (int u = 0; u < DP / 16; ++u) o[r][u] = __fmul_rn(o[r][u], keep);
-      }
-      __syncthreads();
-      tile_weighted<B, DP>(o, P, V, ty, tx);
+      for (int u = 0; u < DP / 16; ++u) o[r][u] = 0.0f;
     }
-  }
+    const int p_hi = min(min(i0 + B, a.q_len) - 1 + past, len - 1);
+    if (p_hi >= i0 + past) {
+      load_rows<B, DP>(Q, a.q + head * a.q_len * a.dim, i0, a.q_len, a.dim);
+      const lnn::KeyTiles tiles(i0 + past, p_hi, a.window, a.sinks, B);
+      for (int t = 0; t < tiles.count; ++t) {
+        const int j0 = tiles.at(t) * B;
+        __syncthreads();
+        load_rows<B, DP>(K, a.k + kv, j0, a.kv_len, a.dim);
+        load_rows<B, DP>(V, a.v + kv, j0, a.kv_len, a.dim);
+        __syncthreads();
+        float s[R][R];
+        tile_product<B, DP>(s, Q, K, ty, tx);
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int i = i0 + ty + 16 * r;
-    if (i >= a.q_len) continue;
-    const bool empty = i + past > p_hi;
-    const float inv = empty ? 0.0f : __fdiv_rn(1.0f, l[r]);
-    float* to = a.o + (head * a.q_len + i) * a.dim;
+        for (int r = 0; r < R; ++r) {
+          const int p = i0 + ty + 16 * r + past;
+          float top = -CUDART_INF_F;
 #pragma unroll
-    for (int u = 0; u < DP / 16; ++u)
-      if (tx + 16 * u < a.dim) to[tx + 16 * u] = empty ? 0.0f : __fmul_rn(o[r][u], inv);
-    if (tx == 0) a.lse[head * a.q_len + i] = empty ? CUDART_INF_F : __fadd_rn(m[r], log2f(l[r]));
-  }
+          for (int c = 0; c < R; ++c) {
+            s[r][c] = p <= p_hi && lnn::attn_visible(p, j0 + tx + 16 * c, a.window, a.sinks) ? __fmul_rn(s[r][c], factor)
+                                                                                              : -CUDART_INF_F;
+            top = fmaxf(top, s[r][c]);
+          }
+          top = fmaxf(m[r], row_max(top));
+          const float base = top == -CUDART_INF_F ? 0.0f : top;
+          const float keep = exp2_fast(__fsub_rn(m[r], base));
+          float sum = 0.0f;
+#pragma unroll
+          for (int c = 0; c < R; ++c) {
+            const float e = exp2_fast(__fsub_rn(s[r][c], base));
+            sum = __fadd_rn(sum, e);
+            P[(ty + 16 * r) * (B + 1) + tx + 16 * c] = e;
+          }
+          l[r] = __fadd_rn(__fmul_rn(l[r], keep), row_sum(sum));
+          m[r] = top;
+#pragma unroll
+          for (int u = 0; u < DP / 16; ++u) o[r][u] = __fmul_rn(o[r][u], keep);
+        }
+        __syncthreads();
+        tile_weighted<B, DP>(o, P, V, ty, tx);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = i0 + ty + 16 * r;
+      if (i >= a.q_len) continue;
+      const bool empty = i + past > p_hi;
+      const float inv = empty ? 0.0f : __fdiv_rn(1.0f, l[r]);
+      float* to = a.o + (head * a.q_len + i) * a.dim;
+#pragma unroll
+      for (int u = 0; u < DP / 16; ++u)
+        if (tx + 16 * u < a.dim) to[tx + 16 * u] = empty ? 0.0f : __fmul_rn(o[r][u], inv);
+      if (tx == 0) a.lse[head * a.q_len + i] = empty ? CUDART_INF_F : __fadd_rn(m[r], log2f(l[r]));
+    }
   }
   if (a.beside) lnn::wait_at_end();
 }
@@ -179,59 +179,59 @@ simt_dq_kernel(const AttnArgs a) {
   const bool left = !a.info || lnn::any_group_left(a);
   const int tiles_q = (a.q_len + B - 1) / B, past = a.kv_len - a.q_len;
   for (int64_t work = blockIdx.x; left && work < (int64_t)tiles_q * a.q_heads * a.batch; work += gridDim.x) {
-  const int h = (int)(work / tiles_q % a.q_heads), b = (int)(work / tiles_q / a.q_heads);
-  const int i0 = (int)(work % tiles_q) * B;
-  if (a.info && lnn::group_ok(a, b, h / (a.q_heads / a.kv_heads))) continue;
-  __syncthreads();
-  const int len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
-  const int64_t head = (int64_t)b * a.q_heads + h;
-  const int64_t kv = ((int64_t)b * a.kv_heads + h / (a.q_heads / a.kv_heads)) * a.kv_len * a.dim;
-  const float factor = a.scale * lnn::kLog2e;
-  float g[R][DP / 16], lse[R], delta[R];
+    const int h = (int)(work / tiles_q % a.q_heads), b = (int)(work / tiles_q / a.q_heads);
+    const int i0 = (int)(work % tiles_q) * B;
+    if (a.info && lnn::group_ok(a, b, h / (a.q_heads / a.kv_heads))) continue;
+    __syncthreads();
+    const int len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
+    const int64_t head = (int64_t)b * a.q_heads + h;
+    const int64_t kv = ((int64_t)b * a.kv_heads + h / (a.q_heads / a.kv_heads)) * a.kv_len * a.dim;
+    const float factor = a.scale * lnn::kLog2e;
+    float g[R][DP / 16], lse[R], delta[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int i = i0 + ty + 16 * r;
-    lse[r] = i < a.q_len ? a.lse[head * a.q_len + i] : CUDART_INF_F;
-    delta[r] = i < a.q_len ? a.delta[head * a.delta_pitch + i] : 0.0f;
+    for (int r = 0; r < R; ++r) {
+      const int i = i0 + ty + 16 * r;
+      lse[r] = i < a.q_len ? a.lse[head * a.q_len + i] : CUDART_INF_F;
+      delta[r] = i < a.q_len ? a.delta[head * a.delta_pitch + i] : 0.0f;
 #pragma unroll
-    for (int u = 0; u < DP / 16; ++u) g[r][u] = 0.0f;
-  }
-  const int p_hi = min(min(i0 + B, a.q_len) - 1 + past, len - 1);
-  if (p_hi >= i0 + past) {
-    load_rows<B, DP>(Q, a.q + head * a.q_len * a.dim, i0, a.q_len, a.dim);
-    load_rows<B, DP>(D, a.dout + head * a.q_len * a.dim, i0, a.q_len, a.dim);
-    const lnn::KeyTiles tiles(i0 + past, p_hi, a.window, a.sinks, B);
-    for (int t = 0; t < tiles.count; ++t) {
-      const int j0 = tiles.at(t) * B;
-      __syncthreads();
-      load_rows<B, DP>(K, a.k + kv, j0, a.kv_len, a.dim);
-      load_rows<B, DP>(V, a.v + kv, j0, a.kv_len, a.dim);
-      __syncthreads();
-      float s[R][R], dp[R][R];
-      tile_product<B, DP>(s, Q, K, ty, tx);
-      tile_product<B, DP>(dp, D, V, ty, tx);
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int c = 0; c < R; ++c) {
-          const int p = i0 + ty + 16 * r + past;
-          const bool seen = p <= p_hi && lnn::attn_visible(p, j0 + tx + 16 * c, a.window, a.sinks);
-          const float e = exp2_fast(__fsub_rn(__fmul_rn(s[r][c], factor), lse[r]));
-          S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fsub_rn(dp[r][c], delta[r])), a.scale) : 0.0f;
-        }
-      __syncthreads();
-      tile_weighted<B, DP>(g, S, K, ty, tx);
+      for (int u = 0; u < DP / 16; ++u) g[r][u] = 0.0f;
     }
-  }
+    const int p_hi = min(min(i0 + B, a.q_len) - 1 + past, len - 1);
+    if (p_hi >= i0 + past) {
+      load_rows<B, DP>(Q, a.q + head * a.q_len * a.dim, i0, a.q_len, a.dim);
+      load_rows<B, DP>(D, a.dout + head * a.q_len * a.dim, i0, a.q_len, a.dim);
+      const lnn::KeyTiles tiles(i0 + past, p_hi, a.window, a.sinks, B);
+      for (int t = 0; t < tiles.count; ++t) {
+        const int j0 = tiles.at(t) * B;
+        __syncthreads();
+        load_rows<B, DP>(K, a.k + kv, j0, a.kv_len, a.dim);
+        load_rows<B, DP>(V, a.v + kv, j0, a.kv_len, a.dim);
+        __syncthreads();
+        float s[R][R], dp[R][R];
+        tile_product<B, DP>(s, Q, K, ty, tx);
+        tile_product<B, DP>(dp, D, V, ty, tx);
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int i = i0 + ty + 16 * r;
-    if (i >= a.q_len) continue;
-    float* to = a.dq + (head * a.q_len + i) * a.dim;
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int u = 0; u < DP / 16; ++u)
-      if (tx + 16 * u < a.dim) to[tx + 16 * u] = a.acc_q ? __fadd_rn(to[tx + 16 * u], g[r][u]) : g[r][u];
-  }
+          for (int c = 0; c < R; ++c) {
+            const int p = i0 + ty + 16 * r + past;
+            const bool seen = p <= p_hi && lnn::attn_visible(p, j0 + tx + 16 * c, a.window, a.sinks);
+            const float e = exp2_fast(__fsub_rn(__fmul_rn(s[r][c], factor), lse[r]));
+            S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fsub_rn(dp[r][c], delta[r])), a.scale) : 0.0f;
+          }
+        __syncthreads();
+        tile_weighted<B, DP>(g, S, K, ty, tx);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = i0 + ty + 16 * r;
+      if (i >= a.q_len) continue;
+      float* to = a.dq + (head * a.q_len + i) * a.dim;
+#pragma unroll
+      for (int u = 0; u < DP / 16; ++u)
+        if (tx + 16 * u < a.dim) to[tx + 16 * u] = a.acc_q ? __fadd_rn(to[tx + 16 * u], g[r][u]) : g[r][u];
+    }
   }
   if (a.beside) lnn::wait_at_end();
 }
@@ -248,64 +248,64 @@ simt_dkv_kernel(const AttnArgs a) {
   const bool left = !a.info || lnn::any_group_left(a);
   const int tiles_k = (a.kv_len + B - 1) / B, past = a.kv_len - a.q_len, group = a.q_heads / a.kv_heads;
   for (int64_t work = blockIdx.x; left && work < (int64_t)tiles_k * a.kv_heads * a.batch; work += gridDim.x) {
-  const int hk = (int)(work / tiles_k % a.kv_heads), b = (int)(work / tiles_k / a.kv_heads);
-  const int j0 = (int)(work % tiles_k) * B;
-  if (a.info && lnn::group_ok(a, b, hk)) continue;
-  __syncthreads();
-  const int len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
-  const int64_t kv = ((int64_t)b * a.kv_heads + hk) * a.kv_len * a.dim;
-  const float factor = a.scale * lnn::kLog2e;
-  float gk[R][DP / 16], gv[R][DP / 16];
+    const int hk = (int)(work / tiles_k % a.kv_heads), b = (int)(work / tiles_k / a.kv_heads);
+    const int j0 = (int)(work % tiles_k) * B;
+    if (a.info && lnn::group_ok(a, b, hk)) continue;
+    __syncthreads();
+    const int len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
+    const int64_t kv = ((int64_t)b * a.kv_heads + hk) * a.kv_len * a.dim;
+    const float factor = a.scale * lnn::kLog2e;
+    float gk[R][DP / 16], gv[R][DP / 16];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int u = 0; u < DP / 16; ++u) gk[r][u] = gv[r][u] = 0.0f;
-  const lnn::QuerySpan span(j0, min(j0 + B, a.kv_len) - 1, a.window, a.sinks, past, len);
-  if (span.hi >= span.lo) {
-    load_rows<B, DP>(K, a.k + kv, j0, a.kv_len, a.dim);
-    load_rows<B, DP>(V, a.v + kv, j0, a.kv_len, a.dim);
-    for (int h = hk * group; h < (hk + 1) * group; ++h) {
-      const int64_t head = (int64_t)b * a.q_heads + h;
-      for (int i0 = (span.lo - past) / B * B; i0 + past <= span.hi; i0 += B) {
-        __syncthreads();
-        load_rows<B, DP>(Q, a.q + head * a.q_len * a.dim, i0, a.q_len, a.dim);
-        load_rows<B, DP>(D, a.dout + head * a.q_len * a.dim, i0, a.q_len, a.dim);
-        __syncthreads();
-        float s[R][R], dp[R][R];
-        tile_product<B, DP>(s, K, Q, ty, tx);
-        tile_product<B, DP>(dp, V, D, ty, tx);
+      for (int u = 0; u < DP / 16; ++u) gk[r][u] = gv[r][u] = 0.0f;
+    const lnn::QuerySpan span(j0, min(j0 + B, a.kv_len) - 1, a.window, a.sinks, past, len);
+    if (span.hi >= span.lo) {
+      load_rows<B, DP>(K, a.k + kv, j0, a.kv_len, a.dim);
+      load_rows<B, DP>(V, a.v + kv, j0, a.kv_len, a.dim);
+      for (int h = hk * group; h < (hk + 1) * group; ++h) {
+        const int64_t head = (int64_t)b * a.q_heads + h;
+        for (int i0 = (span.lo - past) / B * B; i0 + past <= span.hi; i0 += B) {
+          __syncthreads();
+          load_rows<B, DP>(Q, a.q + head * a.q_len * a.dim, i0, a.q_len, a.dim);
+          load_rows<B, DP>(D, a.dout + head * a.q_len * a.dim, i0, a.q_len, a.dim);
+          __syncthreads();
+          float s[R][R], dp[R][R];
+          tile_product<B, DP>(s, K, Q, ty, tx);
+          tile_product<B, DP>(dp, V, D, ty, tx);
 #pragma unroll
-        for (int c = 0; c < R; ++c) {
-          const int i = i0 + tx + 16 * c, p = i + past;
-          const float lse = i < a.q_len ? __ldg(a.lse + head * a.q_len + i) : CUDART_INF_F;
-          const float delta = i < a.q_len ? __ldg(a.delta + head * a.delta_pitch + i) : 0.0f;
+          for (int c = 0; c < R; ++c) {
+            const int i = i0 + tx + 16 * c, p = i + past;
+            const float lse = i < a.q_len ? __ldg(a.lse + head * a.q_len + i) : CUDART_INF_F;
+            const float delta = i < a.q_len ? __ldg(a.delta + head * a.delta_pitch + i) : 0.0f;
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const bool seen = i < a.q_len && p < len && lnn::attn_visible(p, j0 + ty + 16 * r, a.window, a.sinks);
-            const float e = seen ? exp2_fast(__fsub_rn(__fmul_rn(s[r][c], factor), lse)) : 0.0f;
-            P[(ty + 16 * r) * (B + 1) + tx + 16 * c] = e;
-            S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fsub_rn(dp[r][c], delta)), a.scale) : 0.0f;
+            for (int r = 0; r < R; ++r) {
+              const bool seen = i < a.q_len && p < len && lnn::attn_visible(p, j0 + ty + 16 * r, a.window, a.sinks);
+              const float e = seen ? exp2_fast(__fsub_rn(__fmul_rn(s[r][c], factor), lse)) : 0.0f;
+              P[(ty + 16 * r) * (B + 1) + tx + 16 * c] = e;
+              S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fsub_rn(dp[r][c], delta)), a.scale) : 0.0f;
+            }
           }
+          __syncthreads();
+          tile_weighted<B, DP>(gv, P, D, ty, tx);
+          tile_weighted<B, DP>(gk, S, Q, ty, tx);
         }
-        __syncthreads();
-        tile_weighted<B, DP>(gv, P, D, ty, tx);
-        tile_weighted<B, DP>(gk, S, Q, ty, tx);
       }
     }
-  }
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int j = j0 + ty + 16 * r;
-    if (j >= a.kv_len) continue;
+    for (int r = 0; r < R; ++r) {
+      const int j = j0 + ty + 16 * r;
+      if (j >= a.kv_len) continue;
 #pragma unroll
-    for (int u = 0; u < DP / 16; ++u) {
-      const int c = tx + 16 * u;
-      if (c >= a.dim) continue;
-      const int64_t at = kv + (int64_t)j * a.dim + c;
-      if (a.dk) a.dk[at] = a.acc_k ? __fadd_rn(a.dk[at], gk[r][u]) : gk[r][u];
-      if (a.dv) a.dv[at] = a.acc_v ? __fadd_rn(a.dv[at], gv[r][u]) : gv[r][u];
+      for (int u = 0; u < DP / 16; ++u) {
+        const int c = tx + 16 * u;
+        if (c >= a.dim) continue;
+        const int64_t at = kv + (int64_t)j * a.dim + c;
+        if (a.dk) a.dk[at] = a.acc_k ? __fadd_rn(a.dk[at], gk[r][u]) : gk[r][u];
+        if (a.dv) a.dv[at] = a.acc_v ? __fadd_rn(a.dv[at], gv[r][u]) : gv[r][u];
+      }
     }
-  }
   }
   if (a.beside) lnn::wait_at_end();
 }
@@ -625,8 +625,8 @@ step_kernel(const StepArgs a) {
   step_finish<GC, NV>(a, p, t, smem);
 }
 
-// Rows of 16-byte units: the slots of a share are one piece of memory, which bulk copies bring into a ring of stages in
-// shared memory; two blocks per SM have up to 192 KB on the way.  FULL: dim = 32 NV.
+// Bound by HBM (figures at the top).  Rows of 16-byte units: the slots of a share are one piece of memory, which bulk copies
+// bring into a ring of stages in shared memory; two blocks per SM have up to 192 KB on the way.  FULL: dim = 32 NV.
 template <int GC, int NV, bool FULL>
 __global__ void __launch_bounds__(kThreads, 2)
 step_bulk_kernel(const StepArgs a) {

@@ -45,10 +45,11 @@ constexpr int kRowsM = 128;                      // stationary rows
 
 // ---- preparation -----------------------------------------------------------------------------------
 // One pass over each operand: split, row norms (what bounds dS), and for dO the rows of dO * O and the denominators
-// with a padded pitch.  Bound by HBM, with about 5 us of dependent latencies in front and behind (24 heads of 8192 rows of 128
-// values, 200 MB: 35 us).  Eight values to a lane: half the address arithmetic and shuffles of four.  The scale of a head is guessed from 32 of its rows, so that the largest value of them is in
-// [2^8, 2^9); the true maximum may be 2^7 times that before fp16 overflows.  A head beyond it, or with values that are
-// not finite, is marked and goes to the FP32-pipe kernels.
+// with a padded pitch.  Bound by HBM, with about 5 us of dependent latencies in front and behind (24 heads of 8192 rows
+// of 128 values, 200 MB: 35 us).  Eight values to a lane: half the address arithmetic and shuffles of four.
+// The scale of a head is guessed from 32 of its rows, so that the largest value of them is in [2^8, 2^9); the true
+// maximum may be 2^7 times that before fp16 overflows.  A head beyond it, or with values that are not finite, is marked
+// and goes to the FP32-pipe kernels.
 constexpr int kPrepThreads = 256;
 constexpr int kPrepRows = 64;                    // a block takes a multiple of them
 constexpr int kPrepBlocksPerSm = 4;
