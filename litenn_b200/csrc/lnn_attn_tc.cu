@@ -570,7 +570,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
         mbar_arrive(smem_u32(&bar_w_full[nr % NW]));
       }
       __syncwarp();
+      // (what the work before still needs must not wait for the next one with steps: that one's place among the works may be
+      // free only when the one before is finished)
       if (k.steps == 0 || k.skip) {
+        if (!S::TWO && late.any && !load_z(late)) { ok = false; break; }
+        late.any = false;
         if (following < t.works) make_work<MODE, DP>(ahead, t, following, some_left);
         continue;
       }
@@ -680,7 +684,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       const Work k = works[nr % NW];
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bar_w_empty[nr % NW]));
-      if (k.steps == 0 || k.skip) continue;
+      if (k.steps == 0 || k.skip) {
+        if (late.any && !out(late)) { ok = false; break; }
+        late.any = false;
+        continue;
+      }
       if (!warp_wait(smem_u32(&bar_x_full), nw & 1, abort_flag, status, 23, w)) { ok = false; break; }
       Steps<MODE, DP> step(t, k);
       int n16 = (step.n + 15) & ~15;
@@ -876,10 +884,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       const Work& k = works[slot];
       const int steps = k.steps, row0 = k.row0;
       if (k.skip || steps == 0) {
+        // (behind the results that are still to be stored)
+        if (pending >= 0 && (!drain(g - 1) || !finish(pending, m, l, times))) { ok = false; break; }
+        pending = -1;
         if (!k.skip) {
-          // nothing is seen: zeros (behind the results that are still to be stored)
-          if (pending >= 0 && (!drain(g - 1) || !finish(pending, m, l, times))) { ok = false; break; }
-          pending = -1;
+          // nothing is seen: zeros
           if (!finish(slot, 0.0f, 1.0f, 1.0f)) { ok = false; break; }
         } else {
           __syncwarp();

@@ -416,6 +416,31 @@ def test_sink_attention(nn_gpu, case):
         assert_bit_exact(x.get_grad().np(), g + g, name)
 
 
+@pytest.mark.parametrize("D", [64, 72])
+def test_sequences_without_a_position_between_long_ones(nn_gpu, D):
+    """Six tiles of 128 heads for each of which a block has two empty ones between two full ones."""
+    nn = nn_gpu
+    B, H, S, window, sinks = 8, 16, 768, 100, 3
+    lens, full = [768, 0, 0, 768, 0, 0, 0, 300], [0, 3, 7]
+    rng = np.random.default_rng(31)
+    q, k, v, do = (rng.standard_normal((B, H, S, D)).astype(np.float32) for _ in range(4))
+    seen, scale = visible(S, S, window, sinks, [lens[b] for b in full]), D ** -0.5
+    r = [torch.tensor(x[full], dtype=torch.float64, requires_grad=True) for x in (q, k, v)]
+    o = plain_attention(*r, seen, scale)
+    d64 = torch.tensor(do[full], dtype=torch.float64)
+    o.backward(d64)
+    bounds = attention_bounds(*[x.detach() for x in r], d64, seen, scale)
+    t = [nn.Tensor_from_value(x) for x in (q, k, v)]
+    trainable(nn, *t)
+    y = nn.sink_attention(*t, window, sinks, lengths_t=nn.Tensor_from_value(np.array(lens, np.float32)))
+    nn.backward({y: nn.Tensor_from_value(do)})
+    rest = [b for b in range(B) if b not in full]
+    for name, g, w, b in zip(("o", "dq", "dk", "dv"), [y] + [x.get_grad() for x in t], [o.detach()] + [x.grad for x in r], bounds):
+        g = g.np()
+        assert not g[rest].any(), name
+        close(g[full], w.numpy(), b.detach().numpy() + 1e-30, name)
+
+
 def test_sink_attention_masked_places_hold_anything(nn_gpu):
     """Keys that a row does not see do not reach it, whatever they hold, even where its neighbours see them."""
     nn = nn_gpu
