@@ -78,6 +78,7 @@ struct PrepArgs {
   const float *o, *lse;
   float *lse_p, *delta_p;
   int pitch;
+  int* taken;                    // [4] works that have been taken, of each pass
   int* status;
 };
 
@@ -93,6 +94,7 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
   __shared__ int last_block;
   lnn::wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES, c = lane % LANES * 8;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 4) a.taken[threadIdx.x] = 0;
   int head = blockIdx.y, ti = 0;
   while (head >= a.t[ti].heads) head -= a.t[ti++].heads;
   const PrepTensor& t = a.t[ti];
@@ -245,6 +247,7 @@ struct TcArgs {
   const float* norms;            // squares, DQ: of dO's rows, DK: of V's
   int pitch, width;
   int works;
+  int* taken;                    // works that CTAs have taken so far
   int beside;                    // runs beside the pass in front of it, which shares only operands with it
   const uint32_t* x2;            // DQ: dO, DK: V, split
   // FWD, DQ: the works from `whole` on are cut into `splits` each (few tiles, or few in the last round of the SMs)
@@ -287,6 +290,7 @@ struct Work {
   int i_lo, nq, q_hi, hq0, q0;           // keys: first query, tiles of queries per head, position of the last query; first step
   int split_up;                          // one of several works of its rows
   int skip;                              // the FP32 pipe's
+  int end;                               // there is none: the last was taken
   int part;                              // its place among the parts
   int ek, ev, eq, eo;                    // exponents of the scales (eq, eo: of query head h)
   float norm_v, norm_do;
@@ -558,27 +562,41 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       __syncwarp();
       return true;
     };
-    // A work is made out while the one before it is loaded: its rows are asked for the moment that their place is free.
+    // Works are taken one by one, the longest first, so that SMs that come late or meet short ones even out.  Results do not
+    // depend on who takes what.  A work is made out while the one before it is loaded: its rows are asked for the moment
+    // that their place is free.
+    const auto take = [&]() {
+      int w = 0;
+      if (lane == 0) w = atomicAdd(t.taken, 1);
+      return __shfl_sync(0xffffffffu, w, 0);
+    };
     Work k = {}, ahead = {};
-    if (blockIdx.x < t.works) make_work<MODE, DP>(ahead, t, blockIdx.x, some_left);
-    for (int w = blockIdx.x; ok && w < t.works; w += gridDim.x, ++nr) {
-      const int following = w + gridDim.x;
+    const auto take_ahead = [&]() {
+      const int w = take();
+      ahead = Work{};
+      if (w < t.works) make_work<MODE, DP>(ahead, t, w, some_left);
+      else ahead.end = 1;
+    };
+    take_ahead();
+    for (; ok; ++nr) {
       k = ahead;
-      if (!warp_wait(smem_u32(&bar_w_empty[nr % NW]), ((nr / NW) & 1) ^ 1, abort_flag, status, 13, w)) { ok = false; break; }
+      if (k.end && !S::TWO && late.any && !load_z(late)) { ok = false; break; }
+      if (!warp_wait(smem_u32(&bar_w_empty[nr % NW]), ((nr / NW) & 1) ^ 1, abort_flag, status, 13, nr)) { ok = false; break; }
       if (lane == 0) {
         works[nr % NW] = k;
         mbar_arrive(smem_u32(&bar_w_full[nr % NW]));
       }
       __syncwarp();
+      if (k.end) break;
       // (what the work before still needs must not wait for the next one with steps: that one's place among the works may be
       // free only when the one before is finished)
       if (k.steps == 0 || k.skip) {
         if (!S::TWO && late.any && !load_z(late)) { ok = false; break; }
         late.any = false;
-        if (following < t.works) make_work<MODE, DP>(ahead, t, following, some_left);
+        take_ahead();
         continue;
       }
-      if (!warp_wait(smem_u32(&bar_x_empty), (nw & 1) ^ 1, abort_flag, status, 11, w)) { ok = false; break; }
+      if (!warp_wait(smem_u32(&bar_x_empty), (nw & 1) ^ 1, abort_flag, status, 11, nr)) { ok = false; break; }
       if (elect_one()) {
         const int xh = S::KEYS ? k.b * t.a.kv_heads + k.hk : k.b * t.a.q_heads + k.h;
         const uint32_t bx = smem_u32(&bar_x_full);
@@ -616,11 +634,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           late = z;
         }
         step.next(t, k);
-        if (s == 0 && following < t.works) make_work<MODE, DP>(ahead, t, following, some_left);
+        if (s == 0) take_ahead();
       }
       ++nw;
     }
-    if (ok && !S::TWO && late.any) load_z(late);
   } else if (warp == 1) {
     // ---- MMAs -------------------------------------------------------------------------------------
     // K-major tiles of 128-byte rows (128-byte swizzle); the same bytes are an MN-major operand when the rows are K:
@@ -679,9 +696,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       __syncwarp();
       return true;
     };
-    for (int w = blockIdx.x; ok && w < t.works; w += gridDim.x, ++nr) {
-      if (!warp_wait(smem_u32(&bar_w_full[nr % NW]), (nr / NW) & 1, abort_flag, status, 27, w)) { ok = false; break; }
+    for (; ok; ++nr) {
+      if (!warp_wait(smem_u32(&bar_w_full[nr % NW]), (nr / NW) & 1, abort_flag, status, 27, nr)) { ok = false; break; }
       const Work k = works[nr % NW];
+      if (k.end) break;
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bar_w_empty[nr % NW]));
       if (k.steps == 0 || k.skip) {
@@ -689,7 +707,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
         late.any = false;
         continue;
       }
-      if (!warp_wait(smem_u32(&bar_x_full), nw & 1, abort_flag, status, 23, w)) { ok = false; break; }
+      if (!warp_wait(smem_u32(&bar_x_full), nw & 1, abort_flag, status, 23, nr)) { ok = false; break; }
       Steps<MODE, DP> step(t, k);
       int n16 = (step.n + 15) & ~15;
       const int steps = k.steps;
@@ -704,7 +722,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
             // (whoever brings the second operand first finishes the work before: its last step cannot wait for this one)
             if (late.any && !out(late)) { ok = false; break; }
             late.any = false;
-            if (!warp_wait(smem_u32(&bar_x2_full), nw & 1, abort_flag, status, 28, w)) { ok = false; break; }
+            if (!warp_wait(smem_u32(&bar_x2_full), nw & 1, abort_flag, status, 28, nr)) { ok = false; break; }
           }
           if (!warp_wait(smem_u32(&bar_y_full[g % NY]), (g / NY) & 1, abort_flag, status, 26, g)) { ok = false; break; }
           tc_fence_after();
@@ -878,10 +896,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       return true;
     };
     int nr = 0, nw = 0;
-    for (int w = blockIdx.x; ok && w < t.works; w += gridDim.x, ++nr) {
+    for (; ok; ++nr) {
       const int slot = nr % NW;
-      if (!warp_wait(smem_u32(&bar_w_full[slot]), (nr / NW) & 1, abort_flag, status, 33, w)) { ok = false; break; }
+      if (!warp_wait(smem_u32(&bar_w_full[slot]), (nr / NW) & 1, abort_flag, status, 33, nr)) { ok = false; break; }
       const Work& k = works[slot];
+      if (k.end) break;
       const int steps = k.steps, row0 = k.row0;
       if (k.skip || steps == 0) {
         // (behind the results that are still to be stored)
@@ -912,7 +931,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       if (S::TWO) {
         // The second stationary operand into TMEM, once the products of the work before are over: this warp's fourth of
         // the columns of its rows, hi and lo (what is no row of the tensor is zero).
-        if (!warp_wait(smem_u32(&bar_x_empty), (nw & 1) ^ 1, abort_flag, status, 34, w)) { ok = false; break; }
+        if (!warp_wait(smem_u32(&bar_x_empty), (nw & 1) ^ 1, abort_flag, status, 34, nr)) { ok = false; break; }
         const int64_t lo_at = (int64_t)(S::KEYS ? a.batch * a.kv_heads : a.batch * a.q_heads) * rows * (t.width / 2);
         const uint32_t* src = t.x2 + ((int64_t)xh * rows + row) * (t.width / 2) + part * (DP / 8);
         tc_fence_after();
@@ -1239,10 +1258,10 @@ void plan_keys(const lnn::Device* d, TcArgs& t) {
   }
 }
 
-// Works of a pass over queries: those of the last round of the SMs, or all where they are few, may be cut.  A pass with others
-// behind it leaves its last round to them (8192 positions of 8 heads with gradients: 1084 us with DQ's last round cut, 1071).
+// Works of a pass over queries: those of the last round of the SMs, or all where they are few, may be cut.  A pass beside
+// others fills their gaps with whole ones (8192 positions of 8 heads with gradients: 1080 us with DQ's last round cut, 1073).
 template <int MODE, int DP>
-void plan_queries(const lnn::Device* d, TcArgs& t, bool last) {
+void plan_queries(const lnn::Device* d, TcArgs& t, bool alone) {
   constexpr int BN = Shape<MODE, DP>::BN;
   const AttnArgs& a = t.a;
   t.tiles = (a.q_len + kRowsM - 1) / kRowsM;
@@ -1253,7 +1272,7 @@ void plan_queries(const lnn::Device* d, TcArgs& t, bool last) {
   const int64_t steps = rest > 0 ? (std::min<int64_t>(a.sinks, lowest) + BN - 1) / BN + (p_hi - lowest) / BN + 1 : 0;
   double best = (rest > 0 ? 1.0 : 0.0) * ((double)steps + kWorkCost);
   t.splits = 1;
-  for (int splits = 2; splits <= 32 && splits <= steps && rest > 0 && (last || full == 0); ++splits) {
+  for (int splits = 2; splits <= 32 && splits <= steps && rest > 0 && (alone || full == 0); ++splits) {
     const double cost = (double)((rest * splits + d->sm_count - 1) / d->sm_count) * ((double)((steps + splits - 1) / splits) + kWorkCost) +
                         kPartCost * (double)(rest * splits) + kMergeCost;
     if (cost < best) { best = cost; t.splits = splits; }
@@ -1293,9 +1312,10 @@ int prepare(lnn::Device* d, AttnArgs& a, Operands& op, bool backward) {
   const int64_t heads = 2 * nk + (backward ? 2 : 1) * nq;
   const int64_t norm_words = backward ? nk * a.kv_len + nq * a.q_len : 0, col_words = backward ? 2 * nq * p.pitch : 0;
   const int64_t info_words = (heads * (int64_t)sizeof(HeadInfo) / 4 + 3) / 4 * 4;
-  rc = op.small.get((uint64_t)(info_words + (col_words + 3) / 4 * 4 + 2 * heads * p.blocks + norm_words) * 4);
+  rc = op.small.get((uint64_t)(4 + info_words + (col_words + 3) / 4 * 4 + 2 * heads * p.blocks + norm_words) * 4);
   if (rc) return rc;
   float* s = op.small.as<float>();
+  p.taken = (int*)s; s += 4;
   p.info = (HeadInfo*)s; s += info_words;
   p.lse_p = s; p.delta_p = s + col_words / 2; s += (col_words + 3) / 4 * 4;       // (16-byte aligned: the pitch is a multiple of 8)
   p.block_max = s; s += heads * p.blocks;
@@ -1328,8 +1348,8 @@ struct QueriesPass {
   TcArgs t;
   int64_t n = 0;
   QueriesPass(lnn::Device* d, const TcArgs& args) : parts(d), t(args) {}
-  int run(lnn::Device* d, const Operands& op, bool last) {
-    plan_queries<MODE, DP>(d, t, last);
+  int run(lnn::Device* d, const Operands& op, bool alone) {
+    plan_queries<MODE, DP>(d, t, alone);
     n = t.works - t.whole;
     if (n > 0) {
       const int rc = parts.get((uint64_t)n * kRowsM * (DP * 4 + (MODE == FWD ? 8 : 0)));
@@ -1355,6 +1375,7 @@ int tc_fwd(lnn::Device* d, AttnArgs a) {
   TcArgs t = {};
   t.a = a;
   t.width = op.p.width;
+  t.taken = op.p.taken;
   QueriesPass<FWD, DP> pass(d, t);
   a.beside = 1;
   if ((rc = pass.run(d, op, true)) || (rc = lnn::attn_simt_fwd(d, a))) return rc;      // (the latter: the heads that were marked)
@@ -1391,15 +1412,19 @@ int tc_bwd(lnn::Device* d, AttnArgs a) {
   QueriesPass<DQ, DP> q(d, t);
   KeysPass<DV, DP> v(d, t);
   KeysPass<DK, DP> k(d, t);
+  k.t.taken = op.p.taken;
+  v.t.taken = op.p.taken + 1;
+  q.t.taken = op.p.taken + 2;
   q.t.norms = op.p.t[3].norms;
   q.t.x2 = (const uint32_t*)op.p.t[3].hi;
   k.t.norms = op.p.t[2].norms;
   k.t.x2 = (const uint32_t*)op.p.t[2].hi;
-  v.t.beside = a.dq != nullptr;
-  k.t.beside = a.dq || a.dv;
-  if (a.dq && (rc = q.run(d, op, !a.dk && !a.dv))) return rc;
-  if (a.dv && (rc = v.run(d, op))) return rc;
+  // the pass of the longest works first, that of the shortest last
+  v.t.beside = a.dk != nullptr;
+  q.t.beside = a.dk || a.dv;
   if (a.dk && (rc = k.run(d, op))) return rc;
+  if (a.dv && (rc = v.run(d, op))) return rc;
+  if (a.dq && (rc = q.run(d, op, !a.dk && !a.dv))) return rc;
   a.delta = op.p.delta_p;
   a.delta_pitch = op.p.pitch;
   a.beside = 1;
