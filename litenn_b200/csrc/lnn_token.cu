@@ -374,7 +374,7 @@ int embedding_bwd(lnn::Device* d, T* dtable, const T* dy, const float* ids, int6
   for (int i = 0; i < 2; ++i) { a.keys[i] = buf + i * pad; a.at[i] = buf + (2 + i) * pad; }
   a.ids = ids; a.n = tokens; a.vocab = vocab; a.status = d->status_dev;
   a.passes = 1;
-  while ((vocab >> (8 * a.passes)) != 0) ++a.passes;             // (keys go up to vocab)
+  while (((int64_t)vocab >> (8 * a.passes)) != 0) ++a.passes;             // (keys go up to vocab)
   const int64_t floats = accumulate ? 0 : (int64_t)vocab * units * (int64_t)(sizeof(T) / 4);
   float* table = reinterpret_cast<float*>(dtable);
   a.lead = table;

@@ -42,7 +42,7 @@ def some_ids(rng, n, vocab, kind):
 @pytest.mark.parametrize("n,vocab,dim,kind", [
     (1, 1, 1, "all"), (1, 7, 3, "all"), (1, 9, 4, "padded"), (31, 2, 4, "mixed"), (32, 1, 5, "same"), (33, 300, 8, "same"),
     (1000, 3, 17, "mixed"), (4097, 300, 64, "all"), (2500, 70000, 8, "mixed"), (700, 255, 1028, "mixed"),
-    (513, 256, 4, "padded"), (5000, 5, 260, "same")])
+    (513, 256, 4, "padded"), (5000, 5, 260, "same"), (70001, 3, 5, "same"), (16385, 50001, 12, "all"), (300, 1 << 24, 1, "mixed")])
 def test_embedding(nn_gpu, n, vocab, dim, kind):
     nn = nn_gpu
     rng = np.random.default_rng(n + vocab)
