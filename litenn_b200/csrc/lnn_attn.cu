@@ -216,7 +216,7 @@ simt_dq_kernel(const AttnArgs a) {
           for (int c = 0; c < R; ++c) {
             const int p = i0 + ty + 16 * r + past;
             const bool seen = p <= p_hi && lnn::attn_visible(p, j0 + tx + 16 * c, a.window, a.sinks);
-            const float e = exp2_fast(__fsub_rn(__fmul_rn(s[r][c], factor), lse[r]));
+            const float e = exp2_fast(fminf(__fsub_rn(__fmul_rn(s[r][c], factor), lse[r]), 0.0f));      // (1 at most, whatever rounding says)
             S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fsub_rn(dp[r][c], delta[r])), a.scale) : 0.0f;
           }
         __syncthreads();
@@ -282,7 +282,7 @@ simt_dkv_kernel(const AttnArgs a) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
               const bool seen = i < a.q_len && p < len && lnn::attn_visible(p, j0 + ty + 16 * r, a.window, a.sinks);
-              const float e = seen ? exp2_fast(__fsub_rn(__fmul_rn(s[r][c], factor), lse)) : 0.0f;
+              const float e = seen ? exp2_fast(fminf(__fsub_rn(__fmul_rn(s[r][c], factor), lse), 0.0f)) : 0.0f;
               P[(ty + 16 * r) * (B + 1) + tx + 16 * c] = e;
               S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fsub_rn(dp[r][c], delta)), a.scale) : 0.0f;
             }

@@ -971,8 +971,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           if (MODE == DV) factor = pow2f_int(eo - 14);
           if (S::TWO) {
             cdp = pow2f_int(eo + k.ev);
-            // |dP - delta| <= 2 |dO| |V|: below 2^15 after scaling
-            const float bound = fmaxf(2.0f * norm * (MODE == DK ? norm_do : k.norm_v), 0.0009765625f);
+            // |dP| <= |dO| |V|, and |delta| <= |dO| times the largest |V| of the head: below 2^15 after scaling
+            const float bound = fmaxf(MODE == DK ? norm_do * (norm + k.norm_v) : 2.0f * norm * k.norm_v, 0.0009765625f);
             row_exp = 14 - ((int)(__float_as_uint(bound) >> 23) - 127) - (eo + k.ev);
             if (MODE == DK) factor = pow2f_int(eq - row_exp);
           }
@@ -1080,7 +1080,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
                 }
                 float x, y;
                 unpack2(fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), c2, up), x, y);
-                wt[i] = pack2(exp2_fast(x), exp2_fast(y));
+                // (a weight is 1 at most, however far scores of 10^6 and more are off)
+                wt[i] = pack2(exp2_fast(fminf(x, exponent)), exp2_fast(fminf(y, exponent)));
                 if (S::TWO)
                   wt[i] = mul2(wt[i], fma2(pack2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), cdp2, less));
               }

@@ -505,6 +505,39 @@ def test_sink_attention_one_tensor_in_three_places(nn_gpu):
     assert np.linalg.norm(t.get_grad().np().reshape(x.shape) - r.grad.numpy()) <= 1e-5 * float(r.grad.norm())
 
 
+@pytest.mark.parametrize("D", [1, 64, 128])
+def test_sink_attention_with_rows_of_nothing(nn_gpu, D):
+    """Rows of zeros, and some of tiny values, in each of the inputs."""
+    nn = nn_gpu
+    case = (1, 4, 2, 300, 300, D, 150, 4, None)
+    inputs, lens = attention_inputs(case)
+    for i, x in enumerate(inputs):
+        x[:, :, i::7] = 0.0
+        x[:, :, i + 3::11] *= np.float32(1e-6)
+    q, k, v, do = inputs
+    seen, scale = visible(300, 300, 150, 4, lens), D ** -0.5
+    r = [torch.tensor(x, dtype=torch.float64, requires_grad=True) for x in (q, k, v)]
+    o = plain_attention(*r, seen, scale)
+    d64 = torch.tensor(do, dtype=torch.float64)
+    o.backward(d64)
+    bounds = attention_bounds(*[x.detach() for x in r], d64, seen, scale)
+    # Beside errors relative to the terms: lo ends at fp16's smallest step, 2^-24, where the head's largest value is 2^8 or more, so
+    # that an operand is off by step = 2^-33 of its largest.  A weight is off by `weight` through q and k then, dP - delta by D
+    # products of which each has two such operands, and what they are multiplied with (k: 1 weight in all, q and dO: n) by one.
+    step, n = 2.0 ** -33, 300 * 2
+    Q, K, V, DO = (float(np.abs(x).max()) for x in inputs)
+    weight = 2 * (2 * step * scale * D * Q * K)
+    ds = scale * D * DO * V * (2 * weight + 2 * step + 2 * step)
+    rest = (V * (weight + step), K * ds, n * Q * ds, n * DO * (weight + step))
+    t = [nn.Tensor_from_value(x) for x in (q, k, v)]
+    trainable(nn, *t)
+    y = nn.sink_attention(*t, 150, 4)
+    nn.backward({y: nn.Tensor_from_value(do)})
+    for name, g, w, b, c in zip(("o", "dq", "dk", "dv"), [y] + [x.get_grad() for x in t], [o.detach()] + [x.grad for x in r], bounds,
+                                rest):
+        close(g.np(), w.numpy(), b.detach().numpy() + c, name)
+
+
 def test_sink_attention_with_a_negative_scale(nn_gpu):
     nn = nn_gpu
     (q, k, v, do), lens = attention_inputs((1, 2, 1, 150, 150, 64, 60, 4, None))
