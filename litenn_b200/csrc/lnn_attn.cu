@@ -878,7 +878,7 @@ int lnn_sink_attn_fwd(int dev, uint64_t O, uint64_t LSE, uint64_t Q, uint64_t K,
   LNN_REQUIRE(O && LSE && Q && K && V, "bad arguments");
   AttnArgs a = attn_args(d, g, Q, K, V, LEN);
   a.o = out(O); a.lse = out(LSE);
-  return lnn::attn_tc_applicable(a, false) ? lnn::attn_tc_fwd(d, a) : lnn::attn_simt_fwd(d, a);
+  return lnn::attn_tc_applicable(a) ? lnn::attn_tc_fwd(d, a) : lnn::attn_simt_fwd(d, a);
 }
 
 int lnn_sink_attn_bwd(int dev, uint64_t dQ, uint64_t dK, uint64_t dV, uint64_t Q, uint64_t K, uint64_t V, uint64_t O, uint64_t LSE,
@@ -891,7 +891,7 @@ int lnn_sink_attn_bwd(int dev, uint64_t dQ, uint64_t dK, uint64_t dV, uint64_t Q
   a.o = out(O); a.lse = out(LSE); a.dout = in(dO);
   a.dq = out(dQ); a.dk = out(dK); a.dv = out(dV);
   a.acc_q = acc_q; a.acc_k = acc_k; a.acc_v = acc_v;
-  if (lnn::attn_tc_applicable(a, true)) return lnn::attn_tc_bwd(d, a);
+  if (lnn::attn_tc_applicable(a)) return lnn::attn_tc_bwd(d, a);
   const int64_t rows = (int64_t)g->batch * g->q_heads * g->q_len;
   lnn::Scratch delta(d);
   rc = delta.get((uint64_t)rows * 4);

@@ -118,7 +118,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // On the FP32 pipe; with `info`, only the heads that the tensor cores have left.  Gradients: those that are not null.
 int attn_simt_fwd(Device* d, const AttnArgs& a);
 int attn_simt_bwd(Device* d, const AttnArgs& a);
-bool attn_tc_applicable(const AttnArgs& a, bool backward);
+bool attn_tc_applicable(const AttnArgs& a);
 int attn_tc_fwd(Device* d, const AttnArgs& a);
 int attn_tc_bwd(Device* d, const AttnArgs& a);
 int attn_delta(Device* d, float* delta, const float* dout, const float* o, int64_t rows, int dim);

@@ -648,11 +648,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
     const auto scores = [&](uint32_t d, uint32_t ax, uint32_t by, uint32_t id) {
       const uint32_t a = K_LO + (ax >> 4), b = K_LO + (by >> 4);
 #pragma unroll
-      for (int pr = 0; pr < 3; ++pr)                            // lo hi, hi lo, hi hi
+      for (int pr = 0; pr < 3; ++pr)      // q's lo k's hi, hi lo, hi hi: in this order in all passes, whose scores are the same to the bit
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks)
-          if (ks < ksteps) mma_ss(d, a + (pr == 0 ? S::X_PART / 16 : 0) + (ks / 4) * (kRowsM * 128 / 16) + (ks % 4) * 2,
-                 b + (pr == 1 ? S::Y_PART / 16 : 0) + (ks / 4) * (BN * 128 / 16) + (ks % 4) * 2, DESC_HI, id, pr + ks > 0);
+          if (ks < ksteps) mma_ss(d, a + (pr == (S::KEYS ? 1 : 0) ? S::X_PART / 16 : 0) + (ks / 4) * (kRowsM * 128 / 16) + (ks % 4) * 2,
+                 b + (pr == (S::KEYS ? 0 : 1) ? S::Y_PART / 16 : 0) + (ks / 4) * (BN * 128 / 16) + (ks % 4) * 2, DESC_HI, id, pr + ks > 0);
     };
     const auto second_scores = [&](uint32_t d, uint32_t by, uint32_t id) {      // dO or V from TMEM: DP / 2 columns of hi, then of lo
       const uint32_t a = tmem + S::T_X2, b = K_LO + (by >> 4);
@@ -1446,10 +1446,11 @@ namespace lnn {
 // Short sequences are the FP32-pipe kernels': one launch in place of three, or three in place of five, and a tile of 128 rows would
 // be half empty.  us for 32 heads, FP32 pipe / tensor cores: of 64 values, 64 positions 10.3 / 15.2, 96 positions 17.5 / 15.5, with
 // gradients 32.5 / 40.0 and 46.5 / 39.6; of 128 values, 32 positions 9.9 / 16.8, 64 positions 16.5 / 18.2, 96 positions 22.8 / 19.4,
-// with gradients (theirs always here) 37.7 / 41.1, 53.6 / 45.9 and 78.8 / 49.4.
-bool attn_tc_applicable(const AttnArgs& a, bool backward) {
+// with gradients 32.6 / 41.1, 55.4 / 45.9 and 78.8 / 49.4.  (The same for both directions: the gradients' scores are to
+// be those that the denominators were made of.)
+bool attn_tc_applicable(const AttnArgs& a) {
   const int64_t heads = 2ll * a.batch * (a.q_heads + a.kv_heads);
-  if (a.dim <= 64 ? a.kv_len <= 64 : a.kv_len <= 32 && !backward) return false;
+  if (a.kv_len <= (a.dim <= 64 ? 64 : 32)) return false;
   return a.dim <= 128 && heads <= kTileCounters && heads < 65536;
 }
 int attn_tc_fwd(Device* d, const AttnArgs& a) { return a.dim <= 64 ? tc_fwd<64>(d, a) : tc_fwd<128>(d, a); }
