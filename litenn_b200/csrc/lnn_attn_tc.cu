@@ -18,8 +18,8 @@
 // What bounds it, for heads of 128 values: FWD and DV the way of the stream from L2 to shared memory (128 KB for a tile of 128 x
 // 128, about 3800 clocks where the products take 3120; with a quarter of the loads 3200), DQ and DK the gaps between the products
 // (3500 clocks for 128 x 64, 2780 of them products), and the turn from one tile of rows to the next (its first loads, 64 KB of
-// results: two to three steps).  Under load the SMs run at 1.6 of their 1.9 GHz.  8192 positions, 16 heads, window 1024: 206 us,
-// 314 TFLOP/s (three products each: 551 is the most); 8 heads over 2, window 2048: FWD 171, DQ 306, DV 186, DK 337 us.
+// results: two to three steps).  Under load the SMs run at 1.6 of their 1.9 GHz.  8192 positions, 16 heads, window 1024: 197 us,
+// 328 TFLOP/s (three products each: 551 is the most); 8 heads over 2, window 2048: FWD 171, DQ 306, DV 186, DK 337 us.
 //
 // A persistent CTA of 576 threads per SM: warp 0 loads (TMA), one thread of warp 1 issues the MMAs, warps 2-17 (four per
 // quarter of the TMEM lanes, a fourth of the columns each) turn scores into weights, write them back to TMEM as the A operand
