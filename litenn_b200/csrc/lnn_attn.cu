@@ -784,7 +784,8 @@ int launch_step(lnn::Device* d, StepArgs& a, bool vec) {
     bytes = std::max(join, (size_t)a.stages * stage);
     kernel = a.dim == NV * 32 ? step_bulk_kernel<GC, NV, true> : step_bulk_kernel<GC, NV, false>;
   }
-  if (bytes > 48 * 1024) LNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  if (bytes > 47 * 1024)                                         // (barriers come on top)
+    LNN_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.splits, (unsigned)(a.kv_heads * a.group_chunks), (unsigned)a.batch);
   cfg.blockDim = dim3(kThreads);

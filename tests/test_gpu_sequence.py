@@ -619,7 +619,7 @@ def test_sink_attention_gradient_against_differences(nn_gpu):
 # ---------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("B,Hq,Hkv,D,window,sinks", [
     (1, 1, 1, 1, 1, 0), (2, 2, 1, 3, 5, 2), (3, 6, 3, 64, 20, 4), (2, 8, 1, 80, 7, 0), (1, 5, 1, 128, 40, 3), (2, 3, 3, 130, 9, 1),
-    (1, 4, 2, 256, 33, 5), (1, 16, 2, 96, 12, 1), (2, 2, 2, 32, 700, 30)])
+    (1, 4, 2, 256, 33, 5), (1, 16, 2, 96, 12, 1), (2, 2, 2, 32, 700, 30), (2, 2, 2, 96, 20, 3)])
 def test_steps_equal_attention_over_the_whole(nn_gpu, B, Hq, Hkv, D, window, sinks):
     """A prompt into the cache, then one token after another, past the end of the ring."""
     nn = nn_gpu
