@@ -93,9 +93,10 @@ int lnn_host_free(void* ptr);
 /* number of kernels this library has launched on the device since lnn_init */
 int lnn_launch_count(int dev, uint64_t* count);
 /* Read-and-clear the device status word that bounded waits in the tile kernels set when they
- * give up ({LNN_E_TIMEOUT, role, tile, step}).  While the word is set, later tile kernels return
+ * give up ({LNN_E_TIMEOUT, role, tile, step}).  While it says so, later tile kernels return
  * at once, so their outputs are not results; lnn_sync and lnn_d2h read the word with the
  * synchronisation they perform anyway and return LNN_E_TIMEOUT (clearing it) when it is set.
+ * LNN_E_INVALID in it (a number that is no token or no length) stops no kernel.
  * The reference has no counterpart: an OpenCL kernel that waits forever hangs the queue. */
 int lnn_device_status(int dev, int* status);
 /* Test hook: writes the status word from the host, as if a wait had expired (no kernel runs). */

@@ -513,7 +513,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
   if (t.beside) lnn::start_next();
   else lnn::wait_for_previous();
   // an earlier kernel gave up: leave as a whole CTA (the decision must be uniform)
-  if (threadIdx.x == 0) abort_flag_smem = (*(volatile int*)status == LNN_E_TIMEOUT) ? 2 : 0;
+  if (threadIdx.x == 0) abort_flag_smem = wait_expired(status) ? 2 : 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

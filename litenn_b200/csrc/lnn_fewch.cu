@@ -141,7 +141,7 @@ fewch_conv_kernel(const __grid_constant__ FcParams p) {
   __shared__ uint32_t wmax_smem;
   __shared__ float bias_s[256];
 
-  if (threadIdx.x == 0) { abort_flag_smem = (*(volatile int*)p.status != 0) ? 2 : 0; wmax_smem = 0u; }
+  if (threadIdx.x == 0) { abort_flag_smem = wait_expired(p.status) ? 2 : 0; wmax_smem = 0u; }
   __syncthreads();
   if (abort_flag_smem == 2) return;
 

@@ -201,7 +201,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tmAh, const __grid_constant__ CUte
   __shared__ int abort_flag_smem;
 
   // an earlier CTA already gave up: leave as a whole CTA (the decision must be uniform)
-  if (threadIdx.x == 0) abort_flag_smem = (*(volatile int*)p.status != 0) ? 2 : 0;
+  if (threadIdx.x == 0) abort_flag_smem = wait_expired(p.status) ? 2 : 0;
   __syncthreads();
   if (abort_flag_smem == 2) return;
 
@@ -674,7 +674,7 @@ tc_halo_kernel(const __grid_constant__ CUtensorMap tmAh, const __grid_constant__
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag_smem;
 
-  if (threadIdx.x == 0) abort_flag_smem = (*(volatile int*)p.status != 0) ? 2 : 0;
+  if (threadIdx.x == 0) abort_flag_smem = wait_expired(p.status) ? 2 : 0;
   __syncthreads();
   if (abort_flag_smem == 2) return;
 
@@ -1495,7 +1495,7 @@ prep_batch_kernel(const __grid_constant__ PrepBatchParams p) {
     while (*(volatile unsigned int*)p.barrier < gridDim.x) {
       if (clock64() - t0 > kWaitBudget) {
         gave_up = 1;
-        if (atomicCAS(p.status, 0, LNN_E_TIMEOUT) == 0) { p.status[1] = 20; p.status[2] = (int)blockIdx.x; p.status[3] = 0; }
+        report_expired_wait(p.status, 20, (int)blockIdx.x, 0);
         break;
       }
     }

@@ -44,6 +44,15 @@ __device__ __forceinline__ uint32_t mbar_test_wait(uint32_t bar, uint32_t parity
       : "memory");
   return ok;
 }
+// The device status word.  A wait that expired outranks a bad number (LNN_E_INVALID), which changes nothing but the report:
+// kernels behind the former return at once, behind the latter they run.
+static_assert(LNN_E_TIMEOUT < LNN_E_INVALID && LNN_E_INVALID < 0, "atomicMin keeps the one that counts");
+__device__ __forceinline__ bool wait_expired(const int* status) {
+  return *reinterpret_cast<const volatile int*>(status) == LNN_E_TIMEOUT;
+}
+__device__ __forceinline__ void report_expired_wait(int* status, int role, int tile, int step) {
+  if (atomicMin(status, LNN_E_TIMEOUT) != LNN_E_TIMEOUT) { status[1] = role; status[2] = tile; status[3] = step; }
+}
 // Bounded wait.  Returns false when the budget ran out or another role aborted.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                           int* status, int role, int step) {
@@ -54,11 +63,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     if (*abort_flag) return false;
     if (clock64() - t0 > kWaitBudget) {
       *abort_flag = 1;
-      if (atomicCAS(status, 0, LNN_E_TIMEOUT) == 0) {
-        status[1] = role;
-        status[2] = (int)(blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z));
-        status[3] = step;
-      }
+      report_expired_wait(status, role, (int)(blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z)), step);
       return false;
     }
   }
