@@ -85,7 +85,8 @@ int lnn_wait_prefetch(int dev);
 /* The mirror image for results: a device->host copy ordered after the work enqueued so far but
  * on its own stream, so that the next batch's kernels do not wait for it; the source buffer must
  * stay allocated until lnn_wait_readback (which blocks the host) returns.  `dst` should be
- * pinned (lnn_host_alloc).  ref: minicl/CLBuffer.py:99-115 is the blocking form */
+ * pinned (lnn_host_alloc).  lnn_wait_readback returns the device status as lnn_sync does (an error is
+ * about all work queued before the call).  ref: minicl/CLBuffer.py:99-115 is the blocking form */
 int lnn_d2h_readback(int dev, void* dst, uint64_t src, uint64_t bytes);
 int lnn_wait_readback(int dev);
 int lnn_host_alloc(uint64_t bytes, void** ptr);   /* pinned host memory */
@@ -94,8 +95,8 @@ int lnn_host_free(void* ptr);
 int lnn_launch_count(int dev, uint64_t* count);
 /* Read-and-clear the device status word that bounded waits in the tile kernels set when they
  * give up ({LNN_E_TIMEOUT, role, tile, step}).  While it says so, later tile kernels return
- * at once, so their outputs are not results; lnn_sync and lnn_d2h read the word with the
- * synchronisation they perform anyway and return LNN_E_TIMEOUT (clearing it) when it is set.
+ * at once, so their outputs are not results; lnn_sync, lnn_d2h and lnn_wait_readback read the word
+ * with the synchronisation they perform anyway and return LNN_E_TIMEOUT (clearing it) when it is set.
  * LNN_E_INVALID in it (a number that is no token or no length) stops no kernel.
  * The reference has no counterpart: an OpenCL kernel that waits forever hangs the queue. */
 int lnn_device_status(int dev, int* status);
@@ -424,7 +425,7 @@ int lnn_optimizer_step_many(int dev, int kind, int count, const uint64_t* V, con
 /* ---- operators on tokens ---------------------------------------------------------------
  * Token numbers and lengths are whole numbers in fp32 (exact to 2^24).  A token below zero marks a padded place: zeros,
  * no gradient.  A number that is no row of the table, or a length that is none, counts as padding and leaves
- * LNN_E_INVALID in the device status, which the next lnn_sync or lnn_d2h returns.
+ * LNN_E_INVALID in the device status, which the next lnn_sync, lnn_d2h or lnn_wait_readback returns.
  * Nothing in the reference corresponds to them. */
 
 /* Y[n] = scale * TABLE[IDS[n]];  dTABLE[v] (+)= scale * sum of dY[n] over the n with IDS[n] = v, in the order of n */

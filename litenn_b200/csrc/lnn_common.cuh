@@ -26,6 +26,7 @@ struct Device {
   uint64_t launches = 0;
   int* status_dev = nullptr;                     // device status word (bounded waits)
   int* status_host = nullptr;                    // pinned mirror
+  int* status_readback = nullptr;                // pinned, for the read-back stream
   unsigned int* tile_counters = nullptr;         // kTileCounters arrival counters, zero between launches
   unsigned int* grid_barrier = nullptr;          // two words, zero between launches (cooperative kernels)
   void* nccl_comm = nullptr;

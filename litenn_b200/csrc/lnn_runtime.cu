@@ -156,6 +156,7 @@ int lnn_init(int dev) {
   LNN_CUDA(cudaMalloc(&d->status_dev, sizeof(int) * 4));
   LNN_CUDA(cudaMemset(d->status_dev, 0, sizeof(int) * 4));
   LNN_CUDA(cudaMallocHost(&d->status_host, sizeof(int) * 4));
+  LNN_CUDA(cudaMallocHost(&d->status_readback, sizeof(int) * 4));
   LNN_CUDA(cudaMalloc(&d->tile_counters, sizeof(unsigned int) * kTileCounters));
   LNN_CUDA(cudaMemset(d->tile_counters, 0, sizeof(unsigned int) * kTileCounters));
   LNN_CUDA(cudaMalloc(&d->grid_barrier, sizeof(unsigned int) * 2));
@@ -195,6 +196,7 @@ int lnn_shutdown(int dev) {
                      (unsigned long long)d->allocated_bytes);
   cudaFree(d->status_dev);
   cudaFreeHost(d->status_host);
+  cudaFreeHost(d->status_readback);
   cudaFree(d->grid_barrier);
   cudaFree(d->tile_counters);
   cudaStreamDestroy(d->stream);
@@ -316,8 +318,11 @@ int lnn_d2h_readback(int dev, void* dst, uint64_t src, uint64_t bytes) {
 
 int lnn_wait_readback(int dev) {
   LNN_DEV(d, dev);
+  // The status word behind the results.  It may already tell of work queued after them: the report, as that of lnn_sync, is
+  // about everything queued so far.
+  LNN_CUDA(cudaMemcpyAsync(d->status_readback, d->status_dev, sizeof(int) * 4, cudaMemcpyDeviceToHost, d->readback_stream));
   LNN_CUDA(cudaStreamSynchronize(d->readback_stream));
-  return LNN_OK;
+  return d->status_readback[0] != 0 ? sync_and_report(d) : LNN_OK;
 }
 
 int lnn_d2d(int dev, uint64_t dst, uint64_t src, uint64_t bytes) {

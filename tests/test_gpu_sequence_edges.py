@@ -71,3 +71,34 @@ def test_products_behind_a_bad_token_number(nn_gpu, which):
     assert_bit_exact(y.np(), want, "result")
     assert_bit_exact(b_t.np(), after, "weights after the step")
     nn.devices.wait()
+
+
+def test_a_readback_reports_bad_numbers(nn_gpu):
+    """Results that are read on the stream of their own come with the same report as those of np()."""
+    nn = nn_gpu
+    from litenn_b200 import _lib
+    lib, dev = _lib.get_lib(), nn.devices.get_current()[0].index
+    ids_t, table_t = nn.Tensor_from_value(np.array([1, 7], np.float32)), nn.Tensor_from_value(np.ones((7, 4), np.float32))
+    good = nn.Tensor_from_value(np.array([1, 6], np.float32))
+    host = ctypes.c_void_p()
+    lib.lnn_host_alloc(32, ctypes.byref(host))
+    try:
+        for _ in range(2):
+            y = nn.embedding(ids_t, table_t)
+            lib.lnn_d2h_readback(dev, host, y._ptr(0), 32)
+            with pytest.raises(nn.LnnError, match="token number of an embedding"):
+                lib.lnn_wait_readback(dev)
+            # reported once
+            y = nn.embedding(good, table_t)
+            lib.lnn_d2h_readback(dev, host, y._ptr(0), 32)
+            lib.lnn_wait_readback(dev)
+            assert list((ctypes.c_float * 8).from_address(host.value)) == [1.0] * 8
+            assert (y.np() == 1).all()
+        # a wait that expired, too (the word is written from the host)
+        lib.lnn_debug_set_status(dev, _lib.E_TIMEOUT, 1, 7, 3)
+        lib.lnn_d2h_readback(dev, host, y._ptr(0), 32)
+        with pytest.raises(nn.LnnError, match="role 1, tile 7, step 3"):
+            lib.lnn_wait_readback(dev)
+        nn.devices.wait()
+    finally:
+        lib.lnn_host_free(host)
