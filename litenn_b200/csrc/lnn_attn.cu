@@ -419,6 +419,7 @@ struct StepArgs {
   int batch, q_heads, kv_heads, dim, window, sinks, splits, group_chunks;
   int stage_slots, stages;
   float scale;
+  float down, up;                        // powers of two, down * up = 1: see StepSums
   int* status;
 };
 
@@ -466,8 +467,11 @@ struct StepPlace {
 };
 
 // The softmax of a group of eight lanes over the keys it has seen, for GC heads.  m is no maximum but a score that no other
-// is more than kSlack above: a weight of 2^kSlack costs fp32 nothing, and short streams would move a maximum all the time.
-constexpr float kSlack = 30.0f;
+// is more than kSlack above: short streams would move a maximum all the time.  Weights of up to 2^kSlack meet the values
+// times `down`, a power of two for which the sum over all slots is below half of the largest value: an average of finite
+// values is finite.  (The other end: a term is off by 2^-149 / down at most, which is below the normal numbers up to 2^14 slots.)
+constexpr int kSlackBits = 8;
+constexpr float kSlack = (float)kSlackBits;
 template <int GC, int NV>
 struct StepSums {
   uint64_t o[GC][2 * NV];                                        // pairs of values
@@ -483,7 +487,7 @@ struct StepSums {
   }
   // scores s[g][k] (the same in all eight lanes) of KEYS keys, of which the first `real` are there, and their values
   template <int KEYS>
-  __device__ __forceinline__ void take(const float (&s)[GC][KEYS], int real, const uint64_t (&v)[KEYS][2 * NV]) {
+  __device__ __forceinline__ void take(const float (&s)[GC][KEYS], int real, const uint64_t (&v)[KEYS][2 * NV], float down) {
     bool far = false;
 #pragma unroll
     for (int g = 0; g < GC; ++g)
@@ -508,7 +512,8 @@ struct StepSums {
 #pragma unroll
       for (int k = 0; k < KEYS; ++k) {
         const float e = k < real ? exp2_fast(__fsub_rn(s[g][k], m[g])) : 0.0f;
-        const uint64_t e2 = lnn_tc::pack2(e, e);
+        const float low = __fmul_rn(e, down);
+        const uint64_t e2 = lnn_tc::pack2(low, low);
         l[g] = __fadd_rn(l[g], e);
 #pragma unroll
         for (int u = 0; u < 2 * NV; ++u) o[g][u] = lnn_tc::fma2(e2, v[k][u], o[g][u]);
@@ -592,7 +597,7 @@ __device__ __forceinline__ void step_finish(const StepArgs& a, const StepPlace& 
     const auto of_rank = [&](int r) { return (a.splits > 1 ? cluster.map_shared_rank(block, r) : block) + g * kRow; };
     constexpr std::integral_constant<int, kMaxSplits> most{};
     const float sum = join(of_rank, most, a.splits, NV * 32 + 1).x;
-    a.o[p.oq + i] = __fdiv_rn(join(of_rank, most, a.splits, c).x, sum);
+    a.o[p.oq + i] = __fmul_rn(__fdiv_rn(join(of_rank, most, a.splits, c).x, sum), a.up);
   }
   if (a.splits > 1) cluster.sync();                      // nobody leaves while its shared memory is being read
 }
@@ -639,7 +644,7 @@ step_kernel(const StepArgs a) {
 #pragma unroll
       for (int x = 4; x > 0; x >>= 1) s[g][0] = __fadd_rn(s[g][0], __shfl_xor_sync(0xffffffffu, s[g][0], x));
     }
-    t.template take<1>(s, slot < p.end ? 1 : 0, v);
+    t.template take<1>(s, slot < p.end ? 1 : 0, v, a.down);
   }
   step_append(a, p);
   step_finish<GC, NV>(a, p, t, smem);
@@ -745,7 +750,7 @@ step_bulk_kernel(const StepArgs a) {
         for (int g = 0; g < HEADS; ++g)
 #pragma unroll
           for (int k = 0; k < KEYS; ++k) s[g][k] = __fadd_rn(s[g][k], __shfl_xor_sync(0xffffffffu, s[g][k], y));
-      t.template take<KEYS>(s, real, x);
+      t.template take<KEYS>(s, real, x, a.down);
     }
     __syncwarp();
     if (lane == 0) lnn_tc::mbar_arrive(lnn_tc::smem_u32(&empty[stage]));
@@ -926,6 +931,9 @@ int lnn_sink_attn_step(int dev, uint64_t O, uint64_t Q, uint64_t K, uint64_t V, 
   a.lengths = in(LEN); a.lengths_out = out(LEN_OUT);
   a.batch = batch; a.q_heads = q_heads; a.kv_heads = kv_heads; a.dim = dim; a.window = window; a.sinks = sinks;
   a.scale = scale; a.status = d->status_dev;
+  int bits = kSlackBits + 1;
+  while ((1 << (bits - kSlackBits - 1)) < window + sinks) ++bits;
+  a.up = (float)(1ll << bits); a.down = 1.0f / a.up;
   const bool vec = dim % 4 == 0 && ((Q | K | V | CK | CV) & 15) == 0;
   if (dim <= 32) return launch_step<1>(d, a, vec);
   if (dim <= 64) return launch_step<2>(d, a, vec);

@@ -102,3 +102,36 @@ def test_a_readback_reports_bad_numbers(nn_gpu):
         nn.devices.wait()
     finally:
         lib.lnn_host_free(host)
+
+
+# ---------------------------------------------------------------------------------------------
+# values up to the largest
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("size", [3.2e38, 1.0, 1e-30])
+@pytest.mark.parametrize("rise", [0.0, 0.9, 20.0])
+@pytest.mark.parametrize("Hq,D,slots", [(1, 64, 40), (4, 64, 700), (3, 3, 50), (2, 96, 2100), (1, 256, 300), (2, 130, 90)])
+def test_steps_over_values_up_to_the_largest(nn_gpu, Hq, D, slots, rise, size):
+    """An average of values is between them, whatever they are and however the scores rise along the cache (in steps, to
+    the base two, of `rise`)."""
+    nn = nn_gpu
+    rng = np.random.default_rng(D)
+    q = np.zeros((1, Hq, D), np.float32)
+    q[..., 0] = 1.0
+    k = np.zeros((1, 1, slots + 1, D), np.float32)
+    k[0, 0, :, 0] = (np.arange(slots + 1) * rise).astype(np.float32)
+    v = (rng.uniform(0.5, 1.0, (1, 1, slots + 1, D)) * size).astype(np.float32)
+    cache = nn.SinkCache(1, 1, slots + 1, 0, D)
+    cache.k.set(k)
+    cache.v.set(v)
+    cache.set_lengths(slots)
+    scale = float(np.float32(np.log(2.0)))
+    y = nn.sink_attention_step(nn.Tensor_from_value(q), nn.Tensor_from_value(k[:, :, -1]), nn.Tensor_from_value(v[:, :, -1]), cache, scale=scale).np()
+    x = k[0, 0, :, 0].astype(np.float64) * scale
+    w = np.exp(x - x.max())
+    want = np.einsum("n,nd->d", w / w.sum(), v[0, 0].astype(np.float64) / size)
+    # a score of up to 2^11 * 20 is off by three roundings of it (times ln 2: less than one each), its weight by twice that and
+    # by 2^-21; sums of n terms
+    top = float(x.max())
+    bound = 2 * 3 * U * min(top, 90 + 30) + 2.0 ** -21 + (slots + 8) * U + (6 * U * top if rise else 0)
+    # (what is below the normal numbers: half of the smallest step for each term, times the power of two in front of the sum)
+    base.close(y[0].astype(np.float64) / size, np.broadcast_to(want, (Hq, D)), bound + 2.0 ** -126 / size)
