@@ -139,7 +139,7 @@ simt_fwd_kernel(const AttnArgs a) {
           for (int c = 0; c < R; ++c) {
             const float e = exp2_fast(__fsub_rn(s[r][c], base));
             sum = __fadd_rn(sum, e);
-            P[(ty + 16 * r) * (B + 1) + tx + 16 * c] = e;
+            P[(ty + 16 * r) * (B + 1) + tx + 16 * c] = __fmul_rn(e, a.down);
           }
           l[r] = __fadd_rn(__fmul_rn(l[r], keep), row_sum(sum));
           m[r] = top;
@@ -159,7 +159,7 @@ simt_fwd_kernel(const AttnArgs a) {
       float* to = a.o + (head * a.q_len + i) * a.dim;
 #pragma unroll
       for (int u = 0; u < DP / 16; ++u)
-        if (tx + 16 * u < a.dim) to[tx + 16 * u] = empty ? 0.0f : __fmul_rn(o[r][u], inv);
+        if (tx + 16 * u < a.dim) to[tx + 16 * u] = empty ? 0.0f : __fmul_rn(__fmul_rn(o[r][u], inv), a.up);
       if (tx == 0) a.lse[head * a.q_len + i] = empty ? CUDART_INF_F : __fadd_rn(m[r], log2f(l[r]));
     }
   }
@@ -835,6 +835,9 @@ AttnArgs attn_args(lnn::Device* d, const lnn_attn_geom* g, uint64_t Q, uint64_t 
   a.dim = g->dim; a.scale = g->scale;
   a.window = g->window < g->kv_len ? g->window : g->kv_len;       // (positions end there: no sum below passes 2^31)
   a.sinks = g->sinks < g->kv_len ? g->sinks : g->kv_len;
+  int bits = 1;
+  while ((1 << (bits - 1)) < g->kv_len) ++bits;
+  a.up = (float)(1 << bits); a.down = 1.0f / a.up;
   a.status = d->status_dev;
   return a;
 }

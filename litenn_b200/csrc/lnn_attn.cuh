@@ -29,6 +29,7 @@ struct AttnArgs {
   int batch, q_heads, kv_heads, q_len, kv_len, dim;
   int window, sinks;
   float scale;
+  float down, up;                // powers of two, down * up = 1: kv_len weights times any value times `down` stay below the largest
   int* status;
   const HeadInfo* info;          // of q's, k's, v's and (backward) dout's heads, or null: see group_ok
   int backward;

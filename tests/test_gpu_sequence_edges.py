@@ -135,3 +135,18 @@ def test_steps_over_values_up_to_the_largest(nn_gpu, Hq, D, slots, rise, size):
     bound = 2 * 3 * U * min(top, 90 + 30) + 2.0 ** -21 + (slots + 8) * U + (6 * U * top if rise else 0)
     # (what is below the normal numbers: half of the smallest step for each term, times the power of two in front of the sum)
     base.close(y[0].astype(np.float64) / size, np.broadcast_to(want, (Hq, D)), bound + 2.0 ** -126 / size)
+
+
+@pytest.mark.parametrize("S,D", [(40, 16), (64, 200), (150, 64), (300, 128)])
+def test_attention_over_values_up_to_the_largest(nn_gpu, S, D):
+    nn = nn_gpu
+    rng = np.random.default_rng(D)
+    q, k = (rng.standard_normal((1, 2, S, D)).astype(np.float32) for _ in range(2))
+    v = rng.uniform(0.5, 1.0, (1, 2, S, D)).astype(np.float32)
+    seen = base.visible(S, S, S, 0, (S,))
+    want = base.plain_attention(*[torch.tensor(x, dtype=torch.float64) for x in (q, k, v)], seen, D ** -0.5).numpy()
+    for size in (1.0, 2.0 ** 127, 2.0 ** -100):
+        got = nn.sink_attention(*[nn.Tensor_from_value(x) for x in (q, k, v * np.float32(size))], S).np().astype(np.float64) / size
+        # scores off by (D + 8) 2^-22 of their terms' magnitudes, weights by twice that and 2^-20, sums of S terms
+        mag = float(np.einsum("bhtd,bhsd->bhts", np.abs(q), np.abs(k)).max()) * D ** -0.5
+        base.close(got, want, 2 * (D + 8) * 2.0 ** -22 * mag + 2.0 ** -20 + (S + 8) * 2.0 ** -23)
