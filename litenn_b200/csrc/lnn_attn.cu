@@ -21,6 +21,7 @@ namespace {
 namespace cg = cooperative_groups;
 using lnn::AttnArgs;
 using lnn::exp2_fast;
+using lnn::min_or_nan;
 
 constexpr int kThreads = 256;           // 16 x 16
 
@@ -216,7 +217,7 @@ simt_dq_kernel(const AttnArgs a) {
           for (int c = 0; c < R; ++c) {
             const int p = i0 + ty + 16 * r + past;
             const bool seen = p <= p_hi && lnn::attn_visible(p, j0 + tx + 16 * c, a.window, a.sinks);
-            const float e = exp2_fast(fminf(__fsub_rn(__fmul_rn(s[r][c], factor), lse[r]), 0.0f));      // (1 at most, whatever rounding says)
+            const float e = exp2_fast(min_or_nan(__fsub_rn(__fmul_rn(s[r][c], factor), lse[r]), 0.0f));      // (1 at most, whatever rounding says)
             S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fsub_rn(dp[r][c], delta[r])), a.scale) : 0.0f;
           }
         __syncthreads();
@@ -282,7 +283,7 @@ simt_dkv_kernel(const AttnArgs a) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
               const bool seen = i < a.q_len && p < len && lnn::attn_visible(p, j0 + ty + 16 * r, a.window, a.sinks);
-              const float e = seen ? exp2_fast(fminf(__fsub_rn(__fmul_rn(s[r][c], factor), lse), 0.0f)) : 0.0f;
+              const float e = seen ? exp2_fast(min_or_nan(__fsub_rn(__fmul_rn(s[r][c], factor), lse), 0.0f)) : 0.0f;
               P[(ty + 16 * r) * (B + 1) + tx + 16 * c] = e;
               S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fsub_rn(dp[r][c], delta)), a.scale) : 0.0f;
             }

@@ -108,6 +108,12 @@ __device__ __forceinline__ bool any_group_left(const AttnArgs& a) {
   return __syncthreads_or(left) != 0;
 }
 
+// The smaller of the two, or NaN where one of them is (fminf would drop it, and a weight of NaN would become one of 1).
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 // 2^x with a relative error of 2^-22, 0 below the normal numbers
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;

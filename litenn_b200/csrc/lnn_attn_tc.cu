@@ -35,6 +35,7 @@ using namespace lnn_tc;
 using lnn::AttnArgs;
 using lnn::HeadInfo;
 using lnn::exp2_fast;
+using lnn::min_or_nan;
 
 enum { FWD = 0, DV = 1, DQ = 2, DK = 3 };
 
@@ -1081,7 +1082,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
                 float x, y;
                 unpack2(fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), c2, up), x, y);
                 // (a weight is 1 at most, however far scores of 10^6 and more are off)
-                wt[i] = pack2(exp2_fast(fminf(x, exponent)), exp2_fast(fminf(y, exponent)));
+                wt[i] = pack2(exp2_fast(min_or_nan(x, exponent)), exp2_fast(min_or_nan(y, exponent)));
                 if (S::TWO)
                   wt[i] = mul2(wt[i], fma2(pack2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), cdp2, less));
               }

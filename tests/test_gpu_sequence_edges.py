@@ -150,3 +150,36 @@ def test_attention_over_values_up_to_the_largest(nn_gpu, S, D):
         # scores off by (D + 8) 2^-22 of their terms' magnitudes, weights by twice that and 2^-20, sums of S terms
         mag = float(np.einsum("bhtd,bhsd->bhts", np.abs(q), np.abs(k)).max()) * D ** -0.5
         base.close(got, want, 2 * (D + 8) * 2.0 ** -22 * mag + 2.0 ** -20 + (S + 8) * 2.0 ** -23)
+
+
+# ---------------------------------------------------------------------------------------------
+# what is not a number
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("S,D,window", [(30, 16, 9), (60, 64, 20), (300, 64, 40), (300, 128, 40), (100, 200, 30)])
+@pytest.mark.parametrize("which", ["query", "key"])
+@pytest.mark.parametrize("only_values", [False, True])
+def test_what_is_not_a_number_reaches_the_gradients(nn_gpu, S, D, window, which, only_values):
+    """A query row, or a key, of NaN: the gradients of what that query (all that see that key) sees are NaN, the others not."""
+    nn = nn_gpu
+    rng = np.random.default_rng(S + D)
+    q, k, v, do = (rng.standard_normal((1, 2, S, D)).astype(np.float32) for _ in range(4))
+    at = S // 2
+    seen = base.visible(S, S, window, 0, (S,))[0, 0].numpy()
+    if which == "query":
+        q[:, 0, at, 0] = np.nan
+        bad_rows = np.arange(S) == at
+    else:
+        k[:, 0, at, 0] = np.nan
+        bad_rows = seen[:, at]
+    bad_keys = seen[bad_rows].any(0)
+    t = [nn.Tensor_from_value(x) for x in (q, k, v)]
+    base.trainable(nn, *(t[2:] if only_values else t))
+    y = nn.sink_attention(*t, window)
+    nn.backward({y: nn.Tensor_from_value(do)})
+    got = {"o": (y.np(), bad_rows), "dv": (t[2].get_grad().np(), bad_keys)}
+    if not only_values:
+        got["dq"], got["dk"] = (t[0].get_grad().np(), bad_rows), (t[1].get_grad().np(), bad_keys)
+    for name, (x, bad) in got.items():
+        assert np.isfinite(x[0, 1]).all(), name
+        assert np.isfinite(x[0, 0][~bad]).all(), name
+        assert np.isnan(x[0, 0][bad]).all(), name
