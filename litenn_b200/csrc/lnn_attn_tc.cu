@@ -253,7 +253,7 @@ struct TcArgs {
   const uint32_t* x2;            // DQ: dO, DK: V, split
   // FWD, DQ: the works from `whole` on are cut into `splits` each (few tiles, or few in the last round of the SMs)
   int whole;
-  float2* stats;                 // FWD: [part][128] maximum and sum of a row
+  float2* stats;                 // FWD: [part][128] maximum (of what was accumulated) and sum of a row
   // DV, DK: keys below sinks take `splits_sink` works per tile of rows, the others `splits`
   int tiles, sink_tiles, splits_sink, splits;
   float* parts;                  // [part][128][DP] of the tiles that have several works
@@ -280,6 +280,11 @@ template <int MODE, int DP> struct Shape {
 // only the tiles with sinks are cut.
 __device__ __forceinline__ int64_t parts_per_head(const TcArgs& t) {
   return (int64_t)t.sink_tiles * t.splits_sink + (t.splits > 1 ? (int64_t)(t.tiles - t.sink_tiles) * t.splits : 0);
+}
+
+// Accumulated scores times this are scores to the base two.  (2^-126 in place of 0: masked scores stay -inf)
+__device__ __forceinline__ float score_factor(const AttnArgs& a, int eq, int ek) {
+  return fmaxf(__fmul_rn(__fmul_rn(fabsf(a.scale), lnn::kLog2e), pow2f_int(eq + ek)), 1.17549435e-38f);
 }
 
 // A tile of 128 stationary rows and the steps of its stream.  The loading warp works it out (divisions, the sequence's
@@ -820,7 +825,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           mul = 1.0f;
           if (part == 0) t.stats[(int64_t)k.part * kRowsM + row_in] = make_float2(empty ? -CUDART_INF_F : top, empty ? 0.0f : sum);
         } else if (part == 0 && row < rows)
-          a.lse[(int64_t)xh * rows + row] = empty ? CUDART_INF_F : __fadd_rn(top, __fsub_rn(log2f(sum), 14.0f));
+          a.lse[(int64_t)xh * rows + row] = empty ? CUDART_INF_F : fmaf(top, score_factor(a, k.eq, k.ek), __fsub_rn(log2f(sum), 14.0f));
         dst = a.o;
       } else if (MODE == DQ) {
         mul = factor_of;
@@ -967,8 +972,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
             eq = lnn::info_of(a, 0, qh).e; eo = io.e; norm_do = io.norm;
           }
           cur_head = qh;
-          // (2^-126 in place of 0: masked scores stay -inf)
-          c = fmaxf(__fmul_rn(__fmul_rn(fabsf(a.scale), lnn::kLog2e), pow2f_int(eq + k.ek)), 1.17549435e-38f);
+          c = score_factor(a, eq, k.ek);
           if (MODE == DV) factor = pow2f_int(eo - 14);
           if (S::TWO) {
             cdp = pow2f_int(eo + k.ev);
@@ -1017,10 +1021,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           float tops[kParts];
           if (!share(exchange[g & 1], top, tops)) { ok = false; break; }
           top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-          const float now = fmaxf(m, __fmul_rn(top, c));
+          // (differences of scores before the factor: exact near the maximum, whose weight is 2^14 however large the scores are)
+          const float now = fmaxf(m, top);
           const float at = now == -CUDART_INF_F ? 0.0f : now;
-          const float keep = exp2_fast(__fsub_rn(m, at));
-          const uint64_t c2 = pack2(c, c), shift = pack2(14.0f - at, 14.0f - at);
+          const float keep = exp2_fast(__fmul_rn(__fsub_rn(m, at), c));
+          const uint64_t c2 = pack2(c, c), less = pack2(-at, -at), shift = pack2(14.0f, 14.0f);
           uint64_t sum = 0;
           if (col0 < n) {
 #pragma unroll
@@ -1037,7 +1042,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 float x, y;
-                unpack2(fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), c2, shift), x, y);
+                unpack2(fma2(add2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), less), c2, shift), x, y);
                 wt[i] = pack2(exp2_fast(x), exp2_fast(y));
                 sum = add2(sum, wt[i]);
               }
@@ -1176,6 +1181,7 @@ attn_merge_kernel(const __grid_constant__ TcArgs t) {
   if (!lnn::group_ok(a, b, hk)) return;
   const int past = a.kv_len - a.q_len, len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
   const float scale_v = MODE == FWD ? pow2f_int(lnn::info_of(a, 2, b * a.kv_heads + hk).e) : 1.0f;
+  const float c = MODE == FWD ? score_factor(a, lnn::info_of(a, 0, head).e, lnn::info_of(a, 1, b * a.kv_heads + hk).e) : 1.0f;
   const int64_t part0 = (int64_t)work * t.splits;
   for (int i = threadIdx.x; i < ROWS * DP / 4; i += 256) {
     const int r = first + i / (DP / 4), col = i % (DP / 4) * 4, row = row0 + r;
@@ -1192,7 +1198,7 @@ attn_merge_kernel(const __grid_constant__ TcArgs t) {
       float f = 1.0f;
       if (MODE == FWD) {
         const float2 st = __ldg(t.stats + (part0 + k) * kRowsM + r);
-        f = exp2_fast(__fsub_rn(st.x, base));
+        f = exp2_fast(__fmul_rn(__fsub_rn(st.x, base), c));
         total = fmaf(f, st.y, total);
       }
       s = make_float4(fmaf(x.x, f, s.x), fmaf(x.y, f, s.y), fmaf(x.z, f, s.z), fmaf(x.w, f, s.w));
@@ -1202,7 +1208,7 @@ attn_merge_kernel(const __grid_constant__ TcArgs t) {
     if (MODE == FWD) {
       const bool empty = row + past >= len;
       const float mul = empty ? 0.0f : __fmul_rn(__fdiv_rn(1.0f, total), scale_v);
-      if (col == 0) a.lse[(int64_t)head * a.q_len + row] = empty ? CUDART_INF_F : __fadd_rn(top, __fsub_rn(log2f(total), 14.0f));
+      if (col == 0) a.lse[(int64_t)head * a.q_len + row] = empty ? CUDART_INF_F : fmaf(top, c, __fsub_rn(log2f(total), 14.0f));
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         if (col + u < a.dim) a.o[at + u] = empty ? 0.0f : __fmul_rn(v[u], mul);

@@ -183,3 +183,40 @@ def test_what_is_not_a_number_reaches_the_gradients(nn_gpu, S, D, window, which,
         assert np.isfinite(x[0, 1]).all(), name
         assert np.isfinite(x[0, 0][~bad]).all(), name
         assert np.isnan(x[0, 0][bad]).all(), name
+
+
+# ---------------------------------------------------------------------------------------------
+# scores far from zero
+# ---------------------------------------------------------------------------------------------
+SCORES = [1e3, 1e5, 1e6, 3e7, 1e8, 3e9, 1e12]
+WINNERS = [(40, 16, 1), (300, 64, 2), (300, 128, 2), (140, 200, 1), (1500, 64, 1), (1200, 128, 1)]
+
+
+def clear_winners(S, D, heads, score):
+    """q, k, v, dO in which each query has one key far above all others, or two that are equal; the weights, and how far off
+    they may be."""
+    rng = np.random.default_rng(S + D)
+    k = rng.choice([-1.0, 1.0], (heads, S, D)).astype(np.float32)
+    k[:, 1::4] = k[:, 0:k[:, 1::4].shape[1] * 4:4]          # keys 4 n and 4 n + 1 are the same
+    winner = np.array([[rng.integers(0, i + 1) for i in range(S)] for _ in range(heads)])
+    q = (np.take_along_axis(k, winner[..., None], 1) * np.float32(score / D)).astype(np.float32)
+    v, do = (rng.standard_normal((heads, S, D)).astype(np.float32) for _ in range(2))
+    dots = np.einsum("hid,hjd->hij", q.astype(np.float64), k.astype(np.float64))
+    dots[:, np.triu(np.ones((S, S), bool), 1)] = -np.inf
+    w = np.exp(dots - dots.max(-1, keepdims=True))
+    w /= w.sum(-1, keepdims=True)
+    # Equal keys have equal scores.  A weight is off by 2^-20, and by what errors of the others' scores, (D + 8) 2^-22 of them, make
+    # of their weights, which are `clear` at most.
+    clear = float(np.sort(w, -1)[..., :-2].max())
+    return q, k, v, do, w, 2.0 ** -20 + S * min(1.0, clear * np.exp(min(2 * (D + 8) * 2.0 ** -22 * score, 600.0)))
+
+
+@pytest.mark.parametrize("score", SCORES)
+@pytest.mark.parametrize("S,D,heads", WINNERS)
+def test_clear_winners_at_any_score(nn_gpu, S, D, heads, score):
+    """The weight of the winner is one, or a half each of two, however large the scores are."""
+    nn = nn_gpu
+    q, k, v, _, w, off = clear_winners(S, D, heads, score)
+    got = nn.sink_attention(*[nn.Tensor_from_value(x[None]) for x in (q, k, v)], S, scale=1.0).np()[0]
+    o = w @ v.astype(np.float64)
+    base.close(got, o, off * np.abs(v).max() + 2.0 ** -21 * np.abs(o), "o")
