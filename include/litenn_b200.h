@@ -447,7 +447,7 @@ int lnn_token_logit_bwd_acc(int dev, uint64_t dX, uint64_t X, uint64_t STATS, ui
 /* Causal attention with a sliding window and `sinks` first tokens that stay visible.  Q, O [batch][q_heads][q_len][dim],
  * K, V [batch][kv_heads][kv_len][dim]; query i is at position p = i + kv_len - q_len and sees key j when p < LEN[batch],
  * j <= p and (p - j < window or j < sinks).  Rows that see nothing give zeros.  LEN may be 0 (kv_len everywhere).
- * LSE [batch][q_heads][q_len] is kept for the gradients; a gradient whose pointer is 0 is not computed. */
+ * LSE [batch][q_heads][q_len][2] (logarithms as sums of two floats) is kept for the gradients; a gradient whose pointer is 0 is not computed. */
 typedef struct lnn_attn_geom {
   int batch, q_heads, kv_heads, q_len, kv_len, dim, window, sinks;
   float scale;

@@ -101,7 +101,7 @@ simt_fwd_kernel(const AttnArgs a) {
     const int len = lnn::attn_length(a.lengths, b, a.kv_len, a.status);
     const int64_t head = (int64_t)b * a.q_heads + h;
     const int64_t kv = ((int64_t)b * a.kv_heads + h / (a.q_heads / a.kv_heads)) * a.kv_len * a.dim;
-    const float factor = a.scale * lnn::kLog2e;
+    const float factor = fabsf(a.scale) * lnn::kLog2e, sign = a.scale < 0.0f ? -1.0f : 1.0f;
     float o[R][DP / 16], m[R], l[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -128,17 +128,17 @@ simt_fwd_kernel(const AttnArgs a) {
           float top = -CUDART_INF_F;
 #pragma unroll
           for (int c = 0; c < R; ++c) {
-            s[r][c] = p <= p_hi && lnn::attn_visible(p, j0 + tx + 16 * c, a.window, a.sinks) ? __fmul_rn(s[r][c], factor)
-                                                                                              : -CUDART_INF_F;
+            s[r][c] = p <= p_hi && lnn::attn_visible(p, j0 + tx + 16 * c, a.window, a.sinks) ? __fmul_rn(s[r][c], sign) : -CUDART_INF_F;
             top = fmaxf(top, s[r][c]);
           }
           top = fmaxf(m[r], row_max(top));
           const float base = top == -CUDART_INF_F ? 0.0f : top;
-          const float keep = exp2_fast(__fsub_rn(m[r], base));
+          // (differences of scores before the factor, which may be 0)
+          const float keep = m[r] == -CUDART_INF_F ? 0.0f : exp2_fast(__fmul_rn(__fsub_rn(m[r], base), factor));
           float sum = 0.0f;
 #pragma unroll
           for (int c = 0; c < R; ++c) {
-            const float e = exp2_fast(__fsub_rn(s[r][c], base));
+            const float e = s[r][c] == -CUDART_INF_F ? 0.0f : exp2_fast(__fmul_rn(__fsub_rn(s[r][c], base), factor));
             sum = __fadd_rn(sum, e);
             P[(ty + 16 * r) * (B + 1) + tx + 16 * c] = __fmul_rn(e, a.down);
           }
@@ -161,12 +161,17 @@ simt_fwd_kernel(const AttnArgs a) {
 #pragma unroll
       for (int u = 0; u < DP / 16; ++u)
         if (tx + 16 * u < a.dim) to[tx + 16 * u] = empty ? 0.0f : __fmul_rn(__fmul_rn(o[r][u], inv), a.up);
-      if (tx == 0) a.lse[head * a.q_len + i] = empty ? CUDART_INF_F : __fadd_rn(m[r], log2f(l[r]));
+      if (tx == 0)
+        reinterpret_cast<float2*>(a.lse)[head * a.q_len + i] = empty ? make_float2(CUDART_INF_F, 0.0f) : lnn::log_sum(m[r], factor, l[r]);
     }
   }
   if (a.beside) lnn::wait_at_end();
 }
 
+// 2^(factor s - lse), 1 at most whatever rounding says
+__device__ __forceinline__ float weight(float s, float factor, float2 lse) {
+  return exp2_fast(min_or_nan(__fsub_rn(fmaf(s, factor, -lse.x), lse.y), 0.0f));
+}
 // P = 2^(factor S - lse) and dS = scale P (dP - delta) of a tile: rows are queries (KEYS false) or keys (true)
 template <int B, int DP>
 __global__ void __launch_bounds__(kThreads)
@@ -188,11 +193,12 @@ simt_dq_kernel(const AttnArgs a) {
     const int64_t head = (int64_t)b * a.q_heads + h;
     const int64_t kv = ((int64_t)b * a.kv_heads + h / (a.q_heads / a.kv_heads)) * a.kv_len * a.dim;
     const float factor = a.scale * lnn::kLog2e;
-    float g[R][DP / 16], lse[R], delta[R];
+    float g[R][DP / 16], delta[R];
+    float2 lse[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int i = i0 + ty + 16 * r;
-      lse[r] = i < a.q_len ? a.lse[head * a.q_len + i] : CUDART_INF_F;
+      lse[r] = i < a.q_len ? __ldg(reinterpret_cast<const float2*>(a.lse) + head * a.q_len + i) : make_float2(CUDART_INF_F, 0.0f);
       delta[r] = i < a.q_len ? a.delta[head * a.delta_pitch + i] : 0.0f;
 #pragma unroll
       for (int u = 0; u < DP / 16; ++u) g[r][u] = 0.0f;
@@ -217,7 +223,7 @@ simt_dq_kernel(const AttnArgs a) {
           for (int c = 0; c < R; ++c) {
             const int p = i0 + ty + 16 * r + past;
             const bool seen = p <= p_hi && lnn::attn_visible(p, j0 + tx + 16 * c, a.window, a.sinks);
-            const float e = exp2_fast(min_or_nan(__fsub_rn(__fmul_rn(s[r][c], factor), lse[r]), 0.0f));      // (1 at most, whatever rounding says)
+            const float e = weight(s[r][c], factor, lse[r]);
             S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fsub_rn(dp[r][c], delta[r])), a.scale) : 0.0f;
           }
         __syncthreads();
@@ -278,12 +284,12 @@ simt_dkv_kernel(const AttnArgs a) {
 #pragma unroll
           for (int c = 0; c < R; ++c) {
             const int i = i0 + tx + 16 * c, p = i + past;
-            const float lse = i < a.q_len ? __ldg(a.lse + head * a.q_len + i) : CUDART_INF_F;
+            const float2 lse = i < a.q_len ? __ldg(reinterpret_cast<const float2*>(a.lse) + head * a.q_len + i) : make_float2(CUDART_INF_F, 0.0f);
             const float delta = i < a.q_len ? __ldg(a.delta + head * a.delta_pitch + i) : 0.0f;
 #pragma unroll
             for (int r = 0; r < R; ++r) {
               const bool seen = i < a.q_len && p < len && lnn::attn_visible(p, j0 + ty + 16 * r, a.window, a.sinks);
-              const float e = seen ? exp2_fast(min_or_nan(__fsub_rn(__fmul_rn(s[r][c], factor), lse), 0.0f)) : 0.0f;
+              const float e = seen ? weight(s[r][c], factor, lse) : 0.0f;
               P[(ty + 16 * r) * (B + 1) + tx + 16 * c] = e;
               S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fsub_rn(dp[r][c], delta)), a.scale) : 0.0f;
             }
@@ -885,7 +891,7 @@ int lnn_sink_attn_fwd(int dev, uint64_t O, uint64_t LSE, uint64_t Q, uint64_t K,
   LNN_DEV(d, dev);
   int rc = check_geom(g);
   if (rc) return rc;
-  LNN_REQUIRE(O && LSE && Q && K && V, "bad arguments");
+  LNN_REQUIRE(O && LSE && LSE % 8 == 0 && Q && K && V, "bad arguments");
   AttnArgs a = attn_args(d, g, Q, K, V, LEN);
   a.o = out(O); a.lse = out(LSE);
   return lnn::attn_tc_applicable(a) ? lnn::attn_tc_fwd(d, a) : lnn::attn_simt_fwd(d, a);
@@ -896,7 +902,7 @@ int lnn_sink_attn_bwd(int dev, uint64_t dQ, uint64_t dK, uint64_t dV, uint64_t Q
   LNN_DEV(d, dev);
   int rc = check_geom(g);
   if (rc) return rc;
-  LNN_REQUIRE(Q && K && V && O && LSE && dO, "bad arguments");
+  LNN_REQUIRE(Q && K && V && O && LSE && LSE % 8 == 0 && dO, "bad arguments");
   AttnArgs a = attn_args(d, g, Q, K, V, LEN);
   a.o = out(O); a.lse = out(LSE); a.dout = in(dO);
   a.dq = out(dQ); a.dk = out(dK); a.dv = out(dV);

@@ -5,6 +5,8 @@
 //   p < length,  j <= p  and  (p - j < window  or  j < sinks).
 // Rows that see nothing (padding behind a sequence's length) give zeros and receive and pass on no gradient.
 #pragma once
+#include <float.h>
+#include <math_constants.h>
 #include "lnn_common.cuh"
 
 namespace lnn {
@@ -20,7 +22,7 @@ struct AttnArgs {
   const float *q, *k, *v;        // [batch][q_heads][q_len][dim], [batch][kv_heads][kv_len][dim]
   const float* lengths;          // [batch] whole numbers, or null: kv_len everywhere
   float* o;
-  float* lse;                    // [batch][q_heads][q_len]: log2 of the softmax' denominator, +inf where nothing is seen
+  float* lse;                    // [batch][q_heads][q_len][2]: log2 of the softmax' denominator, see log_sum; +inf, 0 where nothing is seen
   const float* dout;             // gradient of o
   const float* delta;            // [batch][q_heads][delta_pitch]: rows of dout * o summed
   int64_t delta_pitch;
@@ -113,6 +115,15 @@ __device__ __forceinline__ float min_or_nan(float a, float b) {
   float y;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
+}
+// log2 of a softmax' denominator, c top + log2(sum) where sum is of 2^(c (s - top)), as the sum of two floats: 24 bits of it
+// would leave a weight 2^(c s - log_sum) nothing to go by once scores are large (half a step is 2^-11 at 10^4 and 1 at 10^7).  The
+// difference fma(c, s, -hi) is rounded at its own size.  NaN where the scores themselves are past fp32's range.
+__device__ __forceinline__ float2 log_sum(float top, float c, float sum) {
+  const float p = __fmul_rn(top, c), q = log2f(sum);
+  if (!(fabsf(p) <= FLT_MAX)) return make_float2(CUDART_NAN_F, 0.0f);
+  const float hi = __fadd_rn(p, q), b = __fsub_rn(hi, p);
+  return make_float2(hi, __fadd_rn(fmaf(top, c, -p), __fadd_rn(__fsub_rn(p, __fsub_rn(hi, b)), __fsub_rn(q, b))));
 }
 // 2^x with a relative error of 2^-22, 0 below the normal numbers
 __device__ __forceinline__ float exp2_fast(float x) {

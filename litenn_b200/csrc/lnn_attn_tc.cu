@@ -77,13 +77,15 @@ struct PrepArgs {
   unsigned int* counters;        // one per head, zero between launches
   // the last tensor is dO
   const float *o, *lse;
-  float *lse_p, *delta_p;
+  float *lse_p, *delta_p;        // lse_p: -hi, -hi, -lo, -lo of two rows
   int pitch;
   int* taken;                    // [4] works that have been taken, of each pass
   int* status;
 };
 
 struct Eight { float4 a, b; };
+// hi of a row's logarithm, lo is two floats behind: two rows are read together
+__device__ __forceinline__ int64_t lse_at(int64_t head, int pitch, int row) { return head * 2 * pitch + (row >> 1) * 4 + (row & 1); }
 
 // VEC: rows of whole, aligned quads
 template <int DP, bool VEC>
@@ -204,12 +206,17 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
     }
   }
   if (is_do) {
+    const auto put_lse = [&](int r, float2 v) {
+      float* to = a.lse_p + lse_at(head, a.pitch, r);
+      to[0] = -v.x;
+      to[2] = -v.y;
+    };
     for (int r = blockIdx.x * a.block_rows + threadIdx.x; r < r_end; r += kPrepThreads)
-      a.lse_p[(int64_t)head * a.pitch + r] = r < end ? __ldg(a.lse + (int64_t)head * t.rows + r) : CUDART_INF_F;
+      put_lse(r, r < end ? __ldg(reinterpret_cast<const float2*>(a.lse) + (int64_t)head * t.rows + r) : make_float2(CUDART_INF_F, 0.0f));
     if ((int)blockIdx.x == blocks - 1)                           // columns that exist in no head
       for (int r = t.rows + threadIdx.x; r < a.pitch; r += kPrepThreads) {
         a.delta_p[(int64_t)head * a.pitch + r] = 0.0f;
-        a.lse_p[(int64_t)head * a.pitch + r] = CUDART_INF_F;
+        put_lse(r, make_float2(CUDART_INF_F, 0.0f));
       }
   }
   top = __all_sync(0xffffffffu, finite) ? warp_max(top) : CUDART_INF_F;
@@ -244,7 +251,7 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
 // ---- the passes ----------------------------------------------------------------------------------------
 struct TcArgs {
   AttnArgs a;
-  const float *lse_p, *delta_p;  // [q head][pitch]
+  const float *lse_p, *delta_p;  // [q head][2 pitch] (see PrepArgs), [q head][pitch]
   const float* norms;            // squares, DQ: of dO's rows, DK: of V's
   int pitch, width;
   int works;
@@ -269,7 +276,7 @@ template <int MODE, int DP> struct Shape {
   static constexpr int NY = TWO ? 3 : (DP == 128 ? 1 : 2), NZ = TWO ? 2 : (DP == 128 ? 1 : 2);
   static constexpr int NS = TWO ? 2 : 3;                         // score buffers (and of dP)
   static constexpr int NO = TWO ? NY : NZ;                       // steps that a completed result is told apart over
-  static constexpr uint32_t SMEM = X_BYTES + (NY + NZ) * Y_BYTES + 1024;
+  static constexpr uint32_t TILES = X_BYTES + (NY + NZ) * Y_BYTES;
   // TMEM columns: DQ and DK keep their second stationary operand (dO, V) there, which leaves shared memory for a third
   // stream tile and makes its products faster (33 instead of 50 clocks for 64 columns)
   static constexpr uint32_t T_DP = NS * BN, T_OUT = T_DP + (TWO ? NS * BN : 0), T_X2 = T_OUT + DP;
@@ -281,6 +288,8 @@ template <int MODE, int DP> struct Shape {
 __device__ __forceinline__ int64_t parts_per_head(const TcArgs& t) {
   return (int64_t)t.sink_tiles * t.splits_sink + (t.splits > 1 ? (int64_t)(t.tiles - t.sink_tiles) * t.splits : 0);
 }
+
+constexpr float kWeightUnit = 1.0f / 16384.0f;      // weights are 2^14 times what they stand for
 
 // Accumulated scores times this are scores to the base two.  (2^-126 in place of 0: masked scores stay -inf)
 __device__ __forceinline__ float score_factor(const AttnArgs& a, int eq, int ek) {
@@ -492,7 +501,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
   // are complete: DK, when its Y slot is (OUT(g) is over); DV, when Y(g + 4) is loaded: S(g + 4 - NY) waited for them.
   constexpr int NC = S::TWO ? NY : 4;
   __shared__ uint64_t bar_c_full[NC];
-  __shared__ __align__(16) float col_lse[S::KEYS ? NC : 1][BN], col_delta[MODE == DK ? NC : 1][BN];
+  __shared__ __align__(16) float col_lse[S::KEYS ? NC : 1][2 * BN], col_delta[MODE == DK ? NC : 1][BN];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &abort_flag_smem;
@@ -518,8 +527,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
   }
   if (t.beside) lnn::start_next();
   else lnn::wait_for_previous();
-  // an earlier kernel gave up: leave as a whole CTA (the decision must be uniform)
-  if (threadIdx.x == 0) abort_flag_smem = wait_expired(status) ? 2 : 0;
+  // an earlier kernel gave up, or the tiles have no place: leave as a whole CTA (the decision must be uniform)
+  if (threadIdx.x == 0) {
+    uint32_t dynamic;
+    asm("mov.u32 %0, %%dynamic_smem_size;" : "=r"(dynamic));
+    const bool fits = base + S::TILES <= smem_u32(smem_raw) + dynamic;
+    if (!fits) report_expired_wait(status, 36, (int)blockIdx.x, 0);
+    abort_flag_smem = !fits || wait_expired(status) ? 2 : 0;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -627,8 +642,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           if (S::KEYS) {
             const int64_t at = (int64_t)z.head * t.pitch + z.r;
             const uint32_t bc = smem_u32(&bar_c_full[g % NC]);
-            mbar_expect_tx(bc, (MODE == DK ? 2 : 1) * BN * 4);
-            bulk_load(smem_u32(&col_lse[g % NC][0]), t.lse_p + at, BN * 4, bc);
+            mbar_expect_tx(bc, (MODE == DK ? 3 : 2) * BN * 4);
+            bulk_load(smem_u32(&col_lse[g % NC][0]), t.lse_p + 2 * at, 2 * BN * 4, bc);
             if (MODE == DK) bulk_load(smem_u32(&col_delta[g % NC][0]), t.delta_p + at, BN * 4, bc);
           }
         }
@@ -825,7 +840,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           mul = 1.0f;
           if (part == 0) t.stats[(int64_t)k.part * kRowsM + row_in] = make_float2(empty ? -CUDART_INF_F : top, empty ? 0.0f : sum);
         } else if (part == 0 && row < rows)
-          a.lse[(int64_t)xh * rows + row] = empty ? CUDART_INF_F : fmaf(top, score_factor(a, k.eq, k.ek), __fsub_rn(log2f(sum), 14.0f));
+          reinterpret_cast<float2*>(a.lse)[(int64_t)xh * rows + row] =
+              empty ? make_float2(CUDART_INF_F, 0.0f) : lnn::log_sum(top, score_factor(a, k.eq, k.ek), __fmul_rn(sum, kWeightUnit));
         dst = a.o;
       } else if (MODE == DQ) {
         mul = factor_of;
@@ -926,12 +942,13 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       const float m_old = m, l_old = l, times_old = times;
       m = -CUDART_INF_F;
       l = 0.0f;
-      float row_lse = CUDART_INF_F, row_delta = 0.0f;              // DQ
+      float row_hi = -CUDART_INF_F, row_lo = 0.0f, row_delta = 0.0f;      // DQ: - logarithm of the denominator, in two; delta
       int row_exp = 0;                                             // DQ, DK: dS is scaled by 2^row_exp
       float norm = 0.0f;
       if (S::TWO && row < rows) norm = sqrtf(__ldg(t.norms + (int64_t)xh * rows + row));
       if (MODE == DQ && row < rows) {
-        row_lse = __ldg(t.lse_p + (int64_t)xh * t.pitch + row);
+        row_hi = __ldg(t.lse_p + lse_at(xh, t.pitch, row));
+        row_lo = __ldg(t.lse_p + lse_at(xh, t.pitch, row) + 2);
         row_delta = __ldg(t.delta_p + (int64_t)xh * t.pitch + row);
       }
       if (S::TWO) {
@@ -1058,9 +1075,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
         } else {
           if (col0 < n) {
             const float exponent = S::TWO ? (float)row_exp : 14.0f;
-            const uint64_t c2 = pack2(c, c), cdp2 = pack2(cdp, cdp), e2 = pack2(exponent, exponent), minus = pack2(-1.0f, -1.0f);
-            uint64_t up = pack2(exponent - row_lse, exponent - row_lse), less = pack2(-row_delta, -row_delta);
-            const float* cl = &col_lse[S::KEYS ? g % NC : 0][S::KEYS ? col0 : 0];
+            const uint64_t c2 = pack2(c, c), cdp2 = pack2(cdp, cdp), e2 = pack2(exponent, exponent);
+            uint64_t hi = pack2(row_hi, row_hi), up = pack2(exponent + row_lo, exponent + row_lo), less = pack2(-row_delta, -row_delta);
+            const float* cl = &col_lse[S::KEYS ? g % NC : 0][S::KEYS ? 2 * col0 : 0];
             const float* cd = &col_delta[MODE == DK ? g % NC : 0][MODE == DK ? col0 : 0];
 #pragma unroll
             for (int q = 0; q < COLS / 16; ++q) {
@@ -1077,16 +1094,17 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 if (S::KEYS) {                                     // (a warp reads one address)
-                  const float2 l2 = *reinterpret_cast<const float2*>(cl + q * 16 + 2 * i);
-                  up = fma2(pack2(l2.x, l2.y), minus, e2);
+                  const float4 l4 = *reinterpret_cast<const float4*>(cl + (q * 16 + 2 * i) * 2);
+                  hi = pack2(l4.x, l4.y);
+                  up = add2(pack2(l4.z, l4.w), e2);
                   if (S::TWO) {
                     const float2 d2 = *reinterpret_cast<const float2*>(cd + q * 16 + 2 * i);
                     less = pack2(-d2.x, -d2.y);
                   }
                 }
                 float x, y;
-                unpack2(fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), c2, up), x, y);
-                // (a weight is 1 at most, however far scores of 10^6 and more are off)
+                unpack2(add2(fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), c2, hi), up), x, y);
+                // (a weight is 1 at most, whatever rounding says)
                 wt[i] = pack2(exp2_fast(min_or_nan(x, exponent)), exp2_fast(min_or_nan(y, exponent)));
                 if (S::TWO)
                   wt[i] = mul2(wt[i], fma2(pack2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), cdp2, less));
@@ -1208,7 +1226,9 @@ attn_merge_kernel(const __grid_constant__ TcArgs t) {
     if (MODE == FWD) {
       const bool empty = row + past >= len;
       const float mul = empty ? 0.0f : __fmul_rn(__fdiv_rn(1.0f, total), scale_v);
-      if (col == 0) a.lse[(int64_t)head * a.q_len + row] = empty ? CUDART_INF_F : fmaf(top, c, __fsub_rn(log2f(total), 14.0f));
+      if (col == 0)
+        reinterpret_cast<float2*>(a.lse)[(int64_t)head * a.q_len + row] =
+            empty ? make_float2(CUDART_INF_F, 0.0f) : lnn::log_sum(top, c, __fmul_rn(total, kWeightUnit));
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         if (col + u < a.dim) a.o[at + u] = empty ? 0.0f : __fmul_rn(v[u], mul);
@@ -1232,9 +1252,17 @@ int operand_map(CUtensorMap* tm, const void* base, int width, int rows, int64_t 
 template <int MODE, int DP>
 int launch_pass(lnn::Device* d, const CUtensorMap* x, const CUtensorMap* y, const CUtensorMap* z, const TcArgs& t) {
   using S = Shape<MODE, DP>;
-  static_assert(S::SMEM + 2048 <= 227 * 1024, "shared memory");
-  LNN_CUDA(cudaFuncSetAttribute(attn_tc_kernel<MODE, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
-  LNN_CUDA(lnn::launch_chained(d, attn_tc_kernel<MODE, DP>, std::min(t.works, d->sm_count), kAttnThreads, S::SMEM, *x, *y, *z, t));
+  // The tiles begin at a multiple of 1024, for which there is that much room where the block has it; DK at 128 values leaves 256
+  // bytes: enough behind what the kernel declares itself, and the kernel looks whether it is.
+  static size_t declared = 0;
+  if (declared == 0) {
+    cudaFuncAttributes attr;
+    LNN_CUDA(cudaFuncGetAttributes(&attr, attn_tc_kernel<MODE, DP>));
+    declared = attr.sharedSizeBytes;
+  }
+  const size_t bytes = std::min<size_t>(S::TILES + 1024, 227 * 1024 - declared);
+  LNN_CUDA(cudaFuncSetAttribute(attn_tc_kernel<MODE, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  LNN_CUDA(lnn::launch_chained(d, attn_tc_kernel<MODE, DP>, std::min(t.works, d->sm_count), kAttnThreads, bytes, *x, *y, *z, t));
   LNN_CHECK_LAUNCH(d);
   return LNN_OK;
 }
@@ -1318,14 +1346,14 @@ int prepare(lnn::Device* d, AttnArgs& a, Operands& op, bool backward) {
   p.blocks = (int)row_blocks(a.kv_len);
   p.pitch = (a.q_len + 7) / 8 * 8 + kRowsM;
   const int64_t heads = 2 * nk + (backward ? 2 : 1) * nq;
-  const int64_t norm_words = backward ? nk * a.kv_len + nq * a.q_len : 0, col_words = backward ? 2 * nq * p.pitch : 0;
+  const int64_t norm_words = backward ? nk * a.kv_len + nq * a.q_len : 0, col_words = backward ? 3 * nq * p.pitch : 0;
   const int64_t info_words = (heads * (int64_t)sizeof(HeadInfo) / 4 + 3) / 4 * 4;
   rc = op.small.get((uint64_t)(4 + info_words + (col_words + 3) / 4 * 4 + 2 * heads * p.blocks + norm_words) * 4);
   if (rc) return rc;
   float* s = op.small.as<float>();
   p.taken = (int*)s; s += 4;
   p.info = (HeadInfo*)s; s += info_words;
-  p.lse_p = s; p.delta_p = s + col_words / 2; s += (col_words + 3) / 4 * 4;       // (16-byte aligned: the pitch is a multiple of 8)
+  p.lse_p = s; p.delta_p = s + 2 * nq * p.pitch; s += (col_words + 3) / 4 * 4;       // (16-byte aligned: the pitch is a multiple of 8)
   p.block_max = s; s += heads * p.blocks;
   p.block_norm = s; s += heads * p.blocks;
   float *norm_v = backward ? s : nullptr, *norm_do = backward ? s + nk * a.kv_len : nullptr;

@@ -222,7 +222,7 @@ def sink_attention(q_t, k_t, v_t, window, sinks=0, scale=None, lengths_t=None):
         if lengths_t.shape.size != B:
             raise ValueError(f"lengths_t must have {B} elements, one per sequence, got {lengths_t.shape}")
     geom = _geom(B, Hq, Hkv, T, S, D, min(window, S), min(sinks, S), scale)
-    output_t, lse_t = _out(q_t.shape, "sink_attention"), _out(_shape(B, Hq, T))
+    output_t, lse_t = _out(q_t.shape, "sink_attention"), _out(_shape(B, Hq, T, 2))
     output_t._gradfns = _AttentionGrad(q_t, k_t, v_t, lengths_t, lse_t, geom)
     for i, dev in _each_device():
         _call.lnn_sink_attn_fwd(i, dev, output_t, lse_t, q_t, k_t, v_t, lengths_t, geom.address)

@@ -220,3 +220,27 @@ def test_clear_winners_at_any_score(nn_gpu, S, D, heads, score):
     got = nn.sink_attention(*[nn.Tensor_from_value(x[None]) for x in (q, k, v)], S, scale=1.0).np()[0]
     o = w @ v.astype(np.float64)
     base.close(got, o, off * np.abs(v).max() + 2.0 ** -21 * np.abs(o), "o")
+
+
+@pytest.mark.parametrize("score", SCORES)
+@pytest.mark.parametrize("S,D,heads", WINNERS)
+def test_gradients_of_clear_winners_at_any_score(nn_gpu, S, D, heads, score):
+    nn = nn_gpu
+    q, k, v, do, w, off = clear_winners(S, D, heads, score)
+    t = [nn.Tensor_from_value(x[None]) for x in (q, k, v)]
+    base.trainable(nn, *t)
+    nn.backward({nn.sink_attention(*t, S, scale=1.0): nn.Tensor_from_value(do[None])})
+    q, k, v, do = (x.astype(np.float64) for x in (q, k, v, do))
+    ds = w * (np.einsum("hid,hjd->hij", do, v) - (do * (w @ v)).sum(-1, keepdims=True))
+    want = {"dq": ds @ k, "dk": np.swapaxes(ds, 1, 2) @ q, "dv": np.swapaxes(w, 1, 2) @ do}
+    got = dict(zip(("dq", "dk", "dv"), [x.get_grad().np()[0] for x in t]))
+    # dP - delta: D products each, of (D + 8) 2^-22 of their magnitudes; dS is held as two fp16 numbers under a bound of 2^15 that is
+    # at most 16 |dO| |V| (two powers of two, the sum of dP and delta, the largest of a head for a row's): what is below 2^-39 of
+    # that is lost.
+    mag = np.einsum("hid,hjd->hij", np.abs(do), np.abs(v))
+    mag = mag + (w * mag).sum(-1, keepdims=True)
+    lost = 2.0 ** -39 * 16 * np.linalg.norm(do, axis=-1).max() * np.linalg.norm(v, axis=-1).max()
+    ds_off = (w * ((D + 8) * 2.0 ** -22) + off * (w > 1e-3)) * mag + 2.0 ** -21 * np.abs(ds) + lost
+    base.close(got["dv"], want["dv"], (off + (S + 8) * U) * np.abs(do).sum(1, keepdims=True), "dv")
+    base.close(got["dq"], want["dq"], ds_off @ np.abs(k), "dq")
+    base.close(got["dk"], want["dk"], np.swapaxes(ds_off, 1, 2) @ np.abs(q), "dk")
