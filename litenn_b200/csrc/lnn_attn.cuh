@@ -98,7 +98,8 @@ __device__ __forceinline__ bool group_ok(const AttnArgs& a, int b, int hk) {
     ok = ok && q.ok && abs(q.e) <= 100 && abs(q.e + k.e) <= 100;
     if (a.backward) {
       const HeadInfo o = info_of(a, 3, h);
-      ok = ok && o.ok && abs(o.e) <= 100 && abs(o.e + v.e) <= 100 && abs(q.e + o.e + v.e) <= 90 && abs(k.e + o.e + v.e) <= 90;
+      // (weights times 2^row_exp, 2^-26 2^-(o.e + v.e) or more, are above fp32's smallest down to 2^-44: what is left of 2^-40 in fp16)
+      ok = ok && o.ok && abs(o.e) <= 100 && o.e + v.e >= -100 && o.e + v.e <= 56 && abs(q.e + o.e + v.e) <= 90 && abs(k.e + o.e + v.e) <= 90;
     }
   }
   return ok;

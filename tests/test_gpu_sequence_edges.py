@@ -244,3 +244,35 @@ def test_gradients_of_clear_winners_at_any_score(nn_gpu, S, D, heads, score):
     base.close(got["dv"], want["dv"], (off + (S + 8) * U) * np.abs(do).sum(1, keepdims=True), "dv")
     base.close(got["dq"], want["dq"], ds_off @ np.abs(k), "dq")
     base.close(got["dk"], want["dk"], np.swapaxes(ds_off, 1, 2) @ np.abs(q), "dk")
+
+
+@pytest.mark.parametrize("size_v,size_do", [(1e18, 1e14), (1e19, 1e2), (1e12, 1e8), (1.0, 1.0), (1e-18, 1e-8)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_gradients_through_small_weights(nn_gpu, D, size_v, size_do):
+    """Keys whose weights are 10^-4 to 10^-10 in every row keep their gradients however large dO V is."""
+    nn = nn_gpu
+    S, scale = 200, 1.0
+    rng = np.random.default_rng(D)
+    q, k, v, do = (rng.standard_normal((1, 1, S, D)).astype(np.float32) for _ in range(4))
+    q *= np.float32(0.05)
+    q[..., 0] = 1.0
+    k[..., 0] = 0.0
+    k[:, :, 20:60, 0] = rng.uniform(-20.0, -8.0, 40)
+    v, do = v * np.float32(size_v), do * np.float32(size_do)
+    seen = base.visible(S, S, S, 0, (S,))
+    r = [torch.tensor(x, dtype=torch.float64, requires_grad=True) for x in (q, k, v)]
+    o = base.plain_attention(*r, seen, scale)
+    d64 = torch.tensor(do, dtype=torch.float64)
+    o.backward(d64)
+    bounds = base.attention_bounds(*[x.detach() for x in r], d64, seen, scale)
+    # what is below 2^-39 of the bound of dS, at most 16 |dO| |V|, is lost (see above), and so are weights below 2^-39
+    lost = 2.0 ** -39 * 16 * np.linalg.norm(do.astype(np.float64), axis=-1).max() * np.linalg.norm(v.astype(np.float64), axis=-1).max()
+    rest = (2.0 ** -39 * np.abs(v).max() * S, lost * np.abs(k).sum(2, keepdims=True), lost * np.abs(q).sum(2, keepdims=True),
+            2.0 ** -39 * np.abs(do).sum(2, keepdims=True))
+    t = [nn.Tensor_from_value(x) for x in (q, k, v)]
+    base.trainable(nn, *t)
+    y = nn.sink_attention(*t, S, scale=scale)
+    nn.backward({y: nn.Tensor_from_value(do)})
+    for name, g, w, b, c in zip(("o", "dq", "dk", "dv"), [y] + [x.get_grad() for x in t], [o.detach()] + [x.grad for x in r], bounds,
+                                rest):
+        base.close(g.np(), w.numpy(), b.detach().numpy() + c, name)
