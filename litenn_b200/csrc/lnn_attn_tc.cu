@@ -48,9 +48,11 @@ constexpr int kRowsM = 128;                      // stationary rows
 // One pass over each operand: split, row norms (what bounds dS), and for dO the rows of dO * O and the denominators
 // with a padded pitch.  Bound by HBM, with about 5 us of dependent latencies in front and behind (24 heads of 8192 rows
 // of 128 values, 200 MB: 35 us).  Eight values to a lane: half the address arithmetic and shuffles of four.
-// The scale of a head is guessed from 32 of its rows, so that the largest value of them is in [2^8, 2^9); the true
-// maximum may be 2^7 times that before fp16 overflows.  A head beyond it, or with values that are not finite, is marked
-// and goes to the FP32-pipe kernels.
+// The scale of a head is guessed from 32 of its rows, the last among them, so that the largest value of them is in [2^8, 2^9);
+// the true maximum may be 2^7 times that before fp16 overflows.  A head beyond it, or with values that are not finite, is
+// marked and goes to the FP32-pipe kernels: a scale for such an outlier would cost the others their low bits.  Where the 32 rows
+// are zero and others are not (dO of a loss on few tokens), the block that ends last splits the head once more with the
+// scale of its true maximum.
 constexpr int kPrepThreads = 256;
 constexpr int kPrepRows = 64;                    // a block takes a multiple of them
 constexpr int kPrepBlocksPerSm = 4;
@@ -71,7 +73,7 @@ struct PrepArgs {
   const float* lengths;
   int kv_len;
   HeadInfo* info;                // [all heads of all tensors]
-  float* block_max;              // [head][blocks]: largest magnitudes after scaling, +inf: not finite
+  float* block_max;              // [head][blocks]: largest magnitudes, +inf: not finite
   float* block_norm;
   int blocks, block_rows;        // row blocks of the longest tensor, rows of a block
   unsigned int* counters;        // one per head, zero between launches
@@ -95,6 +97,7 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
   constexpr int kWarps = kPrepThreads / 32, STRIDE = kWarps * ROWS, BATCH = 2;
   __shared__ float red[kWarps], red_norm[kWarps];
   __shared__ int last_block;
+  __shared__ float head_max;
   lnn::wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LANES, c = lane % LANES * 8;
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 4) a.taken[threadIdx.x] = 0;
@@ -135,7 +138,7 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
       if (is_do && real) y[u] = load(src_o + (int64_t)r * dim);
     }
   };
-  const int r_first = blockIdx.x * a.block_rows + warp * ROWS + sub, r_end = min((int)(blockIdx.x + 1) * a.block_rows, t.rows);
+  int r_first = blockIdx.x * a.block_rows + warp * ROWS + sub, r_end = min((int)(blockIdx.x + 1) * a.block_rows, t.rows);
   fetch(r_first);
   // the scale, from rows spread over those that are real (the same ones in every block of the head; what is not a number is
   // left out here and found below)
@@ -144,7 +147,7 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
   if (span > 0) {
 #pragma unroll
     for (int i = warp * ROWS + sub; i < kSampleRows; i += STRIDE) {
-      const Eight v = load(src + (int64_t)(first + (int)((int64_t)i * span / kSampleRows)) * dim);
+      const Eight v = load(src + (int64_t)(first + (int)((int64_t)i * (span - 1) / (kSampleRows - 1))) * dim);
       top = fmaxf(fmaxf(top, fmaxf(fabsf(v.a.x), fabsf(v.a.y))), fmaxf(fabsf(v.a.z), fabsf(v.a.w)));
       top = fmaxf(fmaxf(top, fmaxf(fabsf(v.b.x), fabsf(v.b.y))), fmaxf(fabsf(v.b.z), fabsf(v.b.w)));
     }
@@ -155,96 +158,117 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) top = fmaxf(top, red[w]);
   const int ebits = (int)(__float_as_uint(top) >> 23);
-  const int e = top == 0.0f || ebits == 255 ? 0 : ebits - 127 - 8;
-  const float factor = t.sign * pow2f_int(max(-126, min(127, -e)));       // (|e| > 100 is not taken anyway)
-  const uint64_t factor2 = pack2(factor, factor), minus = pack2(-1.0f, -1.0f);
+  int e = top == 0.0f || ebits == 255 ? 0 : ebits - 127 - 8;
+  const bool nothing = top == 0.0f;                               // the sample says
+  const uint64_t minus = pack2(-1.0f, -1.0f);
   __syncthreads();
 
   __half* hi = t.hi + (int64_t)head * t.rows * a.width + c;
   __half* lo = hi + (int64_t)t.heads * t.rows * a.width;
-  float top_norm = 0.0f;
-  bool finite = true;
-  top = 0.0f;
-  for (int r0 = r_first; r0 - sub < r_end; r0 += BATCH * STRIDE) {      // (the same turns for both rows of a warp)
-    if (r0 != r_first) fetch(r0);
+  for (bool again = false;; again = true) {
+    const float factor = t.sign * pow2f_int(max(-126, min(127, -e)));     // (|e| > 100 is not taken anyway)
+    const uint64_t factor2 = pack2(factor, factor);
+    float top_norm = 0.0f;
+    bool number = true;
+    top = 0.0f;
+    for (int r0 = r_first; r0 - sub < r_end; r0 += BATCH * STRIDE) {      // (the same turns for both rows of a warp)
+      if (r0 != r_first) fetch(r0);
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      const int r = r0 + u * STRIDE;
-      const bool in = r < r_end;
-      if (is_do) {
-        const float half = fmaf(x[u].a.w, y[u].a.w, fmaf(x[u].a.z, y[u].a.z, fmaf(x[u].a.y, y[u].a.y, __fmul_rn(x[u].a.x, y[u].a.x))));
-        const float delta = row_total(fmaf(x[u].b.w, y[u].b.w, fmaf(x[u].b.z, y[u].b.z, fmaf(x[u].b.y, y[u].b.y, fmaf(x[u].b.x, y[u].b.x, half)))));
-        if (c == 0 && in) a.delta_p[(int64_t)head * a.pitch + r] = delta;
-      }
-      uint32_t h[4], l[4];
-      float norm = 0.0f;
+      for (int u = 0; u < BATCH; ++u) {
+        const int r = r0 + u * STRIDE;
+        const bool in = r < r_end;
+        if (is_do) {
+          const float half = fmaf(x[u].a.w, y[u].a.w, fmaf(x[u].a.z, y[u].a.z, fmaf(x[u].a.y, y[u].a.y, __fmul_rn(x[u].a.x, y[u].a.x))));
+          const float delta = row_total(fmaf(x[u].b.w, y[u].b.w, fmaf(x[u].b.z, y[u].b.z, fmaf(x[u].b.y, y[u].b.y, fmaf(x[u].b.x, y[u].b.x, half)))));
+          if (c == 0 && in) a.delta_p[(int64_t)head * a.pitch + r] = delta;
+        }
+        uint32_t h[4], l[4];
+        float norm = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float4& w = k < 2 ? x[u].a : x[u].b;
-        const uint64_t v = mul2(k & 1 ? pack2(w.z, w.w) : pack2(w.x, w.y), factor2);
-        float p, q;
-        unpack2(v, p, q);
-        top = fmaxf(top, fmaxf(fabsf(p), fabsf(q)));
-        norm = fmaf(q, q, fmaf(p, p, norm));
-        const __half2 hh = __floats2half2_rn(p, q);
-        const float2 f = __half22float2(hh);
-        unpack2(fma2(pack2(f.x, f.y), minus, v), p, q);
-        const __half2 ll = __floats2half2_rn(p, q);
-        h[k] = *reinterpret_cast<const uint32_t*>(&hh);
-        l[k] = *reinterpret_cast<const uint32_t*>(&ll);
-      }
-      finite = finite && norm <= 3.0e38f;                         // (false for what is not a number)
-      if (in && c < a.width) {
-        *reinterpret_cast<uint4*>(hi + (int64_t)r * a.width) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(lo + (int64_t)r * a.width) = make_uint4(l[0], l[1], l[2], l[3]);
-      }
-      if (with_norms) {
-        norm = row_total(norm);
-        top_norm = fmaxf(top_norm, norm);
-        if (c == 0 && in) t.norms[(int64_t)head * t.rows + r] = norm;
+        for (int k = 0; k < 4; ++k) {
+          const float4& w = k < 2 ? x[u].a : x[u].b;
+          top = fmaxf(top, k & 1 ? fmaxf(fabsf(w.z), fabsf(w.w)) : fmaxf(fabsf(w.x), fabsf(w.y)));
+          const uint64_t v = mul2(k & 1 ? pack2(w.z, w.w) : pack2(w.x, w.y), factor2);
+          float p, q;
+          unpack2(v, p, q);
+          norm = fmaf(q, q, fmaf(p, p, norm));
+          const __half2 hh = __floats2half2_rn(p, q);
+          const float2 f = __half22float2(hh);
+          unpack2(fma2(pack2(f.x, f.y), minus, v), p, q);
+          const __half2 ll = __floats2half2_rn(p, q);
+          h[k] = *reinterpret_cast<const uint32_t*>(&hh);
+          l[k] = *reinterpret_cast<const uint32_t*>(&ll);
+        }
+        number = number && norm == norm;
+        if (in && c < a.width) {
+          *reinterpret_cast<uint4*>(hi + (int64_t)r * a.width) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(lo + (int64_t)r * a.width) = make_uint4(l[0], l[1], l[2], l[3]);
+        }
+        if (with_norms) {
+          norm = row_total(norm);
+          top_norm = fmaxf(top_norm, norm);
+          if (c == 0 && in) t.norms[(int64_t)head * t.rows + r] = norm;
+        }
       }
     }
-  }
-  if (is_do) {
-    const auto put_lse = [&](int r, float2 v) {
-      float* to = a.lse_p + lse_at(head, a.pitch, r);
-      to[0] = -v.x;
-      to[2] = -v.y;
-    };
-    for (int r = blockIdx.x * a.block_rows + threadIdx.x; r < r_end; r += kPrepThreads)
-      put_lse(r, r < end ? __ldg(reinterpret_cast<const float2*>(a.lse) + (int64_t)head * t.rows + r) : make_float2(CUDART_INF_F, 0.0f));
-    if ((int)blockIdx.x == blocks - 1)                           // columns that exist in no head
-      for (int r = t.rows + threadIdx.x; r < a.pitch; r += kPrepThreads) {
-        a.delta_p[(int64_t)head * a.pitch + r] = 0.0f;
-        put_lse(r, make_float2(CUDART_INF_F, 0.0f));
+    if (is_do && !again) {
+      const auto put_lse = [&](int r, float2 v) {
+        float* to = a.lse_p + lse_at(head, a.pitch, r);
+        to[0] = -v.x;
+        to[2] = -v.y;
+      };
+      for (int r = blockIdx.x * a.block_rows + threadIdx.x; r < r_end; r += kPrepThreads)
+        put_lse(r, r < end ? __ldg(reinterpret_cast<const float2*>(a.lse) + (int64_t)head * t.rows + r) : make_float2(CUDART_INF_F, 0.0f));
+      if ((int)blockIdx.x == blocks - 1)                           // columns that exist in no head
+        for (int r = t.rows + threadIdx.x; r < a.pitch; r += kPrepThreads) {
+          a.delta_p[(int64_t)head * a.pitch + r] = 0.0f;
+          put_lse(r, make_float2(CUDART_INF_F, 0.0f));
+        }
+    }
+    top = __all_sync(0xffffffffu, number) ? warp_max(top) : CUDART_INF_F;
+    top_norm = warp_max(top_norm);
+    if (lane == 0) { red[warp] = top; red_norm[warp] = top_norm; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < kWarps; ++w) { top = fmaxf(top, red[w]); top_norm = fmaxf(top_norm, red_norm[w]); }
+      if (again) {
+        a.info[blockIdx.y] = HeadInfo{e, 1, sqrtf(top_norm)};
+        last_block = 0;
+      } else {
+        const int64_t at = (int64_t)blockIdx.y * a.blocks;
+        __stcg(a.block_max + at + blockIdx.x, top);
+        __stcg(a.block_norm + at + blockIdx.x, top_norm);
+        __threadfence();
+        last_block = atomicAdd(a.counters + blockIdx.y, 1u) == (unsigned)blocks - 1;
       }
-  }
-  top = __all_sync(0xffffffffu, finite) ? warp_max(top) : CUDART_INF_F;
-  top_norm = warp_max(top_norm);
-  if (lane == 0) { red[warp] = top; red_norm[warp] = top_norm; }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kWarps; ++w) { top = fmaxf(top, red[w]); top_norm = fmaxf(top_norm, red_norm[w]); }
-    const int64_t at = (int64_t)blockIdx.y * a.blocks;
-    __stcg(a.block_max + at + blockIdx.x, top);
-    __stcg(a.block_norm + at + blockIdx.x, top_norm);
-    __threadfence();
-    last_block = atomicAdd(a.counters + blockIdx.y, 1u) == (unsigned)blocks - 1;
-  }
-  __syncthreads();
-  if (!last_block || warp != 0) return;
-  __threadfence();
-  top = 0.0f;
-  top_norm = 0.0f;
-  for (int i = lane; i < blocks; i += 32) {
-    top = fmaxf(top, __ldcg(a.block_max + (int64_t)blockIdx.y * a.blocks + i));
-    top_norm = fmaxf(top_norm, __ldcg(a.block_norm + (int64_t)blockIdx.y * a.blocks + i));
-  }
-  top = warp_max(top);
-  top_norm = warp_max(top_norm);
-  if (lane == 0) {
-    a.info[blockIdx.y] = HeadInfo{e, top == 0.0f || (top >= 4.0f && top < 65000.0f), sqrtf(top_norm)};
-    a.counters[blockIdx.y] = 0;
+    }
+    __syncthreads();
+    if (!last_block) return;
+    if (warp == 0) {
+      __threadfence();
+      top = 0.0f;
+      top_norm = 0.0f;
+      for (int i = lane; i < blocks; i += 32) {
+        top = fmaxf(top, __ldcg(a.block_max + (int64_t)blockIdx.y * a.blocks + i));
+        top_norm = fmaxf(top_norm, __ldcg(a.block_norm + (int64_t)blockIdx.y * a.blocks + i));
+      }
+      top = warp_max(top);
+      top_norm = warp_max(top_norm);
+      if (lane == 0) {
+        const float scaled = __fmul_rn(top, fabsf(factor));
+        a.info[blockIdx.y] = HeadInfo{e, top == 0.0f || (scaled >= 4.0f && scaled < 65000.0f), sqrtf(top_norm)};
+        a.counters[blockIdx.y] = 0;
+        head_max = top;
+      }
+    }
+    if (!nothing) return;
+    __syncthreads();
+    top = head_max;
+    if (top == 0.0f || !(top < CUDART_INF_F)) return;
+    e = (int)(__float_as_uint(top) >> 23) - 127 - 14;              // the largest in [2^14, 2^15)
+    r_first = warp * ROWS + sub;
+    r_end = t.rows;
+    fetch(r_first);
   }
 }
 

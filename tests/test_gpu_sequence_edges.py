@@ -276,3 +276,80 @@ def test_gradients_through_small_weights(nn_gpu, D, size_v, size_do):
     for name, g, w, b, c in zip(("o", "dq", "dk", "dv"), [y] + [x.get_grad() for x in t], [o.detach()] + [x.grad for x in r], bounds,
                                 rest):
         base.close(g.np(), w.numpy(), b.detach().numpy() + c, name)
+
+
+# ---------------------------------------------------------------------------------------------
+# gradients that are zero nearly everywhere
+# ---------------------------------------------------------------------------------------------
+def sparse_rows(S, where):
+    rows = np.zeros(S, bool)
+    if where == "last":
+        rows[S - 20:] = True                                  # the loss is on the answer
+    elif where == "turns":
+        rows[S // 3:S // 3 + 9] = True
+    else:
+        rows[S // 2 + 1] = True
+    return rows
+
+
+@pytest.mark.parametrize("where", ["last", "turns", "one"])
+@pytest.mark.parametrize("S,D", [(300, 64), (1000, 128), (900, 40)])
+def test_gradient_of_some_rows(nn_gpu, S, D, where):
+    nn = nn_gpu
+    case = (1, 4, 2, S, S, D, S // 2, 4, None)
+    (q, k, v, do), lens = base.attention_inputs(case)
+    do[:, :, ~sparse_rows(S, where)] = 0.0
+    do *= np.float32(3e-4)
+    seen, scale = base.visible(S, S, S // 2, 4, lens), D ** -0.5
+    r = [torch.tensor(x, dtype=torch.float64, requires_grad=True) for x in (q, k, v)]
+    o = base.plain_attention(*r, seen, scale)
+    d64 = torch.tensor(do, dtype=torch.float64)
+    o.backward(d64)
+    bounds = base.attention_bounds(*[x.detach() for x in r], d64, seen, scale)
+    t = [nn.Tensor_from_value(x) for x in (q, k, v)]
+    base.trainable(nn, *t)
+    y = nn.sink_attention(*t, S // 2, 4)
+    nn.backward({y: nn.Tensor_from_value(do)})
+    for name, g, w, b in zip(("o", "dq", "dk", "dv"), [y] + [x.get_grad() for x in t], [o.detach()] + [x.grad for x in r], bounds):
+        g = g.np()
+        base.close(g, w.numpy(), b.detach().numpy() + 1e-30, name)
+        norm = float(w.norm())
+        assert np.linalg.norm(g - w.numpy()) <= 1e-5 * norm + bounds[4].get(name, 0.0) + 1e-30, name
+
+
+@pytest.mark.parametrize("where", ["last", "turns", "one"])
+def test_gradient_of_some_rows_stays_on_the_tensor_cores(nn_gpu, where):
+    """The device time of the gradients with dO of zeros but in some rows, against that of a dense dO (the FP32 pipe takes ten
+    times as long and more)."""
+    nn = nn_gpu
+    from litenn_b200 import _lib
+    S, H, D = 4096, 8, 128
+    rng = np.random.default_rng(2)
+    t = [nn.Tensor_from_value(rng.standard_normal((1, H, S, D)).astype(np.float32)) for _ in range(3)]
+    do = rng.standard_normal((1, H, S, D)).astype(np.float32)
+    some = np.where(sparse_rows(S, where)[None, None, :, None], do, np.float32(0))
+    opt = base.trainable(nn, *t)
+
+    lib, dev = _lib.get_lib(), nn.devices.get_current()[0].index
+    ev, ms = [ctypes.c_uint64(), ctypes.c_uint64()], ctypes.c_float()
+    for e in ev:
+        lib.lnn_event_create(dev, ctypes.byref(e))
+
+    def pass_time(do_t):
+        times = []
+        for _ in range(4):
+            opt.zero_grad()
+            y = nn.sink_attention(*t, S)
+            nn.devices.wait()
+            lib.lnn_event_record(dev, ev[0].value)
+            nn.backward({y: do_t})
+            lib.lnn_event_record(dev, ev[1].value)
+            nn.devices.wait()
+            lib.lnn_event_elapsed_ms(dev, ev[0].value, ev[1].value, ctypes.byref(ms))
+            times.append(ms.value)
+        return min(times)
+
+    dense, sparse = pass_time(nn.Tensor_from_value(do)), pass_time(nn.Tensor_from_value(some))
+    for e in ev:
+        lib.lnn_event_destroy(dev, e.value)
+    assert sparse < 3 * dense, (sparse, dense)
