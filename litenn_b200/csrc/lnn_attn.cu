@@ -172,7 +172,7 @@ simt_fwd_kernel(const AttnArgs a) {
 __device__ __forceinline__ float weight(float s, float factor, float2 lse) {
   return exp2_fast(min_or_nan(__fsub_rn(fmaf(s, factor, -lse.x), lse.y), 0.0f));
 }
-// P = 2^(factor S - lse) and dS = scale P (dP - delta) of a tile: rows are queries (KEYS false) or keys (true)
+// P = 2^(factor S - lse) and dS = scale P (dP + delta) of a tile: rows are queries (KEYS false) or keys (true)
 template <int B, int DP>
 __global__ void __launch_bounds__(kThreads)
 simt_dq_kernel(const AttnArgs a) {
@@ -224,7 +224,7 @@ simt_dq_kernel(const AttnArgs a) {
             const int p = i0 + ty + 16 * r + past;
             const bool seen = p <= p_hi && lnn::attn_visible(p, j0 + tx + 16 * c, a.window, a.sinks);
             const float e = weight(s[r][c], factor, lse[r]);
-            S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fsub_rn(dp[r][c], delta[r])), a.scale) : 0.0f;
+            S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fadd_rn(dp[r][c], delta[r])), a.scale) : 0.0f;
           }
         __syncthreads();
         tile_weighted<B, DP>(g, S, K, ty, tx);
@@ -291,7 +291,7 @@ simt_dkv_kernel(const AttnArgs a) {
               const bool seen = i < a.q_len && p < len && lnn::attn_visible(p, j0 + ty + 16 * r, a.window, a.sinks);
               const float e = seen ? weight(s[r][c], factor, lse) : 0.0f;
               P[(ty + 16 * r) * (B + 1) + tx + 16 * c] = e;
-              S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fsub_rn(dp[r][c], delta)), a.scale) : 0.0f;
+              S[(ty + 16 * r) * (B + 1) + tx + 16 * c] = seen ? __fmul_rn(__fmul_rn(e, __fadd_rn(dp[r][c], delta)), a.scale) : 0.0f;
             }
           }
           __syncthreads();
@@ -327,7 +327,7 @@ attn_delta_kernel(float* __restrict__ delta, const float* __restrict__ dout, con
   for (int c = threadIdx.x & 31; c < dim; c += 32) s = fmaf(__ldg(dout + row * dim + c), __ldg(o + row * dim + c), s);
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, x));
-  if ((threadIdx.x & 31) == 0) delta[row] = s;
+  if ((threadIdx.x & 31) == 0) delta[row] = -s;
 }
 
 template <int B, int DP, class Kernel>

@@ -24,7 +24,7 @@ struct AttnArgs {
   float* o;
   float* lse;                    // [batch][q_heads][q_len][2]: log2 of the softmax' denominator, see log_sum; +inf, 0 where nothing is seen
   const float* dout;             // gradient of o
-  const float* delta;            // [batch][q_heads][delta_pitch]: rows of dout * o summed
+  const float* delta;            // [batch][q_heads][delta_pitch]: - rows of dout * o summed
   int64_t delta_pitch;
   float *dq, *dk, *dv;
   int acc_q, acc_k, acc_v;

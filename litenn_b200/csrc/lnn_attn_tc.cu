@@ -79,7 +79,7 @@ struct PrepArgs {
   unsigned int* counters;        // one per head, zero between launches
   // the last tensor is dO
   const float *o, *lse;
-  float *lse_p, *delta_p;        // lse_p: -hi, -hi, -lo, -lo of two rows
+  float *lse_p, *delta_p;        // lse_p: -hi, -hi, 14 - lo, 14 - lo of two rows
   int pitch;
   int* taken;                    // [4] works that have been taken, of each pass
   int* status;
@@ -180,7 +180,7 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
         if (is_do) {
           const float half = fmaf(x[u].a.w, y[u].a.w, fmaf(x[u].a.z, y[u].a.z, fmaf(x[u].a.y, y[u].a.y, __fmul_rn(x[u].a.x, y[u].a.x))));
           const float delta = row_total(fmaf(x[u].b.w, y[u].b.w, fmaf(x[u].b.z, y[u].b.z, fmaf(x[u].b.y, y[u].b.y, fmaf(x[u].b.x, y[u].b.x, half)))));
-          if (c == 0 && in) a.delta_p[(int64_t)head * a.pitch + r] = delta;
+          if (c == 0 && in) a.delta_p[(int64_t)head * a.pitch + r] = -delta;
         }
         uint32_t h[4], l[4];
         float norm = 0.0f;
@@ -215,7 +215,7 @@ attn_prep_kernel(const __grid_constant__ PrepArgs a) {
       const auto put_lse = [&](int r, float2 v) {
         float* to = a.lse_p + lse_at(head, a.pitch, r);
         to[0] = -v.x;
-        to[2] = -v.y;
+        to[2] = 14.0f - v.y;
       };
       for (int r = blockIdx.x * a.block_rows + threadIdx.x; r < r_end; r += kPrepThreads)
         put_lse(r, r < end ? __ldg(reinterpret_cast<const float2*>(a.lse) + (int64_t)head * t.rows + r) : make_float2(CUDART_INF_F, 0.0f));
@@ -966,14 +966,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
       const float m_old = m, l_old = l, times_old = times;
       m = -CUDART_INF_F;
       l = 0.0f;
-      float row_hi = -CUDART_INF_F, row_lo = 0.0f, row_delta = 0.0f;      // DQ: - logarithm of the denominator, in two; delta
+      float row_hi = -CUDART_INF_F, row_up = 0.0f, row_less = 0.0f;      // DQ: see PrepArgs
       int row_exp = 0;                                             // DQ, DK: dS is scaled by 2^row_exp
       float norm = 0.0f;
       if (S::TWO && row < rows) norm = sqrtf(__ldg(t.norms + (int64_t)xh * rows + row));
       if (MODE == DQ && row < rows) {
         row_hi = __ldg(t.lse_p + lse_at(xh, t.pitch, row));
-        row_lo = __ldg(t.lse_p + lse_at(xh, t.pitch, row) + 2);
-        row_delta = __ldg(t.delta_p + (int64_t)xh * t.pitch + row);
+        row_up = __ldg(t.lse_p + lse_at(xh, t.pitch, row) + 2);
+        row_less = __ldg(t.delta_p + (int64_t)xh * t.pitch + row);
       }
       if (S::TWO) {
         // The second stationary operand into TMEM, once the products of the work before are over: this warp's fourth of
@@ -1098,9 +1098,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
           keep_before = keep;
         } else {
           if (col0 < n) {
-            const float exponent = S::TWO ? (float)row_exp : 14.0f;
-            const uint64_t c2 = pack2(c, c), cdp2 = pack2(cdp, cdp), e2 = pack2(exponent, exponent);
-            uint64_t hi = pack2(row_hi, row_hi), up = pack2(exponent + row_lo, exponent + row_lo), less = pack2(-row_delta, -row_delta);
+            const float exponent = S::TWO ? (float)row_exp : 14.0f, more = exponent - 14.0f;
+            const uint64_t c2 = pack2(c, c), cdp2 = pack2(cdp, cdp), more2 = pack2(more, more);
+            uint64_t hi = pack2(row_hi, row_hi), up = pack2(row_up + more, row_up + more), less = pack2(row_less, row_less);
             const float* cl = &col_lse[S::KEYS ? g % NC : 0][S::KEYS ? 2 * col0 : 0];
             const float* cd = &col_delta[MODE == DK ? g % NC : 0][MODE == DK ? col0 : 0];
 #pragma unroll
@@ -1120,10 +1120,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
                 if (S::KEYS) {                                     // (a warp reads one address)
                   const float4 l4 = *reinterpret_cast<const float4*>(cl + (q * 16 + 2 * i) * 2);
                   hi = pack2(l4.x, l4.y);
-                  up = add2(pack2(l4.z, l4.w), e2);
+                  up = S::TWO ? add2(pack2(l4.z, l4.w), more2) : pack2(l4.z, l4.w);
                   if (S::TWO) {
                     const float2 d2 = *reinterpret_cast<const float2*>(cd + q * 16 + 2 * i);
-                    less = pack2(-d2.x, -d2.y);
+                    less = pack2(d2.x, d2.y);
                   }
                 }
                 float x, y;
