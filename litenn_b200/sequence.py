@@ -256,10 +256,10 @@ class SinkCache:
 
     def set_lengths(self, value):
         """A tensor, array or list of `batch` whole numbers, or one number for all."""
-        if isinstance(value, (int, float)):
-            value = np.full(self.batch, value, np.float32)
-        elif not isinstance(value, Tensor):
+        if not isinstance(value, Tensor):
             value = np.asarray(value, np.float32)
+            if value.ndim == 0:
+                value = np.full(self.batch, value)
         if (value.shape.size if isinstance(value, Tensor) else value.size) != self.batch:
             raise ValueError(f"lengths must have {self.batch} elements")
         if not isinstance(value, Tensor):

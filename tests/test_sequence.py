@@ -143,3 +143,10 @@ def test_an_embedding_module_saves_its_table(fake):
     assert [t.get_name() for t in m.trainables()] == ["Embedding.weight"]
     assert tuple(m(T(2, 2)).shape) == (2, 2, 3)
     assert "num_tokens:5" in str(m)
+
+
+@pytest.mark.parametrize("number", [3, 3.0, np.int64(3), np.float32(3), np.array(3)])
+def test_one_number_is_the_length_of_all(fake, number):
+    c = nn.SinkCache(2, 1, 4, 1, 8)
+    c.set_lengths(number)
+    assert c.lengths.np().tolist() == [3, 3]
