@@ -37,10 +37,9 @@ def _shape(*dims):
 
 
 def _whole(name, value, lowest):
-    n = int(value)
-    if n != value or n < lowest:
+    if not abs(value) < float("inf") or int(value) != value or value < lowest:
         raise ValueError(f"{name} {value} must be a whole number, at least {lowest}")
-    return n
+    return int(value)
 
 
 # =============================================================================================

@@ -150,3 +150,11 @@ def test_one_number_is_the_length_of_all(fake, number):
     c = nn.SinkCache(2, 1, 4, 1, 8)
     c.set_lengths(number)
     assert c.lengths.np().tolist() == [3, 3]
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan"), -float("inf")])
+def test_spans_that_are_not_finite_are_refused(fake, bad):
+    q = T(1, 1, 3, 4)
+    refused("window", nn.sink_attention, q, q, q, bad)
+    refused("sinks", nn.sink_attention, q, q, q, 2, bad)
+    refused("window", nn.SinkCache, 1, 1, bad, 0, 4)
