@@ -353,3 +353,61 @@ def test_gradient_of_some_rows_stays_on_the_tensor_cores(nn_gpu, where):
     for e in ev:
         lib.lnn_event_destroy(dev, e.value)
     assert sparse < 3 * dense, (sparse, dense)
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v", "k and do"])
+@pytest.mark.parametrize("S,D,past", [(300, 64, 0), (700, 128, 100), (150, 40, 0)])
+def test_operands_of_some_rows(nn_gpu, S, D, past, which):
+    """Operands whose rows are zero but for a few between those that the guess of the scale looks at."""
+    nn = nn_gpu
+    case = (2, 4, 2, S - past, S, D, S // 2, 3, None)
+    inputs, _ = base.attention_inputs(case)
+    lens = (S, S - 40)
+    for name, x in zip(("q", "k", "v", "do"), inputs):
+        if name in which.split():
+            keep = np.zeros(x.shape[2], bool)
+            keep[x.shape[2] // 2 + 1:x.shape[2] // 2 + 3] = True
+            x[:, :, ~keep] = 0.0
+            x *= np.float32(700.0 if name == "do" else 2.0 ** -7)
+    q, k, v, do = inputs
+    seen, scale = base.visible(S - past, S, S // 2, 3, lens), D ** -0.5
+    r = [torch.tensor(x, dtype=torch.float64, requires_grad=True) for x in (q, k, v)]
+    o = base.plain_attention(*r, seen, scale)
+    d64 = torch.tensor(do, dtype=torch.float64)
+    o.backward(d64)
+    bounds = base.attention_bounds(*[x.detach() for x in r], d64, seen, scale)
+    t = [nn.Tensor_from_value(x) for x in (q, k, v)]
+    base.trainable(nn, *t)
+    y = nn.sink_attention(*t, S // 2, 3, lengths_t=nn.Tensor_from_value(np.array(lens, np.float32)))
+    nn.backward({y: nn.Tensor_from_value(do)})
+    for name, g, w, b in zip(("o", "dq", "dk", "dv"), [y] + [x.get_grad() for x in t], [o.detach()] + [x.grad for x in r], bounds):
+        base.close(g.np(), w.numpy(), b.detach().numpy() + 1e-30, name)
+
+
+@pytest.mark.parametrize("S,D", [(40, 16), (300, 64), (100, 200)])
+def test_a_scale_of_nothing_is_the_mean(nn_gpu, S, D):
+    """All weights of a row are the same, whatever the products are, and nothing reaches q and k."""
+    nn = nn_gpu
+    rng = np.random.default_rng(S)
+    q, k, v, do = (rng.standard_normal((1, 2, S, D)).astype(np.float32) for _ in range(4))
+    k *= np.float32(1e3)
+    t = [nn.Tensor_from_value(x) for x in (q, k, v)]
+    base.trainable(nn, *t)
+    y = nn.sink_attention(*t, 7, scale=0.0)
+    nn.backward({y: nn.Tensor_from_value(do)})
+    w = base.visible(S, S, 7, 0, (S,))[0, 0].numpy().astype(np.float64)
+    w /= w.sum(-1, keepdims=True)
+    off = 2.0 ** -20 + 16 * U
+    base.close(y.np(), np.einsum("ij,bhjd->bhid", w, v.astype(np.float64)), off * np.abs(v).max(), "o")
+    base.close(t[2].get_grad().np(), np.einsum("ij,bhid->bhjd", w, do.astype(np.float64)), off * 7 * np.abs(do).max(), "dv")
+    assert not t[0].get_grad().np().any() and not t[1].get_grad().np().any()
+
+
+# ---------------------------------------------------------------------------------------------
+# borders between the kernels
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("case", [(2, 4, 2, S, S, D, w, 2, None) for D in (72, 128) for S in (32, 33, 64) for w in (10, 100)] +
+                         [(2, 4, 2, S, S, D, 20, 2, None) for D in (16, 64) for S in (64, 65)] +
+                         [(1, 2, 1, 1, S, 128, S, 0, None) for S in (32, 33)])
+def test_attention_at_the_borders_of_its_kernels(nn_gpu, case):
+    base.test_sink_attention(nn_gpu, case)
