@@ -35,7 +35,6 @@ using namespace lnn_tc;
 using lnn::AttnArgs;
 using lnn::HeadInfo;
 using lnn::exp2_fast;
-using lnn::min_or_nan;
 
 enum { FWD = 0, DV = 1, DQ = 2, DK = 3 };
 
@@ -1128,8 +1127,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__
                 }
                 float x, y;
                 unpack2(add2(fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), c2, hi), up), x, y);
-                // (a weight is 1 at most, whatever rounding says)
-                wt[i] = pack2(exp2_fast(min_or_nan(x, exponent)), exp2_fast(min_or_nan(y, exponent)));
+                // (1 at most but for the last bits: the scores are those of FWD to the bit, the logarithm has no step of its own)
+                wt[i] = pack2(exp2_fast(x), exp2_fast(y));
                 if (S::TWO)
                   wt[i] = mul2(wt[i], fma2(pack2(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), cdp2, less));
               }
