@@ -11,15 +11,18 @@
 //   DQ   rows are queries:  S, dP = dO V^T, dS = P (dP - delta), dQ += dS K
 //   DV   rows are keys:     S^T = K Q^T, P^T, dV += P^T dO
 //   DK   rows are keys:     S^T, dP^T = V dO^T, dS^T, dK += dS^T Q
+// Scores of 10^7 and more are as good as others: weights come from differences of scores (FWD), or from scores that are those of
+// FWD to the bit and a logarithm of the denominator that is kept in two floats.
 // Each sum has one owner: no atomics, results do not change from run to run.  dV and dK are separate passes (S^T is computed
 // twice) because 128 stationary rows of K and V of 128 values leave room in shared memory for two tiles of Q and one
 // of dO, not for two of both.
 //
-// What bounds it, for heads of 128 values: FWD and DV the way of the stream from L2 to shared memory (128 KB for a tile of 128 x
-// 128, about 3800 clocks where the products take 3120; with a quarter of the loads 3200), DQ and DK the gaps between the products
-// (3500 clocks for 128 x 64, 2780 of them products), and the turn from one tile of rows to the next (its first loads, 64 KB of
-// results: two to three steps).  Under load the SMs run at 1.6 of their 1.9 GHz.  8192 positions, 16 heads, window 1024: 197 us,
-// 328 TFLOP/s (three products each: 551 is the most); 8 heads over 2, window 2048: FWD 171, DQ 306, DV 186, DK 337 us.
+// What bounds it, for heads of 128 values: waiting, not a rate.  Counters of 8 heads over 2 of 4096 positions, window 1024 (of the
+// clocks in which an SM is active): tensor pipe FWD 47, DV 56, DQ 44, DK 48 %, issue slots 33 to 39 %; of their peaks L1 28 to 33 %, L2 9
+// to 21 %, DRAM 5 to 7 %.  FWD and DV have one slot each for K and V (Q and dO), whose next load begins when the products of the last
+// are over; DQ and DK have gaps between dependent products; and a tile of rows begins with its first loads and ends with
+// 64 KB of results (two to three steps).  Under load the SMs run at 1.6 of their 1.9 GHz.  8192 positions, 16 heads, window
+// 1024: 199 us, 325 TFLOP/s (three products each: 551 is the most); 8 heads over 2, window 2048: FWD 166, DQ 304, DV 187, DK 337 us.
 //
 // A persistent CTA of 576 threads per SM: warp 0 loads (TMA), one thread of warp 1 issues the MMAs, warps 2-17 (four per
 // quarter of the TMEM lanes, a fourth of the columns each) turn scores into weights, write them back to TMEM as the A operand
@@ -1508,7 +1511,7 @@ namespace lnn {
 // be half empty.  us for 32 heads, FP32 pipe / tensor cores: of 64 values, 64 positions 10.3 / 15.2, 96 positions 17.5 / 15.5, with
 // gradients 32.5 / 40.0 and 46.5 / 39.6; of 128 values, 32 positions 9.9 / 16.8, 64 positions 16.5 / 18.2, 96 positions 22.8 / 19.4,
 // with gradients 32.6 / 41.1, 55.4 / 45.9 and 78.8 / 49.4.  (The same for both directions: the gradients' scores are to
-// be those that the denominators were made of.)
+// be those that the denominators were made of.  Only a head whose dO the split form does not hold goes back by the other way.)
 bool attn_tc_applicable(const AttnArgs& a) {
   const int64_t heads = 2ll * a.batch * (a.q_heads + a.kv_heads);
   if (a.kv_len <= (a.dim <= 64 ? 64 : 32)) return false;

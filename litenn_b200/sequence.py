@@ -4,7 +4,7 @@ visible, its cache for one token after another, the logarithm of a token's proba
 They follow the op layer (ops.py): shapes are checked on the host, a result tensor with its grad functions is made, and
 one C-ABI call per current device does the work.  Token numbers and lengths are whole numbers in ordinary fp32 tensors,
 exact up to 2^24.  A token below zero marks a padded place.  A number that is no row of the table, or no length, is taken
-for padding and raises LnnError (E_INVALID) when a result is next read.
+for padding and raises LnnError (E_INVALID) when a result is next read; what is queued meanwhile runs.
 """
 from functools import lru_cache, partial
 
